@@ -378,6 +378,75 @@ VFB_API int vfb_nvfp4_gemm_quant(const void *A, const void *sfa, const void *W, 
                                  int64_t K, const vfb_epilogue *ep, const float *out_global_scale,
                                  void *out_codes, void *out_sf, void *stream);
 
+/* ---- NVFP4 weight, 16-bit activations ------------------------------------
+ * The product of a few rows with an NVFP4 weight whose activations are not
+ * quantised (single tokens, small batches), beside the W4A4 GEMM above:
+ *   y[m,n] = bf16( alpha * sum_k x[m,k] * e2m1(W[n,k]) * e4m3(sf[n,k/16]) + bias[n] )
+ * with exact products, fp32 accumulation and one rounding at the end.  x:
+ * bf16 (dtype 0) or fp16 (dtype 1) [M,K], row stride ldx >= K, any alignment
+ * of its element type.  w_codes / w_sf: the packed weight [N,K/2] and its 128x4 scales as in
+ * vfb_nvfp4_gemm.  alpha: fp32 device scalar.  bias: bf16 [N] or NULL.  out:
+ * bf16 [M,N], row stride ldo >= N.  Requires K % 64 == 0, N % 128 == 0,
+ * 16-byte aligned w_codes, 4-byte aligned w_sf, and a `workspace` of
+ * vfb_nvfp4_weight_only_workspace_bytes(M, N, K) bytes (0: may be NULL),
+ * 256-byte aligned, that no other call in flight uses.  Every row of x is
+ * brought to fp16 by a power of two of its own (exact for elements within
+ * 2^-30 of the row's largest magnitude).  No reference counterpart: the
+ * reference always quantises the activations. */
+VFB_API int64_t vfb_nvfp4_weight_only_workspace_bytes(int64_t M, int64_t N, int64_t K);
+VFB_API int vfb_nvfp4_weight_only(const void *x, int32_t dtype, int64_t M, int64_t ldx,
+                                  const void *w_codes, const void *w_sf, const float *alpha,
+                                  const void *bias, int64_t N, int64_t K, void *out, int64_t ldo,
+                                  void *workspace, int64_t workspace_bytes, void *stream);
+
+/* ---- attention over packed sequences ---------------------------------------
+ * What stands between the QKV projection's planes and the attention output
+ * projection (the dense attention of the reference's block,
+ * src/vflash/native/h3_native_denoiser.py:543-550, generalised to packed
+ * sequences, grouped heads, causal masks and cached keys).  For query row i of
+ * a sequence with nq query rows and nk keys, and head h reading key/value head
+ * h / (heads / kv_heads):
+ *   s_j = scale * q_i . k_j  for j < limit(i),
+ *   limit(i) = causal ? min(nk, i + 1 + nk - nq) : nk
+ *   out_i = sum_j exp(s_j - max s) v_j / sum_j exp(s_j - max s)
+ *   lse_i = log sum_j exp(s_j)                            (natural logarithm)
+ * Sums and statistics are fp32; exp values are rounded to the operands' type
+ * for the second product.  Keys at or beyond limit(i) never reach row i,
+ * whatever they hold (infinities and NaN included).  A row with no key is 0
+ * with lse = -inf.
+ * Rows: sequence b has the query rows [cu_seqlens_q[b], cu_seqlens_q[b+1]) and
+ * the keys from row cu_seqlens_k[b]: up to cu_seqlens_k[b+1], or lengths_k[b]
+ * of them (clamped to the slot) when lengths_k != NULL.  The three are device
+ * int32 arrays ([batch+1], [batch+1], [batch]), non-decreasing, starting at 0;
+ * cu_seqlens_q == NULL means one sequence of all rows, cu_seqlens_k == NULL the
+ * query's offsets.  Offsets beyond the buffers are clamped to them.  Rows of
+ * `out` behind the last sequence are written as zeros when fill_tail, else left
+ * as they are; rows of `lse` behind it become -inf. */
+typedef struct vfb_attention_args {
+  const void *q, *k, *v;       /* bf16 (dtype 0) or fp16 (dtype 1), [rows, heads, dim], unit dim stride */
+  void *out;                   /* the same type, [total_q, heads, dim]; may not alias q, k or v */
+  float *lse;                  /* [heads, total_q] contiguous, or NULL */
+  int64_t q_token_stride, q_head_stride;  /* strides in elements, multiples of 8; bases 16-byte aligned */
+  int64_t k_token_stride, k_head_stride;
+  int64_t v_token_stride, v_head_stride;
+  int64_t out_token_stride, out_head_stride;
+  int64_t total_q, total_k;    /* rows of q and of k / v, < 2^31 */
+  int32_t heads, kv_heads;     /* heads % kv_heads == 0 */
+  int32_t dim;                 /* 8 <= dim <= 128, dim % 8 == 0 */
+  int32_t dtype;
+  const int32_t *cu_seqlens_q, *cu_seqlens_k, *lengths_k;
+  int32_t batch;               /* sequences (1 when cu_seqlens_q == NULL) */
+  int32_t causal;
+  float scale;                 /* positive, finite */
+  int32_t fill_tail;
+  void *workspace;             /* vfb_attention_workspace_bytes() bytes, 256-byte aligned; NULL when that is 0. */
+  int64_t workspace_bytes;     /* No other call in flight may use it. */
+} vfb_attention_args;
+
+/* Bytes of workspace these arguments need (0 when none), or -1 when they are refused. */
+VFB_API int64_t vfb_attention_workspace_bytes(const vfb_attention_args *args);
+VFB_API int vfb_attention(const vfb_attention_args *args, void *stream);
+
 /* ---- strict-BF16 elementwise steps -----------------------------------------
  * Standalone versions of the epilogues above, for callers whose GEMM is not
  * this library's.  bf16 tensors; the last dimension is contiguous and its

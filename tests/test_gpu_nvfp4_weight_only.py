@@ -1,0 +1,217 @@
+"""The weight-only NVFP4 product against 64-bit sums of the exactly decoded weights.
+
+Bound per element: the final rounding (2^-8 of the value, bf16), fp32 sums of
+exact products (K/16 + 64 dependent additions of 2^-24 each, relative to the
+sum of magnitudes), the power-of-two fp16 form of the activations (2^-38 of
+the row's largest magnitude times the sum of the weights' magnitudes) and one
+fp32 rounding for alpha and the bias each.
+"""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import nvfp4
+from vflash_b200 import _lib
+from vflash_b200.kernels import attention, nvfp4_quantize, nvfp4_weight_only
+from vflash_b200.native.h3_attention import PackedAttention
+from vflash_b200.native.h3_nvfp4_linear import NVFP4Execution, NVFP4Weight
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+def weight_of(n, k, seed):
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    w = (torch.randn(n, k, generator=gen, device=DEV) * 0.02).to(BF16)
+    scale = (448.0 * 6.0 / w.float().abs().max()).reshape(())
+    packed, sf = nvfp4_quantize(w, scale)
+    return NVFP4Weight(packed, sf.reshape(n, k // 16), (1.0 / scale).reshape(()), torch.ones((), device=DEV))
+
+
+def decoded(weight):
+    n, k = weight.out_features, weight.in_features
+    w = nvfp4.dequantize(weight.packed.cpu().numpy(), weight.scales.cpu().numpy().reshape(-1), n, k)
+    return torch.from_numpy(w).to(DEV)
+
+
+def activations(rows, k, seed, dtype, gain=1.0):
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randn(rows, k, generator=gen, device=DEV) * gain
+    x[torch.rand(rows, k, generator=gen, device=DEV) < 0.002] *= 20
+    return x.to(dtype)
+
+
+def check(got, x, weight, bias):
+    w, xd, alpha = decoded(weight), x.double(), weight.alpha.double()
+    want = alpha * (xd @ w.T)
+    size = alpha * (xd.abs() @ w.abs().T)
+    if bias is not None:
+        want = want + bias.double()
+        size = size + bias.double().abs()
+    k = x.shape[1]
+    bound = (2.0**-8 * want.abs() + (k / 16 + 64 + 4) * 2.0**-24 * size
+             + 2.0**-38 * alpha * xd.abs().amax(dim=1, keepdim=True) * w.abs().sum(dim=1) + 1e-38)
+    error = (got.double() - want).abs()
+    assert got.dtype == BF16 and got.shape == want.shape
+    assert (error <= bound).all(), f"{(error / bound).max().item():.2f} times the bound"
+    assert _lib.device_status(clear=True) == _lib.VFB_OK
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("rows", [1, 2, 3, 7, 8, 9, 16, 17, 31, 33, 70])
+@pytest.mark.parametrize("n,k", [(128, 64), (256, 192), (384, 1024), (128, 4160), (1152, 512)])
+def test_against_the_decoded_weight(rows, n, k, dtype, with_bias):
+    weight = weight_of(n, k, n + k)
+    x = activations(rows, k, rows, dtype)
+    bias = activations(1, n, 5, BF16)[0] if with_bias else None
+    check(nvfp4_weight_only(x, weight.packed, weight.scales, weight.alpha, bias), x, weight, bias)
+
+
+@pytest.mark.parametrize("n,k", [(4096, 4096), (12288, 4096), (4096, 16384), (5376, 14336)])
+@pytest.mark.parametrize("rows", [1, 5])
+def test_model_sizes(n, k, rows):
+    weight = weight_of(n, k, 3)
+    x = activations(rows, k, 4, BF16)
+    check(nvfp4_weight_only(x, weight.packed, weight.scales, weight.alpha), x, weight, None)
+
+
+def test_every_code_and_scale_decodes_exactly():
+    """One activation of 1 per row of x: the output is that weight times alpha, exact in bf16."""
+    n, k = 128, 256
+    rng = np.random.default_rng(0)
+    codes = rng.integers(0, 16, (n, k), dtype=np.uint8)
+    scales = rng.permutation(np.arange(n * k // 16) % 127).astype(np.uint8)  # every finite e4m3 >= 0
+    flat = np.zeros(n * (k // 16), dtype=np.uint8)
+    flat[nvfp4.sf_offsets(n, k // 16).reshape(-1)] = scales
+    weight = NVFP4Weight(torch.from_numpy(nvfp4.pack(codes)).to(DEV), torch.from_numpy(flat.reshape(n, -1)).to(DEV),
+                         torch.tensor(0.5, device=DEV), torch.ones((), device=DEV))
+    w = decoded(weight)
+    for dtype in (BF16, FP16):
+        x = torch.eye(k, dtype=dtype, device=DEV)
+        got = nvfp4_weight_only(x, weight.packed, weight.scales, weight.alpha)
+        assert torch.equal(got.double(), 0.5 * w.T)
+
+
+def test_whole_numbers_are_exact():
+    n, k = 256, 2048
+    rng = np.random.default_rng(1)
+    codes = rng.integers(0, 16, (n, k), dtype=np.uint8)
+    weight = NVFP4Weight(torch.from_numpy(nvfp4.pack(codes)).to(DEV),
+                         torch.full((n, k // 16), 0x40, dtype=torch.uint8, device=DEV),  # e4m3 2.0: whole weights
+                         torch.ones((), device=DEV), torch.ones((), device=DEV))
+    x = torch.randint(-8, 9, (5, k), generator=torch.Generator(device=DEV).manual_seed(2), device=DEV).to(BF16)
+    got = nvfp4_weight_only(x, weight.packed, weight.scales, weight.alpha)
+    assert torch.equal(got, (x.double() @ decoded(weight).T).to(BF16))
+
+
+@pytest.mark.parametrize("gain", [1e-30, 1e-6, 1e6, 1e30])
+def test_activation_ranges(gain):
+    weight = weight_of(256, 512, 8)
+    x = activations(4, 512, 9, BF16, gain)
+    x[1] *= 1e-3  # rows of very different sizes
+    x[2] = 0
+    check(nvfp4_weight_only(x, weight.packed, weight.scales, weight.alpha), x, weight, None)
+
+
+def test_activations_that_are_not_finite():
+    weight = weight_of(256, 512, 8)
+    x = activations(4, 512, 9, BF16)
+    want = nvfp4_weight_only(x, weight.packed, weight.scales, weight.alpha)
+    x[1, 77] = float("nan")
+    x[2, 300] = float("inf")
+    got = nvfp4_weight_only(x, weight.packed, weight.scales, weight.alpha)
+    assert torch.equal(got[[0, 3]], want[[0, 3]])
+    assert torch.isnan(got[1]).all()
+    column = decoded(weight)[:, 300]
+    assert torch.equal(torch.isnan(got[2]), column == 0)  # inf * 0
+    assert torch.equal(got[2][column > 0] == torch.inf, torch.ones_like(column[column > 0], dtype=torch.bool))
+    assert torch.equal(got[2][column < 0] == -torch.inf, torch.ones_like(column[column < 0], dtype=torch.bool))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_strides_and_alignment(dtype):
+    weight = weight_of(384, 320, 2)
+    wide = activations(9, 331, 3, dtype)
+    out = torch.full((9, 400), 7.0, dtype=BF16, device=DEV)
+    for shift in (0, 1, 3, 8):  # rows that start on any element
+        x = wide[:, shift:shift + 320]
+        got = nvfp4_weight_only(x, weight.packed, weight.scales, weight.alpha, out=out[:, shift:shift + 384])
+        check(got, x, weight, None)
+        assert torch.equal(got, nvfp4_weight_only(x.contiguous(), weight.packed, weight.scales, weight.alpha))
+    assert (out[:, 8 + 384:] == 7.0).all()
+
+
+def test_execution_keeps_leading_dimensions_and_rounds_fp32_first():
+    weight = weight_of(128, 192, 2)
+    x = activations(6, 192, 3, torch.float32).reshape(2, 3, 192)
+    engine = NVFP4Execution()
+    got = engine.weight_only_linear(x, weight)
+    assert got.shape == (2, 3, 128) and engine.calls == 1 and engine.rows == 6
+    check(got.reshape(6, 128), x.reshape(6, 192).to(BF16), weight, None)
+
+
+def test_graph_replay_and_the_same_bits_on_two_streams():
+    weight = weight_of(1024, 2048, 2)
+    x = activations(3, 2048, 3, BF16)
+    run = lambda: nvfp4_weight_only(x, weight.packed, weight.scales, weight.alpha)  # noqa: E731
+    want = run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    graph.replay()
+    assert torch.equal(got, want)
+    x.copy_(activations(3, 2048, 30, BF16))
+    graph.replay()
+    check(got, x, weight, None)
+    want = run()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        outs = []
+        for stream in streams:
+            with torch.cuda.stream(stream):
+                outs.append(run())
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for o in outs)
+
+
+def test_single_token_step():
+    """The operators as a serving step uses them: weight-only QKV, attention over cached keys, weight-only output."""
+    heads, kv, dim, hidden, batch, slot = 8, 2, 64, 512, 3, 300
+    qkv, out = weight_of((heads + 2 * kv) * dim, hidden, 1), weight_of(hidden, heads * dim, 2)
+    engine = NVFP4Execution()
+    x = activations(batch, hidden, 3, BF16)
+    lengths = [299, 1, 130]
+    k_cache = activations(batch * slot, kv * dim, 4, BF16).reshape(-1, kv, dim)
+    v_cache = activations(batch * slot, kv * dim, 5, BF16).reshape(-1, kv, dim)
+    cu_q = torch.arange(batch + 1, dtype=torch.int32, device=DEV)
+    used = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    rows = torch.arange(batch, device=DEV) * slot + used.long() - 1
+
+    def step():
+        planes = engine.weight_only_linear(x, qkv)
+        q, k, v = planes.split([heads * dim, kv * dim, kv * dim], dim=-1)
+        k_cache[rows] = k.reshape(batch, kv, dim)
+        v_cache[rows] = v.reshape(batch, kv, dim)
+        y = PackedAttention(heads, kv, causal=True)(q, k_cache.reshape(-1, kv * dim), v_cache.reshape(-1, kv * dim),
+                                                    cu_q, cu_q * slot, lengths_k=used)
+        return q, y, engine.weight_only_linear(y, out)
+
+    q, y, z = step()
+    check(z, y, out, None)
+    want = attention(q.reshape(batch, heads, dim), k_cache, v_cache, cu_q, cu_q * slot, lengths_k=used)
+    assert torch.equal(y.reshape(batch, heads, dim), want)
+    for b, n in enumerate(lengths):
+        keys = k_cache[b * slot:b * slot + n].double()
+        values = v_cache[b * slot:b * slot + n].double()
+        for h in range(heads):
+            p = torch.softmax(keys[:, h // 4] @ q[b, h * dim:(h + 1) * dim].double() * dim**-0.5, dim=0)
+            ref, size = p @ values[:, h // 4], p @ values[:, h // 4].abs()
+            # one rounding of the output and one of every probability, and 2^-12 for all that is kept in fp32
+            bound = 2.0**-8 * ref.abs() + (2.0**-8 + 2.0**-12) * size
+            assert ((y[b, h * dim:(h + 1) * dim].double() - ref).abs() <= bound).all()

@@ -63,6 +63,25 @@ class Epilogue(ctypes.Structure):
     ]
 
 
+class AttentionArgs(ctypes.Structure):
+    """Mirror of ``vfb_attention_args``."""
+
+    _fields_ = [
+        *[(name, _vp) for name in ("q", "k", "v", "out", "lse")],
+        *[(name, _c_int64) for name in ("q_token_stride", "q_head_stride", "k_token_stride", "k_head_stride",
+                                        "v_token_stride", "v_head_stride", "out_token_stride", "out_head_stride",
+                                        "total_q", "total_k")],
+        *[(name, ctypes.c_int32) for name in ("heads", "kv_heads", "dim", "dtype")],
+        *[(name, _vp) for name in ("cu_seqlens_q", "cu_seqlens_k", "lengths_k")],
+        ("batch", ctypes.c_int32),
+        ("causal", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("fill_tail", ctypes.c_int32),
+        ("workspace", _vp),
+        ("workspace_bytes", _c_int64),
+    ]
+
+
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "vfb_last_error": (ctypes.c_char_p, []),
     "vfb_version": (ctypes.c_char_p, []),
@@ -131,6 +150,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_vp, _vp, _vp, _vp, _vp, _vp, _c_int64, _c_int64, _c_int64, ctypes.POINTER(Epilogue), _vp, _vp, _vp,
          _vp],
     ),
+    "vfb_nvfp4_weight_only_workspace_bytes": (_c_int64, [_c_int64, _c_int64, _c_int64]),
+    "vfb_nvfp4_weight_only": (
+        ctypes.c_int,
+        [_vp, ctypes.c_int32, _c_int64, _c_int64, _vp, _vp, _vp, _vp, _c_int64, _c_int64, _vp, _c_int64, _vp,
+         _c_int64, _vp],
+    ),
+    "vfb_attention_workspace_bytes": (_c_int64, [ctypes.POINTER(AttentionArgs)]),
+    "vfb_attention": (ctypes.c_int, [ctypes.POINTER(AttentionArgs), _vp]),
     "vfb_silu_mul": (ctypes.c_int, [_vp, _c_int64, _c_int64, _vp, _c_int64, _vp]),
     "vfb_ffn_adapter_silu": (
         ctypes.c_int, [_vp, _vp, _c_int64, _c_int64, ctypes.c_float, _vp, _c_int64, _vp]),

@@ -561,3 +561,174 @@ def _nvfp4_gemm_quant(a_codes, a_sf, w_packed, w_scales, alpha, alpha_div, ep: E
                                       sf.data_ptr(), _lib.stream_handle(device))
     _lib.check(rc, "vfb_nvfp4_gemm_quant")
     return codes, sf
+
+
+def _workspace(nbytes: int, device):
+    """A 256-byte aligned buffer of ``nbytes`` from torch's allocator: the tensor to keep and its address."""
+    if nbytes == 0:
+        return None, None
+    buffer = torch.empty(nbytes, device=device, dtype=torch.uint8)  # the allocator aligns to 512 bytes
+    return buffer, buffer.data_ptr()
+
+
+def nvfp4_weight_only(matrix: torch.Tensor, w_packed: torch.Tensor, w_scales: torch.Tensor, alpha: torch.Tensor,
+                      bias: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``bf16(alpha * matrix @ W^T + bias)`` for an NVFP4 weight and activations that stay in 16 bits.
+
+    ``matrix`` bf16 or fp16 ``[M, K]`` (unit column stride, any row stride),
+    ``w_packed`` uint8 ``[N, K/2]`` and ``w_scales`` uint8 (128x4 layout) as
+    ``nvfp4_gemm`` takes them, ``alpha`` an fp32 scalar tensor, ``bias`` bf16
+    ``[N]``.  K % 64 == 0, N % 128 == 0.  Made for few rows (one token, a small
+    batch); any M works, re-reading the weight for every block of rows.
+    """
+    if matrix.dtype not in (BF16, torch.float16) or matrix.ndim != 2 or matrix.stride(1) != 1 and matrix.shape[1] > 1:
+        raise KernelInputError("the weight-only NVFP4 product needs a bf16/fp16 [M, K] matrix with unit column stride")
+    rows, k = matrix.shape
+    device = matrix.device
+    if (w_packed.dtype != torch.uint8 or w_packed.ndim != 2 or 2 * w_packed.shape[1] != k
+            or not w_packed.is_contiguous()):
+        raise KernelInputError("NVFP4 weight codes must be contiguous uint8 [N, K/2]")
+    n = w_packed.shape[0]
+    if n == 0 or k == 0 or k % 64 or n % 128:
+        raise KernelInputError("the weight-only NVFP4 product needs K % 64 == 0, N % 128 == 0")
+    if w_scales.dtype != torch.uint8 or w_scales.numel() != n * (k // 16) or not w_scales.is_contiguous():
+        raise KernelInputError("NVFP4 weight scales differ from the 128x4 layout")
+    if alpha.dtype != torch.float32 or alpha.numel() != 1:
+        raise KernelInputError("NVFP4 alpha must be an fp32 scalar tensor")
+    if bias is not None and (bias.dtype != BF16 or bias.shape != (n,) or not bias.is_contiguous()):
+        raise KernelInputError("NVFP4 bias must be contiguous bf16 [N]")
+    if not (_aligned(w_packed) and _aligned(w_scales, 4)):
+        raise KernelInputError("NVFP4 weight codes must be 16-byte aligned, scales 4-byte aligned")
+    if out is None:
+        out = torch.empty((rows, n), device=device, dtype=BF16)
+    elif out.dtype != BF16 or out.shape != (rows, n) or out.stride(1) != 1:
+        raise KernelInputError("the weight-only NVFP4 output must be bf16 [M, N] with unit column stride")
+    for t in (w_packed, w_scales, alpha, bias, out):
+        if t is not None and t.device != device:
+            raise KernelInputError("weight-only NVFP4 operands must share one device")
+    if rows == 0:
+        return out
+    lib = _lib.load()
+    with torch.cuda.device(device):
+        need = lib.vfb_nvfp4_weight_only_workspace_bytes(rows, n, k)
+        keep, workspace = _workspace(need, device)
+        rc = lib.vfb_nvfp4_weight_only(
+            matrix.data_ptr(), 0 if matrix.dtype == BF16 else 1, rows, max(matrix.stride(0), k),
+            w_packed.data_ptr(), w_scales.data_ptr(), alpha.data_ptr(), _lib.ptr(bias), n, k, out.data_ptr(),
+            max(out.stride(0), n), workspace, need, _lib.stream_handle(device))
+    _lib.check(rc, "vfb_nvfp4_weight_only")
+    return out
+
+
+# ---------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------
+def _head_strides(t: torch.Tensor, name: str) -> tuple[int, int]:
+    """Token and head strides of a ``[rows, heads, dim]`` tensor; a dimension of one element takes a packed stride."""
+    rows, heads, dim = t.shape
+    if t.stride(2) != 1 and dim > 1:
+        raise KernelInputError(f"attention {name} needs a unit stride over the head dimension")
+    head = t.stride(1) if heads > 1 else dim
+    token = t.stride(0) if rows > 1 else max(heads * dim, heads * head)
+    if head % 8 or token % 8 or head < dim or token < dim or (rows and not _aligned(t)):
+        raise KernelInputError(f"attention {name} needs 16-byte aligned rows (strides of 8 elements, not expanded)")
+    return token, head
+
+
+def _check_offsets(t: torch.Tensor, entries: int | None, device, name: str) -> None:
+    if (t.dtype != torch.int32 or t.ndim != 1 or not t.is_contiguous() or t.device != device or not _aligned(t, 4)
+            or entries is not None and t.shape[0] != entries):
+        raise KernelInputError(f"attention {name} must be contiguous int32 on the queries' device"
+                               + ("" if entries is None else f" with {entries} entries"))
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: torch.Tensor | None = None,
+              cu_seqlens_k: torch.Tensor | None = None, *, lengths_k: torch.Tensor | None = None,
+              causal: bool = False, scale: float | None = None, out: torch.Tensor | None = None,
+              return_lse: bool = False):
+    """Softmax attention over packed sequences (``vfb_attention``).
+
+    ``q`` ``[total_q, heads, dim]``, ``k`` and ``v`` ``[total_k, kv_heads, dim]``,
+    all bf16 or all fp16, ``dim`` a multiple of 8 up to 128 with unit stride,
+    other strides free (multiples of 8 elements); head ``h`` reads key head
+    ``h // (heads // kv_heads)``.  Sequence ``b`` has the query rows
+    ``cu_seqlens_q[b]:cu_seqlens_q[b+1]`` and the keys of the same entries of
+    ``cu_seqlens_k`` (default: the queries' offsets), of which only the first
+    ``lengths_k[b]`` count when ``lengths_k`` is given (a cache of fixed slots).
+    The offsets are int32 device tensors that start at 0 and do not decrease;
+    without them all rows are one sequence.  ``causal`` lets the last query row
+    of a sequence see its last key.  ``scale`` defaults to ``dim ** -0.5``.
+
+    Returns ``[total_q, heads, dim]`` in the inputs' type, with ``return_lse``
+    also the fp32 ``[heads, total_q]`` log-sum-exp of the scaled scores.  A row
+    without keys is 0 (lse -inf), and so is a row behind the last sequence,
+    except in a given ``out``, where those rows stay as they were.  Inference
+    only; the scores never leave the SM.
+    """
+    if q.ndim != 3 or k.ndim != 3 or v.ndim != 3:
+        raise KernelInputError("attention operands must be [rows, heads, dim]")
+    total_q, heads, dim = q.shape
+    total_k, kv_heads = k.shape[:2]
+    device = q.device
+    if q.dtype not in (BF16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise KernelInputError("attention needs q, k and v all bf16 or all fp16")
+    if k.shape != v.shape or k.shape[2] != dim or kv_heads < 1 or heads < 1 or heads % kv_heads:
+        raise KernelInputError("attention needs k and v of one shape, q's dim, and heads divisible by kv_heads")
+    if not 8 <= dim <= 128 or dim % 8:
+        raise KernelInputError("attention needs a head dimension of 8 to 128, a multiple of 8")
+    if max(total_q, total_k) >= 2**31:
+        raise KernelInputError("attention rows must stay below 2^31")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        raise KernelInputError("attention is inference-only")
+    scale = dim ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise KernelInputError("attention scale must be positive and finite")
+    for t in (k, v):
+        if t.device != device:
+            raise KernelInputError("attention operands must share one device")
+    a = _lib.AttentionArgs()
+    if cu_seqlens_q is None:
+        if cu_seqlens_k is not None:
+            raise KernelInputError("attention cu_seqlens_k needs cu_seqlens_q")
+        batch = 1
+    else:
+        _check_offsets(cu_seqlens_q, None, device, "cu_seqlens_q")
+        batch = cu_seqlens_q.shape[0] - 1
+        if batch < 1:
+            raise KernelInputError("attention cu_seqlens_q needs at least two entries")
+        a.cu_seqlens_q = cu_seqlens_q.data_ptr()
+        if cu_seqlens_k is not None:
+            _check_offsets(cu_seqlens_k, batch + 1, device, "cu_seqlens_k")
+            a.cu_seqlens_k = cu_seqlens_k.data_ptr()
+        elif total_k != total_q:
+            raise KernelInputError("attention keys of another length than the queries need cu_seqlens_k")
+    if lengths_k is not None:
+        _check_offsets(lengths_k, batch, device, "lengths_k")
+        a.lengths_k = lengths_k.data_ptr()
+    a.q_token_stride, a.q_head_stride = _head_strides(q, "q")
+    a.k_token_stride, a.k_head_stride = _head_strides(k, "k")
+    a.v_token_stride, a.v_head_stride = _head_strides(v, "v")
+    fresh = out is None
+    if fresh:
+        out = torch.empty((total_q, heads, dim), device=device, dtype=q.dtype)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != device:
+        raise KernelInputError("attention out differs from q's shape, type or device")
+    a.out_token_stride, a.out_head_stride = _head_strides(out, "out")
+    lse = torch.empty((heads, total_q), device=device, dtype=torch.float32) if return_lse else None
+    if total_q:
+        require_sm100(device)
+        a.q, a.k, a.v, a.out, a.lse = (_lib.ptr(t) for t in (q, k, v, out, lse))
+        a.total_q, a.total_k, a.heads, a.kv_heads, a.dim = total_q, total_k, heads, kv_heads, dim
+        a.dtype = 0 if q.dtype == BF16 else 1
+        a.batch, a.causal, a.scale, a.fill_tail = batch, int(causal), scale, int(fresh)
+        lib = _lib.load()
+        args = ctypes.byref(a)
+        need = lib.vfb_attention_workspace_bytes(args)
+        if need < 0:
+            raise KernelInputError(f"attention: {_lib.last_error()}")
+        with torch.cuda.device(device):
+            keep, a.workspace = _workspace(need, device)
+            a.workspace_bytes = need
+            rc = lib.vfb_attention(args, _lib.stream_handle(device))
+        _lib.check(rc, "vfb_attention")
+    return (out, lse) if return_lse else out

@@ -7,11 +7,12 @@ with its gated residual ``residual + gate * projected`` (551-556, 366-367),
 the FFN input ``[F, H]`` (568) and the FFN output ``[H, F]`` with its gated
 residual (570-575).  The stack measured here uses the GELU-tanh FFN of the
 fused-FFN benchmark (``F = 4H``); the packed SwiGLU input of 369-373 is the
-``swiglu`` activation of ``RowFP8Execution.ffn``.  Attention and the
-modulation/normalisation steps are not part of this path: ``block_linears``
-feeds the V plane to the attention output projection in attention's place,
-so the four GEMMs run at their real shapes on real data, and the gate is a
-caller-supplied ``[1, H]`` row, fused into the GEMM epilogues.
+``swiglu`` activation of ``RowFP8Execution.ffn``.  The
+modulation/normalisation steps are not part of this path, and attention
+(543-550) is when the caller passes a ``PackedAttention``; without one
+``block_linears`` feeds the V plane to the attention output projection in
+attention's place, so the four GEMMs run at their real shapes on real data.
+The gate is a caller-supplied ``[1, H]`` row, fused into the GEMM epilogues.
 
 Weights live in a ``PinnedHostArena`` and reach the GPU through an
 ``FP8BlockRing`` (two device slots, side copy stream), or stay resident.
@@ -25,6 +26,7 @@ from collections.abc import Iterable
 
 import torch
 
+from .h3_attention import PackedAttention
 from .h3_fp8_linear import RowFP8Execution
 from .h3_parallel import FP8Weight
 from .h3_pinned_arena import ALIGN, BlockLayout, FP8BlockRing, PinnedHostArena, pin_blocks
@@ -41,14 +43,21 @@ def block_flops(rows: int, hidden: int, ffn: int) -> int:
 
 
 def block_linears(execution: RowFP8Execution, weights: dict[str, FP8Weight], hidden: torch.Tensor,
-                  gate: torch.Tensor) -> torch.Tensor:
+                  gate: torch.Tensor, *, attention: PackedAttention | None = None,
+                  cu_seqlens: torch.Tensor | None = None) -> torch.Tensor:
     """One block's linears on ``hidden`` ``[rows, 1, H]`` (bf16) with gate ``[1, H]``.
 
-    qkv -> (V as attention output) -> attention_out with gated residual ->
-    FFN (GELU-tanh up, per-token requant, down with gated residual).
+    qkv -> attention (without ``attention``: V as its output) -> attention_out
+    with gated residual -> FFN (GELU-tanh up, per-token requant, down with gated
+    residual).  ``cu_seqlens`` splits the rows into samples that attend only to
+    themselves (``kernels.attention``); without it they are one sample.
     """
+    if attention is None and cu_seqlens is not None:
+        raise ValueError("cu_seqlens splits the rows for attention, which was not given")
     qkv = weights["qkv"]
-    _q, _k, v = execution.qkv_linear(hidden, qkv.codes, qkv.row_scale)
+    q, k, v = execution.qkv_linear(hidden, qkv.codes, qkv.row_scale)
+    if attention is not None:
+        v = attention(q, k, v, cu_seqlens)
     out = weights["attention_out"]
     hidden = execution.gate_residual_linear(v, out.codes, out.row_scale, hidden, gate)
     up, down = weights["ffn_in"], weights["ffn_out"]
@@ -62,7 +71,7 @@ class FP8BlockStack:
     ``blocks`` yields one ``{name: FP8Weight}`` dict per block (any device);
     each is packed, this rank's byte range is pinned, and the source may be
     freed afterwards.  ``forward(hidden, gate)`` runs every block on the
-    current stream.
+    current stream, with its attention when ``attention`` is given.
     """
 
     def __init__(self, blocks: Iterable[dict[str, FP8Weight]], hidden: int, ffn: int, device, *,
@@ -113,22 +122,23 @@ class FP8BlockStack:
     def weight_bytes_per_block(self) -> int:
         return self.layout.nbytes
 
-    def capture(self, hidden: torch.Tensor, gate: torch.Tensor):
+    def capture(self, hidden: torch.Tensor, gate: torch.Tensor, *, attention: PackedAttention | None = None,
+                cu_seqlens: torch.Tensor | None = None):
         """CUDA graph of ``forward`` over a resident stack; returns ``replay() -> output``.
 
         The stack runs once eagerly first (loading every block and setting up
         the kernels), then the block loop is captured; a replay reads the
-        current contents of ``hidden`` and ``gate`` and rewrites the returned
-        output tensor.  One graph launch replaces the per-block host work of
+        current contents of ``hidden`` and ``gate`` (and ``cu_seqlens``) and
+        rewrites the returned output tensor.  One graph launch replaces the per-block host work of
         issuing 8 kernels per block.
         """
         if not self.ring.resident:
             raise ValueError("graph capture needs a resident stack")
-        self.forward(hidden, gate)
+        self.forward(hidden, gate, attention=attention, cu_seqlens=cu_seqlens)
         torch.cuda.synchronize(self.ring.device)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
-            out = self.ring.run(hidden, lambda w, h: block_linears(self.execution, w, h, gate), wait_ready=False)
+            out = self.ring.run(hidden, self._block(gate, attention, cu_seqlens), wait_ready=False)
 
         def replay() -> torch.Tensor:
             graph.replay()
@@ -137,7 +147,11 @@ class FP8BlockStack:
         replay.graph = graph
         return replay
 
-    def forward(self, hidden: torch.Tensor, gate: torch.Tensor) -> torch.Tensor:
+    def _block(self, gate, attention, cu_seqlens):
+        return lambda w, h: block_linears(self.execution, w, h, gate, attention=attention, cu_seqlens=cu_seqlens)
+
+    def forward(self, hidden: torch.Tensor, gate: torch.Tensor, *, attention: PackedAttention | None = None,
+                cu_seqlens: torch.Tensor | None = None) -> torch.Tensor:
         if hidden.ndim != 3 or hidden.shape[1] != 1 or hidden.shape[2] != self.hidden:
             raise ValueError("block stack input must be bf16 [rows, 1, hidden]")
-        return self.ring.run(hidden, lambda w, h: block_linears(self.execution, w, h, gate))
+        return self.ring.run(hidden, self._block(gate, attention, cu_seqlens))

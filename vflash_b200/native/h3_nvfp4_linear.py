@@ -19,7 +19,8 @@ from functools import cache
 import torch
 
 from .. import _lib
-from ..kernels import Epilogue, nvfp4_gemm, nvfp4_norm_modulate_quantize, nvfp4_quantize
+from ..kernels import (Epilogue, nvfp4_gemm, nvfp4_norm_modulate_quantize, nvfp4_quantize,
+                       nvfp4_weight_only)
 from .h3_fp8_linear import NormModulate
 
 SF_LAYOUT_128x4 = "128x4"
@@ -193,6 +194,36 @@ class NVFP4Execution:
         self.rows += matrix.shape[0]
         output = output.reshape(*shape[:-1], weight.out_features)
         return output if bias is None else output + bias
+
+    def weight_only_linear(self, values, weight: NVFP4Weight, bias=None):
+        """``bf16(weight.alpha * values @ W^T + bias)`` with the activations left in 16 bits.
+
+        ``W[n, k] = e2m1(code) * e4m3(scale)`` exactly; ``weight.input_scale``
+        (the W4A4 path's activation calibration) plays no part.  For single
+        tokens and small batches, where ``linear`` would pad to a 128-row tile
+        and quantise the activations for nothing: the call is bound by reading
+        the weight once.  fp32 values are first rounded to bf16, as in
+        ``linear``; sums are fp32, with one rounding after the bias.
+        """
+        if (
+            values.ndim < 1
+            or values.shape[-1] != weight.in_features
+            or values.dtype not in (torch.bfloat16, torch.float16, torch.float32)
+            or values.device != weight.packed.device
+        ):
+            raise ValueError("NVFP4 input differs from its frozen matrix")
+        if torch.is_grad_enabled() and values.requires_grad:
+            raise ValueError("NVFP4 execution is inference-only")
+        _require_device(values.device)
+        self._check_bias(values, bias, weight.out_features)
+        matrix = values.to(torch.bfloat16) if values.dtype == torch.float32 else values
+        matrix = matrix.reshape(-1, weight.in_features)
+        if matrix.shape[0] == 0:
+            raise ValueError("NVFP4 input rows must be nonempty")
+        output = nvfp4_weight_only(matrix, weight.packed, weight.scales, weight.alpha, bias)
+        self.calls += 1
+        self.rows += matrix.shape[0]
+        return output.reshape(*values.shape[:-1], weight.out_features)
 
     # -- fused entry points (opt-in): the strict-BF16 step after the linear runs
     # in the GEMM's epilogue, as for RowFP8Execution
