@@ -1,0 +1,113 @@
+// Walks the attention kernel's work order on the CPU: every key tile of every
+// job is visited exactly once, pieces use distinct slots, and the join finds
+// exactly the pieces of each job that was cut.
+//
+// Reads cases from standard input, one a line:
+//   split blocks grid groups job_tokens causal has_offsets batch total_q total_k  cu_q...  cu_k...  lengths_or_-1...
+// and prints "ok <cases> <cut jobs>" or the first contradiction.
+#include <cstdio>
+#include <cstdlib>
+#include <map>
+#include <set>
+#include <tuple>
+#include <vector>
+
+#include "attention_plan.h"
+
+using namespace vfb::attn;
+
+static long long read_int() {
+  long long x;
+  if (std::scanf("%lld", &x) != 1) std::exit(3);
+  return x;
+}
+
+int main() {
+  long long cases = 0, cuts = 0, split;
+  while (std::scanf("%lld", &split) == 1) {
+    Plan p = {};
+    p.blocks = static_cast<int32_t>(read_int());
+    const long long grid = read_int();
+    p.groups = static_cast<int32_t>(read_int());
+    p.job_tokens = static_cast<int32_t>(read_int());
+    p.causal = static_cast<int32_t>(read_int());
+    const long long offsets = read_int();
+    p.batch = static_cast<int32_t>(read_int());
+    p.total_q = read_int();
+    p.total_k = read_int();
+    std::vector<int32_t> cu_q, cu_k, lengths;
+    for (int i = 0; i <= p.batch; ++i) cu_q.push_back(static_cast<int32_t>(read_int()));
+    for (int i = 0; i <= p.batch; ++i) cu_k.push_back(static_cast<int32_t>(read_int()));
+    for (int i = 0; i < p.batch; ++i) lengths.push_back(static_cast<int32_t>(read_int()));
+    if (offsets) {
+      p.cu_q = cu_q.data();
+      p.cu_k = cu_k.data();
+    }
+    if (lengths[0] >= 0) p.len_k = lengths.data();
+
+    using Job = std::tuple<int, int, int>;  // sequence, group, tile
+    std::map<Job, std::set<int>> done;
+    std::map<int, std::pair<Job, std::pair<int, int>>> pieces;  // slot -> job, key tiles
+    std::set<int> empty_slots;
+    const int n = static_cast<int>(split ? p.blocks : grid);
+    std::map<Job, bool> whole;
+    for (int block = 0; block < n; ++block) {
+      Order order;
+      bool share = true;
+      if (split) share = order.init_share(p, block);
+      else order.init_whole(p, block, static_cast<int32_t>(grid));
+      if (share && order.empty()) empty_slots.insert(2 * block);
+      Segment s;
+      while (order.next(p, s)) {
+        const Job job{s.b, s.group, s.tile};
+        if (s.seq.tiles <= s.tile || s.tile < 0 || s.group < 0 || s.group >= p.groups) return std::printf("bad job\n"), 1;
+        const int tiles = Order::tiles_of(p, s.seq, s.tile);
+        if (s.t0 < 0 || s.t1 > tiles || s.t1 < s.t0) return std::printf("bad tiles %d %d of %d\n", s.t0, s.t1, tiles), 1;
+        for (int t = s.t0; t < s.t1; ++t)
+          if (!done[job].insert(t).second) return std::printf("tile twice\n"), 1;
+        done[job];
+        if (s.slot < 0) {
+          if (s.t0 != 0 || s.t1 != tiles || whole.count(job)) return std::printf("whole job wrong\n"), 1;
+          whole[job] = true;
+        } else {
+          if (!split || s.slot >= 2 * p.blocks || !pieces.emplace(s.slot, std::make_pair(job, std::make_pair(s.t0, s.t1))).second)
+            return std::printf("slot %d\n", s.slot), 1;
+          if (whole.count(job)) return std::printf("piece of a whole job\n"), 1;
+        }
+      }
+    }
+    for (int b = 0; b < num_seqs(p); ++b) {
+      const Seq s = sequence(p, b);
+      for (int g = 0; g < p.groups; ++g)
+        for (int t = 0; t < s.tiles; ++t) {
+          const auto it = done.find(Job{b, g, t});
+          if (it == done.end() || static_cast<int>(it->second.size()) != Order::tiles_of(p, s, t))
+            return std::printf("job %d %d %d not done\n", b, g, t), 1;
+        }
+    }
+    std::map<Job, std::set<int>> by_job;
+    for (const auto &x : pieces) by_job[x.second.first].insert(x.first);
+    std::set<Job> joined;
+    for (int c = 1; split && c < p.blocks; ++c) {
+      Join j;
+      if (!join_at(p, c, j)) continue;
+      const Job job{j.job.b, j.job.group, j.job.tile};
+      if (!joined.insert(job).second) return std::printf("joined twice\n"), 1;
+      std::set<int> slots{j.first};
+      for (int i = j.c; i <= j.last; ++i) slots.insert(2 * i);
+      std::set<int> real;
+      for (int x : slots) {
+        const auto it = pieces.find(x);
+        if (it != pieces.end() && it->second.first == job) real.insert(x);
+        else if (!empty_slots.count(x)) return std::printf("join reads slot %d that nothing wrote\n", x), 1;
+      }
+      if (real != by_job[job]) return std::printf("join misses pieces\n"), 1;
+      ++cuts;
+    }
+    for (const auto &x : by_job)
+      if (!joined.count(x.first)) return std::printf("pieces never joined\n"), 1;
+    ++cases;
+  }
+  std::printf("ok %lld %lld\n", cases, cuts);
+  return 0;
+}

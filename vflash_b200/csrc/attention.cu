@@ -1,104 +1,859 @@
-// Attention over packed sequences (vfb_attention): one warp per query row and
-// head, scores of 32 keys at a time (one key per lane), running maximum and
-// sum in fp32, only the keys the row may see.
+// Attention over packed sequences (vfb_attention) on tcgen05.
+//
+// For one tile of 128 query rows (the group's heads of as many tokens as fit,
+// row = token * pack + head in group) and the keys it sees, 128 at a time:
+//   S = Q K^T            tcgen05, fp32 in TMEM
+//   m' = max(m, row max) P = exp2((S - m') * scale * log2 e)   registers
+//   l = l * 2^(m - m') + row sum of P
+//   O = O * 2^(m - m') + P V      tcgen05, P (16 bit) read from TMEM
+//   out = O / l,  lse = m * scale + ln l
+// S and O never leave the SM.  m only moves (and O is only multiplied) when the
+// maximum grows by more than kHold binary orders, so P may reach 2^kHold; the
+// result is the same to rounding and the pass over O in TMEM is rare.
+//
+// Roles of a block of twelve warps, one block on an SM:
+//   warps 0-3, 4-7  softmax of stage 0 and stage 1, one thread per row
+//   warp 8          TMA loads: Q tiles, then K and V tiles through one ring
+//   warp 9          MMA issue
+//   warps 10, 11    clean the V tiles that hold keys some row must not see
+// The two stages keep the tensor cores busy with one tile's products while the
+// other's exponentials run.  They are
+//   PAIR: two tiles of query rows against the same keys (many query rows), or
+//   ALT:  one tile of query rows against even and odd key tiles, joined at the
+//         end (few query rows: single tokens, short pieces).
+//
+// TMEM (512 columns): S0 | S1 | O0 | O1, 128 columns each; P overwrites the
+// first 64 columns of its S.  tcgen05 operations of one thread run in order,
+// so S(j+1) may be issued behind the P V(j) that still reads P.
+//
+// Keys behind a row's limit: their scores become -inf, so P = 0; but 0 * inf
+// and 0 * NaN would still spoil the second product.  Warps 10 and 11 therefore
+// zero, in the key tiles that any row of the block sees only in part, the V
+// rows behind the sequence's end and (causal) every element that is not
+// finite; the latter are added back at the end to the rows that do see them.
 #include "common.cuh"
+#include "attention_plan.h"
 
 namespace vfb {
 namespace {
 
-struct Params {
-  vfb_attention_args a;
-  float scale_log2;
+using attn::Plan;
+using attn::Segment;
+
+constexpr int kTile = 128;           // query rows in a tile, and keys in a key tile
+constexpr int kPanelBytes = 16384;   // 128 rows x 64 elements of 16 bits, 128-byte swizzle
+constexpr int kThreads = 384;
+constexpr int kRingSlots = 10;       // at most
+constexpr float kHold = 8.0f;
+constexpr float kLn2 = 0.693147180559945309f;
+
+// Rows of a workspace slot (one piece of a job): both tiles of PAIR.
+constexpr int kSlotRows = 2 * kTile;
+
+template <int DP, bool PAIR>
+struct Layout {
+  static constexpr int panels = DP / 64;
+  static constexpr int tile_bytes = panels * kPanelBytes;
+  static constexpr int q_bytes = (PAIR ? 2 : 1) * tile_bytes;
+  static constexpr int ring = DP == 128 ? (PAIR ? 5 : 6) : (PAIR ? 8 : 10);
+  static constexpr int smem = 1024 + q_bytes + ring * tile_bytes;  // tiles start on 1024 bytes
 };
 
-template <typename T>
-__device__ __forceinline__ float widen(T x);
-template <>
-__device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <>
-__device__ __forceinline__ float widen(__half x) { return __half2float(x); }
-__device__ __forceinline__ void narrow(float f, __nv_bfloat16 *p) { *p = __float2bfloat16_rn(f); }
-__device__ __forceinline__ void narrow(float f, __half *p) { *p = __float2half_rn(f); }
+struct Params {
+  Plan plan;
+  const void *v;
+  void *out;
+  float *lse;
+  int64_t v_token_stride, v_head_stride, out_token_stride, out_head_stride;
+  int32_t heads, pack, tokens;    // heads in a tile, tokens in a tile (pack * tokens <= 128)
+  int32_t group_heads;            // query heads of one key/value head
+  int32_t dim, fill_tail, split;
+  float scale_log2;
+  float *part_o, *part_lse;       // workspace: [slot][kSlotRows][dim], [slot][kSlotRows]
+  int *status;
+};
 
-// Offsets are clamped to the buffers, so no input makes the kernel leave them.
-__device__ __forceinline__ int64_t clamp64(int64_t x, int64_t lo, int64_t hi) {
-  return x < lo ? lo : (x > hi ? hi : x);
+struct Shared {
+  uint64_t q_full, q_empty;
+  uint64_t kv_full[kRingSlots], kv_empty[kRingSlots];
+  uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
+  // a V tile to be cleaned is on its way into the slot, and is clean: the MMA
+  // warp waits for the latter before the slot is given back, so neither barrier
+  // can run ahead of who waits for it
+  uint64_t v_todo[kRingSlots], v_clean[kRingSlots];
+  uint64_t stats_full, stats_empty, drain;
+  uint32_t tmem;
+  int abort;
+  int dirty;  // a non-finite element of V was taken out of a tile
+  float2 stats[kTile];  // ALT: (m, l) of stage 1's rows
+};
+static_assert(sizeof(Shared) + Layout<128, true>::smem <= 232448 && sizeof(Shared) + Layout<128, false>::smem <= 232448,
+              "shared memory of a block");
+
+// ---- small helpers -----------------------------------------------------------
+__device__ __forceinline__ void tma_load_3d(void *smem_dst, const CUtensorMap *map, uint64_t *bar, int32_t x,
+                                            int32_t y, int32_t z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+// D (+)= A B^T, 16-bit operands from shared memory.
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+// D (+)= A B^T with A (16 bit, two elements to a column) in TMEM.
+__device__ __forceinline__ void mma_f16_tmem_a(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc,
+                                               uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b_desc), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+// Descriptor of a V tile read with the head dimension as N: rows of 64
+// contiguous N elements (128 bytes, swizzled), eight K rows to 1024 bytes, the
+// next 64 N elements one panel further.
+__device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t smem_addr) {
+  uint64_t desc = 0;
+  desc |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+  desc |= static_cast<uint64_t>(kPanelBytes >> 4) << 16;  // leading offset: next 64 elements of N
+  desc |= static_cast<uint64_t>(1024 >> 4) << 32;         // stride offset: next eight rows of K
+  desc |= static_cast<uint64_t>(1) << 46;
+  desc |= static_cast<uint64_t>(2) << 61;
+  return desc;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(128) attention_rows_kernel(Params p) {
-  const vfb_attention_args &a = p.a;
-  const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (item >= a.total_q * a.heads) return;
-  const int64_t row = item / a.heads;
-  const int head = static_cast<int>(item - row * a.heads);
-  const int kv = head / (a.heads / a.kv_heads);
-  int64_t q0 = 0, q1 = a.total_q, k0 = 0, nk = a.total_k;
-  bool behind = false;
-  if (a.cu_seqlens_q != nullptr) {
-    int lo = 0, hi = a.batch;  // the last sequence that starts at or before the row
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (a.cu_seqlens_q[mid] <= row) lo = mid; else hi = mid;
-    }
-    while (lo + 1 < a.batch && a.cu_seqlens_q[lo + 1] <= row) ++lo;
-    q0 = clamp64(a.cu_seqlens_q[lo], 0, a.total_q);
-    q1 = clamp64(a.cu_seqlens_q[lo + 1], q0, a.total_q);
-    behind = row >= q1;
-    const int32_t *cu_k = a.cu_seqlens_k != nullptr ? a.cu_seqlens_k : a.cu_seqlens_q;
-    k0 = clamp64(cu_k[lo], 0, a.total_k);
-    nk = clamp64(cu_k[lo + 1], k0, a.total_k) - k0;
-    if (a.lengths_k != nullptr) nk = clamp64(a.lengths_k[lo], 0, nk);
-  } else if (a.lengths_k != nullptr) {
-    nk = clamp64(a.lengths_k[0], 0, nk);
-  }
-  int64_t limit = nk;
-  if (a.causal) limit = clamp64(row - q0 + 1 + nk - (q1 - q0), 0, nk);
-  if (behind) limit = 0;
+__device__ __forceinline__ constexpr uint32_t idesc_f16(int n, bool b_mn_major) {
+  const uint32_t fmt = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  return (1u << 4) | (fmt << 7) | (fmt << 10) | (b_mn_major ? 1u << 16 : 0u) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
+}
 
-  const T *q = static_cast<const T *>(a.q) + row * a.q_token_stride + head * a.q_head_stride;
-  const T *k = static_cast<const T *>(a.k) + k0 * a.k_token_stride + kv * a.k_head_stride;
-  const T *v = static_cast<const T *>(a.v) + k0 * a.v_token_stride + kv * a.v_head_stride;
-  float m = -INFINITY, l = 0.0f, acc[4] = {};
-  for (int64_t j0 = 0; j0 < limit; j0 += 32) {
-    const int64_t j = j0 + lane;
-    float s = -INFINITY;
-    if (j < limit) {
-      s = 0.0f;
-      for (int d = 0; d < a.dim; ++d) s = fmaf(widen(q[d]), widen(k[j * a.k_token_stride + d]), s);
+__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t *r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+      "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Maximum that keeps NaN.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  return pack_bf16x2(lo, hi);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t exponent_mask() {  // both halves of a word
+  return std::is_same<T, __nv_bfloat16>::value ? 0x7F807F80u : 0x7C007C00u;
+}
+
+// ---- what every role derives from a segment --------------------------------------
+template <bool PAIR>
+struct Work {
+  int64_t row0;       // first query row of the job in q
+  int32_t rows0;      // its index in the sequence
+  int32_t count;      // tokens of the job
+  int32_t n[2];       // key tiles of each stage
+  int32_t first_masked;  // key tiles from here on are seen in part by some row
+  int32_t min_seen;   // keys that the job's first row sees
+  __device__ __forceinline__ Work(const Params &p, const Segment &s) {
+    rows0 = s.tile * p.plan.job_tokens;
+    row0 = s.seq.q0 + rows0;
+    count = min(p.plan.job_tokens, s.seq.nq - rows0);
+    min_seen = attn::keys_seen(p.plan, s.seq, static_cast<int64_t>(rows0) + 1);
+    first_masked = min_seen / attn::KEYS;
+    const int32_t tiles = max(s.t1 - s.t0, 0);
+    if (PAIR) {
+      // stage 0's rows may see fewer keys than the job's last row
+      const int32_t seen0 =
+          attn::keys_seen(p.plan, s.seq, static_cast<int64_t>(rows0) + min(p.tokens, count));
+      const int32_t t1 = min(s.t1, (seen0 + attn::KEYS - 1) / attn::KEYS);
+      n[0] = max(t1 - s.t0, 0);
+      n[1] = count > p.tokens ? tiles : 0;
+    } else {
+      n[0] = (tiles + 1) / 2;
+      n[1] = tiles / 2;
     }
-    float top = s;
-    bool nan = s != s;
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-    if (__any_sync(~0u, nan)) top = NAN;
-    const float m_new = top != top || m != m ? NAN : fmaxf(m, top);
-    const float base = m_new == -INFINITY ? 0.0f : m_new;
-    const float e = j < limit ? exp2f((s - base) * p.scale_log2) : 0.0f;
-    const float alpha = m == -INFINITY ? 0.0f : exp2f((m - base) * p.scale_log2);
-    l = l * alpha + e;
-    for (int i = 0; i < 4; ++i) acc[i] *= alpha;
-    const int n = static_cast<int>(limit - j0 < 32 ? limit - j0 : 32);
-    for (int t = 0; t < n; ++t) {
-      const float w = __shfl_sync(~0u, e, t);
-      for (int i = 0; i < 4; ++i) {
-        const int d = lane + 32 * i;
-        if (d < a.dim) acc[i] = fmaf(w, widen(v[(j0 + t) * a.v_token_stride + d]), acc[i]);
+  }
+  __device__ __forceinline__ int32_t tiles() const { return PAIR ? max(n[0], n[1]) : n[0] + n[1]; }
+};
+
+// Running position in the ring of K and V tiles.
+template <int RING>
+struct RingPos {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void step() {
+    if (++slot == RING) {
+      slot = 0;
+      phase ^= 1;
+    }
+  }
+};
+
+// ---- softmax of one stage ----------------------------------------------------------
+// Row state, and the loop over a segment's key tiles.
+template <typename T, int DP, bool PAIR>
+struct Softmax {
+  const Params &p;
+  Shared &sh;
+  const uint32_t tmem_s, tmem_o;  // this warp's lanes
+  const int stage;
+  float m, l;          // running maximum (raw scores, as used) and sum
+  uint32_t s_phase = 0;
+
+  __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t phase) {
+    return warp_wait(bar, phase, &sh.abort, p.status);
+  }
+
+  // `limit`: keys this row sees.  `live`: some row of the warp is a row of the job.
+  __device__ __forceinline__ bool run(int32_t t0, int32_t n, int32_t stride, int32_t limit, bool live, int lane) {
+    m = -INFINITY;
+    l = 0.0f;
+    for (int32_t i = 0; i < n; ++i) {
+      if (!wait(&sh.s_full[stage], s_phase)) return false;
+      s_phase ^= 1;
+      tc_fence_after();
+      if (live) tile((t0 + i * stride) * attn::KEYS, limit, i > 0);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.p_full[stage]);
+    }
+    return true;
+  }
+
+  __device__ __forceinline__ void tile(int32_t key0, int32_t limit, bool scale_o) {
+    float s[128];
+    {
+      uint32_t(&r)[4][32] = reinterpret_cast<uint32_t(&)[4][32]>(s);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32_issue(tmem_s + 32 * c, r[c]);
+      tmem_ld_wait();
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld_fence(r[c]);
+    }
+    const int32_t seen = limit - key0;
+    if (__any_sync(0xffffffffu, seen < attn::KEYS)) {
+#pragma unroll
+      for (int j = 0; j < 128; ++j)
+        if (j >= seen) s[j] = -INFINITY;
+    }
+    float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+    for (int j = 4; j < 124; j += 8) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top[i] = max3_nan(top[i], s[j + 2 * i], s[j + 2 * i + 1]);
+    }
+    top[0] = max3_nan(top[0], s[124], s[125]);
+    top[1] = max3_nan(top[1], s[126], s[127]);
+    const float peak = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], m);
+    // true also for a NaN score; not while no key has been seen
+    const bool move = !((peak - m) * p.scale_log2 <= kHold) && peak != -INFINITY;
+    if (__any_sync(0xffffffffu, move)) {
+      const float alpha = !move ? 1.0f : m == -INFINITY ? 0.0f : ex2((m - peak) * p.scale_log2);
+      if (move) {
+        m = peak;
+        l *= alpha;
+      }
+      if (scale_o) {
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 32) {
+          uint32_t r[32];
+          tmem_ld_32x32b_x32_issue(tmem_o + c, r);
+          tmem_ld_wait();
+          tmem_ld_fence(r);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * alpha);
+          tmem_st_32x32b_x32(tmem_o + c, r);
+        }
       }
     }
-    m = m_new;
+    const float base = m == -INFINITY ? 0.0f : m * p.scale_log2;
+    float sum[4] = {};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t packed[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const float a = ex2(fmaf(s[64 * h + 2 * j], p.scale_log2, -base));
+        const float b = ex2(fmaf(s[64 * h + 2 * j + 1], p.scale_log2, -base));
+        sum[(2 * j) & 3] += a;
+        sum[(2 * j + 1) & 3] += b;
+        packed[j] = pack2<T>(a, b);
+      }
+      tmem_st_32x32b_x32(tmem_s + 32 * h, packed);
+    }
+    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    tmem_st_wait();
   }
-  for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
-  if (!behind || a.fill_tail) {
-    T *out = static_cast<T *>(a.out) + row * a.out_token_stride + head * a.out_head_stride;
-    for (int i = 0; i < 4; ++i) {
-      const int d = lane + 32 * i;
-      if (d < a.dim) narrow(limit > 0 ? acc[i] / l : 0.0f, out + d);
+};
+
+// ---- kernel ------------------------------------------------------------------------
+template <typename T, int DP, bool PAIR>
+__global__ void __launch_bounds__(kThreads, 1)
+    attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                     const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Params p) {
+  using L = Layout<DP, PAIR>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem =
+      reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t *s_q = smem;
+  uint8_t *s_kv = smem + L::q_bytes;
+  __shared__ Shared sh;
+
+  const int warp = threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
+  if (threadIdx.x == 0) {
+    mbar_init(&sh.q_full, 1);
+    mbar_init(&sh.q_empty, 1);
+    for (int i = 0; i < L::ring; ++i) {
+      mbar_init(&sh.kv_full[i], 1);
+      mbar_init(&sh.kv_empty[i], 1);
+      mbar_init(&sh.v_todo[i], 1);
+      mbar_init(&sh.v_clean[i], 2);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.s_full[i], 1);
+      mbar_init(&sh.p_full[i], 4);
+      mbar_init(&sh.o_full[i], 1);
+      mbar_init(&sh.o_empty[i], 4);
+    }
+    mbar_init(&sh.stats_full, 4);
+    mbar_init(&sh.stats_empty, 4);
+    mbar_init(&sh.drain, 1);
+    sh.abort = 0;
+    sh.dirty = 0;
+    fence_mbar_init();
+  }
+  if (warp == 8 && lane == 0) {
+    tma_prefetch_desc(&map_q);
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
+  }
+  if (warp == 9) {
+    tmem_alloc(&sh.tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  grid_dependency_wait();  // q, k, v and the offsets may come from the kernel before
+  grid_launch_dependents();
+
+  attn::Order order;
+  bool has_share = false;  // of evenly cut work, where the workspace is in use
+  if (p.split) has_share = order.init_share(p.plan, blockIdx.x);
+  else order.init_whole(p.plan, blockIdx.x, gridDim.x);
+  Segment seg;
+
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int stage = warp / 4;
+    const int row = (warp % 4) * 32 + lane;  // of the tile, and TMEM lane
+    const uint32_t lanes = tmem + (static_cast<uint32_t>((warp % 4) * 32) << 16);
+    Softmax<T, DP, PAIR> sm{p, sh, lanes + 128 * stage, lanes + 256 + 128 * stage, stage};
+    uint32_t o_phase[2] = {0, 0}, stats_phase = 0;
+    const int token_in_tile = row / p.pack;
+    const int head_in_tile = row - token_in_tile * p.pack;
+    if (has_share && order.empty() && stage == 0) {
+      // a share cut to nothing: its slot may be counted among a job's pieces
+      float *lse = p.part_lse + static_cast<int64_t>(2 * blockIdx.x) * kSlotRows;
+      lse[row] = -INFINITY;
+      lse[row + kTile] = -INFINITY;
+    }
+    while (order.next(p.plan, seg)) {
+      const Work<PAIR> w(p, seg);
+      const int token = token_in_tile + (PAIR ? stage * p.tokens : 0);  // of the job
+      const bool valid = token_in_tile < p.tokens && token < w.count;
+      const int32_t limit =
+          valid ? attn::keys_seen(p.plan, seg.seq, static_cast<int64_t>(w.rows0) + token + 1) : 0;
+      const bool live = __any_sync(0xffffffffu, valid);
+      if (!sm.run(PAIR ? seg.t0 : seg.t0 + stage, w.n[stage], PAIR ? 1 : 2, limit, live, lane)) break;
+      float m = sm.m, l = sm.l;
+      bool have[2] = {w.n[stage] > 0, false};  // accumulators that hold something for this row
+      float f[2] = {1.0f, 0.0f};
+      if (PAIR) {
+        if (have[0]) {
+          if (!warp_wait(&sh.o_full[stage], o_phase[stage], &sh.abort, p.status)) break;
+          o_phase[stage] ^= 1;
+        }
+      } else {
+        // stage 1 hands its statistics over; stage 0 joins the two accumulators
+        if (stage == 1) {
+          if (!warp_wait(&sh.stats_empty, stats_phase ^ 1, &sh.abort, p.status)) break;
+          sh.stats[row] = make_float2(m, l);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.stats_full);
+          stats_phase ^= 1;
+          continue;
+        }
+        if (!warp_wait(&sh.stats_full, stats_phase, &sh.abort, p.status)) break;
+        stats_phase ^= 1;
+        const float2 other = sh.stats[row];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.stats_empty);
+        bool ok = true;
+        for (int i = 0; i < 2; ++i) {
+          if (w.n[i] == 0) continue;
+          ok = ok && warp_wait(&sh.o_full[i], o_phase[i], &sh.abort, p.status);
+          o_phase[i] ^= 1;
+        }
+        if (!ok) break;
+        have[1] = w.n[1] > 0;
+        const float joint = max3_nan(m, other.x, m);
+        const float shift = joint == -INFINITY ? 0.0f : joint;
+        f[0] = m == -INFINITY ? 0.0f : ex2((m - shift) * p.scale_log2);
+        f[1] = other.x == -INFINITY ? 0.0f : ex2((other.x - shift) * p.scale_log2);
+        m = joint;
+        l = l * f[0] + other.y * f[1];
+      }
+      tc_fence_after();
+      // A row of infinite scores is NaN however its exponentials were rounded.
+      if (m == INFINITY) l = NAN;
+      const int64_t piece_end = attn::min64(limit, static_cast<int64_t>(seg.t1) * attn::KEYS);
+      const bool none = piece_end <= static_cast<int64_t>(seg.t0) * attn::KEYS;
+      const float inv = none ? 0.0f : 1.0f / l;
+      const int64_t out_row = w.row0 + token;
+      const int head = seg.group * p.pack + head_in_tile;
+      const bool behind = p.plan.cu_q != nullptr && seg.b == p.plan.batch;
+      T *out = static_cast<T *>(p.out) + out_row * p.out_token_stride + head * p.out_head_stride;
+      float *part = nullptr;
+      if (seg.slot >= 0) {
+        const int64_t at = static_cast<int64_t>(seg.slot) * kSlotRows + (PAIR ? stage * kTile : 0) + row;
+        part = p.part_o + at * p.dim;
+        if (valid) p.part_lse[at] = none ? -INFINITY : m * p.scale_log2 + log2f(l);
+      } else if (valid && p.lse != nullptr) {
+        p.lse[head * p.plan.total_q + out_row] = none ? -INFINITY : (m * p.scale_log2 + log2f(l)) * kLn2;
+      }
+      const bool dirty = *reinterpret_cast<volatile int *>(&sh.dirty) != 0;
+      if (live) {
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 32) {
+          if (c >= p.dim) break;
+          float o[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = 0.0f;
+          if (have[0]) {
+            uint32_t r[32];
+            tmem_ld_32x32b_x32_issue(lanes + 256 + (PAIR ? 128 * stage : 0) + c, r);
+            tmem_ld_wait();
+            tmem_ld_fence(r);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = f[0] == 0.0f ? 0.0f : __uint_as_float(r[j]) * f[0];
+          }
+          if (!PAIR && have[1]) {
+            uint32_t r[32];
+            tmem_ld_32x32b_x32_issue(lanes + 256 + 128 + c, r);
+            tmem_ld_wait();
+            tmem_ld_fence(r);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] += f[1] == 0.0f ? 0.0f : __uint_as_float(r[j]) * f[1];
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = none ? 0.0f : o[j] * inv;
+          if (valid && dirty && !none) {
+            // the elements that were taken out, for the rows that see them
+            const int kv_head = seg.group * p.pack / p.group_heads;
+            const int64_t from = static_cast<int64_t>(max(w.first_masked, seg.t0)) * attn::KEYS;
+            const T *v = static_cast<const T *>(p.v) + kv_head * p.v_head_stride + seg.seq.k0 * p.v_token_stride;
+            for (int64_t key = from; key < piece_end; ++key) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const float x = c + j < p.dim ? static_cast<float>(v[key * p.v_token_stride + c + j]) : 0.0f;
+                if (!(fabsf(x) < INFINITY)) o[j] += x;
+              }
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 32; j += 8) {
+            if (!valid || c + j >= p.dim) continue;
+            if (part != nullptr) {
+              float4 *dst = reinterpret_cast<float4 *>(part + c + j);
+              dst[0] = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+              dst[1] = make_float4(o[j + 4], o[j + 5], o[j + 6], o[j + 7]);
+            } else if (!behind || p.fill_tail) {
+              uint4 t;
+              t.x = pack2<T>(o[j], o[j + 1]);
+              t.y = pack2<T>(o[j + 2], o[j + 3]);
+              t.z = pack2<T>(o[j + 4], o[j + 5]);
+              t.w = pack2<T>(o[j + 6], o[j + 7]);
+              *reinterpret_cast<uint4 *>(out + c + j) = t;
+            }
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (have[0]) mbar_arrive(&sh.o_empty[PAIR ? stage : 0]);
+        if (!PAIR && have[1]) mbar_arrive(&sh.o_empty[1]);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (warp == 8) {
+      // ---------------- TMA producer ----------------
+      RingPos<L::ring> pos;
+      uint32_t q_phase = 0;
+      bool ok = true;
+      uint32_t issued = 0;  // slots that were ever loaded
+      const bool leader = elect_one();
+      const auto load = [&](const CUtensorMap *map, int32_t kv_head, int64_t key, bool masked) {
+        ok = ok && warp_wait(&sh.kv_empty[pos.slot], pos.phase ^ 1, &sh.abort, p.status);
+        if (ok && leader) {
+          mbar_arrive_expect_tx(&sh.kv_full[pos.slot], L::tile_bytes);
+          for (int i = 0; i < L::panels; ++i)
+            tma_load_3d(s_kv + pos.slot * L::tile_bytes + i * kPanelBytes, map, &sh.kv_full[pos.slot], 64 * i,
+                        kv_head, static_cast<int32_t>(key));
+          if (masked) mbar_arrive(&sh.v_todo[pos.slot]);
+        }
+        if (ok) issued |= 1u << pos.slot;
+        if (ok) pos.step();
+      };
+      bool q_loaded = false;
+      while (ok && order.next(p.plan, seg)) {
+        const Work<PAIR> w(p, seg);
+        const int32_t tiles = w.tiles();
+        if (tiles == 0) continue;
+        if (!warp_wait(&sh.q_empty, q_phase ^ 1, &sh.abort, p.status)) break;
+        const int used = PAIR && w.count > p.tokens ? 2 : 1;
+        if (leader) {
+          mbar_arrive_expect_tx(&sh.q_full, used * L::panels * p.pack * p.tokens * 128);
+          for (int t = 0; t < used; ++t)
+            for (int i = 0; i < L::panels; ++i)
+              tma_load_3d(s_q + t * L::tile_bytes + i * kPanelBytes, &map_q, &sh.q_full, 64 * i, seg.group * p.pack,
+                          static_cast<int32_t>(w.row0 + t * p.tokens));
+        }
+        q_loaded = true;
+        q_phase ^= 1;
+        const int32_t kv_head = seg.group * p.pack / p.group_heads;
+        const int64_t k0 = seg.seq.k0 + static_cast<int64_t>(seg.t0) * attn::KEYS;
+        if (PAIR) {
+          for (int32_t i = 0; i < tiles && ok; ++i) {
+            load(&map_k, kv_head, k0 + static_cast<int64_t>(i) * attn::KEYS, false);
+            load(&map_v, kv_head, k0 + static_cast<int64_t>(i) * attn::KEYS, seg.t0 + i >= w.first_masked);
+          }
+        } else {
+          load(&map_k, kv_head, k0, false);
+          if (tiles > 1) load(&map_k, kv_head, k0 + attn::KEYS, false);
+          for (int32_t i = 0; i < tiles && ok; ++i) {
+            load(&map_v, kv_head, k0 + static_cast<int64_t>(i) * attn::KEYS, seg.t0 + i >= w.first_masked);
+            if (i + 2 < tiles) load(&map_k, kv_head, k0 + static_cast<int64_t>(i + 2) * attn::KEYS, false);
+          }
+        }
+      }
+      // every load has landed before the block ends (a finished run waits for nothing here)
+      if (q_loaded) warp_wait(&sh.q_full, q_phase ^ 1, &sh.abort, p.status);
+      for (int i = 0; i < L::ring; ++i) {
+        const uint32_t last = i < pos.slot ? pos.phase : pos.phase ^ 1;
+        if (issued >> i & 1) warp_wait(&sh.kv_full[i], last, &sh.abort, p.status);
+      }
+    } else if (warp == 9) {
+      // ---------------- MMA issue ----------------
+      const bool leader = elect_one();
+      const uint32_t d16 = static_cast<uint32_t>((p.dim + 15) / 16);  // steps of K in Q K^T
+      const uint32_t idesc_s = idesc_f16<T>(attn::KEYS, false);
+      const uint32_t idesc_o = idesc_f16<T>(static_cast<int>(d16) * 16, true);
+      const uint32_t q_addr = smem_u32(s_q), kv_addr = smem_u32(s_kv);
+      RingPos<L::ring> pos;      // the item that is waited for next
+      uint32_t q_phase = 0, p_phase[2] = {0, 0}, o_phase[2] = {1, 1};
+      uint32_t v_phase = 0;  // a bit for every slot
+      bool ok = true;
+      const auto wait = [&](uint64_t *bar, uint32_t phase) {
+        ok = ok && warp_wait(bar, phase, &sh.abort, p.status);
+        return ok;
+      };
+      const auto commit = [&](uint64_t *bar) {
+        if (leader) tc_commit(bar);
+        __syncwarp();
+      };
+      const auto product_s = [&](int stage, int slot) {  // S = Q K^T
+        if (leader) {
+          const uint32_t a = q_addr + (PAIR ? stage * L::tile_bytes : 0);
+          const uint32_t b = kv_addr + slot * L::tile_bytes;
+          for (uint32_t k = 0; k < d16; ++k) {
+            const uint32_t at = (k / 4) * kPanelBytes + (k % 4) * 32;
+            mma_f16(tmem + 128 * stage, sw128_kmajor_desc(a + at), sw128_kmajor_desc(b + at), idesc_s, k > 0);
+          }
+        }
+        __syncwarp();
+      };
+      const auto product_o = [&](int stage, int slot, bool accumulate) {  // O (+)= P V
+        if (leader) {
+          const uint32_t b = kv_addr + slot * L::tile_bytes;
+#pragma unroll
+          for (uint32_t k = 0; k < attn::KEYS / 16; ++k)
+            mma_f16_tmem_a(tmem + 256 + 128 * stage, tmem + 128 * stage + 8 * k, sw128_mnmajor_desc(b + k * 2048),
+                           idesc_o, accumulate || k > 0);
+        }
+        __syncwarp();
+      };
+      while (ok && order.next(p.plan, seg)) {
+        const Work<PAIR> w(p, seg);
+        const int32_t tiles = w.tiles();
+        if (tiles == 0) continue;
+        if (!wait(&sh.q_full, q_phase)) break;
+        q_phase ^= 1;
+        if (PAIR) {
+          for (int32_t j = 0; j <= tiles && ok; ++j) {
+            const int v_slot = pos.slot;
+            if (j > 0) {
+              if (!wait(&sh.kv_full[pos.slot], pos.phase)) break;
+              pos.step();
+              if (seg.t0 + j - 1 >= w.first_masked) {
+                if (!wait(&sh.v_clean[v_slot], v_phase >> v_slot & 1)) break;
+                v_phase ^= 1u << v_slot;
+              }
+            }
+            const int k_slot = pos.slot;
+            if (j < tiles) {
+              if (!wait(&sh.kv_full[pos.slot], pos.phase)) break;
+              pos.step();
+            }
+            for (int s = 0; s < 2 && ok; ++s) {
+              if (j > 0 && j <= w.n[s]) {
+                if (!wait(&sh.p_full[s], p_phase[s])) break;
+                p_phase[s] ^= 1;
+                if (j == 1) {
+                  if (!wait(&sh.o_empty[s], o_phase[s])) break;
+                  o_phase[s] ^= 1;
+                }
+                tc_fence_after();
+                product_o(s, v_slot, j > 1);
+                if (j == w.n[s]) commit(&sh.o_full[s]);
+              }
+              if (j < w.n[s]) {
+                product_s(s, k_slot);
+                commit(&sh.s_full[s]);
+              }
+            }
+            if (!ok) break;
+            if (j > 0) commit(&sh.kv_empty[v_slot]);
+            if (j < tiles) commit(&sh.kv_empty[k_slot]);
+            if (j == tiles - 1) commit(&sh.q_empty);
+          }
+        } else {
+          const auto scores = [&](int32_t i) {
+            if (!wait(&sh.kv_full[pos.slot], pos.phase)) return;
+            product_s(i & 1, pos.slot);
+            commit(&sh.s_full[i & 1]);
+            commit(&sh.kv_empty[pos.slot]);
+            pos.step();
+            if (i == tiles - 1) commit(&sh.q_empty);
+          };
+          scores(0);
+          if (ok && tiles > 1) scores(1);
+          for (int32_t i = 0; i < tiles && ok; ++i) {
+            const int s = i & 1;
+            if (!wait(&sh.kv_full[pos.slot], pos.phase)) break;
+            if (seg.t0 + i >= w.first_masked) {
+              if (!wait(&sh.v_clean[pos.slot], v_phase >> pos.slot & 1)) break;
+              v_phase ^= 1u << pos.slot;
+            }
+            if (!wait(&sh.p_full[s], p_phase[s])) break;
+            p_phase[s] ^= 1;
+            if (i < 2) {
+              if (!wait(&sh.o_empty[s], o_phase[s])) break;
+              o_phase[s] ^= 1;
+            }
+            tc_fence_after();
+            product_o(s, pos.slot, i > 1);
+            commit(&sh.kv_empty[pos.slot]);
+            pos.step();
+            if (i + 2 >= tiles) commit(&sh.o_full[s]);
+            if (i + 2 < tiles) scores(i + 2);
+          }
+        }
+      }
+      // the products issued last are over before the block ends
+      commit(&sh.drain);
+      warp_wait(&sh.drain, 0, &sh.abort, p.status);
+    } else {
+      // ---------------- cleaning of V tiles ----------------
+      RingPos<L::ring> pos;
+      const int me = (warp - 10) * 32 + lane;
+      uint32_t todo_phase = 0;  // a bit for every slot
+      const auto clean = [&](const Work<PAIR> &w, int32_t t) {
+        const int slot = pos.slot;
+        if (!warp_wait(&sh.v_todo[slot], todo_phase >> slot & 1, &sh.abort, p.status)) return false;
+        todo_phase ^= 1u << slot;
+        if (!warp_wait(&sh.kv_full[slot], pos.phase, &sh.abort, p.status)) return false;
+        uint8_t *tile = s_kv + slot * L::tile_bytes;
+        const int32_t end = min(max(seg.seq.nk - t * attn::KEYS, 0), attn::KEYS);       // rows of the sequence
+        const int32_t all = min(max(w.min_seen - t * attn::KEYS, 0), attn::KEYS);       // rows that every row sees
+        for (int i = me; i < (attn::KEYS - all) * 8 * L::panels; i += 64) {
+          const int panel = i / ((attn::KEYS - all) * 8);
+          const int rest = i - panel * (attn::KEYS - all) * 8;
+          uint4 *at = reinterpret_cast<uint4 *>(tile + panel * kPanelBytes + all * 128) + rest;
+          if (all + rest / 8 >= end) {
+            *at = make_uint4(0, 0, 0, 0);
+            continue;
+          }
+          uint4 x = *at;
+          uint32_t *word = reinterpret_cast<uint32_t *>(&x);
+          uint32_t bad = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t hit = __vcmpeq2(word[j] & exponent_mask<T>(), exponent_mask<T>());
+            word[j] &= ~hit;
+            bad |= hit;
+          }
+          if (bad) {
+            *at = x;
+            *reinterpret_cast<volatile int *>(&sh.dirty) = 1;
+          }
+        }
+        fence_proxy_async_smem();
+        __threadfence_block();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.v_clean[slot]);
+        return true;
+      };
+      bool ok = true;
+      while (ok && order.next(p.plan, seg)) {
+        const Work<PAIR> w(p, seg);
+        const int32_t tiles = w.tiles();
+        if (tiles == 0) continue;
+        if (!PAIR) {
+          pos.step();
+          if (tiles > 1) pos.step();
+        }
+        for (int32_t i = 0; i < tiles && ok; ++i) {
+          if (PAIR) pos.step();
+          if (seg.t0 + i >= w.first_masked) ok = clean(w, seg.t0 + i);
+          pos.step();
+          if (!PAIR && i + 2 < tiles) pos.step();
+        }
+      }
     }
   }
-  if (a.lse != nullptr && lane == 0)
-    a.lse[head * a.total_q + row] =
-        limit > 0 ? (m * p.scale_log2 + log2f(l)) * 0.693147180559945309f : -INFINITY;
+  __syncwarp();
+  __syncthreads();
+  if (warp == 9) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---- joining the pieces of jobs that were cut ------------------------------------------
+constexpr int kJoinRows = 8;  // rows of one block, a warp each
+
+template <typename T>
+__global__ void __launch_bounds__(32 * kJoinRows) attention_join_kernel(const __grid_constant__ Params p) {
+  grid_dependency_wait();
+  attn::Join j;
+  if (!attn::join_at(p.plan, static_cast<int32_t>(blockIdx.x) + 1, j)) return;
+  const int lane = threadIdx.x & 31;
+  const int at = blockIdx.y * kJoinRows + (threadIdx.x >> 5);  // row of the slot
+  const int in_tile = at % kTile;
+  const int token = in_tile / p.pack + at / kTile * p.tokens;
+  const int64_t row0 = static_cast<int64_t>(j.job.tile) * p.plan.job_tokens;
+  if (in_tile / p.pack >= p.tokens || token >= min(static_cast<int64_t>(p.plan.job_tokens), j.job.seq.nq - row0))
+    return;
+  const int pieces = j.last - j.c + 2;
+  const auto slot_row = [&](int i) {
+    return static_cast<int64_t>(i == 0 ? j.first : 2 * (j.c + i - 1)) * kSlotRows + at;
+  };
+  float top = -INFINITY;
+  for (int i = lane; i < pieces; i += 32) top = max3_nan(top, p.part_lse[slot_row(i)], top);
+  for (int o = 16; o; o >>= 1) top = max3_nan(top, __shfl_xor_sync(0xffffffffu, top, o), top);
+  const float base = top == -INFINITY ? 0.0f : top;
+  float sum = 0.0f, acc[4] = {};
+  for (int i = 0; i < pieces; ++i) {
+    const float lse = p.part_lse[slot_row(i)];
+    if (lse == -INFINITY) continue;
+    const float weight = ex2(lse - base);
+    sum += weight;
+    if (lane * 4 < p.dim) {
+      const float4 o = *reinterpret_cast<const float4 *>(p.part_o + slot_row(i) * p.dim + 4 * lane);
+      acc[0] = fmaf(weight, o.x, acc[0]);
+      acc[1] = fmaf(weight, o.y, acc[1]);
+      acc[2] = fmaf(weight, o.z, acc[2]);
+      acc[3] = fmaf(weight, o.w, acc[3]);
+    }
+  }
+  const float inv = top == -INFINITY ? 0.0f : 1.0f / sum;
+  const int head = j.job.group * p.pack + in_tile % p.pack;
+  const int64_t row = j.job.seq.q0 + row0 + token;
+  if (lane * 4 < p.dim) {
+    uint2 t;
+    t.x = pack2<T>(acc[0] * inv, acc[1] * inv);
+    t.y = pack2<T>(acc[2] * inv, acc[3] * inv);
+    *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + row * p.out_token_stride + head * p.out_head_stride +
+                               4 * lane) = t;
+  }
+  if (lane == 0 && p.lse != nullptr)
+    p.lse[head * p.plan.total_q + row] = top == -INFINITY ? -INFINITY : (top + log2f(sum)) * kLn2;
+}
+
+// ---- host side -------------------------------------------------------------------------
+constexpr int kMaxBlocks = 148;  // SMs of a B200: blocks that even shares are cut for
+
+struct Choice {
+  int pack, tokens, groups;
+  bool pair, split;
+  int64_t jobs;  // whole jobs, at most
+};
+
+Choice choose(const vfb_attention_args &a) {
+  Choice c;
+  const int group = a.heads / a.kv_heads;
+  c.pack = group;
+  if (group > kTile)
+    for (c.pack = kTile; group % c.pack; --c.pack) {
+    }
+  c.tokens = kTile / c.pack;
+  c.groups = a.heads / c.pack;
+  // Two tiles of rows share every key tile where a sequence has more than one on average.
+  c.pair = a.total_q > static_cast<int64_t>(c.tokens) * a.batch;
+  const int64_t tokens = static_cast<int64_t>(c.tokens) * (c.pair ? 2 : 1);
+  const int64_t tiles = a.cu_seqlens_q == nullptr
+                            ? (a.total_q + tokens - 1) / tokens
+                            : attn::min64(a.total_q, a.total_q / tokens + a.batch + 1);
+  c.jobs = tiles * c.groups;
+  // Whole jobs balance by themselves when there are many; few keys are not worth cutting.
+  c.split = c.jobs < 4 * kMaxBlocks && a.total_k > 2 * attn::KEYS;
+  return c;
 }
 
 int check_args(const vfb_attention_args *a) {
@@ -121,15 +876,67 @@ int check_args(const vfb_attention_args *a) {
   for (int64_t s : strides)
     if (s < a->dim || s % 8 || s >= (1ll << 38))
       return set_error(VFB_EINVAL, "vfb_attention: strides must be multiples of 8, at least dim");
+  if (choose(*a).jobs >= (1ll << 31)) return set_error(VFB_EINVAL, "vfb_attention: too many rows");
   return VFB_OK;
 }
+
+// [rows, heads, dim] as (dim, heads, rows), boxes of 64 x box_heads x box_rows.
+int make_map(CUtensorMap *map, const void *base, int dtype, int64_t dim, int64_t heads, int64_t rows,
+             int64_t head_stride, int64_t token_stride, int box_heads, int box_rows) {
+  auto encode = tensor_map_encoder();
+  if (encode == nullptr) return set_error(VFB_ECUDA, "cuTensorMapEncodeTiled is unavailable");
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(head_stride) * 2, static_cast<cuuint64_t>(token_stride) * 2};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_rows)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = encode(map, dtype == 0 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                      const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return set_error(VFB_ECUDA, "vfb_attention: cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+  return VFB_OK;
+}
+
+template <typename T, int DP, bool PAIR>
+int launch(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, const Params &p, int64_t jobs, int sms,
+           cudaStream_t stream) {
+  using L = Layout<DP, PAIR>;
+  auto kernel = attention_kernel<T, DP, PAIR>;
+  static std::atomic<uint64_t> smem_set[kMaxAttrDevices];
+  int rc = ensure_smem_optin(reinterpret_cast<const void *>(kernel), L::smem, smem_set);
+  if (rc != VFB_OK) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.split ? p.plan.blocks : jobs), 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = L::smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, q, k, v, p);
+  if (err == cudaSuccess && p.split && p.plan.blocks > 1) {
+    cfg.gridDim = dim3(p.plan.blocks - 1, (PAIR ? 2 : 1) * kTile / kJoinRows, 1);
+    cfg.blockDim = dim3(32 * kJoinRows, 1, 1);
+    cfg.dynamicSmemBytes = 0;
+    err = cudaLaunchKernelEx(&cfg, attention_join_kernel<T>, p);
+  }
+  if (err != cudaSuccess) return set_error(VFB_ECUDA, "vfb_attention launch: %s", cudaGetErrorString(err));
+  return VFB_OK;
+}
+
+int64_t slots_of(const Choice &c) { return c.split ? 2 * kMaxBlocks : 0; }
 
 }  // namespace
 }  // namespace vfb
 
 extern "C" int64_t vfb_attention_workspace_bytes(const vfb_attention_args *args) {
-  if (vfb::check_args(args) != VFB_OK) return -1;
-  return 0;
+  using namespace vfb;
+  if (check_args(args) != VFB_OK) return -1;
+  if (args->total_q == 0) return 0;
+  return slots_of(choose(*args)) * kSlotRows * (args->dim + 1) * static_cast<int64_t>(sizeof(float));
 }
 
 extern "C" int vfb_attention(const vfb_attention_args *args, void *stream) {
@@ -142,15 +949,66 @@ extern "C" int vfb_attention(const vfb_attention_args *args, void *stream) {
     return set_error(VFB_EINVAL, "vfb_attention: NULL pointer");
   if (!aligned16(a.q) || !aligned16(a.k) || !aligned16(a.v) || !aligned16(a.out))
     return set_error(VFB_EINVAL, "vfb_attention: q, k, v and out must be 16-byte aligned");
-  rc = check_device(nullptr);
+  const Choice c = choose(a);
+  const int64_t need = vfb_attention_workspace_bytes(args);
+  if (a.workspace_bytes < need || (need > 0 && (!a.workspace || reinterpret_cast<uintptr_t>(a.workspace) % 256)))
+    return set_error(VFB_EINVAL, "vfb_attention: needs %lld bytes of 256-byte aligned workspace", (long long)need);
+  int sms = 0;
+  rc = check_device(&sms);
   if (rc != VFB_OK) return rc;
-  Params p{a, a.scale * 1.44269504088896341f};
-  const int64_t blocks = (a.total_q * a.heads + 3) / 4;
-  if (blocks > 0x7fffffff) return set_error(VFB_EINVAL, "vfb_attention: too many rows");
+
+  Params p = {};
+  p.plan.cu_q = a.cu_seqlens_q;
+  p.plan.cu_k = a.cu_seqlens_k;
+  p.plan.len_k = a.lengths_k;
+  p.plan.total_q = a.total_q;
+  p.plan.total_k = a.total_k;
+  p.plan.batch = a.batch;
+  p.plan.groups = c.groups;
+  p.plan.job_tokens = c.tokens * (c.pair ? 2 : 1);
+  p.plan.causal = a.causal != 0;
+  p.plan.blocks = sms < kMaxBlocks ? sms : kMaxBlocks;
+  p.v = a.v;
+  p.out = a.out;
+  p.lse = a.lse;
+  p.v_token_stride = a.v_token_stride;
+  p.v_head_stride = a.v_head_stride;
+  p.out_token_stride = a.out_token_stride;
+  p.out_head_stride = a.out_head_stride;
+  p.heads = a.heads;
+  p.pack = c.pack;
+  p.tokens = c.tokens;
+  p.group_heads = a.heads / a.kv_heads;
+  p.dim = a.dim;
+  p.fill_tail = a.fill_tail;
+  p.split = c.split;
+  p.scale_log2 = a.scale * 1.44269504088896341f;
+  if (c.split) {
+    p.part_o = static_cast<float *>(a.workspace);
+    p.part_lse = p.part_o + slots_of(c) * kSlotRows * a.dim;
+  }
+  p.status = device_status_ptr();
+
+  CUtensorMap mq, mk, mv;
+  rc = make_map(&mq, a.q, a.dtype, a.dim, a.heads, a.total_q, a.q_head_stride, a.q_token_stride, c.pack, c.tokens);
+  // without keys nothing is loaded, but a map must stand for something
+  const bool keys = a.total_k > 0;
+  if (rc == VFB_OK)
+    rc = make_map(&mk, keys ? a.k : a.q, a.dtype, a.dim, a.kv_heads, keys ? a.total_k : 1, a.k_head_stride,
+                  a.k_token_stride, 1, attn::KEYS);
+  if (rc == VFB_OK)
+    rc = make_map(&mv, keys ? a.v : a.q, a.dtype, a.dim, a.kv_heads, keys ? a.total_k : 1, a.v_head_stride,
+                  a.v_token_stride, 1, attn::KEYS);
+  if (rc != VFB_OK) return rc;
+
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (a.dtype == 0) attention_rows_kernel<__nv_bfloat16><<<(unsigned)blocks, 128, 0, s>>>(p);
-  else attention_rows_kernel<__half><<<(unsigned)blocks, 128, 0, s>>>(p);
-  cudaError_t err = cudaGetLastError();
-  if (err != cudaSuccess) return set_error(VFB_ECUDA, "vfb_attention launch: %s", cudaGetErrorString(err));
-  return VFB_OK;
+  const auto go = [&](auto type) {
+    using T = decltype(type);
+    if (a.dim > 64)
+      return c.pair ? launch<T, 128, true>(mq, mk, mv, p, c.jobs, sms, s)
+                    : launch<T, 128, false>(mq, mk, mv, p, c.jobs, sms, s);
+    return c.pair ? launch<T, 64, true>(mq, mk, mv, p, c.jobs, sms, s)
+                  : launch<T, 64, false>(mq, mk, mv, p, c.jobs, sms, s);
+  };
+  return a.dtype == 0 ? go(__nv_bfloat16()) : go(__half());
 }
