@@ -386,18 +386,16 @@ VFB_API int vfb_nvfp4_gemm_quant(const void *A, const void *sfa, const void *W, 
  * bf16 (dtype 0) or fp16 (dtype 1) [M,K], row stride ldx >= K, any alignment
  * of its element type.  w_codes / w_sf: the packed weight [N,K/2] and its 128x4 scales as in
  * vfb_nvfp4_gemm.  alpha: fp32 device scalar.  bias: bf16 [N] or NULL.  out:
- * bf16 [M,N], row stride ldo >= N.  Requires K % 64 == 0, N % 128 == 0,
- * 16-byte aligned w_codes, 4-byte aligned w_sf, and a `workspace` of
- * vfb_nvfp4_weight_only_workspace_bytes(M, N, K) bytes (0: may be NULL),
- * 256-byte aligned, that no other call in flight uses.  Every row of x is
- * brought to fp16 by a power of two of its own (exact for elements within
- * 2^-30 of the row's largest magnitude).  No reference counterpart: the
- * reference always quantises the activations. */
-VFB_API int64_t vfb_nvfp4_weight_only_workspace_bytes(int64_t M, int64_t N, int64_t K);
+ * bf16 [M,N], row stride ldo >= N.  Requires K % 64 == 0, K <= 32768,
+ * N % 128 == 0, N <= 1048576, M <= 524288, 16-byte aligned w_codes, 4-byte
+ * aligned w_sf.
+ * bf16 rows are brought to fp16 by a power of two of their own (exact for
+ * elements within 2^-30 of the row's largest magnitude).  No reference
+ * counterpart: the reference always quantises the activations. */
 VFB_API int vfb_nvfp4_weight_only(const void *x, int32_t dtype, int64_t M, int64_t ldx,
                                   const void *w_codes, const void *w_sf, const float *alpha,
                                   const void *bias, int64_t N, int64_t K, void *out, int64_t ldo,
-                                  void *workspace, int64_t workspace_bytes, void *stream);
+                                  void *stream);
 
 /* ---- attention over packed sequences ---------------------------------------
  * What stands between the QKV projection's planes and the attention output

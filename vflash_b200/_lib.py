@@ -150,11 +150,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [_vp, _vp, _vp, _vp, _vp, _vp, _c_int64, _c_int64, _c_int64, ctypes.POINTER(Epilogue), _vp, _vp, _vp,
          _vp],
     ),
-    "vfb_nvfp4_weight_only_workspace_bytes": (_c_int64, [_c_int64, _c_int64, _c_int64]),
     "vfb_nvfp4_weight_only": (
         ctypes.c_int,
-        [_vp, ctypes.c_int32, _c_int64, _c_int64, _vp, _vp, _vp, _vp, _c_int64, _c_int64, _vp, _c_int64, _vp,
-         _c_int64, _vp],
+        [_vp, ctypes.c_int32, _c_int64, _c_int64, _vp, _vp, _vp, _vp, _c_int64, _c_int64, _vp, _c_int64, _vp],
     ),
     "vfb_attention_workspace_bytes": (_c_int64, [ctypes.POINTER(AttentionArgs)]),
     "vfb_attention": (ctypes.c_int, [ctypes.POINTER(AttentionArgs), _vp]),

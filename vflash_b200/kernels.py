@@ -578,8 +578,8 @@ def nvfp4_weight_only(matrix: torch.Tensor, w_packed: torch.Tensor, w_scales: to
     ``matrix`` bf16 or fp16 ``[M, K]`` (unit column stride, any row stride),
     ``w_packed`` uint8 ``[N, K/2]`` and ``w_scales`` uint8 (128x4 layout) as
     ``nvfp4_gemm`` takes them, ``alpha`` an fp32 scalar tensor, ``bias`` bf16
-    ``[N]``.  K % 64 == 0, N % 128 == 0.  Made for few rows (one token, a small
-    batch); any M works, re-reading the weight for every block of rows.
+    ``[N]``.  K % 64 == 0, K <= 32768, N % 128 == 0.  Made for few rows (one token,
+    a small batch); more rows work too, re-reading the weight for every 32.
     """
     if matrix.dtype not in (BF16, torch.float16) or matrix.ndim != 2 or matrix.stride(1) != 1 and matrix.shape[1] > 1:
         raise KernelInputError("the weight-only NVFP4 product needs a bf16/fp16 [M, K] matrix with unit column stride")
@@ -589,8 +589,9 @@ def nvfp4_weight_only(matrix: torch.Tensor, w_packed: torch.Tensor, w_scales: to
             or not w_packed.is_contiguous()):
         raise KernelInputError("NVFP4 weight codes must be contiguous uint8 [N, K/2]")
     n = w_packed.shape[0]
-    if n == 0 or k == 0 or k % 64 or n % 128:
-        raise KernelInputError("the weight-only NVFP4 product needs K % 64 == 0, N % 128 == 0")
+    if n == 0 or k == 0 or k % 64 or k > 32768 or n % 128 or n > 1048576 or rows > 524288:
+        raise KernelInputError("the weight-only NVFP4 product needs K % 64 == 0, K <= 32768, N % 128 == 0, "
+                               "N <= 1048576, M <= 524288")
     if w_scales.dtype != torch.uint8 or w_scales.numel() != n * (k // 16) or not w_scales.is_contiguous():
         raise KernelInputError("NVFP4 weight scales differ from the 128x4 layout")
     if alpha.dtype != torch.float32 or alpha.numel() != 1:
@@ -610,12 +611,10 @@ def nvfp4_weight_only(matrix: torch.Tensor, w_packed: torch.Tensor, w_scales: to
         return out
     lib = _lib.load()
     with torch.cuda.device(device):
-        need = lib.vfb_nvfp4_weight_only_workspace_bytes(rows, n, k)
-        keep, workspace = _workspace(need, device)
         rc = lib.vfb_nvfp4_weight_only(
             matrix.data_ptr(), 0 if matrix.dtype == BF16 else 1, rows, max(matrix.stride(0), k),
             w_packed.data_ptr(), w_scales.data_ptr(), alpha.data_ptr(), _lib.ptr(bias), n, k, out.data_ptr(),
-            max(out.stride(0), n), workspace, need, _lib.stream_handle(device))
+            max(out.stride(0), n), _lib.stream_handle(device))
     _lib.check(rc, "vfb_nvfp4_weight_only")
     return out
 
