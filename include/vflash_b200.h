@@ -386,7 +386,7 @@ VFB_API int vfb_nvfp4_gemm_quant(const void *A, const void *sfa, const void *W, 
  * bf16 (dtype 0) or fp16 (dtype 1) [M,K], row stride ldx >= K, any alignment
  * of its element type.  w_codes / w_sf: the packed weight [N,K/2] and its 128x4 scales as in
  * vfb_nvfp4_gemm.  alpha: fp32 device scalar.  bias: bf16 [N] or NULL.  out:
- * bf16 [M,N], row stride ldo >= N.  Requires K % 64 == 0, K <= 32768,
+ * bf16 [M,N], row stride ldo >= N, no overlap with x.  Requires K % 64 == 0, K <= 32768,
  * N % 128 == 0, N <= 1048576, M <= 524288, 16-byte aligned w_codes, 4-byte
  * aligned w_sf.
  * bf16 rows are brought to fp16 by a power of two of their own (exact for

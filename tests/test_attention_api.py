@@ -37,8 +37,8 @@ def cu(*at, dtype=torch.int32):
     (lambda q, k, v: (torch.zeros(6, 4, 136, dtype=BF16), torch.zeros(6, 2, 136, dtype=BF16),
                       torch.zeros(6, 2, 136, dtype=BF16)), "head dimension"),
     (lambda q, k, v: (q.transpose(1, 2).contiguous().transpose(1, 2), k, v), "unit stride"),
-    (lambda q, k, v: (q, k[:, :1].expand(6, 2, 64), v), "not expanded"),
-    (lambda q, k, v: (q, k, torch.zeros(6, 2 * 64 + 4, dtype=BF16)[:, :128].unflatten(1, (2, 64))), "16-byte"),
+    (lambda q, k, v: (q, k[:, :1].expand(6, 2, 64), v), "strides must be multiples of 8"),
+    (lambda q, k, v: (q, k, torch.zeros(6, 2 * 64 + 4, dtype=BF16)[:, :128].unflatten(1, (2, 64))), "strides must be multiples of 8"),
     (lambda q, k, v: (torch.zeros(6 * 4 * 64 + 1, dtype=BF16)[1:].view(6, 4, 64), k, v), "16-byte"),
     (lambda q, k, v: (q.requires_grad_(), k, v), "inference-only"),
 ])

@@ -146,6 +146,14 @@ def test_strides_and_alignment(dtype):
     assert (out[:, 8 + 384:] == 7.0).all()
 
 
+def test_expanded_rows():
+    weight = weight_of(128, 192, 2)
+    x = activations(1, 192, 3, BF16)
+    got = nvfp4_weight_only(x.expand(5, 192), weight.packed, weight.scales, weight.alpha)
+    want = nvfp4_weight_only(x, weight.packed, weight.scales, weight.alpha)
+    assert torch.equal(got, want.expand(5, 128))
+
+
 def test_execution_keeps_leading_dimensions_and_rounds_fp32_first():
     weight = weight_of(128, 192, 2)
     x = activations(6, 192, 3, torch.float32).reshape(2, 3, 192)

@@ -71,11 +71,14 @@ def test_execution_checks(monkeypatch):
     monkeypatch.setattr(nv, "_require_device", lambda _: None)
     with pytest.raises(ValueError, match="bias"):
         engine.weight_only_linear(torch.zeros(1, 64, dtype=BF16), weight, torch.zeros(128))
+    with pytest.raises(ValueError, match="contiguous"):
+        engine.weight_only_linear(torch.zeros(1, 64, dtype=BF16), weight, torch.zeros(256, dtype=BF16)[::2])
     with pytest.raises(ValueError, match="nonempty"):
         engine.weight_only_linear(torch.zeros(0, 64, dtype=BF16), weight)
     assert engine.calls == 0
 
-    def product(matrix, packed, scales, alpha, bias):
+    def product(matrix, packed, scales, alpha, bias, *, checked):
+        assert checked
         assert matrix.dtype == BF16 and matrix.shape == (6, 64) and alpha is weight.alpha
         return torch.ones(6, 128, dtype=BF16)
 

@@ -876,6 +876,8 @@ int check_args(const vfb_attention_args *a) {
   for (int64_t s : strides)
     if (s < a->dim || s % 8 || s >= (1ll << 38))
       return set_error(VFB_EINVAL, "vfb_attention: strides must be multiples of 8, at least dim");
+  if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out))
+    return set_error(VFB_EINVAL, "vfb_attention: q, k, v and out must be 16-byte aligned");
   if (choose(*a).jobs >= (1ll << 31)) return set_error(VFB_EINVAL, "vfb_attention: too many rows");
   return VFB_OK;
 }
@@ -947,8 +949,6 @@ extern "C" int vfb_attention(const vfb_attention_args *args, void *stream) {
   if (a.total_q == 0) return VFB_OK;
   if (!a.q || !a.out || (a.total_k > 0 && (!a.k || !a.v)))
     return set_error(VFB_EINVAL, "vfb_attention: NULL pointer");
-  if (!aligned16(a.q) || !aligned16(a.k) || !aligned16(a.v) || !aligned16(a.out))
-    return set_error(VFB_EINVAL, "vfb_attention: q, k, v and out must be 16-byte aligned");
   const Choice c = choose(a);
   const int64_t need = vfb_attention_workspace_bytes(args);
   if (a.workspace_bytes < need || (need > 0 && (!a.workspace || reinterpret_cast<uintptr_t>(a.workspace) % 256)))

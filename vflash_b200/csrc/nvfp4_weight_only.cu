@@ -46,15 +46,28 @@ struct Args {
   int64_t ldx, ldo;
   int32_t M, N, K;
   int32_t steps;      // steps of a block's K range
+  uint32_t chunk_inverse;  // 2^32 / (16 * steps), rounded up: exact for the i / (16 * steps) that occur
   int32_t vector_x;   // rows of x are 16-byte aligned
 };
 
-__device__ __forceinline__ uint4 load_stream(const void *p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
+// Loads that are skipped (the registers keep what they held) unless `in`.  The
+// results are only touched when they are multiplied, two steps later.
+__device__ __forceinline__ void load_stream(uint4 &v, const void *p, bool in) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.u32 p, %5, 0;\n\t"
+      "@p ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n\t}"
+      : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)
+      : "l"(p), "r"(static_cast<uint32_t>(in)));
+}
+
+__device__ __forceinline__ void load_word(uint32_t &v, const void *p, bool in) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.u32 p, %2, 0;\n\t"
+      "@p ld.global.nc.u32 %0, [%1];\n\t}"
+      : "+r"(v)
+      : "l"(p), "r"(static_cast<uint32_t>(in)));
 }
 
 // Four bytes of e2m1 pairs -> four f16x2 (low nibble in the low half).
@@ -89,13 +102,6 @@ __device__ __forceinline__ void mma_m16n8k16(float (&d)[4], uint32_t a0, uint32_
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Two elements of x to f32.
-template <typename T>
-__device__ __forceinline__ float2 widen2(uint32_t w) {
-  if (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2 *>(&w));
-  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
-}
-
 // Eight elements of a row of x, zeros behind `left`.
 template <typename T>
 __device__ __forceinline__ uint4 load_x8(const T *p, bool vector, int left) {
@@ -128,17 +134,23 @@ struct Shape {
   static constexpr int sum_bytes = k_warps * rows * tokens * 4;
 };
 
+// Blocks that share an SM (by registers).
+template <int NT, int RU>
+constexpr int blocks_per_sm() { return NT == 1 && RU == 2 ? 3 : 2; }
+
 template <int RU>
 struct Batch {  // the weights of one step
   uint4 w[RU][2];
-  uint16_t s[RU][2];
+  uint32_t s[RU][2];  // four groups' scales, of which a lane uses two
 };
 
 template <typename T, int NT, int RU, int WR>
-__global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 2 : 1) weight_only_kernel(const Args p) {
+__global__ void __launch_bounds__(32 * kWarps, blocks_per_sm<NT, RU>()) weight_only_kernel(const Args p) {
   using S = Shape<NT, RU, WR>;
+  constexpr bool kScaled = std::is_same<T, __nv_bfloat16>::value;  // rows of x carry a power of two
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint32_t row_max[S::tokens];
+  __shared__ float bias[S::rows];
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
   const int split = gridDim.x;  // cluster: blocks along K
   const int part = blockIdx.x;
@@ -150,86 +162,106 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 2 : 1) weight_only_kern
   const int k_begin = part * p.steps * kStep;
   const int steps = max(0, min(p.steps, (p.K - k_begin + kStep - 1) / kStep));
 
+  // weight row of row r of the block: a quarter's rows of all its units
+  const auto feature = [&](int r) {
+    const int first = blockIdx.y * WR * RU, quarter_rows = 4 * RU * WR;
+    return static_cast<int64_t>(first / 8) * 128 + r / quarter_rows * 32 + 4 * (first % 8) + r % quarter_rows;
+  };
+
   grid_dependency_wait();
 
-  // rows g and g + 8 of unit u: see the header
-  const int in_quarter = 4 * (unit0 % 8) + g / 4;
-  const uint8_t *codes = p.codes + (row_block * 128 + (g % 4) * 32 + in_quarter) * (p.K / 2) + k_begin / 2 + 16 * t;
-  const uint8_t *sf = p.sf + row_block * (p.K / 64) * 512 + static_cast<int64_t>(k_begin / 64 + t / 2) * 512 +
-                      in_quarter * 16 + (g % 4) * 4 + (t % 2) * 2;
+  // rows g and g + 8 of unit u: see the header; 32-bit offsets inside the scale tile's 128 rows
+  const uint32_t half_k = p.K / 2;
+  const uint8_t *codes = p.codes + row_block * 128 * half_k;
+  const uint8_t *sf = p.sf + row_block * (p.K / 64) * 512;
+  const uint32_t in_quarter = 4 * (unit0 % 8) + g / 4;
+  const uint32_t code_at = ((g % 4) * 32 + in_quarter) * half_k + k_begin / 2 + 16 * t;
+  const uint32_t sf_at = (k_begin / 64 + t / 2) * 512 + in_quarter * 16 + (g % 4) * 4;
+  const int in_steps = max(0, (p.K - k_begin - 32 * t + kStep - 1) / kStep);
   const auto load = [&](Batch<RU> &b, int step) {
-    const bool in = step < steps && k_begin + step * kStep + 32 * t < p.K;  // K ends on half a step, maybe
+    const bool in = step < min(steps, in_steps);
 #pragma unroll
     for (int u = 0; u < RU; ++u)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        b.w[u][r] = make_uint4(0, 0, 0, 0);
-        b.s[u][r] = 0;
-        if (in) {
-          b.w[u][r] = load_stream(codes + static_cast<int64_t>(4 * u + 2 * r) * (p.K / 2) + step * (kStep / 2));
-          b.s[u][r] = __ldg(reinterpret_cast<const uint16_t *>(sf + (4 * u + 2 * r) * 16 + step * 1024));
-        }
+        load_stream(b.w[u][r], codes + (code_at + (4 * u + 2 * r) * half_k + step * (kStep / 2)), in);
+        load_word(b.s[u][r], sf + (sf_at + (4 * u + 2 * r) * 16 + step * 1024), in);
       }
   };
-  Batch<RU> batch[2];
+  Batch<RU> batch[2] = {};
   load(batch[0], k_warp);
   load(batch[1], k_warp + S::k_warps);
 
+  const float alpha = __ldg(p.alpha);
+  if (tid < S::rows) bias[tid] = p.bias != nullptr ? __bfloat162float(p.bias[feature(tid)]) : 0.0f;
+
   // ---- x to fp16 in shared memory ----
   const int row_bytes = S::row_bytes(p.steps);
-  const T *x = static_cast<const T *>(p.x);
-  const int chunks = steps * (kStep / 8);  // of eight elements, in a row
-  if (!std::is_same<T, __half>::value) {
+  const T *x = static_cast<const T *>(p.x) + m0 * p.ldx;
+  const int chunks = p.steps * (kStep / 8);  // of eight elements, in a row; a multiple of 16
+  const int items = tokens * chunks;
+  const auto row_of = [&](int i) { return static_cast<int>(__umulhi(i, p.chunk_inverse)); };  // i / chunks
+  // chunk 4 * t + i of a step is read by lane t in its i-th pair of products
+  const auto place = [&](int m, int c) {
+    return reinterpret_cast<uint4 *>(smem + m * row_bytes + (c / 16) * 256 + (c % 4) * 64 + (c % 16) / 4 * 16);
+  };
+  if (kScaled) {
     if (tid < S::tokens) row_max[tid] = 0;
     __syncthreads();
-    for (int m = 0; m < tokens; ++m) {
-      uint32_t top = 0;
-      for (int c = tid; c < chunks; c += 32 * kWarps) {
-        const int k = k_begin + 8 * c;
-        const uint4 v = load_x8(x + (m0 + m) * p.ldx + k, p.vector_x, p.K - k);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {  // magnitudes compare as integers; NaN is left out
-          const uint32_t lo = (w[j] << 16) & 0x7FFFFFFFu, hi = w[j] & 0x7FFF0000u;
-          top = max(top, lo > 0x7F800000u ? 0u : lo);
-          top = max(top, hi > 0x7F800000u ? 0u : hi);
-        }
-      }
-      top = __reduce_max_sync(0xffffffffu, top);
-      if (lane == 0 && top) atomicMax(&row_max[m], top);
-    }
-    __syncthreads();
   }
-  for (int m = 0; m < tokens; ++m) {
-    const float factor = std::is_same<T, __half>::value ? 1.0f : power_of_two(row_shift(row_max[m]));
-    for (int c = tid; c < chunks; c += 32 * kWarps) {
-      const int k = k_begin + 8 * c;
-      uint4 v = load_x8(x + (m0 + m) * p.ldx + k, p.vector_x, p.K - k);
-      if (!std::is_same<T, __half>::value) {
-        uint32_t *w = reinterpret_cast<uint32_t *>(&v);
+  for (int i0 = tid; i0 < items; i0 += 4 * 32 * kWarps) {
+    uint4 v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 f = widen2<T>(w[j]);
-          const __half2 h = __floats2half2_rn(f.x * factor, f.y * factor);
-          w[j] = *reinterpret_cast<const uint32_t *>(&h);
-        }
+    for (int j = 0; j < 4; ++j) {
+      const int i = i0 + j * 32 * kWarps, m = row_of(i), c = i - m * chunks;
+      if (i < items) v[j] = load_x8(x + m * p.ldx + k_begin + 8 * c, p.vector_x, p.K - k_begin - 8 * c);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = i0 + j * 32 * kWarps, m = row_of(i), c = i - m * chunks;
+      if (i >= items) break;  // for all 16 lanes of a row's piece at once
+      *place(m, c) = v[j];
+      if (!kScaled) continue;
+      const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+      uint32_t top = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {  // magnitudes compare as integers; NaN is left out
+        const uint32_t lo = (w[e] << 16) & 0x7FFFFFFFu, hi = w[e] & 0x7FFF0000u;
+        top = max(top, lo > 0x7F800000u ? 0u : lo);
+        top = max(top, hi > 0x7F800000u ? 0u : hi);
       }
-      // chunk 4 * t + i of a step is read by lane t in its i-th pair of products
-      const int at = (c / 16) * 256 + (c % 4) * 64 + (c % 16) / 4 * 16;
-      *reinterpret_cast<uint4 *>(smem + m * row_bytes + at) = v;
+      top = __reduce_max_sync(0xFFFFu << (lane & 16), top);
+      if (lane % 16 == 0 && top) atomicMax(&row_max[m], top);
     }
   }
   __syncthreads();
+  if (kScaled) {
+    for (int i = tid; i < items; i += 32 * kWarps) {
+      const int m = row_of(i), c = i - m * chunks;
+      const float factor = power_of_two(row_shift(row_max[m]));
+      uint4 v = *place(m, c);
+      uint32_t *w = reinterpret_cast<uint32_t *>(&v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const __half2 h = __floats2half2_rn(__uint_as_float(w[e] << 16) * factor,
+                                            __uint_as_float(w[e] & 0xFFFF0000u) * factor);
+        w[e] = *reinterpret_cast<const uint32_t *>(&h);
+      }
+      *place(m, c) = v;
+    }
+    __syncthreads();
+  }
 
   // ---- products ----
   float acc[RU][NT][4] = {};
   const auto multiply = [&](const Batch<RU> &b, int step) {
-    uint32_t scale[RU][2][2];  // unit, row, group: the scale in both halves
+    const bool in = step < in_steps;  // K may end on half a step: a zero scale makes any code 0
+    uint32_t scale[RU][2][2];         // unit, row, group: the scale in both halves
 #pragma unroll
     for (int u = 0; u < RU; ++u)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const uint32_t h = decode_e4m3x2(b.s[u][r]);
+        const uint32_t h = decode_e4m3x2(in ? static_cast<uint16_t>(b.s[u][r] >> (16 * (t % 2))) : 0);
         scale[u][r][0] = __byte_perm(h, 0, 0x1010);
         scale[u][r][1] = __byte_perm(h, 0, 0x3232);
       }
@@ -275,20 +307,17 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 2 : 1) weight_only_kern
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        // row of the block: quarter, unit, row of the unit in its quarter
-        const int quarter_rows = 4 * RU * WR;
-        const int row = (g % 4) * quarter_rows + 4 * ((warp % WR) * RU + u) + g / 4 + 2 * (j / 2);
+        const int row = (g % 4) * (4 * RU * WR) + 4 * ((warp % WR) * RU + u) + g / 4 + 2 * (j / 2);
         const int token = 8 * n + 2 * t + j % 2;
         sums[(k_warp * S::tokens + token) * S::rows + row] = acc[u][n][j];
       }
   __syncthreads();
-  const float alpha = __ldg(p.alpha);
   for (int i = tid; i < tokens * S::rows; i += 32 * kWarps) {
     float v = sums[i];
 #pragma unroll
     for (int w = 1; w < S::k_warps; ++w) v += sums[w * S::tokens * S::rows + i];
     v *= alpha;
-    if (!std::is_same<T, __half>::value) v *= power_of_two(-row_shift(row_max[i / S::rows]));
+    if (kScaled) v *= power_of_two(-row_shift(row_max[i / S::rows]));
     sums[i] = v;
   }
   cluster_sync();
@@ -299,11 +328,8 @@ __global__ void __launch_bounds__(32 * kWarps, NT == 1 ? 2 : 1) weight_only_kern
       asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(other) : "r"(map_to_rank(smem_u32(sums + i), c)));
       v += other;
     }
-    const int token = i / S::rows, row = i % S::rows, quarter_rows = 4 * RU * WR;
-    const int64_t first = static_cast<int64_t>(blockIdx.y) * WR * RU;  // unit
-    const int64_t n = first / 8 * 128 + row / quarter_rows * 32 + 4 * (first % 8) + row % quarter_rows;
-    if (p.bias != nullptr) v += __bfloat162float(p.bias[n]);
-    p.out[(m0 + token) * p.ldo + n] = __float2bfloat16_rn(v);
+    const int token = i / S::rows, row = i % S::rows;
+    p.out[(m0 + token) * p.ldo + feature(row)] = __float2bfloat16_rn(v + bias[row]);
   }
   cluster_sync();  // the others have read this block's sums
 }
@@ -314,6 +340,7 @@ int launch(Args p, int split, cudaStream_t stream) {
   auto kernel = weight_only_kernel<T, NT, RU, WR>;
   const int steps = (p.K + kStep - 1) / kStep;
   p.steps = (steps + split - 1) / split;
+  p.chunk_inverse = static_cast<uint32_t>((1ull << 32) / (p.steps * 16)) + 1;
   const int x_bytes = (p.M < S::tokens ? p.M : S::tokens) * S::row_bytes(p.steps);
   const int smem = x_bytes > S::sum_bytes ? x_bytes : S::sum_bytes;
   constexpr int kMost = 200 * 1024;
@@ -340,16 +367,19 @@ int launch(Args p, int split, cudaStream_t stream) {
   return VFB_OK;
 }
 
-// Blocks along K: enough blocks for two on every SM, x of a K range within
-// 96 KB (two blocks on an SM), at least one step for every warp while that lasts.
+// Blocks along K: as many as still run at once, but every warp keeps two steps;
+// more where x of a K range would not let that many blocks share an SM.
 template <typename T, int NT, int RU, int WR>
 int launch_split(const Args &p, int sms, cudaStream_t stream) {
   using S = Shape<NT, RU, WR>;
   const int steps = (p.K + kStep - 1) / kStep;
+  const int tokens = p.M < S::tokens ? p.M : S::tokens;
   const int64_t blocks = static_cast<int64_t>(p.N / S::rows) * ((p.M + S::tokens - 1) / S::tokens);
+  const int resident = blocks_per_sm<NT, RU>();
+  const int x_most = 216 * 1024 / resident;
   int split = 1;
-  while (split < 8 && ((blocks * split < 2 * sms && steps >= 2 * split * S::k_warps) ||
-                       S::tokens * S::row_bytes((steps + split - 1) / split) > 96 * 1024))
+  while (split < 8 && ((2 * blocks * split <= resident * sms && steps >= 4 * split * S::k_warps) ||
+                       tokens * S::row_bytes((steps + split - 1) / split) > x_most))
     split *= 2;
   return launch<T, NT, RU, WR>(p, split, stream);
 }
@@ -357,9 +387,9 @@ int launch_split(const Args &p, int sms, cudaStream_t stream) {
 template <typename T>
 int run(const Args &p, int sms, cudaStream_t s) {
   if (p.M <= 2) return launch_split<T, 1, 2, 1>(p, sms, s);
-  if (p.M <= 8) return launch_split<T, 1, 4, 1>(p, sms, s);
-  if (p.M <= 16 || p.K > 16384) return launch_split<T, 2, 4, 2>(p, sms, s);
-  return launch_split<T, 4, 4, 2>(p, sms, s);
+  if (p.M <= 8) return launch_split<T, 1, 4, 2>(p, sms, s);
+  if (p.M <= 16 || p.K > 16384) return launch_split<T, 2, 2, 4>(p, sms, s);
+  return launch_split<T, 4, 2, 4>(p, sms, s);
 }
 
 constexpr int64_t kMaxK = 32768;

@@ -9,6 +9,7 @@ library, a non-SM100 device or a rejected layout raises.
 from __future__ import annotations
 
 import ctypes
+from contextlib import nullcontext
 from dataclasses import dataclass
 
 import torch
@@ -563,35 +564,22 @@ def _nvfp4_gemm_quant(a_codes, a_sf, w_packed, w_scales, alpha, alpha_div, ep: E
     return codes, sf
 
 
-def _workspace(nbytes: int, device):
-    """A 256-byte aligned buffer of ``nbytes`` from torch's allocator: the tensor to keep and its address."""
-    if nbytes == 0:
-        return None, None
-    buffer = torch.empty(nbytes, device=device, dtype=torch.uint8)  # the allocator aligns to 512 bytes
-    return buffer, buffer.data_ptr()
+_SAME_DEVICE = nullcontext()
 
 
-def nvfp4_weight_only(matrix: torch.Tensor, w_packed: torch.Tensor, w_scales: torch.Tensor, alpha: torch.Tensor,
-                      bias: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
-    """``bf16(alpha * matrix @ W^T + bias)`` for an NVFP4 weight and activations that stay in 16 bits.
+def _on(device: torch.device):
+    """Makes ``device`` current, at no cost where it is (short calls are bound by the host)."""
+    return _SAME_DEVICE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
-    ``matrix`` bf16 or fp16 ``[M, K]`` (unit column stride, any row stride),
-    ``w_packed`` uint8 ``[N, K/2]`` and ``w_scales`` uint8 (128x4 layout) as
-    ``nvfp4_gemm`` takes them, ``alpha`` an fp32 scalar tensor, ``bias`` bf16
-    ``[N]``.  K % 64 == 0, K <= 32768, N % 128 == 0.  Made for few rows (one token,
-    a small batch); more rows work too, re-reading the weight for every 32.
-    """
-    if matrix.dtype not in (BF16, torch.float16) or matrix.ndim != 2 or matrix.stride(1) != 1 and matrix.shape[1] > 1:
-        raise KernelInputError("the weight-only NVFP4 product needs a bf16/fp16 [M, K] matrix with unit column stride")
-    rows, k = matrix.shape
-    device = matrix.device
+
+def _check_weight_only(matrix, w_packed, w_scales, alpha, bias) -> None:
+    k = matrix.shape[1]
     if (w_packed.dtype != torch.uint8 or w_packed.ndim != 2 or 2 * w_packed.shape[1] != k
             or not w_packed.is_contiguous()):
         raise KernelInputError("NVFP4 weight codes must be contiguous uint8 [N, K/2]")
     n = w_packed.shape[0]
-    if n == 0 or k == 0 or k % 64 or k > 32768 or n % 128 or n > 1048576 or rows > 524288:
-        raise KernelInputError("the weight-only NVFP4 product needs K % 64 == 0, K <= 32768, N % 128 == 0, "
-                               "N <= 1048576, M <= 524288")
+    if n == 0 or k == 0 or k % 64 or n % 128:
+        raise KernelInputError("the weight-only NVFP4 product needs K % 64 == 0, N % 128 == 0")
     if w_scales.dtype != torch.uint8 or w_scales.numel() != n * (k // 16) or not w_scales.is_contiguous():
         raise KernelInputError("NVFP4 weight scales differ from the 128x4 layout")
     if alpha.dtype != torch.float32 or alpha.numel() != 1:
@@ -600,42 +588,74 @@ def nvfp4_weight_only(matrix: torch.Tensor, w_packed: torch.Tensor, w_scales: to
         raise KernelInputError("NVFP4 bias must be contiguous bf16 [N]")
     if not (_aligned(w_packed) and _aligned(w_scales, 4)):
         raise KernelInputError("NVFP4 weight codes must be 16-byte aligned, scales 4-byte aligned")
+    for t in (w_packed, w_scales, alpha, bias):
+        if t is not None and t.device != matrix.device:
+            raise KernelInputError("weight-only NVFP4 operands must share one device")
+
+
+def nvfp4_weight_only(matrix: torch.Tensor, w_packed: torch.Tensor, w_scales: torch.Tensor, alpha: torch.Tensor,
+                      bias: torch.Tensor | None = None, out: torch.Tensor | None = None, *,
+                      checked: bool = False) -> torch.Tensor:
+    """``bf16(alpha * matrix @ W^T + bias)`` for an NVFP4 weight and activations that stay in 16 bits.
+
+    ``matrix`` bf16 or fp16 ``[M, K]`` (unit column stride, any row stride),
+    ``w_packed`` uint8 ``[N, K/2]`` and ``w_scales`` uint8 (128x4 layout) as
+    ``nvfp4_gemm`` takes them, ``alpha`` an fp32 scalar tensor, ``bias`` bf16
+    ``[N]``.  K % 64 == 0, K <= 32768, N % 128 == 0.  Made for few rows (one token,
+    a small batch); more rows work too, re-reading the weight for every 32.
+    ``out`` may be a strided view and may not overlap ``matrix``.  ``checked``
+    skips the checks of the weight and the bias, for a caller that made them
+    (an ``NVFP4Weight`` is checked when it is made); the library still checks
+    sizes and alignment.
+    """
+    if matrix.dtype not in (BF16, torch.float16) or matrix.ndim != 2 or matrix.stride(1) != 1 and matrix.shape[1] > 1:
+        raise KernelInputError("the weight-only NVFP4 product needs a bf16/fp16 [M, K] matrix with unit column stride")
+    rows, k = matrix.shape
+    device = matrix.device
+    if not checked:
+        _check_weight_only(matrix, w_packed, w_scales, alpha, bias)
+    n = w_packed.shape[0]
+    if k > 32768 or n > 1048576 or rows > 524288:
+        raise KernelInputError("the weight-only NVFP4 product needs K <= 32768, N <= 1048576, M <= 524288")
+    if rows > 1 and matrix.stride(0) < k:
+        matrix = matrix.contiguous()  # expanded or overlapping rows
     if out is None:
         out = torch.empty((rows, n), device=device, dtype=BF16)
-    elif out.dtype != BF16 or out.shape != (rows, n) or out.stride(1) != 1:
+    elif out.dtype != BF16 or out.shape != (rows, n) or out.stride(1) != 1 or rows > 1 and out.stride(0) < n:
         raise KernelInputError("the weight-only NVFP4 output must be bf16 [M, N] with unit column stride")
-    for t in (w_packed, w_scales, alpha, bias, out):
-        if t is not None and t.device != device:
-            raise KernelInputError("weight-only NVFP4 operands must share one device")
+    elif out.device != device:
+        raise KernelInputError("weight-only NVFP4 operands must share one device")
     if rows == 0:
         return out
     lib = _lib.load()
-    with torch.cuda.device(device):
+    with _on(device):
         rc = lib.vfb_nvfp4_weight_only(
             matrix.data_ptr(), 0 if matrix.dtype == BF16 else 1, rows, max(matrix.stride(0), k),
-            w_packed.data_ptr(), w_scales.data_ptr(), alpha.data_ptr(), _lib.ptr(bias), n, k, out.data_ptr(),
-            max(out.stride(0), n), _lib.stream_handle(device))
-    _lib.check(rc, "vfb_nvfp4_weight_only")
+            w_packed.data_ptr(), w_scales.data_ptr(), alpha.data_ptr(), None if bias is None else bias.data_ptr(),
+            n, k, out.data_ptr(), max(out.stride(0), n), _lib.stream_handle(device))
+    if rc:
+        _lib.check(rc, "vfb_nvfp4_weight_only")
     return out
 
 
 # ---------------------------------------------------------------------------
 # attention
 # ---------------------------------------------------------------------------
-def _head_strides(t: torch.Tensor, name: str) -> tuple[int, int]:
+def _strides(t: torch.Tensor, name: str) -> tuple[int, int]:
     """Token and head strides of a ``[rows, heads, dim]`` tensor; a dimension of one element takes a packed stride."""
     rows, heads, dim = t.shape
-    if t.stride(2) != 1 and dim > 1:
+    token, head, unit = t.stride()
+    if unit != 1:
         raise KernelInputError(f"attention {name} needs a unit stride over the head dimension")
-    head = t.stride(1) if heads > 1 else dim
-    token = t.stride(0) if rows > 1 else max(heads * dim, heads * head)
-    if head % 8 or token % 8 or head < dim or token < dim or (rows and not _aligned(t)):
-        raise KernelInputError(f"attention {name} needs 16-byte aligned rows (strides of 8 elements, not expanded)")
+    if heads == 1:
+        head = dim
+    if rows <= 1:
+        token = heads * head
     return token, head
 
 
 def _check_offsets(t: torch.Tensor, entries: int | None, device, name: str) -> None:
-    if (t.dtype != torch.int32 or t.ndim != 1 or not t.is_contiguous() or t.device != device or not _aligned(t, 4)
+    if (t.dtype != torch.int32 or t.ndim != 1 or not t.is_contiguous() or t.device != device
             or entries is not None and t.shape[0] != entries):
         raise KernelInputError(f"attention {name} must be contiguous int32 on the queries' device"
                                + ("" if entries is None else f" with {entries} entries"))
@@ -682,52 +702,50 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: t
     scale = dim ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < float("inf"):
         raise KernelInputError("attention scale must be positive and finite")
-    for t in (k, v):
-        if t.device != device:
-            raise KernelInputError("attention operands must share one device")
-    a = _lib.AttentionArgs()
-    if cu_seqlens_q is None:
-        if cu_seqlens_k is not None:
-            raise KernelInputError("attention cu_seqlens_k needs cu_seqlens_q")
-        batch = 1
-    else:
+    if k.device != device or v.device != device:
+        raise KernelInputError("attention operands must share one device")
+    at_q = at_k = at_n = None
+    batch = 1
+    if cu_seqlens_q is not None:
         _check_offsets(cu_seqlens_q, None, device, "cu_seqlens_q")
         batch = cu_seqlens_q.shape[0] - 1
         if batch < 1:
             raise KernelInputError("attention cu_seqlens_q needs at least two entries")
-        a.cu_seqlens_q = cu_seqlens_q.data_ptr()
+        at_q = cu_seqlens_q.data_ptr()
         if cu_seqlens_k is not None:
             _check_offsets(cu_seqlens_k, batch + 1, device, "cu_seqlens_k")
-            a.cu_seqlens_k = cu_seqlens_k.data_ptr()
+            at_k = cu_seqlens_k.data_ptr()
         elif total_k != total_q:
             raise KernelInputError("attention keys of another length than the queries need cu_seqlens_k")
+    elif cu_seqlens_k is not None:
+        raise KernelInputError("attention cu_seqlens_k needs cu_seqlens_q")
     if lengths_k is not None:
         _check_offsets(lengths_k, batch, device, "lengths_k")
-        a.lengths_k = lengths_k.data_ptr()
-    a.q_token_stride, a.q_head_stride = _head_strides(q, "q")
-    a.k_token_stride, a.k_head_stride = _head_strides(k, "k")
-    a.v_token_stride, a.v_head_stride = _head_strides(v, "v")
+        at_n = lengths_k.data_ptr()
     fresh = out is None
     if fresh:
         out = torch.empty((total_q, heads, dim), device=device, dtype=q.dtype)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != device:
         raise KernelInputError("attention out differs from q's shape, type or device")
-    a.out_token_stride, a.out_head_stride = _head_strides(out, "out")
     lse = torch.empty((heads, total_q), device=device, dtype=torch.float32) if return_lse else None
+    args = _lib.AttentionArgs(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
+        *_strides(q, "q"), *_strides(k, "k"), *_strides(v, "v"), *_strides(out, "out"), total_q, total_k, heads,
+        kv_heads, dim, 0 if q.dtype == BF16 else 1, at_q, at_k, at_n, batch, causal, scale, fresh)
+    lib = _lib.load()
+    address = ctypes.byref(args)
+    need = lib.vfb_attention_workspace_bytes(address)  # checks strides and alignment too
+    if need < 0:
+        raise KernelInputError(_lib.last_error())
     if total_q:
-        require_sm100(device)
-        a.q, a.k, a.v, a.out, a.lse = (_lib.ptr(t) for t in (q, k, v, out, lse))
-        a.total_q, a.total_k, a.heads, a.kv_heads, a.dim = total_q, total_k, heads, kv_heads, dim
-        a.dtype = 0 if q.dtype == BF16 else 1
-        a.batch, a.causal, a.scale, a.fill_tail = batch, int(causal), scale, int(fresh)
-        lib = _lib.load()
-        args = ctypes.byref(a)
-        need = lib.vfb_attention_workspace_bytes(args)
-        if need < 0:
-            raise KernelInputError(f"attention: {_lib.last_error()}")
-        with torch.cuda.device(device):
-            keep, a.workspace = _workspace(need, device)
-            a.workspace_bytes = need
-            rc = lib.vfb_attention(args, _lib.stream_handle(device))
-        _lib.check(rc, "vfb_attention")
+        if device.type != "cuda":
+            require_sm100(device)  # refuses; a CUDA device is checked by the library
+        with _on(device):
+            if need:
+                workspace = torch.empty(need, device=device, dtype=torch.uint8)  # 512-byte aligned
+                args.workspace = workspace.data_ptr()
+                args.workspace_bytes = need
+            rc = lib.vfb_attention(address, _lib.stream_handle(device))
+        if rc:
+            _lib.check(rc, "vfb_attention")
     return (out, lse) if return_lse else out

@@ -205,25 +205,33 @@ class NVFP4Execution:
         the weight once.  fp32 values are first rounded to bf16, as in
         ``linear``; sums are fp32, with one rounding after the bias.
         """
+        packed = weight.packed
+        shape, device, dtype = values.shape, values.device, values.dtype
+        n, k = packed.shape[0], 2 * packed.shape[1]
         if (
-            values.ndim < 1
-            or values.shape[-1] != weight.in_features
-            or values.dtype not in (torch.bfloat16, torch.float16, torch.float32)
-            or values.device != weight.packed.device
+            not shape
+            or shape[-1] != k
+            or dtype not in (torch.bfloat16, torch.float16, torch.float32)
+            or device != packed.device
         ):
             raise ValueError("NVFP4 input differs from its frozen matrix")
-        if torch.is_grad_enabled() and values.requires_grad:
+        if values.requires_grad and torch.is_grad_enabled():
             raise ValueError("NVFP4 execution is inference-only")
-        _require_device(values.device)
-        self._check_bias(values, bias, weight.out_features)
-        matrix = values.to(torch.bfloat16) if values.dtype == torch.float32 else values
-        matrix = matrix.reshape(-1, weight.in_features)
-        if matrix.shape[0] == 0:
+        _require_device(device)
+        if bias is not None:
+            self._check_bias(values, bias, n)
+            if not bias.is_contiguous():
+                raise ValueError("NVFP4 bias must be contiguous")
+        matrix = values.to(torch.bfloat16) if dtype == torch.float32 else values
+        if len(shape) != 2:
+            matrix = matrix.reshape(-1, k)
+        rows = matrix.shape[0]
+        if rows == 0:
             raise ValueError("NVFP4 input rows must be nonempty")
-        output = nvfp4_weight_only(matrix, weight.packed, weight.scales, weight.alpha, bias)
+        output = nvfp4_weight_only(matrix, packed, weight.scales, weight.alpha, bias, checked=True)
         self.calls += 1
-        self.rows += matrix.shape[0]
-        return output.reshape(*values.shape[:-1], weight.out_features)
+        self.rows += rows
+        return output if len(shape) == 2 else output.reshape(*shape[:-1], n)
 
     # -- fused entry points (opt-in): the strict-BF16 step after the linear runs
     # in the GEMM's epilogue, as for RowFP8Execution
