@@ -49,14 +49,19 @@ int main() {
     std::map<Job, std::set<int>> done;
     std::map<int, std::pair<Job, std::pair<int, int>>> pieces;  // slot -> job, key tiles
     std::set<int> empty_slots;
+    std::vector<Record> records;
     const int n = static_cast<int>(split ? p.blocks : grid);
     std::map<Job, bool> whole;
     for (int block = 0; block < n; ++block) {
       Order order;
-      bool share = true;
-      if (split) share = order.init_share(p, block);
-      else order.init_whole(p, block, static_cast<int32_t>(grid));
-      if (share && order.empty()) empty_slots.insert(2 * block);
+      if (split) {
+        Record record;
+        order.init_share(p, block, record);
+        records.push_back(record);
+        if (order.empty()) empty_slots.insert(2 * block);
+      } else {
+        order.init_whole(p, block, static_cast<int32_t>(grid));
+      }
       Segment s;
       while (order.next(p, s)) {
         const Job job{s.b, s.group, s.tile};
@@ -89,19 +94,29 @@ int main() {
     for (const auto &x : pieces) by_job[x.second.first].insert(x.first);
     std::set<Job> joined;
     for (int c = 1; split && c < p.blocks; ++c) {
-      Join j;
-      if (!join_at(p, c, j)) continue;
-      const Job job{j.job.b, j.job.group, j.job.tile};
-      if (!joined.insert(job).second) return std::printf("joined twice\n"), 1;
-      std::set<int> slots{j.first};
-      for (int i = j.c; i <= j.last; ++i) slots.insert(2 * i);
+      const Record &r = records[c], &before = records[c - 1];
+      if (!join_starts(before, r)) continue;
+      std::set<int> slots{join_first(before, r, c)};
+      for (int i = c; i < p.blocks && records[i].inside && records[i].start == r.start; ++i) slots.insert(2 * i);
       std::set<int> real;
+      std::set<Job> jobs;
       for (int x : slots) {
         const auto it = pieces.find(x);
-        if (it != pieces.end() && it->second.first == job) real.insert(x);
-        else if (!empty_slots.count(x)) return std::printf("join reads slot %d that nothing wrote\n", x), 1;
+        if (it != pieces.end()) {
+          real.insert(x);
+          jobs.insert(it->second.first);
+        } else if (!empty_slots.count(x)) {
+          return std::printf("join reads slot %d that nothing wrote\n", x), 1;
+        }
       }
+      if (jobs.size() != 1) return std::printf("join of several jobs\n"), 1;
+      const Job job = *jobs.begin();
+      if (!joined.insert(job).second) return std::printf("joined twice\n"), 1;
       if (real != by_job[job]) return std::printf("join misses pieces\n"), 1;
+      const Seq s = sequence(p, std::get<0>(job));
+      const int64_t rows0 = static_cast<int64_t>(std::get<2>(job)) * p.job_tokens;
+      if (r.row0 != s.q0 + rows0 || r.group != std::get<1>(job) || r.count != min64(p.job_tokens, s.nq - rows0))
+        return std::printf("record of another job\n"), 1;
       ++cuts;
     }
     for (const auto &x : by_job)

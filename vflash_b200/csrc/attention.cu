@@ -15,7 +15,8 @@
 //   warps 0-3, 4-7  softmax of stage 0 and stage 1, one thread per row
 //   warp 8          TMA loads: Q tiles, then K and V tiles through one ring
 //   warp 9          MMA issue
-//   warps 10, 11    clean the V tiles that hold keys some row must not see
+//   warp 10         cleans the V tiles that hold keys some row must not see
+//   warp 11         works out the block's jobs and hands them to the others
 // The two stages keep the tensor cores busy with one tile's products while the
 // other's exponentials run.  They are
 //   PAIR: two tiles of query rows against the same keys (many query rows), or
@@ -27,8 +28,8 @@
 // so S(j+1) may be issued behind the P V(j) that still reads P.
 //
 // Keys behind a row's limit: their scores become -inf, so P = 0; but 0 * inf
-// and 0 * NaN would still spoil the second product.  Warps 10 and 11 therefore
-// zero, in the key tiles that any row of the block sees only in part, the V
+// and 0 * NaN would still spoil the second product.  Warp 10 therefore
+// zeroes, in the key tiles that any row of the block sees only in part, the V
 // rows behind the sequence's end and (causal) every element that is not
 // finite; the latter are added back at the end to the rows that do see them.
 #include "common.cuh"
@@ -44,6 +45,8 @@ constexpr int kTile = 128;           // query rows in a tile, and keys in a key 
 constexpr int kPanelBytes = 16384;   // 128 rows x 64 elements of 16 bits, 128-byte swizzle
 constexpr int kThreads = 384;
 constexpr int kRingSlots = 10;       // at most
+constexpr int kJobs = 4;             // jobs that the scheduler may be ahead
+constexpr int kJobReaders = 11;      // warps that follow the schedule
 constexpr float kHold = 8.0f;
 constexpr float kLn2 = 0.693147180559945309f;
 
@@ -70,25 +73,9 @@ struct Params {
   int32_t dim, fill_tail, split;
   float scale_log2;
   float *part_o, *part_lse;       // workspace: [slot][kSlotRows][dim], [slot][kSlotRows]
+  attn::Record *records;          // workspace: [block]
   int *status;
 };
-
-struct Shared {
-  uint64_t q_full, q_empty;
-  uint64_t kv_full[kRingSlots], kv_empty[kRingSlots];
-  uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
-  // a V tile to be cleaned is on its way into the slot, and is clean: the MMA
-  // warp waits for the latter before the slot is given back, so neither barrier
-  // can run ahead of who waits for it
-  uint64_t v_todo[kRingSlots], v_clean[kRingSlots];
-  uint64_t stats_full, stats_empty, drain;
-  uint32_t tmem;
-  int abort;
-  int dirty;  // a non-finite element of V was taken out of a tile
-  float2 stats[kTile];  // ALT: (m, l) of stage 1's rows
-};
-static_assert(sizeof(Shared) + Layout<128, true>::smem <= 232448 && sizeof(Shared) + Layout<128, false>::smem <= 232448,
-              "shared memory of a block");
 
 // ---- small helpers -----------------------------------------------------------
 __device__ __forceinline__ void tma_load_3d(void *smem_dst, const CUtensorMap *map, uint64_t *bar, int32_t x,
@@ -185,35 +172,88 @@ __device__ __forceinline__ constexpr uint32_t exponent_mask() {  // both halves 
   return std::is_same<T, __nv_bfloat16>::value ? 0x7F807F80u : 0x7C007C00u;
 }
 
-// ---- what every role derives from a segment --------------------------------------
+// ---- a job (or a piece of one) as the roles see it -----------------------------------
+struct Job {
+  int64_t row0, k0;     // first query row of the job in q, first key row of its sequence
+  int32_t rows0, count; // index of the row in the sequence, tokens of the job (-1: no more jobs)
+  int32_t nq, nk;       // of the sequence
+  int32_t group;        // of heads
+  int32_t t0, t1;       // key tiles
+  int32_t n[2];         // key tiles of each stage
+  int32_t first_masked; // key tiles from here on are seen in part by some row
+  int32_t min_seen;     // keys that the job's first row sees
+  int32_t slot;         // of the workspace for a piece, -1 for a whole job
+  int32_t behind;       // rows behind the last sequence
+  int32_t reserved;
+
+  __device__ __forceinline__ int32_t tiles(bool pair) const { return pair ? max(n[0], n[1]) : n[0] + n[1]; }
+};
+
 template <bool PAIR>
-struct Work {
-  int64_t row0;       // first query row of the job in q
-  int32_t rows0;      // its index in the sequence
-  int32_t count;      // tokens of the job
-  int32_t n[2];       // key tiles of each stage
-  int32_t first_masked;  // key tiles from here on are seen in part by some row
-  int32_t min_seen;   // keys that the job's first row sees
-  __device__ __forceinline__ Work(const Params &p, const Segment &s) {
-    rows0 = s.tile * p.plan.job_tokens;
-    row0 = s.seq.q0 + rows0;
-    count = min(p.plan.job_tokens, s.seq.nq - rows0);
-    min_seen = attn::keys_seen(p.plan, s.seq, static_cast<int64_t>(rows0) + 1);
-    first_masked = min_seen / attn::KEYS;
-    const int32_t tiles = max(s.t1 - s.t0, 0);
-    if (PAIR) {
-      // stage 0's rows may see fewer keys than the job's last row
-      const int32_t seen0 =
-          attn::keys_seen(p.plan, s.seq, static_cast<int64_t>(rows0) + min(p.tokens, count));
-      const int32_t t1 = min(s.t1, (seen0 + attn::KEYS - 1) / attn::KEYS);
-      n[0] = max(t1 - s.t0, 0);
-      n[1] = count > p.tokens ? tiles : 0;
-    } else {
-      n[0] = (tiles + 1) / 2;
-      n[1] = tiles / 2;
-    }
+__device__ __forceinline__ void describe(const Params &p, const Segment &s, Job &j) {
+  j.rows0 = s.tile * p.plan.job_tokens;
+  j.row0 = s.seq.q0 + j.rows0;
+  j.k0 = s.seq.k0;
+  j.count = min(p.plan.job_tokens, s.seq.nq - j.rows0);
+  j.nq = s.seq.nq;
+  j.nk = s.seq.nk;
+  j.group = s.group;
+  j.t0 = s.t0;
+  j.t1 = s.t1;
+  j.min_seen = attn::keys_seen(p.plan, s.seq, static_cast<int64_t>(j.rows0) + 1);
+  j.first_masked = j.min_seen / attn::KEYS;
+  j.slot = s.slot;
+  j.behind = p.plan.cu_q != nullptr && s.b == p.plan.batch;
+  const int32_t tiles = max(s.t1 - s.t0, 0);
+  if (PAIR) {
+    // stage 0's rows may see fewer keys than the job's last row
+    const int32_t seen0 = attn::keys_seen(p.plan, s.seq, static_cast<int64_t>(j.rows0) + min(p.tokens, j.count));
+    j.n[0] = max(min(s.t1, (seen0 + attn::KEYS - 1) / attn::KEYS) - s.t0, 0);
+    j.n[1] = j.count > p.tokens ? tiles : 0;
+  } else {
+    j.n[0] = (tiles + 1) / 2;
+    j.n[1] = tiles / 2;
   }
-  __device__ __forceinline__ int32_t tiles() const { return PAIR ? max(n[0], n[1]) : n[0] + n[1]; }
+}
+
+struct Shared {
+  uint64_t q_full, q_empty;
+  uint64_t kv_full[kRingSlots], kv_empty[kRingSlots];
+  uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
+  // a V tile to be cleaned is on its way into the slot, and is clean: the MMA
+  // warp waits for the latter before the slot is given back, so neither barrier
+  // can run ahead of who waits for it
+  uint64_t v_todo[kRingSlots], v_clean[kRingSlots];
+  uint64_t stats_full, stats_empty, drain;
+  uint64_t job_full[kJobs], job_empty[kJobs];
+  Job jobs[kJobs];
+  uint32_t tmem;
+  int abort;
+  int dirty;  // a non-finite element of V was taken out of a tile
+  float2 stats[kTile];  // ALT: (m, l) of stage 1's rows
+};
+static_assert(sizeof(Shared) + Layout<128, true>::smem <= 232448 && sizeof(Shared) + Layout<128, false>::smem <= 232448,
+              "shared memory of a block");
+
+// A warp's way through the schedule.
+struct JobReader {
+  Shared &sh;
+  int *status;
+  int slot = 0;
+  uint32_t phase = 0;
+
+  // The next job; false when there is none (or a wait ran out).
+  __device__ __forceinline__ bool next(Job &j) {
+    if (!warp_wait(&sh.job_full[slot], phase, &sh.abort, status)) return false;
+    j = sh.jobs[slot];
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.job_empty[slot]);
+    if (++slot == kJobs) {
+      slot = 0;
+      phase ^= 1;
+    }
+    return j.count >= 0;
+  }
 };
 
 // Running position in the ring of K and V tiles.
@@ -348,7 +388,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&sh.kv_full[i], 1);
       mbar_init(&sh.kv_empty[i], 1);
       mbar_init(&sh.v_todo[i], 1);
-      mbar_init(&sh.v_clean[i], 2);
+      mbar_init(&sh.v_clean[i], 1);
+    }
+    for (int i = 0; i < kJobs; ++i) {
+      mbar_init(&sh.job_full[i], 1);
+      mbar_init(&sh.job_empty[i], kJobReaders);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.s_full[i], 1);
@@ -379,11 +423,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   grid_dependency_wait();  // q, k, v and the offsets may come from the kernel before
   grid_launch_dependents();
 
-  attn::Order order;
-  bool has_share = false;  // of evenly cut work, where the workspace is in use
-  if (p.split) has_share = order.init_share(p.plan, blockIdx.x);
-  else order.init_whole(p.plan, blockIdx.x, gridDim.x);
-  Segment seg;
+  JobReader jobs{sh, p.status};
+  Job job;
 
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
@@ -394,22 +435,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t o_phase[2] = {0, 0}, stats_phase = 0;
     const int token_in_tile = row / p.pack;
     const int head_in_tile = row - token_in_tile * p.pack;
-    if (has_share && order.empty() && stage == 0) {
-      // a share cut to nothing: its slot may be counted among a job's pieces
-      float *lse = p.part_lse + static_cast<int64_t>(2 * blockIdx.x) * kSlotRows;
-      lse[row] = -INFINITY;
-      lse[row + kTile] = -INFINITY;
-    }
-    while (order.next(p.plan, seg)) {
-      const Work<PAIR> w(p, seg);
+    while (jobs.next(job)) {
       const int token = token_in_tile + (PAIR ? stage * p.tokens : 0);  // of the job
-      const bool valid = token_in_tile < p.tokens && token < w.count;
-      const int32_t limit =
-          valid ? attn::keys_seen(p.plan, seg.seq, static_cast<int64_t>(w.rows0) + token + 1) : 0;
+      const bool valid = token_in_tile < p.tokens && token < job.count;
+      int32_t limit = valid ? job.nk : 0;
+      if (valid && p.plan.causal)
+        limit = static_cast<int32_t>(
+            min(max(static_cast<int64_t>(job.rows0) + token + 1 + job.nk - job.nq, int64_t{0}), int64_t{job.nk}));
       const bool live = __any_sync(0xffffffffu, valid);
-      if (!sm.run(PAIR ? seg.t0 : seg.t0 + stage, w.n[stage], PAIR ? 1 : 2, limit, live, lane)) break;
+      if (!sm.run(PAIR ? job.t0 : job.t0 + stage, job.n[stage], PAIR ? 1 : 2, limit, live, lane)) break;
       float m = sm.m, l = sm.l;
-      bool have[2] = {w.n[stage] > 0, false};  // accumulators that hold something for this row
+      bool have[2] = {job.n[stage] > 0, false};  // accumulators that hold something for this row
       float f[2] = {1.0f, 0.0f};
       if (PAIR) {
         if (have[0]) {
@@ -433,12 +469,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&sh.stats_empty);
         bool ok = true;
         for (int i = 0; i < 2; ++i) {
-          if (w.n[i] == 0) continue;
+          if (job.n[i] == 0) continue;
           ok = ok && warp_wait(&sh.o_full[i], o_phase[i], &sh.abort, p.status);
           o_phase[i] ^= 1;
         }
         if (!ok) break;
-        have[1] = w.n[1] > 0;
+        have[1] = job.n[1] > 0;
         const float joint = max3_nan(m, other.x, m);
         const float shift = joint == -INFINITY ? 0.0f : joint;
         f[0] = m == -INFINITY ? 0.0f : ex2((m - shift) * p.scale_log2);
@@ -449,16 +485,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       // A row of infinite scores is NaN however its exponentials were rounded.
       if (m == INFINITY) l = NAN;
-      const int64_t piece_end = attn::min64(limit, static_cast<int64_t>(seg.t1) * attn::KEYS);
-      const bool none = piece_end <= static_cast<int64_t>(seg.t0) * attn::KEYS;
+      const int64_t piece_end = attn::min64(limit, static_cast<int64_t>(job.t1) * attn::KEYS);
+      const bool none = piece_end <= static_cast<int64_t>(job.t0) * attn::KEYS;
       const float inv = none ? 0.0f : 1.0f / l;
-      const int64_t out_row = w.row0 + token;
-      const int head = seg.group * p.pack + head_in_tile;
-      const bool behind = p.plan.cu_q != nullptr && seg.b == p.plan.batch;
+      const int64_t out_row = job.row0 + token;
+      const int head = job.group * p.pack + head_in_tile;
       T *out = static_cast<T *>(p.out) + out_row * p.out_token_stride + head * p.out_head_stride;
       float *part = nullptr;
-      if (seg.slot >= 0) {
-        const int64_t at = static_cast<int64_t>(seg.slot) * kSlotRows + (PAIR ? stage * kTile : 0) + row;
+      if (job.slot >= 0) {
+        const int64_t at = static_cast<int64_t>(job.slot) * kSlotRows + (PAIR ? stage * kTile : 0) + row;
         part = p.part_o + at * p.dim;
         if (valid) p.part_lse[at] = none ? -INFINITY : m * p.scale_log2 + log2f(l);
       } else if (valid && p.lse != nullptr) {
@@ -492,9 +527,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int j = 0; j < 32; ++j) o[j] = none ? 0.0f : o[j] * inv;
           if (valid && dirty && !none) {
             // the elements that were taken out, for the rows that see them
-            const int kv_head = seg.group * p.pack / p.group_heads;
-            const int64_t from = static_cast<int64_t>(max(w.first_masked, seg.t0)) * attn::KEYS;
-            const T *v = static_cast<const T *>(p.v) + kv_head * p.v_head_stride + seg.seq.k0 * p.v_token_stride;
+            const int kv_head = job.group * p.pack / p.group_heads;
+            const int64_t from = static_cast<int64_t>(max(job.first_masked, job.t0)) * attn::KEYS;
+            const T *v = static_cast<const T *>(p.v) + kv_head * p.v_head_stride + job.k0 * p.v_token_stride;
             for (int64_t key = from; key < piece_end; ++key) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) {
@@ -510,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               float4 *dst = reinterpret_cast<float4 *>(part + c + j);
               dst[0] = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
               dst[1] = make_float4(o[j + 4], o[j + 5], o[j + 6], o[j + 7]);
-            } else if (!behind || p.fill_tail) {
+            } else if (!job.behind || p.fill_tail) {
               uint4 t;
               t.x = pack2<T>(o[j], o[j + 1]);
               t.y = pack2<T>(o[j + 2], o[j + 3]);
@@ -550,33 +585,32 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ok) pos.step();
       };
       bool q_loaded = false;
-      while (ok && order.next(p.plan, seg)) {
-        const Work<PAIR> w(p, seg);
-        const int32_t tiles = w.tiles();
+      while (ok && jobs.next(job)) {
+        const int32_t tiles = job.tiles(PAIR);
         if (tiles == 0) continue;
         if (!warp_wait(&sh.q_empty, q_phase ^ 1, &sh.abort, p.status)) break;
-        const int used = PAIR && w.count > p.tokens ? 2 : 1;
+        const int used = PAIR && job.count > p.tokens ? 2 : 1;
         if (leader) {
           mbar_arrive_expect_tx(&sh.q_full, used * L::panels * p.pack * p.tokens * 128);
           for (int t = 0; t < used; ++t)
             for (int i = 0; i < L::panels; ++i)
-              tma_load_3d(s_q + t * L::tile_bytes + i * kPanelBytes, &map_q, &sh.q_full, 64 * i, seg.group * p.pack,
-                          static_cast<int32_t>(w.row0 + t * p.tokens));
+              tma_load_3d(s_q + t * L::tile_bytes + i * kPanelBytes, &map_q, &sh.q_full, 64 * i, job.group * p.pack,
+                          static_cast<int32_t>(job.row0 + t * p.tokens));
         }
         q_loaded = true;
         q_phase ^= 1;
-        const int32_t kv_head = seg.group * p.pack / p.group_heads;
-        const int64_t k0 = seg.seq.k0 + static_cast<int64_t>(seg.t0) * attn::KEYS;
+        const int32_t kv_head = job.group * p.pack / p.group_heads;
+        const int64_t k0 = job.k0 + static_cast<int64_t>(job.t0) * attn::KEYS;
         if (PAIR) {
           for (int32_t i = 0; i < tiles && ok; ++i) {
             load(&map_k, kv_head, k0 + static_cast<int64_t>(i) * attn::KEYS, false);
-            load(&map_v, kv_head, k0 + static_cast<int64_t>(i) * attn::KEYS, seg.t0 + i >= w.first_masked);
+            load(&map_v, kv_head, k0 + static_cast<int64_t>(i) * attn::KEYS, job.t0 + i >= job.first_masked);
           }
         } else {
           load(&map_k, kv_head, k0, false);
           if (tiles > 1) load(&map_k, kv_head, k0 + attn::KEYS, false);
           for (int32_t i = 0; i < tiles && ok; ++i) {
-            load(&map_v, kv_head, k0 + static_cast<int64_t>(i) * attn::KEYS, seg.t0 + i >= w.first_masked);
+            load(&map_v, kv_head, k0 + static_cast<int64_t>(i) * attn::KEYS, job.t0 + i >= job.first_masked);
             if (i + 2 < tiles) load(&map_k, kv_head, k0 + static_cast<int64_t>(i + 2) * attn::KEYS, false);
           }
         }
@@ -627,9 +661,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
       };
-      while (ok && order.next(p.plan, seg)) {
-        const Work<PAIR> w(p, seg);
-        const int32_t tiles = w.tiles();
+      while (ok && jobs.next(job)) {
+        const int32_t tiles = job.tiles(PAIR);
         if (tiles == 0) continue;
         if (!wait(&sh.q_full, q_phase)) break;
         q_phase ^= 1;
@@ -639,7 +672,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (j > 0) {
               if (!wait(&sh.kv_full[pos.slot], pos.phase)) break;
               pos.step();
-              if (seg.t0 + j - 1 >= w.first_masked) {
+              if (job.t0 + j - 1 >= job.first_masked) {
                 if (!wait(&sh.v_clean[v_slot], v_phase >> v_slot & 1)) break;
                 v_phase ^= 1u << v_slot;
               }
@@ -650,7 +683,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               pos.step();
             }
             for (int s = 0; s < 2 && ok; ++s) {
-              if (j > 0 && j <= w.n[s]) {
+              if (j > 0 && j <= job.n[s]) {
                 if (!wait(&sh.p_full[s], p_phase[s])) break;
                 p_phase[s] ^= 1;
                 if (j == 1) {
@@ -659,9 +692,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 tc_fence_after();
                 product_o(s, v_slot, j > 1);
-                if (j == w.n[s]) commit(&sh.o_full[s]);
+                if (j == job.n[s]) commit(&sh.o_full[s]);
               }
-              if (j < w.n[s]) {
+              if (j < job.n[s]) {
                 product_s(s, k_slot);
                 commit(&sh.s_full[s]);
               }
@@ -685,7 +718,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int32_t i = 0; i < tiles && ok; ++i) {
             const int s = i & 1;
             if (!wait(&sh.kv_full[pos.slot], pos.phase)) break;
-            if (seg.t0 + i >= w.first_masked) {
+            if (job.t0 + i >= job.first_masked) {
               if (!wait(&sh.v_clean[pos.slot], v_phase >> pos.slot & 1)) break;
               v_phase ^= 1u << pos.slot;
             }
@@ -707,20 +740,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       // the products issued last are over before the block ends
       commit(&sh.drain);
       warp_wait(&sh.drain, 0, &sh.abort, p.status);
-    } else {
+    } else if (warp == 10) {
       // ---------------- cleaning of V tiles ----------------
       RingPos<L::ring> pos;
-      const int me = (warp - 10) * 32 + lane;
       uint32_t todo_phase = 0;  // a bit for every slot
-      const auto clean = [&](const Work<PAIR> &w, int32_t t) {
+      const auto clean = [&](int32_t t) {
         const int slot = pos.slot;
         if (!warp_wait(&sh.v_todo[slot], todo_phase >> slot & 1, &sh.abort, p.status)) return false;
         todo_phase ^= 1u << slot;
         if (!warp_wait(&sh.kv_full[slot], pos.phase, &sh.abort, p.status)) return false;
         uint8_t *tile = s_kv + slot * L::tile_bytes;
-        const int32_t end = min(max(seg.seq.nk - t * attn::KEYS, 0), attn::KEYS);       // rows of the sequence
-        const int32_t all = min(max(w.min_seen - t * attn::KEYS, 0), attn::KEYS);       // rows that every row sees
-        for (int i = me; i < (attn::KEYS - all) * 8 * L::panels; i += 64) {
+        const int32_t end = min(max(job.nk - t * attn::KEYS, 0), attn::KEYS);       // rows of the sequence
+        const int32_t all = min(max(job.min_seen - t * attn::KEYS, 0), attn::KEYS);       // rows that every row sees
+        for (int i = lane; i < (attn::KEYS - all) * 8 * L::panels; i += 32) {
           const int panel = i / ((attn::KEYS - all) * 8);
           const int rest = i - panel * (attn::KEYS - all) * 8;
           uint4 *at = reinterpret_cast<uint4 *>(tile + panel * kPanelBytes + all * 128) + rest;
@@ -749,9 +781,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         return true;
       };
       bool ok = true;
-      while (ok && order.next(p.plan, seg)) {
-        const Work<PAIR> w(p, seg);
-        const int32_t tiles = w.tiles();
+      while (ok && jobs.next(job)) {
+        const int32_t tiles = job.tiles(PAIR);
         if (tiles == 0) continue;
         if (!PAIR) {
           pos.step();
@@ -759,9 +790,39 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int32_t i = 0; i < tiles && ok; ++i) {
           if (PAIR) pos.step();
-          if (seg.t0 + i >= w.first_masked) ok = clean(w, seg.t0 + i);
+          if (job.t0 + i >= job.first_masked) ok = clean(job.t0 + i);
           pos.step();
           if (!PAIR && i + 2 < tiles) pos.step();
+        }
+      }
+    } else {
+      // ---------------- schedule ----------------
+      attn::Order order;
+      if (p.split) {
+        attn::Record record;
+        order.init_share(p.plan, blockIdx.x, record);
+        if (lane == 0) p.records[blockIdx.x] = record;
+        if (order.empty())  // a share cut to nothing may be counted among a job's pieces
+          for (int i = lane; i < kSlotRows; i += 32) p.part_lse[2ll * blockIdx.x * kSlotRows + i] = -INFINITY;
+      } else {
+        order.init_whole(p.plan, blockIdx.x, gridDim.x);
+      }
+      Segment seg;
+      uint32_t phase = 1;
+      for (int slot = 0;;) {
+        const bool more = order.next(p.plan, seg);
+        if (more) describe<PAIR>(p, seg, job);
+        else job.count = -1;
+        if (!warp_wait(&sh.job_empty[slot], phase, &sh.abort, p.status)) break;
+        if (lane == 0) {
+          sh.jobs[slot] = job;
+          mbar_arrive(&sh.job_full[slot]);
+        }
+        __syncwarp();
+        if (!more) break;
+        if (++slot == kJobs) {
+          slot = 0;
+          phase ^= 1;
         }
       }
     }
@@ -781,18 +842,25 @@ constexpr int kJoinRows = 8;  // rows of one block, a warp each
 template <typename T>
 __global__ void __launch_bounds__(32 * kJoinRows) attention_join_kernel(const __grid_constant__ Params p) {
   grid_dependency_wait();
-  attn::Join j;
-  if (!attn::join_at(p.plan, static_cast<int32_t>(blockIdx.x) + 1, j)) return;
   const int lane = threadIdx.x & 31;
+  const int c = static_cast<int>(blockIdx.x) + 1;
+  const attn::Record before = p.records[c - 1], job = p.records[c];
+  if (!attn::join_starts(before, job)) return;
   const int at = blockIdx.y * kJoinRows + (threadIdx.x >> 5);  // row of the slot
   const int in_tile = at % kTile;
   const int token = in_tile / p.pack + at / kTile * p.tokens;
-  const int64_t row0 = static_cast<int64_t>(j.job.tile) * p.plan.job_tokens;
-  if (in_tile / p.pack >= p.tokens || token >= min(static_cast<int64_t>(p.plan.job_tokens), j.job.seq.nq - row0))
-    return;
-  const int pieces = j.last - j.c + 2;
+  if (in_tile / p.pack >= p.tokens || token >= job.count) return;
+  int pieces = 1;  // and one for every record inside the job
+  for (int i0 = c;; i0 += 32) {
+    const int i = i0 + lane;
+    const bool same = i < p.plan.blocks && p.records[i].inside && p.records[i].start == job.start;
+    const unsigned others = __ballot_sync(0xffffffffu, !same);
+    pieces += others ? __ffs(others) - 1 : 32;
+    if (others) break;
+  }
+  const int first = attn::join_first(before, job, c);
   const auto slot_row = [&](int i) {
-    return static_cast<int64_t>(i == 0 ? j.first : 2 * (j.c + i - 1)) * kSlotRows + at;
+    return static_cast<int64_t>(i == 0 ? first : 2 * (c + i - 1)) * kSlotRows + at;
   };
   float top = -INFINITY;
   for (int i = lane; i < pieces; i += 32) top = max3_nan(top, p.part_lse[slot_row(i)], top);
@@ -813,8 +881,8 @@ __global__ void __launch_bounds__(32 * kJoinRows) attention_join_kernel(const __
     }
   }
   const float inv = top == -INFINITY ? 0.0f : 1.0f / sum;
-  const int head = j.job.group * p.pack + in_tile % p.pack;
-  const int64_t row = j.job.seq.q0 + row0 + token;
+  const int head = job.group * p.pack + in_tile % p.pack;
+  const int64_t row = job.row0 + token;
   if (lane * 4 < p.dim) {
     uint2 t;
     t.x = pack2<T>(acc[0] * inv, acc[1] * inv);
@@ -938,7 +1006,9 @@ extern "C" int64_t vfb_attention_workspace_bytes(const vfb_attention_args *args)
   using namespace vfb;
   if (check_args(args) != VFB_OK) return -1;
   if (args->total_q == 0) return 0;
-  return slots_of(choose(*args)) * kSlotRows * (args->dim + 1) * static_cast<int64_t>(sizeof(float));
+  const int64_t slots = slots_of(choose(*args));
+  return slots * kSlotRows * (args->dim + 1) * static_cast<int64_t>(sizeof(float)) +
+         slots / 2 * static_cast<int64_t>(sizeof(attn::Record));
 }
 
 extern "C" int vfb_attention(const vfb_attention_args *args, void *stream) {
@@ -986,6 +1056,7 @@ extern "C" int vfb_attention(const vfb_attention_args *args, void *stream) {
   if (c.split) {
     p.part_o = static_cast<float *>(a.workspace);
     p.part_lse = p.part_o + slots_of(c) * kSlotRows * a.dim;
+    p.records = reinterpret_cast<attn::Record *>(p.part_lse + slots_of(c) * kSlotRows);
   }
   p.status = device_status_ptr();
 

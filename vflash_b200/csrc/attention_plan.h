@@ -14,8 +14,10 @@
 //   and a second kernel joins them in the order of the blocks.
 //
 // Only totals are known on the host: lengths are device data, so the functions
-// here run on the device, on a whole warp with uniform arguments (the lanes
-// read the sequences side by side).  On the host they run as plain loops.
+// here run on the device, on one whole warp of a block with uniform arguments
+// (the lanes read the sequences side by side).  On the host they run as plain
+// loops.  Places on the line are integers below 2^53: quotients are taken in
+// fp64 and corrected, several times faster than 64-bit integer division.
 #pragma once
 
 #include <stdint.h>
@@ -116,19 +118,20 @@ VFB_HD int64_t snap(int64_t off, int64_t keys) {
 }
 
 // ---- scans over the sequences --------------------------------------------------
-struct JobCount {  // jobs of a sequence
-  VFB_HD int64_t operator()(const Plan &p, const Seq &s) const { return static_cast<int64_t>(s.tiles) * p.groups; }
-};
-struct JobLength {  // length of a sequence's jobs
-  VFB_HD int64_t operator()(const Plan &p, const Seq &s) const { return jobs_length(p, s, s.tiles) * p.groups; }
-};
+// Floor of a / b for 0 <= a < 2^53, b > 0, with the fp64 inverse of b.
+VFB_HD int64_t quotient(int64_t a, int64_t b, double inverse) {
+  int64_t q = static_cast<int64_t>(static_cast<double>(a) * inverse);
+  if (q * b > a) --q;
+  else if ((q + 1) * b <= a) ++q;
+  return q;
+}
+
+VFB_HD int64_t line_length(const Plan &p, const Seq &s) { return jobs_length(p, s, s.tiles) * p.groups; }
 
 #ifdef __CUDA_ARCH__
-template <class F>
-__device__ __forceinline__ int64_t warp_prefix(const Plan &p, F f, int32_t b, int64_t &own) {
+__device__ __forceinline__ int64_t warp_inclusive(int64_t sum) {
   const int lane = threadIdx.x & 31;
-  own = b < num_seqs(p) ? f(p, sequence(p, b)) : 0;
-  int64_t sum = own;
+#pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int64_t t = __shfl_up_sync(0xffffffffu, sum, o);
     if (lane >= o) sum += t;
@@ -137,41 +140,59 @@ __device__ __forceinline__ int64_t warp_prefix(const Plan &p, F f, int32_t b, in
 }
 #endif
 
-// Sum over all sequences.
-template <class F>
-VFB_HD int64_t total(const Plan &p, F f) {
-  int64_t sum = 0;
+struct Totals {
+  int64_t length, jobs;
+};
+
+VFB_HD Totals totals(const Plan &p) {
+  Totals t = {0, 0};
 #ifdef __CUDA_ARCH__
-  for (int32_t b = 0; b < num_seqs(p); b += 32) {
-    int64_t own;
-    const int64_t inclusive = warp_prefix(p, f, b + (threadIdx.x & 31), own);
-    sum += __shfl_sync(0xffffffffu, inclusive, 31);
+  for (int32_t b = threadIdx.x & 31; b < num_seqs(p); b += 32) {
+    const Seq s = sequence(p, b);
+    t.length += line_length(p, s);
+    t.jobs += s.tiles;
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    t.length += __shfl_xor_sync(0xffffffffu, t.length, o);
+    t.jobs += __shfl_xor_sync(0xffffffffu, t.jobs, o);
   }
 #else
-  for (int32_t b = 0; b < num_seqs(p); ++b) sum += f(p, sequence(p, b));
+  for (int32_t b = 0; b < num_seqs(p); ++b) {
+    const Seq s = sequence(p, b);
+    t.length += line_length(p, s);
+    t.jobs += s.tiles;
+  }
 #endif
-  return sum;
+  t.jobs *= p.groups;
+  return t;
 }
 
-// The sequence in which position `x` (0 <= x < total) lies; `x` becomes the
-// position inside it.
-template <class F>
-VFB_HD int32_t locate(const Plan &p, F f, int64_t &x) {
+// The sequence in which position `x` lies on the line (LINE) or in the list of
+// jobs; `x` becomes the position inside it.
+template <bool LINE>
+VFB_HD int32_t locate(const Plan &p, int64_t &x) {
 #ifdef __CUDA_ARCH__
-  for (int32_t b = 0; b < num_seqs(p); b += 32) {
-    int64_t own;
-    const int64_t inclusive = warp_prefix(p, f, b + (threadIdx.x & 31), own);
+  for (int32_t b0 = 0; b0 < num_seqs(p); b0 += 32) {
+    const int32_t b = b0 + (threadIdx.x & 31);
+    int64_t own = 0;
+    if (b < num_seqs(p)) {
+      const Seq s = sequence(p, b);
+      own = LINE ? line_length(p, s) : static_cast<int64_t>(s.tiles) * p.groups;
+    }
+    const int64_t inclusive = warp_inclusive(own);
     const unsigned hit = __ballot_sync(0xffffffffu, x < inclusive);
     if (hit) {
       const int at = __ffs(hit) - 1;
       x -= __shfl_sync(0xffffffffu, inclusive - own, at);
-      return b + at;
+      return b0 + at;
     }
     x -= __shfl_sync(0xffffffffu, inclusive, 31);
   }
 #else
   for (int32_t b = 0; b < num_seqs(p); ++b) {
-    const int64_t own = f(p, sequence(p, b));
+    const Seq s = sequence(p, b);
+    const int64_t own = LINE ? line_length(p, s) : static_cast<int64_t>(s.tiles) * p.groups;
     if (x < own) return b;
     x -= own;
   }
@@ -199,10 +220,10 @@ struct Place {
 VFB_HD Place place_at(const Plan &p, int64_t x) {
   Place a;
   int64_t in = x;
-  a.b = locate(p, JobLength(), in);
+  a.b = locate<true>(p, in);
   a.seq = sequence(p, a.b < 0 ? 0 : a.b);
   const int64_t line = jobs_length(p, a.seq, a.seq.tiles);
-  a.group = static_cast<int32_t>(in / line);
+  a.group = static_cast<int32_t>(quotient(in, line, 1.0 / static_cast<double>(line)));
   in -= a.group * line;
   int32_t lo = 0, hi = a.seq.tiles;  // the last tile that starts at or before `in`
   while (hi - lo > 1) {
@@ -223,7 +244,18 @@ VFB_HD int32_t share_blocks(const Plan &p, int64_t length, int64_t jobs) {
 }
 
 // Cut c of `blocks` on a line of `length` before it is moved.
-VFB_HD int64_t cut(int64_t length, int32_t blocks, int32_t c) { return length / blocks * c + length % blocks * c / blocks; }
+VFB_HD int64_t cut(int64_t length, int32_t blocks, int32_t c) {
+  if (c >= blocks) return length;
+  return static_cast<int64_t>(static_cast<double>(length) * c / blocks);
+}
+
+// Where a block's share begins, for the join: `inside` a job (its earlier part
+// belongs to blocks before), and which one.
+struct Record {
+  int64_t start;    // of the job on the line
+  int64_t row0;     // its first query row
+  int32_t group, count, inside, reserved;
+};
 
 class Order {
  public:
@@ -232,28 +264,31 @@ class Order {
     split_ = false;
     next_ = block;
     step_ = step;
-    end_ = total(p, JobCount());
+    end_ = totals(p).jobs;
   }
 
-  // The share of `block`.  `part` reports whether it is one of the blocks that get a share.
-  VFB_HD bool init_share(const Plan &p, int32_t block) {
+  // The share of `block`; `record` is for the join.
+  VFB_HD void init_share(const Plan &p, int32_t block, Record &record) {
     split_ = true;
-    const int64_t length = total(p, JobLength());
-    const int32_t blocks = share_blocks(p, length, total(p, JobCount()));
+    const Totals t = totals(p);
+    const int32_t blocks = share_blocks(p, t.length, t.jobs);
     next_ = end_ = 0;
     block_ = block;
     first_ = true;
-    if (length == 0 || block >= blocks) return false;
-    at_ = place_at(p, cut(length, blocks, block));
+    record = Record{-1, 0, 0, 0, 0, 0};
+    if (t.length == 0 || block >= blocks) return;
+    at_ = place_at(p, cut(t.length, blocks, block));
     next_ = at_.start + at_.off;
-    if (block + 1 == blocks) {
-      end_ = length;
-    } else {
-      const Place e = place_at(p, cut(length, blocks, block + 1));
+    end_ = t.length;
+    if (block + 1 < blocks) {
+      const Place e = place_at(p, cut(t.length, blocks, block + 1));
       end_ = e.start + e.off;
     }
     if (at_.off == OVERHEAD + at_.keys) advance(p);
-    return true;
+    if (at_.b >= num_seqs(p)) return;
+    const int64_t rows0 = static_cast<int64_t>(at_.tile) * p.job_tokens;
+    record = Record{at_.start, at_.seq.q0 + rows0, at_.group,
+                    static_cast<int32_t>(min64(p.job_tokens, at_.seq.nq - rows0)), at_.off > 0, 0};
   }
 
   VFB_HD bool next(const Plan &p, Segment &s) {
@@ -261,10 +296,11 @@ class Order {
     if (!split_) {
       int64_t in = next_;
       next_ += step_;
-      s.b = locate(p, JobCount(), in);
+      s.b = locate<false>(p, in);
       s.seq = sequence(p, s.b < 0 ? 0 : s.b);
-      s.group = static_cast<int32_t>(in / s.seq.tiles);
-      const int32_t i = static_cast<int32_t>(in - static_cast<int64_t>(s.group) * s.seq.tiles);
+      // jobs are fewer than 2^31
+      s.group = static_cast<int32_t>(static_cast<uint32_t>(in) / static_cast<uint32_t>(s.seq.tiles));
+      const int32_t i = static_cast<int32_t>(in) - s.group * s.seq.tiles;
       s.tile = p.causal ? s.seq.tiles - 1 - i : i;  // causal: the longest first
       s.t0 = 0;
       s.t1 = tiles_of(p, s.seq, s.tile);
@@ -318,40 +354,16 @@ class Order {
 };
 
 // ---- joining the pieces ------------------------------------------------------------
-// Cut c (1 <= c < blocks) is the first one inside its job: the job's pieces are
-// then slot `first` and the slots 2 * c, 2 * (c + 1), ... up to 2 * last.
-struct Join {
-  Place job;
-  int32_t first, c, last;
-};
-
-VFB_HD bool join_at(const Plan &p, int32_t c, Join &j) {
-  const int64_t length = total(p, JobLength());
-  if (length == 0) return false;
-  const int32_t blocks = share_blocks(p, length, total(p, JobCount()));
-  if (c < 1 || c >= blocks) return false;
-  j.job = place_at(p, cut(length, blocks, c));
-  const int64_t job_length = OVERHEAD + j.job.keys;
-  if (j.job.off == 0 || j.job.off == job_length) return false;
-  // cuts of the same job, moved the same way
-  const int64_t before = cut(length, blocks, c - 1) - j.job.start;
-  const int64_t previous = before < 0 ? -1 : snap(before, j.job.keys);
-  if (previous > 0) return false;
-  // the block before starts at this job (no earlier job in its share) or in an earlier one
-  bool starts_here = previous == 0;
-  if (before < 0) {
-    const Place b = place_at(p, cut(length, blocks, c - 1));
-    starts_here = b.start + b.off == j.job.start;  // moved to the end of the job before
-  }
-  j.first = 2 * (c - 1) + (starts_here ? 0 : 1);
-  j.c = c;
-  j.last = c;
-  while (j.last + 1 < blocks) {
-    const int64_t raw = cut(length, blocks, j.last + 1) - j.job.start;
-    if (raw >= job_length || snap(raw, j.job.keys) == job_length) break;
-    ++j.last;
-  }
-  return true;
+// Cut c (1 <= c < blocks) is the first one inside its job when its record says
+// `inside` and the one before does not lie inside the same job.  The job's
+// pieces are then slot join_first() and the slots 2 * c, 2 * (c + 1), ... as long as
+// the records stay inside the same job (a share cut to nothing leaves -inf in
+// its slot).
+VFB_HD bool join_starts(const Record &before, const Record &here) {
+  return here.inside && !(before.inside && before.start == here.start);
+}
+VFB_HD int32_t join_first(const Record &before, const Record &here, int32_t c) {
+  return 2 * (c - 1) + (before.start == here.start ? 0 : 1);
 }
 
 }  // namespace attn
