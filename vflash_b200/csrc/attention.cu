@@ -48,6 +48,8 @@ constexpr int kRingSlots = 10;       // at most
 constexpr int kJobs = 4;             // jobs that the scheduler may be ahead
 constexpr int kJobReaders = 11;      // warps that follow the schedule
 constexpr float kHold = 8.0f;
+constexpr int kFmaPairs = 0;         // of every 8 pairs of exponentials, so many on the FMA pipe
+constexpr int kTail = 32;            // keys of a tile whose P is handed over separately
 constexpr float kLn2 = 0.693147180559945309f;
 
 // Rows of a workspace slot (one piece of a job): both tiles of PAIR.
@@ -140,12 +142,64 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
       : "memory");
 }
 
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
+}
+
+// ---- two floats at a time: half the issue slots --------------------------------
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void split(f32x2 v, float &lo, float &hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 2^x on the FMA pipe, for x <= 126: x = n + f with n its nearest integer (read
+// off the low bits of x + 1.5 * 2^23) and |f| <= 1/2, 2^f by a polynomial of
+// degree 4, n added to its exponent.  The coefficients are those of the
+// minimax approximation of 2^f in relative error over [-1/2, 1/2], fitted
+// numerically (iteratively reweighted least squares); error at most 2.7e-6 in
+// fp32.  Below 2^-126 (and for NaN) it is 0.
+__device__ __forceinline__ void exp2_fma(f32x2 x, float &lo, float &hi) {
+  const f32x2 magic = pair(12582912.0f, 12582912.0f), minus = pair(-12582912.0f, -12582912.0f);
+  const f32x2 t = add2(x, magic);
+  const f32x2 f = fma2(add2(t, minus), pair(-1.0f, -1.0f), x);
+  f32x2 y = fma2(f, pair(0.009570086374878883f, 0.009570086374878883f), pair(0.055917851626873016f, 0.055917851626873016f));
+  y = fma2(y, f, pair(0.240247443318367f, 0.240247443318367f));
+  y = fma2(y, f, pair(0.6931217908859253f, 0.6931217908859253f));
+  y = fma2(y, f, pair(0.9999992847442627f, 0.9999992847442627f));
+  float x0, x1, t0, t1, y0, y1;
+  split(x, x0, x1);
+  split(t, t0, t1);
+  split(y, y0, y1);
+  lo = x0 > -126.0f ? __uint_as_float(__float_as_uint(y0) + (__float_as_uint(t0) << 23)) : 0.0f;
+  hi = x1 > -126.0f ? __uint_as_float(__float_as_uint(y1) + (__float_as_uint(t1) << 23)) : 0.0f;
 }
 
 // Maximum that keeps NaN.
@@ -219,7 +273,7 @@ __device__ __forceinline__ void describe(const Params &p, const Segment &s, Job 
 struct Shared {
   uint64_t q_full, q_empty;
   uint64_t kv_full[kRingSlots], kv_empty[kRingSlots];
-  uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
+  uint64_t s_full[2], p_full[2], p_tail[2], o_full[2], o_empty[2];
   // a V tile to be cleaned is on its way into the slot, and is clean: the MMA
   // warp waits for the latter before the slot is given back, so neither barrier
   // can run ahead of who waits for it
@@ -284,23 +338,32 @@ struct Softmax {
     return warp_wait(bar, phase, &sh.abort, p.status);
   }
 
-  // `limit`: keys this row sees.  `live`: some row of the warp is a row of the job.
-  __device__ __forceinline__ bool run(int32_t t0, int32_t n, int32_t stride, int32_t limit, bool live, int lane) {
+  __device__ __forceinline__ void hand_over(uint64_t *bar) {
+    tc_fence_before();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+  }
+
+  // `limit`: keys this row sees.  `live`: some row of the warp is a row of the job;
+  // `valid`: this one is.
+  __device__ __forceinline__ bool run(int32_t t0, int32_t n, int32_t stride, int32_t limit, bool live, bool valid) {
     m = -INFINITY;
     l = 0.0f;
     for (int32_t i = 0; i < n; ++i) {
       if (!wait(&sh.s_full[stage], s_phase)) return false;
       s_phase ^= 1;
       tc_fence_after();
-      if (live) tile((t0 + i * stride) * attn::KEYS, limit, i > 0);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh.p_full[stage]);
+      if (live) {
+        tile((t0 + i * stride) * attn::KEYS, limit, i > 0, valid);
+      } else {
+        hand_over(&sh.p_full[stage]);
+        hand_over(&sh.p_tail[stage]);
+      }
     }
     return true;
   }
 
-  __device__ __forceinline__ void tile(int32_t key0, int32_t limit, bool scale_o) {
+  __device__ __forceinline__ void tile(int32_t key0, int32_t limit, bool scale_o, bool valid) {
     float s[128];
     {
       uint32_t(&r)[4][32] = reinterpret_cast<uint32_t(&)[4][32]>(s);
@@ -310,7 +373,8 @@ struct Softmax {
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld_fence(r[c]);
     }
-    const int32_t seen = limit - key0;
+    // a row that is not part of the job is left alone: nobody reads its results
+    const int32_t seen = valid ? limit - key0 : attn::KEYS;
     if (__any_sync(0xffffffffu, seen < attn::KEYS)) {
 #pragma unroll
       for (int j = 0; j < 128; ++j)
@@ -326,7 +390,7 @@ struct Softmax {
     top[1] = max3_nan(top[1], s[126], s[127]);
     const float peak = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], m);
     // true also for a NaN score; not while no key has been seen
-    const bool move = !((peak - m) * p.scale_log2 <= kHold) && peak != -INFINITY;
+    const bool move = valid && !((peak - m) * p.scale_log2 <= kHold) && peak != -INFINITY;
     if (__any_sync(0xffffffffu, move)) {
       const float alpha = !move ? 1.0f : m == -INFINITY ? 0.0f : ex2((m - peak) * p.scale_log2);
       if (move) {
@@ -347,22 +411,37 @@ struct Softmax {
       }
     }
     const float base = m == -INFINITY ? 0.0f : m * p.scale_log2;
-    float sum[4] = {};
+    const f32x2 scale2 = pair(p.scale_log2, p.scale_log2), base2 = pair(-base, -base);
+    f32x2 sum[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint32_t packed[32];
+    for (int h = 0; h < 4; ++h) {
+      uint32_t packed[16];
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        const float a = ex2(fmaf(s[64 * h + 2 * j], p.scale_log2, -base));
-        const float b = ex2(fmaf(s[64 * h + 2 * j + 1], p.scale_log2, -base));
-        sum[(2 * j) & 3] += a;
-        sum[(2 * j + 1) & 3] += b;
+      for (int j = 0; j < 16; ++j) {
+        const f32x2 x = fma2(pair(s[32 * h + 2 * j], s[32 * h + 2 * j + 1]), scale2, base2);
+        float a, b;
+        if (j % 8 >= 8 - kFmaPairs) {
+          exp2_fma(x, a, b);
+        } else {
+          split(x, a, b);
+          a = ex2(a);
+          b = ex2(b);
+        }
+        sum[j & 1] = add2(sum[j & 1], pair(a, b));
         packed[j] = pack2<T>(a, b);
       }
-      tmem_st_32x32b_x32(tmem_s + 32 * h, packed);
+      tmem_st_32x32b_x16(tmem_s + 16 * h, packed);
+      if (32 * (h + 1) == attn::KEYS - kTail) {
+        tmem_st_wait();
+        hand_over(&sh.p_full[stage]);
+      }
     }
-    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     tmem_st_wait();
+    hand_over(&sh.p_tail[stage]);
+    float a, b, c, d;
+    split(sum[0], a, b);
+    split(sum[1], c, d);
+    l += (a + b) + (c + d);
   }
 };
 
@@ -397,6 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.s_full[i], 1);
       mbar_init(&sh.p_full[i], 4);
+      mbar_init(&sh.p_tail[i], 4);
       mbar_init(&sh.o_full[i], 1);
       mbar_init(&sh.o_empty[i], 4);
     }
@@ -443,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         limit = static_cast<int32_t>(
             min(max(static_cast<int64_t>(job.rows0) + token + 1 + job.nk - job.nq, int64_t{0}), int64_t{job.nk}));
       const bool live = __any_sync(0xffffffffu, valid);
-      if (!sm.run(PAIR ? job.t0 : job.t0 + stage, job.n[stage], PAIR ? 1 : 2, limit, live, lane)) break;
+      if (!sm.run(PAIR ? job.t0 : job.t0 + stage, job.n[stage], PAIR ? 1 : 2, limit, live, valid)) break;
       float m = sm.m, l = sm.l;
       bool have[2] = {job.n[stage] > 0, false};  // accumulators that hold something for this row
       float f[2] = {1.0f, 0.0f};
@@ -629,7 +709,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t idesc_o = idesc_f16<T>(static_cast<int>(d16) * 16, true);
       const uint32_t q_addr = smem_u32(s_q), kv_addr = smem_u32(s_kv);
       RingPos<L::ring> pos;      // the item that is waited for next
-      uint32_t q_phase = 0, p_phase[2] = {0, 0}, o_phase[2] = {1, 1};
+      constexpr uint32_t kHead = (attn::KEYS - kTail) / 16;  // steps of K in P V before the tail
+      uint32_t q_phase = 0, p_phase[2] = {0, 0}, t_phase[2] = {0, 0}, o_phase[2] = {1, 1};
       uint32_t v_phase = 0;  // a bit for every slot
       bool ok = true;
       const auto wait = [&](uint64_t *bar, uint32_t phase) {
@@ -651,11 +732,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
       };
-      const auto product_o = [&](int stage, int slot, bool accumulate) {  // O (+)= P V
+      const auto product_o = [&](int stage, int slot, bool accumulate, uint32_t from, uint32_t to) {  // O (+)= P V
         if (leader) {
           const uint32_t b = kv_addr + slot * L::tile_bytes;
 #pragma unroll
-          for (uint32_t k = 0; k < attn::KEYS / 16; ++k)
+          for (uint32_t k = from; k < to; ++k)
             mma_f16_tmem_a(tmem + 256 + 128 * stage, tmem + 128 * stage + 8 * k, sw128_mnmajor_desc(b + k * 2048),
                            idesc_o, accumulate || k > 0);
         }
@@ -691,7 +772,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                   o_phase[s] ^= 1;
                 }
                 tc_fence_after();
-                product_o(s, v_slot, j > 1);
+                product_o(s, v_slot, j > 1, 0, kHead);
+                if (!wait(&sh.p_tail[s], t_phase[s])) break;
+                t_phase[s] ^= 1;
+                tc_fence_after();
+                product_o(s, v_slot, true, kHead, attn::KEYS / 16);
                 if (j == job.n[s]) commit(&sh.o_full[s]);
               }
               if (j < job.n[s]) {
@@ -729,7 +814,11 @@ __global__ void __launch_bounds__(kThreads, 1)
               o_phase[s] ^= 1;
             }
             tc_fence_after();
-            product_o(s, pos.slot, i > 1);
+            product_o(s, pos.slot, i > 1, 0, kHead);
+            if (!wait(&sh.p_tail[s], t_phase[s])) break;
+            t_phase[s] ^= 1;
+            tc_fence_after();
+            product_o(s, pos.slot, true, kHead, attn::KEYS / 16);
             commit(&sh.kv_empty[pos.slot]);
             pos.step();
             if (i + 2 >= tiles) commit(&sh.o_full[s]);
@@ -752,27 +841,30 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint8_t *tile = s_kv + slot * L::tile_bytes;
         const int32_t end = min(max(job.nk - t * attn::KEYS, 0), attn::KEYS);       // rows of the sequence
         const int32_t all = min(max(job.min_seen - t * attn::KEYS, 0), attn::KEYS);       // rows that every row sees
-        for (int i = lane; i < (attn::KEYS - all) * 8 * L::panels; i += 32) {
-          const int panel = i / ((attn::KEYS - all) * 8);
-          const int rest = i - panel * (attn::KEYS - all) * 8;
-          uint4 *at = reinterpret_cast<uint4 *>(tile + panel * kPanelBytes + all * 128) + rest;
-          if (all + rest / 8 >= end) {
-            *at = make_uint4(0, 0, 0, 0);
-            continue;
-          }
-          uint4 x = *at;
-          uint32_t *word = reinterpret_cast<uint32_t *>(&x);
-          uint32_t bad = 0;
+        // lanes: eight 16-byte pieces of four rows
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t hit = __vcmpeq2(word[j] & exponent_mask<T>(), exponent_mask<T>());
-            word[j] &= ~hit;
-            bad |= hit;
+        for (int panel = 0; panel < L::panels; ++panel) {
+          uint8_t *column = tile + panel * kPanelBytes + lane % 8 * 16;
+#pragma unroll 4
+          for (int r = all + lane / 8; r < end; r += 4) {
+            uint4 *at = reinterpret_cast<uint4 *>(column + r * 128);
+            uint4 x = *at;
+            uint32_t *word = reinterpret_cast<uint32_t *>(&x);
+            uint32_t bad = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t hit = __vcmpeq2(word[j] & exponent_mask<T>(), exponent_mask<T>());
+              word[j] &= ~hit;
+              bad |= hit;
+            }
+            if (bad) {
+              *at = x;
+              *reinterpret_cast<volatile int *>(&sh.dirty) = 1;
+            }
           }
-          if (bad) {
-            *at = x;
-            *reinterpret_cast<volatile int *>(&sh.dirty) = 1;
-          }
+#pragma unroll 4
+          for (int r = end + lane / 8; r < attn::KEYS; r += 4)
+            *reinterpret_cast<uint4 *>(column + r * 128) = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
         __threadfence_block();
@@ -977,7 +1069,7 @@ int launch(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, con
   int rc = ensure_smem_optin(reinterpret_cast<const void *>(kernel), L::smem, smem_set);
   if (rc != VFB_OK) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.split ? p.plan.blocks : jobs), 1, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(p.split ? p.plan.blocks : attn::min64(jobs, sms)), 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
   cfg.dynamicSmemBytes = L::smem;
   cfg.stream = stream;

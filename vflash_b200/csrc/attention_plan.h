@@ -264,7 +264,7 @@ class Order {
     split_ = false;
     next_ = block;
     step_ = step;
-    end_ = totals(p).jobs;
+    end_ = INT64_MAX;
   }
 
   // The share of `block`; `record` is for the join.
@@ -297,7 +297,8 @@ class Order {
       int64_t in = next_;
       next_ += step_;
       s.b = locate<false>(p, in);
-      s.seq = sequence(p, s.b < 0 ? 0 : s.b);
+      if (s.b < 0) return false;
+      s.seq = sequence(p, s.b);
       // jobs are fewer than 2^31
       s.group = static_cast<int32_t>(static_cast<uint32_t>(in) / static_cast<uint32_t>(s.seq.tiles));
       const int32_t i = static_cast<int32_t>(in) - s.group * s.seq.tiles;
