@@ -1,7 +1,7 @@
 // Attention over packed sequences (vfb_attention) on tcgen05.
 //
 // For one tile of 128 query rows (the group's heads of as many tokens as fit,
-// row = token * pack + head in group) and the keys it sees, 128 at a time:
+// row = token * pack + head in group) and the keys it sees, 64 at a time:
 //   S = Q K^T            tcgen05, fp32 in TMEM
 //   m' = max(m, row max) P = exp2((S - m') * scale * log2 e)   registers
 //   l = l * 2^(m - m') + row sum of P
@@ -23,9 +23,15 @@
 //   ALT:  one tile of query rows against even and odd key tiles, joined at the
 //         end (few query rows: single tokens, short pieces).
 //
-// TMEM (512 columns): S0 | S1 | O0 | O1, 128 columns each; P overwrites the
-// first 64 columns of its S.  tcgen05 operations of one thread run in order,
-// so S(j+1) may be issued behind the P V(j) that still reads P.
+// TMEM (512 columns): S of stage 0 (two buffers of 64) | S of stage 1 | O0 | O1,
+// 128 columns each; P overwrites the first 32 columns of its S.  With two
+// buffers the scores of a stage's next tile are there before the softmax of
+// this one ends.  Key tiles of 64 are what makes room for that next to two
+// 128-column O: the product Q K^T then takes 48 instead of 32 cycles a step
+// (its operands are read from shared memory at 128 bytes a cycle), but tiles of
+// 128 keys with one buffer leave the chain S -> softmax -> P V -> next S exposed
+// (measured: 3150 cycles for 128 keys of both stages, of which 2050 are
+// products; with two buffers of 64 the products' 2520 are the bound).
 //
 // Keys behind a row's limit: their scores become -inf, so P = 0; but 0 * inf
 // and 0 * NaN would still spoil the second product.  Warp 10 therefore
@@ -41,15 +47,15 @@ namespace {
 using attn::Plan;
 using attn::Segment;
 
-constexpr int kTile = 128;           // query rows in a tile, and keys in a key tile
-constexpr int kPanelBytes = 16384;   // 128 rows x 64 elements of 16 bits, 128-byte swizzle
+constexpr int kTile = 128;           // query rows in a tile
+constexpr int kQPanel = kTile * 128;       // bytes of a tile's 64 elements of 16 bits, 128-byte swizzle
+constexpr int kKvPanel = attn::KEYS * 128;
 constexpr int kThreads = 384;
-constexpr int kRingSlots = 10;       // at most
-constexpr int kJobs = 4;             // jobs that the scheduler may be ahead
+constexpr int kRingSlots = 16;       // at most
+constexpr int kJobs = 2;             // jobs that the scheduler may be ahead
 constexpr int kJobReaders = 11;      // warps that follow the schedule
 constexpr float kHold = 8.0f;
 constexpr int kFmaPairs = 0;         // of every 8 pairs of exponentials, so many on the FMA pipe
-constexpr int kTail = 32;            // keys of a tile whose P is handed over separately
 constexpr float kLn2 = 0.693147180559945309f;
 
 // Rows of a workspace slot (one piece of a job): both tiles of PAIR.
@@ -58,10 +64,12 @@ constexpr int kSlotRows = 2 * kTile;
 template <int DP, bool PAIR>
 struct Layout {
   static constexpr int panels = DP / 64;
-  static constexpr int tile_bytes = panels * kPanelBytes;
-  static constexpr int q_bytes = (PAIR ? 2 : 1) * tile_bytes;
-  static constexpr int ring = DP == 128 ? (PAIR ? 5 : 6) : (PAIR ? 8 : 10);
-  static constexpr int smem = 1024 + q_bytes + ring * tile_bytes;  // tiles start on 1024 bytes
+  static constexpr int q_tile = panels * kQPanel;
+  static constexpr int kv_tile = panels * kKvPanel;
+  static constexpr int q_bytes = (PAIR ? 2 : 1) * q_tile;
+  static constexpr int ring = DP == 128 ? (PAIR ? 10 : 12) : 16;
+  static constexpr int ahead = PAIR ? 2 : 4;  // key tiles whose S is issued before the first P V
+  static constexpr int smem = 1024 + q_bytes + ring * kv_tile;  // tiles start on 1024 bytes
 };
 
 struct Params {
@@ -116,7 +124,7 @@ __device__ __forceinline__ void mma_f16_tmem_a(uint32_t d, uint32_t a, uint64_t 
 __device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t smem_addr) {
   uint64_t desc = 0;
   desc |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
-  desc |= static_cast<uint64_t>(kPanelBytes >> 4) << 16;  // leading offset: next 64 elements of N
+  desc |= static_cast<uint64_t>(kKvPanel >> 4) << 16;  // leading offset: next 64 elements of N
   desc |= static_cast<uint64_t>(1024 >> 4) << 32;         // stride offset: next eight rows of K
   desc |= static_cast<uint64_t>(1) << 46;
   desc |= static_cast<uint64_t>(2) << 61;
@@ -273,7 +281,7 @@ __device__ __forceinline__ void describe(const Params &p, const Segment &s, Job 
 struct Shared {
   uint64_t q_full, q_empty;
   uint64_t kv_full[kRingSlots], kv_empty[kRingSlots];
-  uint64_t s_full[2], p_full[2], p_tail[2], o_full[2], o_empty[2];
+  uint64_t s_full[2][2], p_full[2][2], pv_done[2], o_full[2], o_empty[2];
   // a V tile to be cleaned is on its way into the slot, and is clean: the MMA
   // warp waits for the latter before the slot is given back, so neither barrier
   // can run ahead of who waits for it
@@ -298,7 +306,7 @@ struct JobReader {
 
   // The next job; false when there is none (or a wait ran out).
   __device__ __forceinline__ bool next(Job &j) {
-    if (!warp_wait(&sh.job_full[slot], phase, &sh.abort, status)) return false;
+    if (!warp_wait_quick(&sh.job_full[slot], phase, &sh.abort, status)) return false;
     j = sh.jobs[slot];
     __syncwarp();
     if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.job_empty[slot]);
@@ -324,24 +332,18 @@ struct RingPos {
 };
 
 // ---- softmax of one stage ----------------------------------------------------------
-// Row state, and the loop over a segment's key tiles.
+// Row state, and the loop over a job's key tiles.
 template <typename T, int DP, bool PAIR>
 struct Softmax {
   const Params &p;
   Shared &sh;
   const uint32_t tmem_s, tmem_o;  // this warp's lanes
   const int stage;
-  float m, l;          // running maximum (raw scores, as used) and sum
-  uint32_t s_phase = 0;
+  float m, l;            // running maximum (raw scores, as used) and sum
+  uint32_t count = 0;    // key tiles of this stage so far, over all jobs
 
   __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t phase) {
-    return warp_wait(bar, phase, &sh.abort, p.status);
-  }
-
-  __device__ __forceinline__ void hand_over(uint64_t *bar) {
-    tc_fence_before();
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+    return warp_wait_quick(bar, phase, &sh.abort, p.status);
   }
 
   // `limit`: keys this row sees.  `live`: some row of the warp is a row of the job;
@@ -349,46 +351,44 @@ struct Softmax {
   __device__ __forceinline__ bool run(int32_t t0, int32_t n, int32_t stride, int32_t limit, bool live, bool valid) {
     m = -INFINITY;
     l = 0.0f;
-    for (int32_t i = 0; i < n; ++i) {
-      if (!wait(&sh.s_full[stage], s_phase)) return false;
-      s_phase ^= 1;
+    for (int32_t i = 0; i < n; ++i, ++count) {
+      if (!wait(&sh.s_full[stage][count & 1], count >> 1 & 1)) return false;
       tc_fence_after();
-      if (live) {
-        tile((t0 + i * stride) * attn::KEYS, limit, i > 0, valid);
-      } else {
-        hand_over(&sh.p_full[stage]);
-        hand_over(&sh.p_tail[stage]);
-      }
+      if (live && !tile((t0 + i * stride) * attn::KEYS, limit, i > 0, valid)) return false;
+      tc_fence_before();
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.p_full[stage][count & 1]);
     }
     return true;
   }
 
-  __device__ __forceinline__ void tile(int32_t key0, int32_t limit, bool scale_o, bool valid) {
-    float s[128];
+  __device__ __forceinline__ bool tile(int32_t key0, int32_t limit, bool scale_o, bool valid) {
+    const uint32_t at = tmem_s + attn::KEYS * (count & 1);
+    float s[64];
     {
-      uint32_t(&r)[4][32] = reinterpret_cast<uint32_t(&)[4][32]>(s);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32_issue(tmem_s + 32 * c, r[c]);
+      uint32_t(&r)[2][32] = reinterpret_cast<uint32_t(&)[2][32]>(s);
+      tmem_ld_32x32b_x32_issue(at, r[0]);
+      tmem_ld_32x32b_x32_issue(at + 32, r[1]);
       tmem_ld_wait();
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_fence(r[c]);
+      tmem_ld_fence(r[0]);
+      tmem_ld_fence(r[1]);
     }
     // a row that is not part of the job is left alone: nobody reads its results
     const int32_t seen = valid ? limit - key0 : attn::KEYS;
     if (__any_sync(0xffffffffu, seen < attn::KEYS)) {
 #pragma unroll
-      for (int j = 0; j < 128; ++j)
+      for (int j = 0; j < 64; ++j)
         if (j >= seen) s[j] = -INFINITY;
     }
-    float top[4] = {s[0], s[1], s[2], s[3]};
+    float top[4] = {m, s[0], s[1], s[2]};
 #pragma unroll
-    for (int j = 4; j < 124; j += 8) {
+    for (int j = 3; j < 59; j += 8) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) top[i] = max3_nan(top[i], s[j + 2 * i], s[j + 2 * i + 1]);
     }
-    top[0] = max3_nan(top[0], s[124], s[125]);
-    top[1] = max3_nan(top[1], s[126], s[127]);
-    const float peak = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], m);
+    top[0] = max3_nan(top[0], s[59], s[60]);
+    top[1] = max3_nan(top[1], s[61], s[62]);
+    const float peak = max3_nan(max3_nan(top[0], top[1], s[63]), top[2], top[3]);
     // true also for a NaN score; not while no key has been seen
     const bool move = valid && !((peak - m) * p.scale_log2 <= kHold) && peak != -INFINITY;
     if (__any_sync(0xffffffffu, move)) {
@@ -398,6 +398,9 @@ struct Softmax {
         l *= alpha;
       }
       if (scale_o) {
+        // The last P V is behind S(count - 2) of its buffer, so at most one phase of pv_done is open here.
+        if (!wait(&sh.pv_done[stage], (count - 1) & 1)) return false;
+        tc_fence_after();
 #pragma unroll 1
         for (int c = 0; c < DP; c += 32) {
           uint32_t r[32];
@@ -413,35 +416,28 @@ struct Softmax {
     const float base = m == -INFINITY ? 0.0f : m * p.scale_log2;
     const f32x2 scale2 = pair(p.scale_log2, p.scale_log2), base2 = pair(-base, -base);
     f32x2 sum[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
+    uint32_t packed[32];
 #pragma unroll
-    for (int h = 0; h < 4; ++h) {
-      uint32_t packed[16];
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const f32x2 x = fma2(pair(s[32 * h + 2 * j], s[32 * h + 2 * j + 1]), scale2, base2);
-        float a, b;
-        if (j % 8 >= 8 - kFmaPairs) {
-          exp2_fma(x, a, b);
-        } else {
-          split(x, a, b);
-          a = ex2(a);
-          b = ex2(b);
-        }
-        sum[j & 1] = add2(sum[j & 1], pair(a, b));
-        packed[j] = pack2<T>(a, b);
+    for (int j = 0; j < 32; ++j) {
+      const f32x2 x = fma2(pair(s[2 * j], s[2 * j + 1]), scale2, base2);
+      float a, b;
+      if (j % 8 >= 8 - kFmaPairs) {
+        exp2_fma(x, a, b);
+      } else {
+        split(x, a, b);
+        a = ex2(a);
+        b = ex2(b);
       }
-      tmem_st_32x32b_x16(tmem_s + 16 * h, packed);
-      if (32 * (h + 1) == attn::KEYS - kTail) {
-        tmem_st_wait();
-        hand_over(&sh.p_full[stage]);
-      }
+      sum[j & 1] = add2(sum[j & 1], pair(a, b));
+      packed[j] = pack2<T>(a, b);
     }
-    tmem_st_wait();
-    hand_over(&sh.p_tail[stage]);
+    tmem_st_32x32b_x32(at, packed);
     float a, b, c, d;
     split(sum[0], a, b);
     split(sum[1], c, d);
     l += (a + b) + (c + d);
+    tmem_st_wait();
+    return true;
   }
 };
 
@@ -474,9 +470,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&sh.job_empty[i], kJobReaders);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&sh.s_full[i], 1);
-      mbar_init(&sh.p_full[i], 4);
-      mbar_init(&sh.p_tail[i], 4);
+      mbar_init(&sh.s_full[i][0], 1);
+      mbar_init(&sh.s_full[i][1], 1);
+      mbar_init(&sh.p_full[i][0], 4);
+      mbar_init(&sh.p_full[i][1], 4);
+      mbar_init(&sh.pv_done[i], 1);
       mbar_init(&sh.o_full[i], 1);
       mbar_init(&sh.o_empty[i], 4);
     }
@@ -529,20 +527,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       float f[2] = {1.0f, 0.0f};
       if (PAIR) {
         if (have[0]) {
-          if (!warp_wait(&sh.o_full[stage], o_phase[stage], &sh.abort, p.status)) break;
+          if (!warp_wait_quick(&sh.o_full[stage], o_phase[stage], &sh.abort, p.status)) break;
           o_phase[stage] ^= 1;
         }
       } else {
         // stage 1 hands its statistics over; stage 0 joins the two accumulators
         if (stage == 1) {
-          if (!warp_wait(&sh.stats_empty, stats_phase ^ 1, &sh.abort, p.status)) break;
+          if (!warp_wait_quick(&sh.stats_empty, stats_phase ^ 1, &sh.abort, p.status)) break;
           sh.stats[row] = make_float2(m, l);
           __syncwarp();
           if (lane == 0) mbar_arrive(&sh.stats_full);
           stats_phase ^= 1;
           continue;
         }
-        if (!warp_wait(&sh.stats_full, stats_phase, &sh.abort, p.status)) break;
+        if (!warp_wait_quick(&sh.stats_full, stats_phase, &sh.abort, p.status)) break;
         stats_phase ^= 1;
         const float2 other = sh.stats[row];
         __syncwarp();
@@ -550,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         for (int i = 0; i < 2; ++i) {
           if (job.n[i] == 0) continue;
-          ok = ok && warp_wait(&sh.o_full[i], o_phase[i], &sh.abort, p.status);
+          ok = ok && warp_wait_quick(&sh.o_full[i], o_phase[i], &sh.abort, p.status);
           o_phase[i] ^= 1;
         }
         if (!ok) break;
@@ -653,11 +651,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t issued = 0;  // slots that were ever loaded
       const bool leader = elect_one();
       const auto load = [&](const CUtensorMap *map, int32_t kv_head, int64_t key, bool masked) {
-        ok = ok && warp_wait(&sh.kv_empty[pos.slot], pos.phase ^ 1, &sh.abort, p.status);
+        ok = ok && warp_wait_quick(&sh.kv_empty[pos.slot], pos.phase ^ 1, &sh.abort, p.status);
         if (ok && leader) {
-          mbar_arrive_expect_tx(&sh.kv_full[pos.slot], L::tile_bytes);
+          mbar_arrive_expect_tx(&sh.kv_full[pos.slot], L::kv_tile);
           for (int i = 0; i < L::panels; ++i)
-            tma_load_3d(s_kv + pos.slot * L::tile_bytes + i * kPanelBytes, map, &sh.kv_full[pos.slot], 64 * i,
+            tma_load_3d(s_kv + pos.slot * L::kv_tile + i * kKvPanel, map, &sh.kv_full[pos.slot], 64 * i,
                         kv_head, static_cast<int32_t>(key));
           if (masked) mbar_arrive(&sh.v_todo[pos.slot]);
         }
@@ -668,77 +666,91 @@ __global__ void __launch_bounds__(kThreads, 1)
       while (ok && jobs.next(job)) {
         const int32_t tiles = job.tiles(PAIR);
         if (tiles == 0) continue;
-        if (!warp_wait(&sh.q_empty, q_phase ^ 1, &sh.abort, p.status)) break;
+        if (!warp_wait_quick(&sh.q_empty, q_phase ^ 1, &sh.abort, p.status)) break;
         const int used = PAIR && job.count > p.tokens ? 2 : 1;
         if (leader) {
           mbar_arrive_expect_tx(&sh.q_full, used * L::panels * p.pack * p.tokens * 128);
           for (int t = 0; t < used; ++t)
             for (int i = 0; i < L::panels; ++i)
-              tma_load_3d(s_q + t * L::tile_bytes + i * kPanelBytes, &map_q, &sh.q_full, 64 * i, job.group * p.pack,
+              tma_load_3d(s_q + t * L::q_tile + i * kQPanel, &map_q, &sh.q_full, 64 * i, job.group * p.pack,
                           static_cast<int32_t>(job.row0 + t * p.tokens));
         }
         q_loaded = true;
         q_phase ^= 1;
         const int32_t kv_head = job.group * p.pack / p.group_heads;
         const int64_t k0 = job.k0 + static_cast<int64_t>(job.t0) * attn::KEYS;
-        if (PAIR) {
-          for (int32_t i = 0; i < tiles && ok; ++i) {
-            load(&map_k, kv_head, k0 + static_cast<int64_t>(i) * attn::KEYS, false);
-            load(&map_v, kv_head, k0 + static_cast<int64_t>(i) * attn::KEYS, job.t0 + i >= job.first_masked);
-          }
-        } else {
-          load(&map_k, kv_head, k0, false);
-          if (tiles > 1) load(&map_k, kv_head, k0 + attn::KEYS, false);
-          for (int32_t i = 0; i < tiles && ok; ++i) {
-            load(&map_v, kv_head, k0 + static_cast<int64_t>(i) * attn::KEYS, job.t0 + i >= job.first_masked);
-            if (i + 2 < tiles) load(&map_k, kv_head, k0 + static_cast<int64_t>(i + 2) * attn::KEYS, false);
-          }
+        for (int32_t i = 0; i < min(tiles, L::ahead); ++i)
+          load(&map_k, kv_head, k0 + static_cast<int64_t>(i) * attn::KEYS, false);
+        for (int32_t i = 0; i < tiles && ok; ++i) {
+          load(&map_v, kv_head, k0 + static_cast<int64_t>(i) * attn::KEYS, job.t0 + i >= job.first_masked);
+          if (i + L::ahead < tiles)
+            load(&map_k, kv_head, k0 + static_cast<int64_t>(i + L::ahead) * attn::KEYS, false);
         }
       }
       // every load has landed before the block ends (a finished run waits for nothing here)
-      if (q_loaded) warp_wait(&sh.q_full, q_phase ^ 1, &sh.abort, p.status);
+      if (q_loaded) warp_wait_quick(&sh.q_full, q_phase ^ 1, &sh.abort, p.status);
       for (int i = 0; i < L::ring; ++i) {
         const uint32_t last = i < pos.slot ? pos.phase : pos.phase ^ 1;
-        if (issued >> i & 1) warp_wait(&sh.kv_full[i], last, &sh.abort, p.status);
+        if (issued >> i & 1) warp_wait_quick(&sh.kv_full[i], last, &sh.abort, p.status);
       }
     } else if (warp == 9) {
       // ---------------- MMA issue ----------------
       const bool leader = elect_one();
-      const uint32_t d16 = static_cast<uint32_t>((p.dim + 15) / 16);  // steps of K in Q K^T
+      // All of TMEM is this block's, so it starts at column 0; constants and loop
+      // counters keep the operands of the products warp-uniform.  Products run
+      // over the padded head dimension: TMA filled the rest with zeros.
       const uint32_t idesc_s = idesc_f16<T>(attn::KEYS, false);
-      const uint32_t idesc_o = idesc_f16<T>(static_cast<int>(d16) * 16, true);
-      const uint32_t q_addr = smem_u32(s_q), kv_addr = smem_u32(s_kv);
+      const uint32_t idesc_o = idesc_f16<T>((p.dim + 15) / 16 * 16, true);
+      const uint64_t q_desc = sw128_kmajor_desc(smem_u32(s_q));
+      const uint64_t k_desc = sw128_kmajor_desc(smem_u32(s_kv)), v_desc = sw128_mnmajor_desc(smem_u32(s_kv));
       RingPos<L::ring> pos;      // the item that is waited for next
-      constexpr uint32_t kHead = (attn::KEYS - kTail) / 16;  // steps of K in P V before the tail
-      uint32_t q_phase = 0, p_phase[2] = {0, 0}, t_phase[2] = {0, 0}, o_phase[2] = {1, 1};
+      uint32_t q_phase = 0, o_phase[2] = {1, 1};
+      uint32_t issued[2] = {0, 0}, joined[2] = {0, 0};  // S and P V of each stage so far, over all jobs
       uint32_t v_phase = 0;  // a bit for every slot
       bool ok = true;
       const auto wait = [&](uint64_t *bar, uint32_t phase) {
-        ok = ok && warp_wait(bar, phase, &sh.abort, p.status);
+        ok = ok && warp_wait_quick(bar, phase, &sh.abort, p.status);
         return ok;
       };
       const auto commit = [&](uint64_t *bar) {
         if (leader) tc_commit(bar);
         __syncwarp();
       };
-      const auto product_s = [&](int stage, int slot) {  // S = Q K^T
+      // `done`: a barrier that the products up to this one complete (or NULL)
+      const auto product_s = [&](int stage, int slot, uint64_t *done, uint64_t *done_too) {  // S = Q K^T
+        const uint64_t a = q_desc + (PAIR ? stage * (L::q_tile >> 4) : 0);
+        const uint64_t b = k_desc + slot * (L::kv_tile >> 4);
+        const uint32_t buffer = issued[stage]++ & 1;
+        const uint32_t d = 128 * stage + attn::KEYS * buffer;
         if (leader) {
-          const uint32_t a = q_addr + (PAIR ? stage * L::tile_bytes : 0);
-          const uint32_t b = kv_addr + slot * L::tile_bytes;
-          for (uint32_t k = 0; k < d16; ++k) {
-            const uint32_t at = (k / 4) * kPanelBytes + (k % 4) * 32;
-            mma_f16(tmem + 128 * stage, sw128_kmajor_desc(a + at), sw128_kmajor_desc(b + at), idesc_s, k > 0);
-          }
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k)
+            mma_f16(d, a + ((k / 4 * kQPanel + k % 4 * 32) >> 4), b + ((k / 4 * kKvPanel + k % 4 * 32) >> 4), idesc_s,
+                    k > 0);
+          tc_commit(&sh.s_full[stage][buffer]);
+          if (done != nullptr) tc_commit(done);
+          if (done_too != nullptr) tc_commit(done_too);
         }
         __syncwarp();
       };
-      const auto product_o = [&](int stage, int slot, bool accumulate, uint32_t from, uint32_t to) {  // O (+)= P V
+      const auto product_o = [&](int stage, int slot, bool first, bool last, uint64_t *done) {  // O (+)= P V
+        const uint32_t buffer = joined[stage] & 1;
+        if (!wait(&sh.p_full[stage][buffer], joined[stage] >> 1 & 1)) return;
+        if (first) {
+          if (!wait(&sh.o_empty[stage], o_phase[stage])) return;
+          o_phase[stage] ^= 1;
+        }
+        ++joined[stage];
+        tc_fence_after();
+        const uint64_t b = v_desc + slot * (L::kv_tile >> 4);
+        const uint32_t a = 128 * stage + attn::KEYS * buffer, d = 256 + 128 * stage;
         if (leader) {
-          const uint32_t b = kv_addr + slot * L::tile_bytes;
 #pragma unroll
-          for (uint32_t k = from; k < to; ++k)
-            mma_f16_tmem_a(tmem + 256 + 128 * stage, tmem + 128 * stage + 8 * k, sw128_mnmajor_desc(b + k * 2048),
-                           idesc_o, accumulate || k > 0);
+          for (int k = 0; k < attn::KEYS / 16; ++k)
+            mma_f16_tmem_a(d, a + 8 * k, b + (k * 2048 >> 4), idesc_o, k > 0 || !first);
+          tc_commit(&sh.pv_done[stage]);
+          if (last) tc_commit(&sh.o_full[stage]);
+          if (done != nullptr) tc_commit(done);
         }
         __syncwarp();
       };
@@ -747,104 +759,69 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (tiles == 0) continue;
         if (!wait(&sh.q_full, q_phase)) break;
         q_phase ^= 1;
-        if (PAIR) {
-          for (int32_t j = 0; j <= tiles && ok; ++j) {
-            const int v_slot = pos.slot;
-            if (j > 0) {
-              if (!wait(&sh.kv_full[pos.slot], pos.phase)) break;
-              pos.step();
-              if (job.t0 + j - 1 >= job.first_masked) {
-                if (!wait(&sh.v_clean[v_slot], v_phase >> v_slot & 1)) break;
-                v_phase ^= 1u << v_slot;
-              }
-            }
-            const int k_slot = pos.slot;
-            if (j < tiles) {
-              if (!wait(&sh.kv_full[pos.slot], pos.phase)) break;
-              pos.step();
-            }
-            for (int s = 0; s < 2 && ok; ++s) {
-              if (j > 0 && j <= job.n[s]) {
-                if (!wait(&sh.p_full[s], p_phase[s])) break;
-                p_phase[s] ^= 1;
-                if (j == 1) {
-                  if (!wait(&sh.o_empty[s], o_phase[s])) break;
-                  o_phase[s] ^= 1;
-                }
-                tc_fence_after();
-                product_o(s, v_slot, j > 1, 0, kHead);
-                if (!wait(&sh.p_tail[s], t_phase[s])) break;
-                t_phase[s] ^= 1;
-                tc_fence_after();
-                product_o(s, v_slot, true, kHead, attn::KEYS / 16);
-                if (j == job.n[s]) commit(&sh.o_full[s]);
-              }
-              if (j < job.n[s]) {
-                product_s(s, k_slot);
-                commit(&sh.s_full[s]);
-              }
-            }
-            if (!ok) break;
-            if (j > 0) commit(&sh.kv_empty[v_slot]);
-            if (j < tiles) commit(&sh.kv_empty[k_slot]);
-            if (j == tiles - 1) commit(&sh.q_empty);
+        // S of key tile i: of both stages (as far as they see it), or of the tile's stage
+        const auto scores = [&](int32_t i) {
+          const int slot = pos.slot;
+          if (!wait(&sh.kv_full[slot], pos.phase)) return;
+          pos.step();
+          uint64_t *q_done = i == tiles - 1 ? &sh.q_empty : nullptr;
+          if (PAIR) {
+            const bool both = i < job.n[0] && i < job.n[1];
+            if (i < job.n[0]) product_s(0, slot, both ? nullptr : &sh.kv_empty[slot], both ? nullptr : q_done);
+            if (i < job.n[1]) product_s(1, slot, &sh.kv_empty[slot], q_done);
+          } else {
+            product_s(i & 1, slot, &sh.kv_empty[slot], q_done);
           }
-        } else {
-          const auto scores = [&](int32_t i) {
-            if (!wait(&sh.kv_full[pos.slot], pos.phase)) return;
-            product_s(i & 1, pos.slot);
-            commit(&sh.s_full[i & 1]);
-            commit(&sh.kv_empty[pos.slot]);
-            pos.step();
-            if (i == tiles - 1) commit(&sh.q_empty);
-          };
-          scores(0);
-          if (ok && tiles > 1) scores(1);
-          for (int32_t i = 0; i < tiles && ok; ++i) {
-            const int s = i & 1;
-            if (!wait(&sh.kv_full[pos.slot], pos.phase)) break;
-            if (job.t0 + i >= job.first_masked) {
-              if (!wait(&sh.v_clean[pos.slot], v_phase >> pos.slot & 1)) break;
-              v_phase ^= 1u << pos.slot;
+        };
+        for (int32_t i = 0; i < min(tiles, L::ahead) && ok; ++i) scores(i);
+        for (int32_t i = 0; i < tiles && ok; ++i) {
+          const int v_slot = pos.slot;
+          if (!wait(&sh.kv_full[v_slot], pos.phase)) break;
+          pos.step();
+          if (job.t0 + i >= job.first_masked) {
+            if (!wait(&sh.v_clean[v_slot], v_phase >> v_slot & 1)) break;
+            v_phase ^= 1u << v_slot;
+          }
+          uint64_t *v_done = &sh.kv_empty[v_slot];
+          if (PAIR) {
+            // S of the next tile but one follows the P V that frees its buffer
+            const int32_t next = i + L::ahead;
+            const int k_slot = pos.slot;
+            uint64_t *k_done = &sh.kv_empty[k_slot], *q_done = next == tiles - 1 ? &sh.q_empty : nullptr;
+            if (next < tiles) {
+              if (!wait(&sh.kv_full[k_slot], pos.phase)) break;
+              pos.step();
             }
-            if (!wait(&sh.p_full[s], p_phase[s])) break;
-            p_phase[s] ^= 1;
-            if (i < 2) {
-              if (!wait(&sh.o_empty[s], o_phase[s])) break;
-              o_phase[s] ^= 1;
-            }
-            tc_fence_after();
-            product_o(s, pos.slot, i > 1, 0, kHead);
-            if (!wait(&sh.p_tail[s], t_phase[s])) break;
-            t_phase[s] ^= 1;
-            tc_fence_after();
-            product_o(s, pos.slot, true, kHead, attn::KEYS / 16);
-            commit(&sh.kv_empty[pos.slot]);
-            pos.step();
-            if (i + 2 >= tiles) commit(&sh.o_full[s]);
-            if (i + 2 < tiles) scores(i + 2);
+            const bool v1 = i < job.n[1], k1 = next < job.n[1];  // stage 1 comes last where it has the tile
+            if (i < job.n[0]) product_o(0, v_slot, i == 0, i == job.n[0] - 1, v1 ? nullptr : v_done);
+            if (ok && next < job.n[0]) product_s(0, k_slot, k1 ? nullptr : k_done, k1 ? nullptr : q_done);
+            if (ok && v1) product_o(1, v_slot, i == 0, i == job.n[1] - 1, v_done);
+            if (ok && k1) product_s(1, k_slot, k_done, q_done);
+          } else {
+            product_o(i & 1, v_slot, i < 2, i + 2 >= tiles, v_done);
+            if (ok && i + L::ahead < tiles) scores(i + L::ahead);
           }
         }
       }
       // the products issued last are over before the block ends
       commit(&sh.drain);
-      warp_wait(&sh.drain, 0, &sh.abort, p.status);
+      warp_wait_quick(&sh.drain, 0, &sh.abort, p.status);
     } else if (warp == 10) {
       // ---------------- cleaning of V tiles ----------------
       RingPos<L::ring> pos;
       uint32_t todo_phase = 0;  // a bit for every slot
       const auto clean = [&](int32_t t) {
         const int slot = pos.slot;
-        if (!warp_wait(&sh.v_todo[slot], todo_phase >> slot & 1, &sh.abort, p.status)) return false;
+        if (!warp_wait_quick(&sh.v_todo[slot], todo_phase >> slot & 1, &sh.abort, p.status)) return false;
         todo_phase ^= 1u << slot;
-        if (!warp_wait(&sh.kv_full[slot], pos.phase, &sh.abort, p.status)) return false;
-        uint8_t *tile = s_kv + slot * L::tile_bytes;
+        if (!warp_wait_quick(&sh.kv_full[slot], pos.phase, &sh.abort, p.status)) return false;
+        uint8_t *tile = s_kv + slot * L::kv_tile;
         const int32_t end = min(max(job.nk - t * attn::KEYS, 0), attn::KEYS);       // rows of the sequence
         const int32_t all = min(max(job.min_seen - t * attn::KEYS, 0), attn::KEYS);       // rows that every row sees
         // lanes: eight 16-byte pieces of four rows
 #pragma unroll
         for (int panel = 0; panel < L::panels; ++panel) {
-          uint8_t *column = tile + panel * kPanelBytes + lane % 8 * 16;
+          uint8_t *column = tile + panel * kKvPanel + lane % 8 * 16;
 #pragma unroll 4
           for (int r = all + lane / 8; r < end; r += 4) {
             uint4 *at = reinterpret_cast<uint4 *>(column + r * 128);
@@ -876,15 +853,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       while (ok && jobs.next(job)) {
         const int32_t tiles = job.tiles(PAIR);
         if (tiles == 0) continue;
-        if (!PAIR) {
-          pos.step();
-          if (tiles > 1) pos.step();
-        }
+        for (int32_t i = 0; i < min(tiles, L::ahead); ++i) pos.step();
         for (int32_t i = 0; i < tiles && ok; ++i) {
-          if (PAIR) pos.step();
           if (job.t0 + i >= job.first_masked) ok = clean(job.t0 + i);
           pos.step();
-          if (!PAIR && i + 2 < tiles) pos.step();
+          if (i + L::ahead < tiles) pos.step();
         }
       }
     } else {
@@ -905,7 +878,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool more = order.next(p.plan, seg);
         if (more) describe<PAIR>(p, seg, job);
         else job.count = -1;
-        if (!warp_wait(&sh.job_empty[slot], phase, &sh.abort, p.status)) break;
+        if (!warp_wait_quick(&sh.job_empty[slot], phase, &sh.abort, p.status)) break;
         if (lane == 0) {
           sh.jobs[slot] = job;
           mbar_arrive(&sh.job_full[slot]);

@@ -464,6 +464,28 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volati
   return __all_sync(0xffffffffu, ok);
 }
 
+// warp_wait for roles that wait several times for every product they issue: no
+// vote while the phase is there or comes soon (38 cycles when it is there, warp_wait
+// 112).  The warp is converged and all lanes ask with one instruction, so
+// they get one answer; only giving up is voted on.
+__device__ __forceinline__ bool warp_wait_quick(uint64_t *bar, uint32_t parity, volatile int *abort_flag,
+                                                int *status) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t start = global_timer_ns();
+  for (;;) {
+    for (int spin = 0; spin < 256; ++spin)
+      if (mbar_try_wait(bar, parity)) return true;
+    const bool expired = global_timer_ns() - start > VFB_WAIT_TIMEOUT_NS;
+    if (__any_sync(0xffffffffu, expired || *abort_flag)) {
+      if (expired) {
+        *abort_flag = 1;
+        record_status(status, VFB_ETIMEOUT);
+      }
+      return false;
+    }
+  }
+}
+
 // ---- CTA pairs (2-CTA clusters) ---------------------------------------------
 __device__ __forceinline__ uint32_t cluster_ctarank() {
   uint32_t r;
