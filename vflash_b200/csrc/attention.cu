@@ -150,15 +150,6 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
       : "memory");
 }
 
-__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
-
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -297,12 +288,25 @@ struct Shared {
 static_assert(sizeof(Shared) + Layout<128, true>::smem <= 232448 && sizeof(Shared) + Layout<128, false>::smem <= 232448,
               "shared memory of a block");
 
-// A warp's way through the schedule.
+// A role's way through the schedule.
 struct JobReader {
   Shared &sh;
   int *status;
   int slot = 0;
   uint32_t phase = 0;
+
+  // `next` for a role of one thread.
+  __device__ __forceinline__ bool next_alone(Job &j) {
+    mbar_wait_through(&sh.job_full[slot], phase, &sh.abort, status);
+    if (*const_cast<volatile int *>(&sh.abort)) return false;
+    j = sh.jobs[slot];
+    mbar_arrive(&sh.job_empty[slot]);
+    if (++slot == kJobs) {
+      slot = 0;
+      phase ^= 1;
+    }
+    return j.count >= 0;
+  }
 
   // The next job; false when there is none (or a wait ran out).
   __device__ __forceinline__ bool next(Job &j) {
@@ -695,34 +699,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     } else if (warp == 9) {
       // ---------------- MMA issue ----------------
-      const bool leader = elect_one();
-      // All of TMEM is this block's, so it starts at column 0; constants and loop
-      // counters keep the operands of the products warp-uniform.  Products run
-      // over the padded head dimension: TMA filled the rest with zeros.
-      const uint32_t idesc_s = idesc_f16<T>(attn::KEYS, false);
-      const uint32_t idesc_o = idesc_f16<T>((p.dim + 15) / 16 * 16, true);
-      const uint64_t q_desc = sw128_kmajor_desc(smem_u32(s_q));
-      const uint64_t k_desc = sw128_kmajor_desc(smem_u32(s_kv)), v_desc = sw128_mnmajor_desc(smem_u32(s_kv));
-      RingPos<L::ring> pos;      // the item that is waited for next
-      uint32_t q_phase = 0, o_phase[2] = {1, 1};
-      uint32_t issued[2] = {0, 0}, joined[2] = {0, 0};  // S and P V of each stage so far, over all jobs
-      uint32_t v_phase = 0;  // a bit for every slot
-      bool ok = true;
-      const auto wait = [&](uint64_t *bar, uint32_t phase) {
-        ok = ok && warp_wait_quick(bar, phase, &sh.abort, p.status);
-        return ok;
-      };
-      const auto commit = [&](uint64_t *bar) {
-        if (leader) tc_commit(bar);
-        __syncwarp();
-      };
-      // `done`: a barrier that the products up to this one complete (or NULL)
-      const auto product_s = [&](int stage, int slot, uint64_t *done, uint64_t *done_too) {  // S = Q K^T
-        const uint64_t a = q_desc + (PAIR ? stage * (L::q_tile >> 4) : 0);
-        const uint64_t b = k_desc + slot * (L::kv_tile >> 4);
-        const uint32_t buffer = issued[stage]++ & 1;
-        const uint32_t d = 128 * stage + attn::KEYS * buffer;
-        if (leader) {
+      // One thread for the whole role: between two products it passes two or three
+      // barriers that are usually ready (38 cycles each), and as a warp with an
+      // elected lane the branches, reconvergence and votes around them took longer
+      // than the products themselves (2240 cycles for the key tile of both stages,
+      // whose products take 1260).  Products run over the padded head dimension:
+      // TMA filled the rest with zeros.
+      if (elect_one()) {
+        const uint32_t idesc_s = idesc_f16<T>(attn::KEYS, false);
+        const uint32_t idesc_o = idesc_f16<T>((p.dim + 15) / 16 * 16, true);
+        const uint64_t q_desc = sw128_kmajor_desc(smem_u32(s_q));
+        const uint64_t k_desc = sw128_kmajor_desc(smem_u32(s_kv)), v_desc = sw128_mnmajor_desc(smem_u32(s_kv));
+        RingPos<L::ring> pos;      // the item that is waited for next
+        uint32_t q_phase = 0, o_phase[2] = {1, 1};
+        uint32_t issued[2] = {0, 0}, joined[2] = {0, 0};  // S and P V of each stage so far, over all jobs
+        uint32_t v_phase = 0;  // a bit for every slot
+        const auto wait = [&](uint64_t *bar, uint32_t phase) { mbar_wait_through(bar, phase, &sh.abort, p.status); };
+        // `done`, `done_too`: barriers that the products up to this one complete (or NULL)
+        const auto product_s = [&](int stage, int slot, uint64_t *done, uint64_t *done_too) {  // S = Q K^T
+          const uint64_t a = q_desc + (PAIR ? stage * (L::q_tile >> 4) : 0);
+          const uint64_t b = k_desc + slot * (L::kv_tile >> 4);
+          const uint32_t buffer = issued[stage]++ & 1;
+          const uint32_t d = 128 * stage + attn::KEYS * buffer;
 #pragma unroll
           for (int k = 0; k < DP / 16; ++k)
             mma_f16(d, a + ((k / 4 * kQPanel + k % 4 * 32) >> 4), b + ((k / 4 * kKvPanel + k % 4 * 32) >> 4), idesc_s,
@@ -730,82 +728,79 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_commit(&sh.s_full[stage][buffer]);
           if (done != nullptr) tc_commit(done);
           if (done_too != nullptr) tc_commit(done_too);
-        }
-        __syncwarp();
-      };
-      const auto product_o = [&](int stage, int slot, bool first, bool last, uint64_t *done) {  // O (+)= P V
-        const uint32_t buffer = joined[stage] & 1;
-        if (!wait(&sh.p_full[stage][buffer], joined[stage] >> 1 & 1)) return;
-        if (first) {
-          if (!wait(&sh.o_empty[stage], o_phase[stage])) return;
-          o_phase[stage] ^= 1;
-        }
-        ++joined[stage];
-        tc_fence_after();
-        const uint64_t b = v_desc + slot * (L::kv_tile >> 4);
-        const uint32_t a = 128 * stage + attn::KEYS * buffer, d = 256 + 128 * stage;
-        if (leader) {
+        };
+        const auto product_o = [&](int stage, int slot, bool first, bool last, uint64_t *done) {  // O (+)= P V
+          const uint32_t buffer = joined[stage] & 1;
+          wait(&sh.p_full[stage][buffer], joined[stage] >> 1 & 1);
+          if (first) {
+            wait(&sh.o_empty[stage], o_phase[stage]);
+            o_phase[stage] ^= 1;
+          }
+          ++joined[stage];
+          tc_fence_after();
+          const uint64_t b = v_desc + slot * (L::kv_tile >> 4);
+          const uint32_t a = 128 * stage + attn::KEYS * buffer, d = 256 + 128 * stage;
 #pragma unroll
           for (int k = 0; k < attn::KEYS / 16; ++k)
             mma_f16_tmem_a(d, a + 8 * k, b + (k * 2048 >> 4), idesc_o, k > 0 || !first);
           tc_commit(&sh.pv_done[stage]);
           if (last) tc_commit(&sh.o_full[stage]);
           if (done != nullptr) tc_commit(done);
-        }
-        __syncwarp();
-      };
-      while (ok && jobs.next(job)) {
-        const int32_t tiles = job.tiles(PAIR);
-        if (tiles == 0) continue;
-        if (!wait(&sh.q_full, q_phase)) break;
-        q_phase ^= 1;
-        // S of key tile i: of both stages (as far as they see it), or of the tile's stage
-        const auto scores = [&](int32_t i) {
-          const int slot = pos.slot;
-          if (!wait(&sh.kv_full[slot], pos.phase)) return;
-          pos.step();
-          uint64_t *q_done = i == tiles - 1 ? &sh.q_empty : nullptr;
-          if (PAIR) {
-            const bool both = i < job.n[0] && i < job.n[1];
-            if (i < job.n[0]) product_s(0, slot, both ? nullptr : &sh.kv_empty[slot], both ? nullptr : q_done);
-            if (i < job.n[1]) product_s(1, slot, &sh.kv_empty[slot], q_done);
-          } else {
-            product_s(i & 1, slot, &sh.kv_empty[slot], q_done);
-          }
         };
-        for (int32_t i = 0; i < min(tiles, L::ahead) && ok; ++i) scores(i);
-        for (int32_t i = 0; i < tiles && ok; ++i) {
-          const int v_slot = pos.slot;
-          if (!wait(&sh.kv_full[v_slot], pos.phase)) break;
-          pos.step();
-          if (job.t0 + i >= job.first_masked) {
-            if (!wait(&sh.v_clean[v_slot], v_phase >> v_slot & 1)) break;
-            v_phase ^= 1u << v_slot;
-          }
-          uint64_t *v_done = &sh.kv_empty[v_slot];
-          if (PAIR) {
-            // S of the next tile but one follows the P V that frees its buffer
-            const int32_t next = i + L::ahead;
-            const int k_slot = pos.slot;
-            uint64_t *k_done = &sh.kv_empty[k_slot], *q_done = next == tiles - 1 ? &sh.q_empty : nullptr;
-            if (next < tiles) {
-              if (!wait(&sh.kv_full[k_slot], pos.phase)) break;
-              pos.step();
+        while (jobs.next_alone(job)) {
+          const int32_t n0 = job.n[0], n1 = job.n[1], tiles = job.tiles(PAIR);
+          const int32_t masked = max(job.first_masked - job.t0, 0);  // tiles from here on
+          if (tiles == 0) continue;
+          wait(&sh.q_full, q_phase);
+          q_phase ^= 1;
+          // S of key tile i: of both stages (as far as they see it), or of the tile's stage
+          const auto scores = [&](int32_t i) {
+            const int slot = pos.slot;
+            wait(&sh.kv_full[slot], pos.phase);
+            pos.step();
+            uint64_t *q_done = i == tiles - 1 ? &sh.q_empty : nullptr;
+            if (PAIR) {
+              const bool both = i < n0 && i < n1;
+              if (i < n0) product_s(0, slot, both ? nullptr : &sh.kv_empty[slot], both ? nullptr : q_done);
+              if (i < n1) product_s(1, slot, &sh.kv_empty[slot], q_done);
+            } else {
+              product_s(i & 1, slot, &sh.kv_empty[slot], q_done);
             }
-            const bool v1 = i < job.n[1], k1 = next < job.n[1];  // stage 1 comes last where it has the tile
-            if (i < job.n[0]) product_o(0, v_slot, i == 0, i == job.n[0] - 1, v1 ? nullptr : v_done);
-            if (ok && next < job.n[0]) product_s(0, k_slot, k1 ? nullptr : k_done, k1 ? nullptr : q_done);
-            if (ok && v1) product_o(1, v_slot, i == 0, i == job.n[1] - 1, v_done);
-            if (ok && k1) product_s(1, k_slot, k_done, q_done);
-          } else {
-            product_o(i & 1, v_slot, i < 2, i + 2 >= tiles, v_done);
-            if (ok && i + L::ahead < tiles) scores(i + L::ahead);
+          };
+          for (int32_t i = 0; i < min(tiles, L::ahead); ++i) scores(i);
+          for (int32_t i = 0; i < tiles; ++i) {
+            const int v_slot = pos.slot;
+            wait(&sh.kv_full[v_slot], pos.phase);
+            pos.step();
+            if (i >= masked) {
+              wait(&sh.v_clean[v_slot], v_phase >> v_slot & 1);
+              v_phase ^= 1u << v_slot;
+            }
+            uint64_t *v_done = &sh.kv_empty[v_slot];
+            if (PAIR) {
+              // S of the next tile but one follows the P V that frees its buffer
+              const int32_t next = i + L::ahead;
+              const int k_slot = pos.slot;
+              uint64_t *k_done = &sh.kv_empty[k_slot], *q_done = next == tiles - 1 ? &sh.q_empty : nullptr;
+              if (next < tiles) {
+                wait(&sh.kv_full[k_slot], pos.phase);
+                pos.step();
+              }
+              const bool v1 = i < n1, k1 = next < n1;  // stage 1 comes last where it has the tile
+              if (i < n0) product_o(0, v_slot, i == 0, i == n0 - 1, v1 ? nullptr : v_done);
+              if (next < n0) product_s(0, k_slot, k1 ? nullptr : k_done, k1 ? nullptr : q_done);
+              if (v1) product_o(1, v_slot, i == 0, i == n1 - 1, v_done);
+              if (k1) product_s(1, k_slot, k_done, q_done);
+            } else {
+              product_o(i & 1, v_slot, i < 2, i + 2 >= tiles, v_done);
+              if (i + L::ahead < tiles) scores(i + L::ahead);
+            }
           }
         }
+        // the products issued last are over before the block ends
+        tc_commit(&sh.drain);
+        wait(&sh.drain, 0);
       }
-      // the products issued last are over before the block ends
-      commit(&sh.drain);
-      warp_wait_quick(&sh.drain, 0, &sh.abort, p.status);
     } else if (warp == 10) {
       // ---------------- cleaning of V tiles ----------------
       RingPos<L::ring> pos;

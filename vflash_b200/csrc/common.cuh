@@ -486,6 +486,25 @@ __device__ __forceinline__ bool warp_wait_quick(uint64_t *bar, uint32_t parity, 
   }
 }
 
+// A bounded wait without an answer, for the MMA issuer: after one that ran out
+// (or another role's abort) the caller goes on, its later waits return at
+// once, and what it issues is discarded with the rest of the run.  Control flow
+// that does not depend on the wait stays warp-uniform for the compiler, which
+// then keeps the products' operands in uniform registers.
+__device__ __forceinline__ void mbar_wait_through(uint64_t *bar, uint32_t parity, volatile int *abort_flag,
+                                                  int *status) {
+  if (mbar_try_wait(bar, parity)) return;
+  const uint64_t start = global_timer_ns();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*abort_flag) return;
+    if (global_timer_ns() - start > VFB_WAIT_TIMEOUT_NS) {
+      *abort_flag = 1;
+      record_status(status, VFB_ETIMEOUT);
+      return;
+    }
+  }
+}
+
 // ---- CTA pairs (2-CTA clusters) ---------------------------------------------
 __device__ __forceinline__ uint32_t cluster_ctarank() {
   uint32_t r;
