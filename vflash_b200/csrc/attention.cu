@@ -11,12 +11,12 @@
 // maximum grows by more than kHold binary orders, so P may reach 2^kHold; the
 // result is the same to rounding and the pass over O in TMEM is rare.
 //
-// Roles of a block of twelve warps, one block on an SM:
+// Roles of a block of sixteen warps, one block on an SM:
 //   warps 0-3, 4-7  softmax of stage 0 and stage 1, one thread per row
 //   warp 8          TMA loads: Q tiles, then K and V tiles through one ring
-//   warp 9          MMA issue
-//   warp 10         cleans the V tiles that hold keys some row must not see
+//   warps 9, 10     MMA issue of stage 0 and stage 1, one thread each
 //   warp 11         works out the block's jobs and hands them to the others
+//   warps 12-15     clean the V tiles that hold keys some row must not see
 // The two stages keep the tensor cores busy with one tile's products while the
 // other's exponentials run.  They are
 //   PAIR: two tiles of query rows against the same keys (many query rows), or
@@ -34,8 +34,8 @@
 // products; with two buffers of 64 the products' 2520 are the bound).
 //
 // Keys behind a row's limit: their scores become -inf, so P = 0; but 0 * inf
-// and 0 * NaN would still spoil the second product.  Warp 10 therefore
-// zeroes, in the key tiles that any row of the block sees only in part, the V
+// and 0 * NaN would still spoil the second product.  Warps 12-15 therefore
+// zero, in the key tiles that any row of the block sees only in part, the V
 // rows behind the sequence's end and (causal) every element that is not
 // finite; the latter are added back at the end to the rows that do see them.
 #include "common.cuh"
@@ -50,10 +50,10 @@ using attn::Segment;
 constexpr int kTile = 128;           // query rows in a tile
 constexpr int kQPanel = kTile * 128;       // bytes of a tile's 64 elements of 16 bits, 128-byte swizzle
 constexpr int kKvPanel = attn::KEYS * 128;
-constexpr int kThreads = 384;
+constexpr int kThreads = 512;
 constexpr int kRingSlots = 16;       // at most
 constexpr int kJobs = 2;             // jobs that the scheduler may be ahead
-constexpr int kJobReaders = 11;      // warps that follow the schedule
+constexpr int kJobReaders = 15;      // warps that follow the schedule
 constexpr float kHold = 8.0f;
 constexpr int kFmaPairs = 0;         // of every 8 pairs of exponentials, so many on the FMA pipe
 constexpr float kLn2 = 0.693147180559945309f;
@@ -462,12 +462,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
     mbar_init(&sh.q_full, 1);
-    mbar_init(&sh.q_empty, 1);
+    mbar_init(&sh.q_empty, 2);
     for (int i = 0; i < L::ring; ++i) {
       mbar_init(&sh.kv_full[i], 1);
-      mbar_init(&sh.kv_empty[i], 1);
+      mbar_init(&sh.kv_empty[i], 2);
       mbar_init(&sh.v_todo[i], 1);
-      mbar_init(&sh.v_clean[i], 1);
+      mbar_init(&sh.v_clean[i], 4);
     }
     for (int i = 0; i < kJobs; ++i) {
       mbar_init(&sh.job_full[i], 1);
@@ -484,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     mbar_init(&sh.stats_full, 4);
     mbar_init(&sh.stats_empty, 4);
-    mbar_init(&sh.drain, 1);
+    mbar_init(&sh.drain, 2);
     sh.abort = 0;
     sh.dirty = 0;
     fence_mbar_init();
@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   Job job;
 
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
     const int stage = warp / 4;
     const int row = (warp % 4) * 32 + lane;  // of the tile, and TMEM lane
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp % 4) * 32) << 16);
@@ -646,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 8) {
       // ---------------- TMA producer ----------------
       RingPos<L::ring> pos;
@@ -697,165 +697,92 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t last = i < pos.slot ? pos.phase : pos.phase ^ 1;
         if (issued >> i & 1) warp_wait_quick(&sh.kv_full[i], last, &sh.abort, p.status);
       }
-    } else if (warp == 9) {
+    } else if (warp == 9 || warp == 10) {
       // ---------------- MMA issue ----------------
-      // One thread for the whole role: between two products it passes two or three
-      // barriers that are usually ready (38 cycles each), and as a warp with an
-      // elected lane the branches, reconvergence and votes around them took longer
-      // than the products themselves (2240 cycles for the key tile of both stages,
-      // whose products take 1260).  Products run over the padded head dimension:
-      // TMA filled the rest with zeros.
+      // One thread for a stage.  Between two products it passes two or three
+      // barriers that are usually ready (38 cycles each) and prepares operands:
+      // as one warp for both stages with an elected lane that took 2240 cycles for a
+      // key tile of both (one thread for both: 1840), whose products take 1260.
+      // Both follow every item of the ring, also those of the other's tiles, so
+      // neither is ever a pass ahead or behind.  Products run over the padded head
+      // dimension: TMA filled the rest with zeros.
       if (elect_one()) {
+        const int stage = warp - 9;
         const uint32_t idesc_s = idesc_f16<T>(attn::KEYS, false);
         const uint32_t idesc_o = idesc_f16<T>((p.dim + 15) / 16 * 16, true);
-        const uint64_t q_desc = sw128_kmajor_desc(smem_u32(s_q));
+        const uint64_t q_desc = sw128_kmajor_desc(smem_u32(s_q) + (PAIR ? stage * L::q_tile : 0));
         const uint64_t k_desc = sw128_kmajor_desc(smem_u32(s_kv)), v_desc = sw128_mnmajor_desc(smem_u32(s_kv));
+        const uint32_t tmem_s = tmem + 128 * stage, tmem_o = tmem + 256 + 128 * stage;
         RingPos<L::ring> pos;      // the item that is waited for next
-        uint32_t q_phase = 0, o_phase[2] = {1, 1};
-        uint32_t issued[2] = {0, 0}, joined[2] = {0, 0};  // S and P V of each stage so far, over all jobs
+        uint32_t q_phase = 0, o_phase = 1;
+        uint32_t issued = 0, joined = 0;  // S and P V so far, over all jobs
         uint32_t v_phase = 0;  // a bit for every slot
         const auto wait = [&](uint64_t *bar, uint32_t phase) { mbar_wait_through(bar, phase, &sh.abort, p.status); };
-        // `done`, `done_too`: barriers that the products up to this one complete (or NULL)
-        const auto product_s = [&](int stage, int slot, uint64_t *done, uint64_t *done_too) {  // S = Q K^T
-          const uint64_t a = q_desc + (PAIR ? stage * (L::q_tile >> 4) : 0);
-          const uint64_t b = k_desc + slot * (L::kv_tile >> 4);
-          const uint32_t buffer = issued[stage]++ & 1;
-          const uint32_t d = 128 * stage + attn::KEYS * buffer;
-#pragma unroll
-          for (int k = 0; k < DP / 16; ++k)
-            mma_f16(d, a + ((k / 4 * kQPanel + k % 4 * 32) >> 4), b + ((k / 4 * kKvPanel + k % 4 * 32) >> 4), idesc_s,
-                    k > 0);
-          tc_commit(&sh.s_full[stage][buffer]);
-          if (done != nullptr) tc_commit(done);
-          if (done_too != nullptr) tc_commit(done_too);
-        };
-        const auto product_o = [&](int stage, int slot, bool first, bool last, uint64_t *done) {  // O (+)= P V
-          const uint32_t buffer = joined[stage] & 1;
-          wait(&sh.p_full[stage][buffer], joined[stage] >> 1 & 1);
-          if (first) {
-            wait(&sh.o_empty[stage], o_phase[stage]);
-            o_phase[stage] ^= 1;
-          }
-          ++joined[stage];
-          tc_fence_after();
-          const uint64_t b = v_desc + slot * (L::kv_tile >> 4);
-          const uint32_t a = 128 * stage + attn::KEYS * buffer, d = 256 + 128 * stage;
-#pragma unroll
-          for (int k = 0; k < attn::KEYS / 16; ++k)
-            mma_f16_tmem_a(d, a + 8 * k, b + (k * 2048 >> 4), idesc_o, k > 0 || !first);
-          tc_commit(&sh.pv_done[stage]);
-          if (last) tc_commit(&sh.o_full[stage]);
-          if (done != nullptr) tc_commit(done);
-        };
         while (jobs.next_alone(job)) {
-          const int32_t n0 = job.n[0], n1 = job.n[1], tiles = job.tiles(PAIR);
+          const int32_t tiles = job.tiles(PAIR), own = job.n[stage];
           const int32_t masked = max(job.first_masked - job.t0, 0);  // tiles from here on
           if (tiles == 0) continue;
           wait(&sh.q_full, q_phase);
           q_phase ^= 1;
-          // S of key tile i: of both stages (as far as they see it), or of the tile's stage
-          const auto scores = [&](int32_t i) {
+          if (own == 0) mbar_arrive(&sh.q_empty);
+          const auto mine = [&](int32_t i) { return PAIR ? i < own : (i & 1) == stage; };
+          const int32_t last = PAIR ? own - 1 : 2 * (own - 1) + stage;  // of this stage's tiles
+          const auto scores = [&](int32_t i) {  // S = Q K^T of key tile i
             const int slot = pos.slot;
             wait(&sh.kv_full[slot], pos.phase);
             pos.step();
-            uint64_t *q_done = i == tiles - 1 ? &sh.q_empty : nullptr;
-            if (PAIR) {
-              const bool both = i < n0 && i < n1;
-              if (i < n0) product_s(0, slot, both ? nullptr : &sh.kv_empty[slot], both ? nullptr : q_done);
-              if (i < n1) product_s(1, slot, &sh.kv_empty[slot], q_done);
-            } else {
-              product_s(i & 1, slot, &sh.kv_empty[slot], q_done);
+            if (!mine(i)) {
+              mbar_arrive(&sh.kv_empty[slot]);
+              return;
             }
+            const uint64_t b = k_desc + slot * (L::kv_tile >> 4);
+            const uint32_t buffer = issued++ & 1;
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k)
+              mma_f16(tmem_s + attn::KEYS * buffer, q_desc + ((k / 4 * kQPanel + k % 4 * 32) >> 4),
+                      b + ((k / 4 * kKvPanel + k % 4 * 32) >> 4), idesc_s, k > 0);
+            tc_commit(&sh.s_full[stage][buffer]);
+            tc_commit(&sh.kv_empty[slot]);
+            if (i == last) tc_commit(&sh.q_empty);
           };
           for (int32_t i = 0; i < min(tiles, L::ahead); ++i) scores(i);
-          for (int32_t i = 0; i < tiles; ++i) {
-            const int v_slot = pos.slot;
-            wait(&sh.kv_full[v_slot], pos.phase);
+          for (int32_t i = 0; i < tiles; ++i) {  // O (+)= P V of key tile i
+            const int slot = pos.slot;
+            wait(&sh.kv_full[slot], pos.phase);
             pos.step();
-            if (i >= masked) {
-              wait(&sh.v_clean[v_slot], v_phase >> v_slot & 1);
-              v_phase ^= 1u << v_slot;
-            }
-            uint64_t *v_done = &sh.kv_empty[v_slot];
-            if (PAIR) {
-              // S of the next tile but one follows the P V that frees its buffer
-              const int32_t next = i + L::ahead;
-              const int k_slot = pos.slot;
-              uint64_t *k_done = &sh.kv_empty[k_slot], *q_done = next == tiles - 1 ? &sh.q_empty : nullptr;
-              if (next < tiles) {
-                wait(&sh.kv_full[k_slot], pos.phase);
-                pos.step();
+            const uint32_t cleaned = v_phase >> slot & 1;
+            if (i >= masked) v_phase ^= 1u << slot;
+            if (mine(i)) {
+              if (i >= masked) wait(&sh.v_clean[slot], cleaned);
+              const uint32_t buffer = joined & 1;
+              wait(&sh.p_full[stage][buffer], joined >> 1 & 1);
+              const bool first = PAIR ? i == 0 : i < 2;
+              if (first) {
+                wait(&sh.o_empty[stage], o_phase);
+                o_phase ^= 1;
               }
-              const bool v1 = i < n1, k1 = next < n1;  // stage 1 comes last where it has the tile
-              if (i < n0) product_o(0, v_slot, i == 0, i == n0 - 1, v1 ? nullptr : v_done);
-              if (next < n0) product_s(0, k_slot, k1 ? nullptr : k_done, k1 ? nullptr : q_done);
-              if (v1) product_o(1, v_slot, i == 0, i == n1 - 1, v_done);
-              if (k1) product_s(1, k_slot, k_done, q_done);
+              ++joined;
+              tc_fence_after();
+              const uint64_t b = v_desc + slot * (L::kv_tile >> 4);
+#pragma unroll
+              for (int k = 0; k < attn::KEYS / 16; ++k)
+                mma_f16_tmem_a(tmem_o, tmem_s + attn::KEYS * buffer + 8 * k, b + (k * 2048 >> 4), idesc_o,
+                               k > 0 || !first);
+              tc_commit(&sh.pv_done[stage]);
+              tc_commit(&sh.kv_empty[slot]);
+              if (i == last) tc_commit(&sh.o_full[stage]);
             } else {
-              product_o(i & 1, v_slot, i < 2, i + 2 >= tiles, v_done);
-              if (i + L::ahead < tiles) scores(i + L::ahead);
+              mbar_arrive(&sh.kv_empty[slot]);
             }
+            // S of the tile whose buffer that P V frees
+            if (i + L::ahead < tiles) scores(i + L::ahead);
           }
         }
         // the products issued last are over before the block ends
         tc_commit(&sh.drain);
         wait(&sh.drain, 0);
       }
-    } else if (warp == 10) {
-      // ---------------- cleaning of V tiles ----------------
-      RingPos<L::ring> pos;
-      uint32_t todo_phase = 0;  // a bit for every slot
-      const auto clean = [&](int32_t t) {
-        const int slot = pos.slot;
-        if (!warp_wait_quick(&sh.v_todo[slot], todo_phase >> slot & 1, &sh.abort, p.status)) return false;
-        todo_phase ^= 1u << slot;
-        if (!warp_wait_quick(&sh.kv_full[slot], pos.phase, &sh.abort, p.status)) return false;
-        uint8_t *tile = s_kv + slot * L::kv_tile;
-        const int32_t end = min(max(job.nk - t * attn::KEYS, 0), attn::KEYS);       // rows of the sequence
-        const int32_t all = min(max(job.min_seen - t * attn::KEYS, 0), attn::KEYS);       // rows that every row sees
-        // lanes: eight 16-byte pieces of four rows
-#pragma unroll
-        for (int panel = 0; panel < L::panels; ++panel) {
-          uint8_t *column = tile + panel * kKvPanel + lane % 8 * 16;
-#pragma unroll 4
-          for (int r = all + lane / 8; r < end; r += 4) {
-            uint4 *at = reinterpret_cast<uint4 *>(column + r * 128);
-            uint4 x = *at;
-            uint32_t *word = reinterpret_cast<uint32_t *>(&x);
-            uint32_t bad = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const uint32_t hit = __vcmpeq2(word[j] & exponent_mask<T>(), exponent_mask<T>());
-              word[j] &= ~hit;
-              bad |= hit;
-            }
-            if (bad) {
-              *at = x;
-              *reinterpret_cast<volatile int *>(&sh.dirty) = 1;
-            }
-          }
-#pragma unroll 4
-          for (int r = end + lane / 8; r < attn::KEYS; r += 4)
-            *reinterpret_cast<uint4 *>(column + r * 128) = make_uint4(0, 0, 0, 0);
-        }
-        fence_proxy_async_smem();
-        __threadfence_block();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.v_clean[slot]);
-        return true;
-      };
-      bool ok = true;
-      while (ok && jobs.next(job)) {
-        const int32_t tiles = job.tiles(PAIR);
-        if (tiles == 0) continue;
-        for (int32_t i = 0; i < min(tiles, L::ahead); ++i) pos.step();
-        for (int32_t i = 0; i < tiles && ok; ++i) {
-          if (job.t0 + i >= job.first_masked) ok = clean(job.t0 + i);
-          pos.step();
-          if (i + L::ahead < tiles) pos.step();
-        }
-      }
-    } else {
+    } else if (warp == 11) {
       // ---------------- schedule ----------------
       attn::Order order;
       if (p.split) {
@@ -883,6 +810,60 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (++slot == kJobs) {
           slot = 0;
           phase ^= 1;
+        }
+      }
+    } else {
+      // ---------------- cleaning of V tiles ----------------
+      RingPos<L::ring> pos;
+      uint32_t todo_phase = 0;  // a bit for every slot
+      const auto clean = [&](int32_t t) {
+        const int slot = pos.slot;
+        if (!warp_wait_quick(&sh.v_todo[slot], todo_phase >> slot & 1, &sh.abort, p.status)) return false;
+        todo_phase ^= 1u << slot;
+        if (!warp_wait_quick(&sh.kv_full[slot], pos.phase, &sh.abort, p.status)) return false;
+        uint8_t *tile = s_kv + slot * L::kv_tile;
+        const int32_t end = min(max(job.nk - t * attn::KEYS, 0), attn::KEYS);       // rows of the sequence
+        const int32_t all = min(max(job.min_seen - t * attn::KEYS, 0), attn::KEYS);       // rows that every row sees
+        const int row = (warp - 12) * 4 + lane / 8;  // lanes: eight 16-byte pieces of four rows
+#pragma unroll
+        for (int panel = 0; panel < L::panels; ++panel) {
+          uint8_t *column = tile + panel * kKvPanel + lane % 8 * 16;
+#pragma unroll 2
+          for (int r = all + row; r < end; r += 16) {
+            uint4 *at = reinterpret_cast<uint4 *>(column + r * 128);
+            uint4 x = *at;
+            uint32_t *word = reinterpret_cast<uint32_t *>(&x);
+            uint32_t bad = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t hit = __vcmpeq2(word[j] & exponent_mask<T>(), exponent_mask<T>());
+              word[j] &= ~hit;
+              bad |= hit;
+            }
+            if (bad) {
+              *at = x;
+              *reinterpret_cast<volatile int *>(&sh.dirty) = 1;
+            }
+          }
+#pragma unroll 2
+          for (int r = end + row; r < attn::KEYS; r += 16)
+            *reinterpret_cast<uint4 *>(column + r * 128) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        __threadfence_block();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.v_clean[slot]);
+        return true;
+      };
+      bool ok = true;
+      while (ok && jobs.next(job)) {
+        const int32_t tiles = job.tiles(PAIR);
+        if (tiles == 0) continue;
+        for (int32_t i = 0; i < min(tiles, L::ahead); ++i) pos.step();
+        for (int32_t i = 0; i < tiles && ok; ++i) {
+          if (job.t0 + i >= job.first_masked) ok = clean(job.t0 + i);
+          pos.step();
+          if (i + L::ahead < tiles) pos.step();
         }
       }
     }
