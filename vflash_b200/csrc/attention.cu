@@ -50,6 +50,8 @@ using attn::Segment;
 constexpr int kTile = 128;           // query rows in a tile
 constexpr int kQPanel = kTile * 128;       // bytes of a tile's 64 elements of 16 bits, 128-byte swizzle
 constexpr int kKvPanel = attn::KEYS * 128;
+constexpr int kBuffers = 128 / attn::KEYS;  // of S, for a stage
+constexpr int kTail = 32;            // keys of a tile whose P is handed over separately
 constexpr int kThreads = 512;
 constexpr int kRingSlots = 16;       // at most
 constexpr int kJobs = 2;             // jobs that the scheduler may be ahead
@@ -67,8 +69,8 @@ struct Layout {
   static constexpr int q_tile = panels * kQPanel;
   static constexpr int kv_tile = panels * kKvPanel;
   static constexpr int q_bytes = (PAIR ? 2 : 1) * q_tile;
-  static constexpr int ring = DP == 128 ? (PAIR ? 10 : 12) : 16;
-  static constexpr int ahead = PAIR ? 2 : 4;  // key tiles whose S is issued before the first P V
+  static constexpr int ring = DP == 128 ? (PAIR ? 640 : 768) / attn::KEYS : 1024 / attn::KEYS;
+  static constexpr int ahead = (PAIR ? 1 : 2) * kBuffers;  // key tiles whose S is issued before the first P V
   static constexpr int smem = 1024 + q_bytes + ring * kv_tile;  // tiles start on 1024 bytes
 };
 
@@ -147,6 +149,15 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
       "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
       "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
       "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 
@@ -272,7 +283,7 @@ __device__ __forceinline__ void describe(const Params &p, const Segment &s, Job 
 struct Shared {
   uint64_t q_full, q_empty;
   uint64_t kv_full[kRingSlots], kv_empty[kRingSlots];
-  uint64_t s_full[2][2], p_full[2][2], pv_done[2], o_full[2], o_empty[2];
+  uint64_t s_full[2][2], p_full[2][2], p_tail[2][2], pv_done[2], o_full[2], o_empty[2];
   // a V tile to be cleaned is on its way into the slot, and is clean: the MMA
   // warp waits for the latter before the slot is given back, so neither barrier
   // can run ahead of who waits for it
@@ -356,43 +367,50 @@ struct Softmax {
     m = -INFINITY;
     l = 0.0f;
     for (int32_t i = 0; i < n; ++i, ++count) {
-      if (!wait(&sh.s_full[stage][count & 1], count >> 1 & 1)) return false;
+      if (!wait(&sh.s_full[stage][count % kBuffers], count / kBuffers & 1)) return false;
       tc_fence_after();
-      if (live && !tile((t0 + i * stride) * attn::KEYS, limit, i > 0, valid)) return false;
-      tc_fence_before();
-      __syncwarp();
-      if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.p_full[stage][count & 1]);
+      if (live) {
+        if (!tile((t0 + i * stride) * attn::KEYS, limit, i > 0, valid)) return false;
+      } else {
+        hand_over(sh.p_full[stage]);
+        hand_over(sh.p_tail[stage]);
+      }
     }
     return true;
   }
 
+  __device__ __forceinline__ void hand_over(uint64_t (&bar)[2]) {
+    tc_fence_before();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&bar[count % kBuffers]);
+  }
+
   __device__ __forceinline__ bool tile(int32_t key0, int32_t limit, bool scale_o, bool valid) {
-    const uint32_t at = tmem_s + attn::KEYS * (count & 1);
-    float s[64];
+    constexpr int N = attn::KEYS;
+    const uint32_t at = tmem_s + N * (count % kBuffers);
+    float s[N];
     {
-      uint32_t(&r)[2][32] = reinterpret_cast<uint32_t(&)[2][32]>(s);
-      tmem_ld_32x32b_x32_issue(at, r[0]);
-      tmem_ld_32x32b_x32_issue(at + 32, r[1]);
+      uint32_t(&r)[N / 32][32] = reinterpret_cast<uint32_t(&)[N / 32][32]>(s);
+#pragma unroll
+      for (int c = 0; c < N / 32; ++c) tmem_ld_32x32b_x32_issue(at + 32 * c, r[c]);
       tmem_ld_wait();
-      tmem_ld_fence(r[0]);
-      tmem_ld_fence(r[1]);
+#pragma unroll
+      for (int c = 0; c < N / 32; ++c) tmem_ld_fence(r[c]);
     }
     // a row that is not part of the job is left alone: nobody reads its results
-    const int32_t seen = valid ? limit - key0 : attn::KEYS;
-    if (__any_sync(0xffffffffu, seen < attn::KEYS)) {
+    const int32_t seen = valid ? limit - key0 : N;
+    if (__any_sync(0xffffffffu, seen < N)) {
 #pragma unroll
-      for (int j = 0; j < 64; ++j)
+      for (int j = 0; j < N; ++j)
         if (j >= seen) s[j] = -INFINITY;
     }
-    float top[4] = {m, s[0], s[1], s[2]};
+    float top[4] = {m, m, m, m};
 #pragma unroll
-    for (int j = 3; j < 59; j += 8) {
+    for (int j = 0; j < N; j += 8) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) top[i] = max3_nan(top[i], s[j + 2 * i], s[j + 2 * i + 1]);
     }
-    top[0] = max3_nan(top[0], s[59], s[60]);
-    top[1] = max3_nan(top[1], s[61], s[62]);
-    const float peak = max3_nan(max3_nan(top[0], top[1], s[63]), top[2], top[3]);
+    const float peak = max3_nan(max3_nan(top[0], top[1], top[2]), top[3], top[3]);
     // true also for a NaN score; not while no key has been seen
     const bool move = valid && !((peak - m) * p.scale_log2 <= kHold) && peak != -INFINITY;
     if (__any_sync(0xffffffffu, move)) {
@@ -402,7 +420,7 @@ struct Softmax {
         l *= alpha;
       }
       if (scale_o) {
-        // The last P V is behind S(count - 2) of its buffer, so at most one phase of pv_done is open here.
+        // S(count) came behind the P V that freed its buffer, so at most one phase of pv_done is open here.
         if (!wait(&sh.pv_done[stage], (count - 1) & 1)) return false;
         tc_fence_after();
 #pragma unroll 1
@@ -420,27 +438,35 @@ struct Softmax {
     const float base = m == -INFINITY ? 0.0f : m * p.scale_log2;
     const f32x2 scale2 = pair(p.scale_log2, p.scale_log2), base2 = pair(-base, -base);
     f32x2 sum[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
-    uint32_t packed[32];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      const f32x2 x = fma2(pair(s[2 * j], s[2 * j + 1]), scale2, base2);
-      float a, b;
-      if (j % 8 >= 8 - kFmaPairs) {
-        exp2_fma(x, a, b);
-      } else {
-        split(x, a, b);
-        a = ex2(a);
-        b = ex2(b);
+    for (int h = 0; h < N / 32; ++h) {
+      uint32_t packed[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const f32x2 x = fma2(pair(s[32 * h + 2 * j], s[32 * h + 2 * j + 1]), scale2, base2);
+        float a, b;
+        if (j % 8 >= 8 - kFmaPairs) {
+          exp2_fma(x, a, b);
+        } else {
+          split(x, a, b);
+          a = ex2(a);
+          b = ex2(b);
+        }
+        sum[j & 1] = add2(sum[j & 1], pair(a, b));
+        packed[j] = pack2<T>(a, b);
       }
-      sum[j & 1] = add2(sum[j & 1], pair(a, b));
-      packed[j] = pack2<T>(a, b);
+      tmem_st_32x32b_x16(at + 16 * h, packed);
+      if (32 * (h + 1) == N - kTail) {
+        tmem_st_wait();
+        hand_over(sh.p_full[stage]);
+      }
     }
-    tmem_st_32x32b_x32(at, packed);
+    tmem_st_wait();
+    hand_over(sh.p_tail[stage]);
     float a, b, c, d;
     split(sum[0], a, b);
     split(sum[1], c, d);
     l += (a + b) + (c + d);
-    tmem_st_wait();
     return true;
   }
 };
@@ -478,6 +504,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&sh.s_full[i][1], 1);
       mbar_init(&sh.p_full[i][0], 4);
       mbar_init(&sh.p_full[i][1], 4);
+      mbar_init(&sh.p_tail[i][0], 4);
+      mbar_init(&sh.p_tail[i][1], 4);
       mbar_init(&sh.pv_done[i], 1);
       mbar_init(&sh.o_full[i], 1);
       mbar_init(&sh.o_empty[i], 4);
@@ -736,7 +764,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               return;
             }
             const uint64_t b = k_desc + slot * (L::kv_tile >> 4);
-            const uint32_t buffer = issued++ & 1;
+            const uint32_t buffer = issued++ % kBuffers;
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k)
               mma_f16(tmem_s + attn::KEYS * buffer, q_desc + ((k / 4 * kQPanel + k % 4 * 32) >> 4),
@@ -754,8 +782,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (i >= masked) v_phase ^= 1u << slot;
             if (mine(i)) {
               if (i >= masked) wait(&sh.v_clean[slot], cleaned);
-              const uint32_t buffer = joined & 1;
-              wait(&sh.p_full[stage][buffer], joined >> 1 & 1);
+              const uint32_t buffer = joined % kBuffers, p_phase = joined / kBuffers & 1;
+              wait(&sh.p_full[stage][buffer], p_phase);
               const bool first = PAIR ? i == 0 : i < 2;
               if (first) {
                 wait(&sh.o_empty[stage], o_phase);
@@ -765,9 +793,14 @@ __global__ void __launch_bounds__(kThreads, 1)
               tc_fence_after();
               const uint64_t b = v_desc + slot * (L::kv_tile >> 4);
 #pragma unroll
-              for (int k = 0; k < attn::KEYS / 16; ++k)
+              for (int k = 0; k < attn::KEYS / 16; ++k) {
+                if (k == (attn::KEYS - kTail) / 16) {
+                  wait(&sh.p_tail[stage][buffer], p_phase);
+                  tc_fence_after();
+                }
                 mma_f16_tmem_a(tmem_o, tmem_s + attn::KEYS * buffer + 8 * k, b + (k * 2048 >> 4), idesc_o,
                                k > 0 || !first);
+              }
               tc_commit(&sh.pv_done[stage]);
               tc_commit(&sh.kv_empty[slot]);
               if (i == last) tc_commit(&sh.o_full[stage]);

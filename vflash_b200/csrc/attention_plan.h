@@ -31,7 +31,7 @@
 namespace vfb {
 namespace attn {
 
-constexpr int KEYS = 64;          // keys in a key tile
+constexpr int KEYS = 128;         // keys in a key tile
 constexpr int64_t OVERHEAD = 256; // a job's fixed cost, in keys
 constexpr int64_t SHARE = 512;    // a block's share is at least this long, unless that leaves jobs without blocks
 
