@@ -3,7 +3,7 @@
 // exactly the pieces of each job that was cut.
 //
 // Reads cases from standard input, one a line:
-//   split blocks grid groups job_tokens causal has_offsets batch total_q total_k  cu_q...  cu_k...  lengths_or_-1...
+//   split blocks key_shift grid groups job_tokens causal has_offsets batch total_q total_k  cu_q...  cu_k...  lengths_or_-1...
 // and prints "ok <cases> <cut jobs>" or the first contradiction.
 #include <cstdio>
 #include <cstdlib>
@@ -27,6 +27,7 @@ int main() {
   while (std::scanf("%lld", &split) == 1) {
     Plan p = {};
     p.blocks = static_cast<int32_t>(read_int());
+    p.key_shift = static_cast<int32_t>(read_int());
     const long long grid = read_int();
     p.groups = static_cast<int32_t>(read_int());
     p.job_tokens = static_cast<int32_t>(read_int());

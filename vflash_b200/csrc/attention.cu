@@ -1,7 +1,7 @@
 // Attention over packed sequences (vfb_attention) on tcgen05.
 //
 // For one tile of 128 query rows (the group's heads of as many tokens as fit,
-// row = token * pack + head in group) and the keys it sees, 64 at a time:
+// row = token * pack + head in group) and the keys it sees, a key tile at a time:
 //   S = Q K^T            tcgen05, fp32 in TMEM
 //   m' = max(m, row max) P = exp2((S - m') * scale * log2 e)   registers
 //   l = l * 2^(m - m') + row sum of P
@@ -11,31 +11,39 @@
 // maximum grows by more than kHold binary orders, so P may reach 2^kHold; the
 // result is the same to rounding and the pass over O in TMEM is rare.
 //
-// Roles of a block of sixteen warps, one block on an SM:
+// Roles of a block of twelve warps, one block on an SM:
 //   warps 0-3, 4-7  softmax of stage 0 and stage 1, one thread per row
 //   warp 8          TMA loads: Q tiles, then K and V tiles through one ring
-//   warps 9, 10     MMA issue of stage 0 and stage 1, one thread each
+//   warp 9          MMA issue, one thread
+//   warp 10         cleans the V tiles that hold keys some row must not see
 //   warp 11         works out the block's jobs and hands them to the others
-//   warps 12-15     clean the V tiles that hold keys some row must not see
 // The two stages keep the tensor cores busy with one tile's products while the
 // other's exponentials run.  They are
 //   PAIR: two tiles of query rows against the same keys (many query rows), or
 //   ALT:  one tile of query rows against even and odd key tiles, joined at the
 //         end (few query rows: single tokens, short pieces).
 //
-// TMEM (512 columns): S of stage 0 (two buffers of 64) | S of stage 1 | O0 | O1,
-// 128 columns each; P overwrites the first 32 columns of its S.  With two
-// buffers the scores of a stage's next tile are there before the softmax of
-// this one ends.  Key tiles of 64 are what makes room for that next to two
-// 128-column O: the product Q K^T then takes 48 instead of 32 cycles a step
-// (its operands are read from shared memory at 128 bytes a cycle), but tiles of
-// 128 keys with one buffer leave the chain S -> softmax -> P V -> next S exposed
-// (measured: 3150 cycles for 128 keys of both stages, of which 2050 are
-// products; with two buffers of 64 the products' 2520 are the bound).
+// TMEM (512 columns): S of stage 0 | S of stage 1 | O0 | O1, 128 columns each; P
+// overwrites the first columns of its S.  PAIR has key tiles of 128 and one
+// buffer of S: the products of a stage's tile, P V and then the next S, run
+// while the other stage is in its softmax.  One thread issues them, stage after
+// stage: with a thread for each, their products mix, both stages get their S at
+// one time and then compete for the exponentials (3900 cycles for a key tile of
+// both instead of 3150).  Key tiles of 64 with two buffers of S take the
+// chain S -> softmax -> P V -> S apart, but Q K^T with N = 64 takes 48 instead
+// of 32 cycles a step (its operands come from shared memory at 128 bytes a
+// cycle), and on long inputs the extra work costs more at the power limit
+// than it gains (16.2 against 14.1 ms for 32760 tokens of 32 heads).  ALT waits
+// for memory instead; there 64 keys mean shorter latencies and less padding.
+//
+// The exponentials (16 a cycle) take as long as the products of D = 128.  Some
+// of them as a polynomial on the FMA pipe shortened neither: the chip is at its
+// power limit here and the extra instructions cost clock (2 of 8: 15.1 against
+// 14.6 ms at the limit, 13.2 against 12.8 ms before it is reached).
 //
 // Keys behind a row's limit: their scores become -inf, so P = 0; but 0 * inf
-// and 0 * NaN would still spoil the second product.  Warps 12-15 therefore
-// zero, in the key tiles that any row of the block sees only in part, the V
+// and 0 * NaN would still spoil the second product.  Warp 10 therefore
+// zeroes, in the key tiles that any row of the block sees only in part, the V
 // rows behind the sequence's end and (causal) every element that is not
 // finite; the latter are added back at the end to the rows that do see them.
 #include "common.cuh"
@@ -49,15 +57,12 @@ using attn::Segment;
 
 constexpr int kTile = 128;           // query rows in a tile
 constexpr int kQPanel = kTile * 128;       // bytes of a tile's 64 elements of 16 bits, 128-byte swizzle
-constexpr int kKvPanel = attn::KEYS * 128;
-constexpr int kBuffers = 128 / attn::KEYS;  // of S, for a stage
 constexpr int kTail = 32;            // keys of a tile whose P is handed over separately
-constexpr int kThreads = 512;
+constexpr int kThreads = 384;
 constexpr int kRingSlots = 16;       // at most
 constexpr int kJobs = 2;             // jobs that the scheduler may be ahead
-constexpr int kJobReaders = 15;      // warps that follow the schedule
+constexpr int kJobReaders = 11;      // warps that follow the schedule
 constexpr float kHold = 8.0f;
-constexpr int kFmaPairs = 0;         // of every 8 pairs of exponentials, so many on the FMA pipe
 constexpr float kLn2 = 0.693147180559945309f;
 
 // Rows of a workspace slot (one piece of a job): both tiles of PAIR.
@@ -65,12 +70,15 @@ constexpr int kSlotRows = 2 * kTile;
 
 template <int DP, bool PAIR>
 struct Layout {
+  static constexpr int keys = PAIR ? 128 : 64;   // in a key tile
+  static constexpr int buffers = 128 / keys;     // of S, for a stage
   static constexpr int panels = DP / 64;
+  static constexpr int kv_panel = keys * 128;    // bytes
   static constexpr int q_tile = panels * kQPanel;
-  static constexpr int kv_tile = panels * kKvPanel;
+  static constexpr int kv_tile = panels * kv_panel;
   static constexpr int q_bytes = (PAIR ? 2 : 1) * q_tile;
-  static constexpr int ring = DP == 128 ? (PAIR ? 640 : 768) / attn::KEYS : 1024 / attn::KEYS;
-  static constexpr int ahead = (PAIR ? 1 : 2) * kBuffers;  // key tiles whose S is issued before the first P V
+  static constexpr int ring = DP == 128 ? (PAIR ? 5 : 12) : (PAIR ? 8 : 16);
+  static constexpr int ahead = PAIR ? 1 : 4;  // key tiles whose S is issued before the first P V
   static constexpr int smem = 1024 + q_bytes + ring * kv_tile;  // tiles start on 1024 bytes
 };
 
@@ -123,10 +131,10 @@ __device__ __forceinline__ void mma_f16_tmem_a(uint32_t d, uint32_t a, uint64_t 
 // Descriptor of a V tile read with the head dimension as N: rows of 64
 // contiguous N elements (128 bytes, swizzled), eight K rows to 1024 bytes, the
 // next 64 N elements one panel further.
-__device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t smem_addr) {
+__device__ __forceinline__ uint64_t sw128_mnmajor_desc(uint32_t smem_addr, uint32_t panel_bytes) {
   uint64_t desc = 0;
   desc |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
-  desc |= static_cast<uint64_t>(kKvPanel >> 4) << 16;  // leading offset: next 64 elements of N
+  desc |= static_cast<uint64_t>(panel_bytes >> 4) << 16;  // leading offset: next 64 elements of N
   desc |= static_cast<uint64_t>(1024 >> 4) << 32;         // stride offset: next eight rows of K
   desc |= static_cast<uint64_t>(1) << 46;
   desc |= static_cast<uint64_t>(2) << 61;
@@ -190,28 +198,6 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
   return r;
 }
 
-// 2^x on the FMA pipe, for x <= 126: x = n + f with n its nearest integer (read
-// off the low bits of x + 1.5 * 2^23) and |f| <= 1/2, 2^f by a polynomial of
-// degree 4, n added to its exponent.  The coefficients are those of the
-// minimax approximation of 2^f in relative error over [-1/2, 1/2], fitted
-// numerically (iteratively reweighted least squares); error at most 2.7e-6 in
-// fp32.  Below 2^-126 (and for NaN) it is 0.
-__device__ __forceinline__ void exp2_fma(f32x2 x, float &lo, float &hi) {
-  const f32x2 magic = pair(12582912.0f, 12582912.0f), minus = pair(-12582912.0f, -12582912.0f);
-  const f32x2 t = add2(x, magic);
-  const f32x2 f = fma2(add2(t, minus), pair(-1.0f, -1.0f), x);
-  f32x2 y = fma2(f, pair(0.009570086374878883f, 0.009570086374878883f), pair(0.055917851626873016f, 0.055917851626873016f));
-  y = fma2(y, f, pair(0.240247443318367f, 0.240247443318367f));
-  y = fma2(y, f, pair(0.6931217908859253f, 0.6931217908859253f));
-  y = fma2(y, f, pair(0.9999992847442627f, 0.9999992847442627f));
-  float x0, x1, t0, t1, y0, y1;
-  split(x, x0, x1);
-  split(t, t0, t1);
-  split(y, y0, y1);
-  lo = x0 > -126.0f ? __uint_as_float(__float_as_uint(y0) + (__float_as_uint(t0) << 23)) : 0.0f;
-  hi = x1 > -126.0f ? __uint_as_float(__float_as_uint(y1) + (__float_as_uint(t1) << 23)) : 0.0f;
-}
-
 // Maximum that keeps NaN.
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float r;
@@ -265,14 +251,14 @@ __device__ __forceinline__ void describe(const Params &p, const Segment &s, Job 
   j.t0 = s.t0;
   j.t1 = s.t1;
   j.min_seen = attn::keys_seen(p.plan, s.seq, static_cast<int64_t>(j.rows0) + 1);
-  j.first_masked = j.min_seen / attn::KEYS;
+  j.first_masked = j.min_seen >> p.plan.key_shift;
   j.slot = s.slot;
   j.behind = p.plan.cu_q != nullptr && s.b == p.plan.batch;
   const int32_t tiles = max(s.t1 - s.t0, 0);
   if (PAIR) {
     // stage 0's rows may see fewer keys than the job's last row
     const int32_t seen0 = attn::keys_seen(p.plan, s.seq, static_cast<int64_t>(j.rows0) + min(p.tokens, j.count));
-    j.n[0] = max(min(s.t1, (seen0 + attn::KEYS - 1) / attn::KEYS) - s.t0, 0);
+    j.n[0] = max(min(s.t1, (seen0 + 127) / 128) - s.t0, 0);
     j.n[1] = j.count > p.tokens ? tiles : 0;
   } else {
     j.n[0] = (tiles + 1) / 2;
@@ -350,6 +336,7 @@ struct RingPos {
 // Row state, and the loop over a job's key tiles.
 template <typename T, int DP, bool PAIR>
 struct Softmax {
+  static constexpr int N = Layout<DP, PAIR>::keys, kBuffers = Layout<DP, PAIR>::buffers;
   const Params &p;
   Shared &sh;
   const uint32_t tmem_s, tmem_o;  // this warp's lanes
@@ -370,7 +357,7 @@ struct Softmax {
       if (!wait(&sh.s_full[stage][count % kBuffers], count / kBuffers & 1)) return false;
       tc_fence_after();
       if (live) {
-        if (!tile((t0 + i * stride) * attn::KEYS, limit, i > 0, valid)) return false;
+        if (!tile((t0 + i * stride) * N, limit, i > 0, valid)) return false;
       } else {
         hand_over(sh.p_full[stage]);
         hand_over(sh.p_tail[stage]);
@@ -386,7 +373,6 @@ struct Softmax {
   }
 
   __device__ __forceinline__ bool tile(int32_t key0, int32_t limit, bool scale_o, bool valid) {
-    constexpr int N = attn::KEYS;
     const uint32_t at = tmem_s + N * (count % kBuffers);
     float s[N];
     {
@@ -445,13 +431,9 @@ struct Softmax {
       for (int j = 0; j < 16; ++j) {
         const f32x2 x = fma2(pair(s[32 * h + 2 * j], s[32 * h + 2 * j + 1]), scale2, base2);
         float a, b;
-        if (j % 8 >= 8 - kFmaPairs) {
-          exp2_fma(x, a, b);
-        } else {
-          split(x, a, b);
-          a = ex2(a);
-          b = ex2(b);
-        }
+        split(x, a, b);
+        a = ex2(a);
+        b = ex2(b);
         sum[j & 1] = add2(sum[j & 1], pair(a, b));
         packed[j] = pack2<T>(a, b);
       }
@@ -477,6 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Params p) {
   using L = Layout<DP, PAIR>;
+  constexpr int kKeys = L::keys, kBuffers = L::buffers;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem =
       reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -488,12 +471,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
     mbar_init(&sh.q_full, 1);
-    mbar_init(&sh.q_empty, 2);
+    mbar_init(&sh.q_empty, 1);
     for (int i = 0; i < L::ring; ++i) {
       mbar_init(&sh.kv_full[i], 1);
-      mbar_init(&sh.kv_empty[i], 2);
+      mbar_init(&sh.kv_empty[i], 1);
       mbar_init(&sh.v_todo[i], 1);
-      mbar_init(&sh.v_clean[i], 4);
+      mbar_init(&sh.v_clean[i], 1);
     }
     for (int i = 0; i < kJobs; ++i) {
       mbar_init(&sh.job_full[i], 1);
@@ -512,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     mbar_init(&sh.stats_full, 4);
     mbar_init(&sh.stats_empty, 4);
-    mbar_init(&sh.drain, 2);
+    mbar_init(&sh.drain, 1);
     sh.abort = 0;
     sh.dirty = 0;
     fence_mbar_init();
@@ -537,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   Job job;
 
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     const int stage = warp / 4;
     const int row = (warp % 4) * 32 + lane;  // of the tile, and TMEM lane
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp % 4) * 32) << 16);
@@ -595,8 +578,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       // A row of infinite scores is NaN however its exponentials were rounded.
       if (m == INFINITY) l = NAN;
-      const int64_t piece_end = attn::min64(limit, static_cast<int64_t>(job.t1) * attn::KEYS);
-      const bool none = piece_end <= static_cast<int64_t>(job.t0) * attn::KEYS;
+      const int64_t piece_end = attn::min64(limit, static_cast<int64_t>(job.t1) * kKeys);
+      const bool none = piece_end <= static_cast<int64_t>(job.t0) * kKeys;
       const float inv = none ? 0.0f : 1.0f / l;
       const int64_t out_row = job.row0 + token;
       const int head = job.group * p.pack + head_in_tile;
@@ -638,7 +621,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (valid && dirty && !none) {
             // the elements that were taken out, for the rows that see them
             const int kv_head = job.group * p.pack / p.group_heads;
-            const int64_t from = static_cast<int64_t>(max(job.first_masked, job.t0)) * attn::KEYS;
+            const int64_t from = static_cast<int64_t>(max(job.first_masked, job.t0)) * kKeys;
             const T *v = static_cast<const T *>(p.v) + kv_head * p.v_head_stride + job.k0 * p.v_token_stride;
             for (int64_t key = from; key < piece_end; ++key) {
 #pragma unroll
@@ -674,7 +657,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     if (warp == 8) {
       // ---------------- TMA producer ----------------
       RingPos<L::ring> pos;
@@ -687,7 +670,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (ok && leader) {
           mbar_arrive_expect_tx(&sh.kv_full[pos.slot], L::kv_tile);
           for (int i = 0; i < L::panels; ++i)
-            tma_load_3d(s_kv + pos.slot * L::kv_tile + i * kKvPanel, map, &sh.kv_full[pos.slot], 64 * i,
+            tma_load_3d(s_kv + pos.slot * L::kv_tile + i * L::kv_panel, map, &sh.kv_full[pos.slot], 64 * i,
                         kv_head, static_cast<int32_t>(key));
           if (masked) mbar_arrive(&sh.v_todo[pos.slot]);
         }
@@ -710,13 +693,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         q_loaded = true;
         q_phase ^= 1;
         const int32_t kv_head = job.group * p.pack / p.group_heads;
-        const int64_t k0 = job.k0 + static_cast<int64_t>(job.t0) * attn::KEYS;
+        const int64_t k0 = job.k0 + static_cast<int64_t>(job.t0) * kKeys;
         for (int32_t i = 0; i < min(tiles, L::ahead); ++i)
-          load(&map_k, kv_head, k0 + static_cast<int64_t>(i) * attn::KEYS, false);
+          load(&map_k, kv_head, k0 + static_cast<int64_t>(i) * kKeys, false);
         for (int32_t i = 0; i < tiles && ok; ++i) {
-          load(&map_v, kv_head, k0 + static_cast<int64_t>(i) * attn::KEYS, job.t0 + i >= job.first_masked);
+          load(&map_v, kv_head, k0 + static_cast<int64_t>(i) * kKeys, job.t0 + i >= job.first_masked);
           if (i + L::ahead < tiles)
-            load(&map_k, kv_head, k0 + static_cast<int64_t>(i + L::ahead) * attn::KEYS, false);
+            load(&map_k, kv_head, k0 + static_cast<int64_t>(i + L::ahead) * kKeys, false);
         }
       }
       // every load has landed before the block ends (a finished run waits for nothing here)
@@ -725,90 +708,100 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t last = i < pos.slot ? pos.phase : pos.phase ^ 1;
         if (issued >> i & 1) warp_wait_quick(&sh.kv_full[i], last, &sh.abort, p.status);
       }
-    } else if (warp == 9 || warp == 10) {
+    } else if (warp == 9) {
       // ---------------- MMA issue ----------------
-      // One thread for a stage.  Between two products it passes two or three
-      // barriers that are usually ready (38 cycles each) and prepares operands:
-      // as one warp for both stages with an elected lane that took 2240 cycles for a
-      // key tile of both (one thread for both: 1840), whose products take 1260.
-      // Both follow every item of the ring, also those of the other's tiles, so
-      // neither is ever a pass ahead or behind.  Products run over the padded head
-      // dimension: TMA filled the rest with zeros.
+      // One thread: between two products it passes two or three barriers that are
+      // usually ready (38 cycles each), which as a warp with an elected lane (branches,
+      // votes, reconvergence) took longer than the products.  Products run over the
+      // padded head dimension: TMA filled the rest with zeros.
       if (elect_one()) {
-        const int stage = warp - 9;
-        const uint32_t idesc_s = idesc_f16<T>(attn::KEYS, false);
+        const uint32_t idesc_s = idesc_f16<T>(kKeys, false);
         const uint32_t idesc_o = idesc_f16<T>((p.dim + 15) / 16 * 16, true);
-        const uint64_t q_desc = sw128_kmajor_desc(smem_u32(s_q) + (PAIR ? stage * L::q_tile : 0));
-        const uint64_t k_desc = sw128_kmajor_desc(smem_u32(s_kv)), v_desc = sw128_mnmajor_desc(smem_u32(s_kv));
-        const uint32_t tmem_s = tmem + 128 * stage, tmem_o = tmem + 256 + 128 * stage;
+        const uint64_t q_desc = sw128_kmajor_desc(smem_u32(s_q)), k_desc = sw128_kmajor_desc(smem_u32(s_kv));
+        const uint64_t v_desc = sw128_mnmajor_desc(smem_u32(s_kv), L::kv_panel);
         RingPos<L::ring> pos;      // the item that is waited for next
-        uint32_t q_phase = 0, o_phase = 1;
-        uint32_t issued = 0, joined = 0;  // S and P V so far, over all jobs
+        uint32_t q_phase = 0, o_phase[2] = {1, 1};
+        uint32_t issued[2] = {0, 0}, joined[2] = {0, 0};  // S and P V of each stage so far, over all jobs
         uint32_t v_phase = 0;  // a bit for every slot
         const auto wait = [&](uint64_t *bar, uint32_t phase) { mbar_wait_through(bar, phase, &sh.abort, p.status); };
+        const auto product_s = [&](int stage, int slot) {  // S = Q K^T
+          const uint64_t a = q_desc + (PAIR ? stage * (L::q_tile >> 4) : 0);
+          const uint64_t b = k_desc + slot * (L::kv_tile >> 4);
+          const uint32_t buffer = issued[stage]++ % kBuffers;
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k)
+            mma_f16(tmem + 128 * stage + kKeys * buffer, a + ((k / 4 * kQPanel + k % 4 * 32) >> 4),
+                    b + ((k / 4 * L::kv_panel + k % 4 * 32) >> 4), idesc_s, k > 0);
+          tc_commit(&sh.s_full[stage][buffer]);
+        };
+        const auto product_o = [&](int stage, int slot, bool first, bool last) {  // O (+)= P V
+          const uint32_t buffer = joined[stage] % kBuffers, phase = joined[stage] / kBuffers & 1;
+          ++joined[stage];
+          wait(&sh.p_full[stage][buffer], phase);
+          if (first) {
+            wait(&sh.o_empty[stage], o_phase[stage]);
+            o_phase[stage] ^= 1;
+          }
+          tc_fence_after();
+          const uint64_t b = v_desc + slot * (L::kv_tile >> 4);
+          const uint32_t a = tmem + 128 * stage + kKeys * buffer;
+#pragma unroll
+          for (int k = 0; k < kKeys / 16; ++k) {
+            if (k == (kKeys - kTail) / 16) {
+              wait(&sh.p_tail[stage][buffer], phase);
+              tc_fence_after();
+            }
+            mma_f16_tmem_a(tmem + 256 + 128 * stage, a + 8 * k, b + (k * 2048 >> 4), idesc_o, k > 0 || !first);
+          }
+          tc_commit(&sh.pv_done[stage]);
+          if (last) tc_commit(&sh.o_full[stage]);
+        };
         while (jobs.next_alone(job)) {
-          const int32_t tiles = job.tiles(PAIR), own = job.n[stage];
+          const int32_t tiles = job.tiles(PAIR), n0 = job.n[0], n1 = job.n[1];
           const int32_t masked = max(job.first_masked - job.t0, 0);  // tiles from here on
           if (tiles == 0) continue;
           wait(&sh.q_full, q_phase);
           q_phase ^= 1;
-          if (own == 0) mbar_arrive(&sh.q_empty);
-          const auto mine = [&](int32_t i) { return PAIR ? i < own : (i & 1) == stage; };
-          const int32_t last = PAIR ? own - 1 : 2 * (own - 1) + stage;  // of this stage's tiles
-          const auto scores = [&](int32_t i) {  // S = Q K^T of key tile i
+          // Scores of key tile i (its K is the next item); with `join`, behind the P V of
+          // tile i - ahead, stage after stage.
+          const auto step = [&](int32_t i, bool join, int v_slot) {
+            const int32_t at = i - L::ahead;
             const int slot = pos.slot;
-            wait(&sh.kv_full[slot], pos.phase);
-            pos.step();
-            if (!mine(i)) {
-              mbar_arrive(&sh.kv_empty[slot]);
-              return;
-            }
-            const uint64_t b = k_desc + slot * (L::kv_tile >> 4);
-            const uint32_t buffer = issued++ % kBuffers;
+            const bool more = i < tiles;
+            bool arrived = false;
+            const auto scores = [&](int s) {
+              if (!arrived) wait(&sh.kv_full[slot], pos.phase);
+              arrived = true;
+              product_s(s, slot);
+            };
+            if (PAIR) {
 #pragma unroll
-            for (int k = 0; k < DP / 16; ++k)
-              mma_f16(tmem_s + attn::KEYS * buffer, q_desc + ((k / 4 * kQPanel + k % 4 * 32) >> 4),
-                      b + ((k / 4 * kKvPanel + k % 4 * 32) >> 4), idesc_s, k > 0);
-            tc_commit(&sh.s_full[stage][buffer]);
-            tc_commit(&sh.kv_empty[slot]);
-            if (i == last) tc_commit(&sh.q_empty);
-          };
-          for (int32_t i = 0; i < min(tiles, L::ahead); ++i) scores(i);
-          for (int32_t i = 0; i < tiles; ++i) {  // O (+)= P V of key tile i
-            const int slot = pos.slot;
-            wait(&sh.kv_full[slot], pos.phase);
-            pos.step();
-            const uint32_t cleaned = v_phase >> slot & 1;
-            if (i >= masked) v_phase ^= 1u << slot;
-            if (mine(i)) {
-              if (i >= masked) wait(&sh.v_clean[slot], cleaned);
-              const uint32_t buffer = joined % kBuffers, p_phase = joined / kBuffers & 1;
-              wait(&sh.p_full[stage][buffer], p_phase);
-              const bool first = PAIR ? i == 0 : i < 2;
-              if (first) {
-                wait(&sh.o_empty[stage], o_phase);
-                o_phase ^= 1;
+              for (int s = 0; s < 2; ++s) {
+                const int32_t n = s == 0 ? n0 : n1;
+                if (join && at < n) product_o(s, v_slot, at == 0, at == n - 1);
+                if (i < n) scores(s);
               }
-              ++joined;
-              tc_fence_after();
-              const uint64_t b = v_desc + slot * (L::kv_tile >> 4);
-#pragma unroll
-              for (int k = 0; k < attn::KEYS / 16; ++k) {
-                if (k == (attn::KEYS - kTail) / 16) {
-                  wait(&sh.p_tail[stage][buffer], p_phase);
-                  tc_fence_after();
-                }
-                mma_f16_tmem_a(tmem_o, tmem_s + attn::KEYS * buffer + 8 * k, b + (k * 2048 >> 4), idesc_o,
-                               k > 0 || !first);
-              }
-              tc_commit(&sh.pv_done[stage]);
-              tc_commit(&sh.kv_empty[slot]);
-              if (i == last) tc_commit(&sh.o_full[stage]);
             } else {
-              mbar_arrive(&sh.kv_empty[slot]);
+              if (join) product_o(at & 1, v_slot, at < 2, at + 2 >= tiles);
+              if (more) scores(i & 1);
             }
-            // S of the tile whose buffer that P V frees
-            if (i + L::ahead < tiles) scores(i + L::ahead);
+            if (join) tc_commit(&sh.kv_empty[v_slot]);
+            if (more) {
+              pos.step();
+              tc_commit(&sh.kv_empty[slot]);
+              if (i == tiles - 1) tc_commit(&sh.q_empty);
+            }
+          };
+          for (int32_t i = 0; i < min(tiles, L::ahead); ++i) step(i, false, 0);
+          for (int32_t i = 0; i < tiles; ++i) {
+            const int v_slot = pos.slot;
+            wait(&sh.kv_full[v_slot], pos.phase);
+            pos.step();
+            if (i >= masked) {
+              wait(&sh.v_clean[v_slot], v_phase >> v_slot & 1);
+              v_phase ^= 1u << v_slot;
+            }
+            step(i + L::ahead, true, v_slot);
           }
         }
         // the products issued last are over before the block ends
@@ -855,14 +848,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         todo_phase ^= 1u << slot;
         if (!warp_wait_quick(&sh.kv_full[slot], pos.phase, &sh.abort, p.status)) return false;
         uint8_t *tile = s_kv + slot * L::kv_tile;
-        const int32_t end = min(max(job.nk - t * attn::KEYS, 0), attn::KEYS);       // rows of the sequence
-        const int32_t all = min(max(job.min_seen - t * attn::KEYS, 0), attn::KEYS);       // rows that every row sees
-        const int row = (warp - 12) * 4 + lane / 8;  // lanes: eight 16-byte pieces of four rows
+        const int32_t end = min(max(job.nk - t * kKeys, 0), kKeys);       // rows of the sequence
+        const int32_t all = min(max(job.min_seen - t * kKeys, 0), kKeys);       // rows that every row sees
+        const int row = lane / 8;  // lanes: eight 16-byte pieces of four rows
 #pragma unroll
         for (int panel = 0; panel < L::panels; ++panel) {
-          uint8_t *column = tile + panel * kKvPanel + lane % 8 * 16;
-#pragma unroll 2
-          for (int r = all + row; r < end; r += 16) {
+          uint8_t *column = tile + panel * L::kv_panel + lane % 8 * 16;
+#pragma unroll 4
+          for (int r = all + row; r < end; r += 4) {
             uint4 *at = reinterpret_cast<uint4 *>(column + r * 128);
             uint4 x = *at;
             uint32_t *word = reinterpret_cast<uint32_t *>(&x);
@@ -878,8 +871,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               *reinterpret_cast<volatile int *>(&sh.dirty) = 1;
             }
           }
-#pragma unroll 2
-          for (int r = end + row; r < attn::KEYS; r += 16)
+#pragma unroll 4
+          for (int r = end + row; r < kKeys; r += 4)
             *reinterpret_cast<uint4 *>(column + r * 128) = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
@@ -994,7 +987,7 @@ Choice choose(const vfb_attention_args &a) {
                             : attn::min64(a.total_q, a.total_q / tokens + a.batch + 1);
   c.jobs = tiles * c.groups;
   // Whole jobs balance by themselves when there are many; few keys are not worth cutting.
-  c.split = c.jobs < 4 * kMaxBlocks && a.total_k > 2 * attn::KEYS;
+  c.split = c.jobs < 4 * kMaxBlocks && a.total_k > 256;
   return c;
 }
 
@@ -1112,6 +1105,7 @@ extern "C" int vfb_attention(const vfb_attention_args *args, void *stream) {
   p.plan.job_tokens = c.tokens * (c.pair ? 2 : 1);
   p.plan.causal = a.causal != 0;
   p.plan.blocks = sms < kMaxBlocks ? sms : kMaxBlocks;
+  p.plan.key_shift = c.pair ? 7 : 6;
   p.v = a.v;
   p.out = a.out;
   p.lse = a.lse;
@@ -1140,10 +1134,10 @@ extern "C" int vfb_attention(const vfb_attention_args *args, void *stream) {
   const bool keys = a.total_k > 0;
   if (rc == VFB_OK)
     rc = make_map(&mk, keys ? a.k : a.q, a.dtype, a.dim, a.kv_heads, keys ? a.total_k : 1, a.k_head_stride,
-                  a.k_token_stride, 1, attn::KEYS);
+                  a.k_token_stride, 1, c.pair ? 128 : 64);
   if (rc == VFB_OK)
     rc = make_map(&mv, keys ? a.v : a.q, a.dtype, a.dim, a.kv_heads, keys ? a.total_k : 1, a.v_head_stride,
-                  a.v_token_stride, 1, attn::KEYS);
+                  a.v_token_stride, 1, c.pair ? 128 : 64);
   if (rc != VFB_OK) return rc;
 
   cudaStream_t s = static_cast<cudaStream_t>(stream);

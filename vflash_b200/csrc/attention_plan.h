@@ -1,7 +1,7 @@
 // The work order of the packed attention kernel, shared with its CPU test.
 //
 // A job is one tile of query rows of one sequence for one group of heads that
-// read the same keys; its keys come in key tiles of KEYS.  Two orders:
+// read the same keys; its keys come in key tiles of 64 or 128 (Plan::key_shift).  Two orders:
 //
 // * whole jobs (`split` false): job i of the list goes to block i (or is
 //   strided over the blocks), every job by itself;
@@ -31,7 +31,6 @@
 namespace vfb {
 namespace attn {
 
-constexpr int KEYS = 128;         // keys in a key tile
 constexpr int64_t OVERHEAD = 256; // a job's fixed cost, in keys
 constexpr int64_t SHARE = 512;    // a block's share is at least this long, unless that leaves jobs without blocks
 
@@ -46,6 +45,7 @@ struct Plan {
   int32_t job_tokens;  // query tokens in a job
   int32_t causal;
   int32_t blocks;      // blocks that even shares are cut for, at most
+  int32_t key_shift;   // log2 of the keys in a key tile
 };
 
 // Sequence b: its rows and keys, clamped to the buffers.  b == batch stands for
@@ -111,10 +111,10 @@ VFB_HD int64_t jobs_length(const Plan &p, const Seq &s, int64_t tiles) {
 
 // Moves a cut at `off` inside a job of `keys` keys to a key tile's border or to
 // one of the job's ends.
-VFB_HD int64_t snap(int64_t off, int64_t keys) {
-  const int64_t tile = off <= OVERHEAD ? 0 : (off - OVERHEAD + KEYS / 2) / KEYS;
-  if (off <= 0 || tile == 0) return 0;
-  return tile * KEYS >= keys ? OVERHEAD + keys : OVERHEAD + tile * KEYS;
+VFB_HD int64_t snap(const Plan &p, int64_t off, int64_t keys) {
+  const int64_t at = off <= OVERHEAD ? 0 : (off - OVERHEAD + (1 << p.key_shift) / 2) >> p.key_shift << p.key_shift;
+  if (at == 0) return 0;
+  return OVERHEAD + min64(at, keys);
 }
 
 // ---- scans over the sequences --------------------------------------------------
@@ -235,7 +235,7 @@ VFB_HD Place place_at(const Plan &p, int64_t x) {
   const int64_t raw = in - jobs_length(p, a.seq, lo);
   a.keys = job_keys(p, a.seq, lo);
   a.start = x - raw;
-  a.off = snap(raw, a.keys);
+  a.off = snap(p, raw, a.keys);
   return a;
 }
 
@@ -315,8 +315,8 @@ class Order {
     s.group = at_.group;
     s.tile = at_.tile;
     const int32_t tiles = tiles_of(p, s.seq, s.tile);
-    s.t0 = at_.off == 0 ? 0 : static_cast<int32_t>(min64((at_.off - OVERHEAD) / KEYS, tiles));
-    s.t1 = stop == job_end ? tiles : static_cast<int32_t>(min64((stop - at_.start - OVERHEAD) / KEYS, tiles));
+    s.t0 = at_.off == 0 ? 0 : static_cast<int32_t>(min64((at_.off - OVERHEAD) >> p.key_shift, tiles));
+    s.t1 = stop == job_end ? tiles : static_cast<int32_t>(min64((stop - at_.start - OVERHEAD) >> p.key_shift, tiles));
     s.slot = at_.off == 0 && stop == job_end ? -1 : 2 * block_ + (first_ ? 0 : 1);
     first_ = false;
     next_ = stop;
@@ -328,7 +328,7 @@ class Order {
 
   static VFB_HD int32_t tiles_of(const Plan &p, const Seq &s, int32_t tile) {
     const int32_t keys = keys_seen(p, s, min64((static_cast<int64_t>(tile) + 1) * p.job_tokens, s.nq));
-    return (keys + KEYS - 1) / KEYS;
+    return static_cast<int32_t>((static_cast<int64_t>(keys) + (1 << p.key_shift) - 1) >> p.key_shift);
   }
 
  private:
