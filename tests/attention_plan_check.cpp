@@ -3,7 +3,7 @@
 // exactly the pieces of each job that was cut.
 //
 // Reads cases from standard input, one a line:
-//   split blocks key_shift grid groups job_tokens causal has_offsets batch total_q total_k  cu_q...  cu_k...  lengths_or_-1...
+//   split blocks key_shift unit_shift grid groups job_tokens causal has_offsets batch total_q total_k  cu_q...  cu_k...  lengths_or_-1...
 // and prints "ok <cases> <cut jobs>" or the first contradiction.
 #include <cstdio>
 #include <cstdlib>
@@ -28,14 +28,15 @@ int main() {
     Plan p = {};
     p.blocks = static_cast<int32_t>(read_int());
     p.key_shift = static_cast<int32_t>(read_int());
+    p.unit_shift = static_cast<int32_t>(read_int());
     const long long grid = read_int();
     p.groups = static_cast<int32_t>(read_int());
-    p.job_tokens = static_cast<int32_t>(read_int());
+    set_job_tokens(p, static_cast<int32_t>(read_int()));
     p.causal = static_cast<int32_t>(read_int());
     const long long offsets = read_int();
     p.batch = static_cast<int32_t>(read_int());
-    p.total_q = read_int();
-    p.total_k = read_int();
+    p.total_q = static_cast<int32_t>(read_int());
+    p.total_k = static_cast<int32_t>(read_int());
     std::vector<int32_t> cu_q, cu_k, lengths;
     for (int i = 0; i <= p.batch; ++i) cu_q.push_back(static_cast<int32_t>(read_int()));
     for (int i = 0; i <= p.batch; ++i) cu_k.push_back(static_cast<int32_t>(read_int()));
@@ -61,13 +62,13 @@ int main() {
         records.push_back(record);
         if (order.empty()) empty_slots.insert(2 * block);
       } else {
-        order.init_whole(p, block, static_cast<int32_t>(grid));
+        order.init_whole(block, static_cast<int32_t>(grid));
       }
       Segment s;
       while (order.next(p, s)) {
         const Job job{s.b, s.group, s.tile};
         if (s.seq.tiles <= s.tile || s.tile < 0 || s.group < 0 || s.group >= p.groups) return std::printf("bad job\n"), 1;
-        const int tiles = Order::tiles_of(p, s.seq, s.tile);
+        const int tiles = tiles_of(p, s.seq, s.tile);
         if (s.t0 < 0 || s.t1 > tiles || s.t1 < s.t0) return std::printf("bad tiles %d %d of %d\n", s.t0, s.t1, tiles), 1;
         for (int t = s.t0; t < s.t1; ++t)
           if (!done[job].insert(t).second) return std::printf("tile twice\n"), 1;
@@ -87,7 +88,7 @@ int main() {
       for (int g = 0; g < p.groups; ++g)
         for (int t = 0; t < s.tiles; ++t) {
           const auto it = done.find(Job{b, g, t});
-          if (it == done.end() || static_cast<int>(it->second.size()) != Order::tiles_of(p, s, t))
+          if (it == done.end() || static_cast<int>(it->second.size()) != tiles_of(p, s, t))
             return std::printf("job %d %d %d not done\n", b, g, t), 1;
         }
     }
@@ -115,8 +116,8 @@ int main() {
       if (!joined.insert(job).second) return std::printf("joined twice\n"), 1;
       if (real != by_job[job]) return std::printf("join misses pieces\n"), 1;
       const Seq s = sequence(p, std::get<0>(job));
-      const int64_t rows0 = static_cast<int64_t>(std::get<2>(job)) * p.job_tokens;
-      if (r.row0 != s.q0 + rows0 || r.group != std::get<1>(job) || r.count != min64(p.job_tokens, s.nq - rows0))
+      const int32_t rows0 = std::get<2>(job) * p.job_tokens;
+      if (r.row0 != s.q0 + rows0 || r.group != std::get<1>(job) || r.count != min32(p.job_tokens, s.nq - rows0))
         return std::printf("record of another job\n"), 1;
       ++cuts;
     }

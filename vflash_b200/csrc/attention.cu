@@ -148,15 +148,15 @@ __device__ __forceinline__ constexpr uint32_t idesc_f16(int n, bool b_mn_major) 
          (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
 }
 
-__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t *r) {
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  __syncwarp();
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
-      "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
-      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
       : "memory");
 }
 
@@ -242,7 +242,7 @@ struct Job {
 template <bool PAIR>
 __device__ __forceinline__ void describe(const Params &p, const Segment &s, Job &j) {
   j.rows0 = s.tile * p.plan.job_tokens;
-  j.row0 = s.seq.q0 + j.rows0;
+  j.row0 = static_cast<int64_t>(s.seq.q0) + j.rows0;
   j.k0 = s.seq.k0;
   j.count = min(p.plan.job_tokens, s.seq.nq - j.rows0);
   j.nq = s.seq.nq;
@@ -250,14 +250,14 @@ __device__ __forceinline__ void describe(const Params &p, const Segment &s, Job 
   j.group = s.group;
   j.t0 = s.t0;
   j.t1 = s.t1;
-  j.min_seen = attn::keys_seen(p.plan, s.seq, static_cast<int64_t>(j.rows0) + 1);
+  j.min_seen = attn::keys_seen(p.plan, s.seq, j.rows0 + 1);
   j.first_masked = j.min_seen >> p.plan.key_shift;
   j.slot = s.slot;
   j.behind = p.plan.cu_q != nullptr && s.b == p.plan.batch;
   const int32_t tiles = max(s.t1 - s.t0, 0);
   if (PAIR) {
     // stage 0's rows may see fewer keys than the job's last row
-    const int32_t seen0 = attn::keys_seen(p.plan, s.seq, static_cast<int64_t>(j.rows0) + min(p.tokens, j.count));
+    const int32_t seen0 = attn::keys_seen(p.plan, s.seq, j.rows0 + min(p.tokens, j.count));
     j.n[0] = max(min(s.t1, (seen0 + 127) / 128) - s.t0, 0);
     j.n[1] = j.count > p.tokens ? tiles : 0;
   } else {
@@ -303,6 +303,21 @@ struct JobReader {
       phase ^= 1;
     }
     return j.count >= 0;
+  }
+
+  // The next job in place, for a warp that reads its fields when it needs them (the
+  // softmax warps have no register to spare) and gives it back with done().
+  __device__ __forceinline__ bool peek() {
+    return warp_wait_quick(&sh.job_full[slot], phase, &sh.abort, status) && here().count >= 0;
+  }
+  __device__ __forceinline__ const Job &here() const { return sh.jobs[slot]; }
+  __device__ __forceinline__ void done() {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.job_empty[slot]);
+    if (++slot == kJobs) {
+      slot = 0;
+      phase ^= 1;
+    }
   }
 
   // The next job; false when there is none (or a wait ran out).
@@ -410,14 +425,12 @@ struct Softmax {
         if (!wait(&sh.pv_done[stage], (count - 1) & 1)) return false;
         tc_fence_after();
 #pragma unroll 1
-        for (int c = 0; c < DP; c += 32) {
-          uint32_t r[32];
-          tmem_ld_32x32b_x32_issue(tmem_o + c, r);
-          tmem_ld_wait();
-          tmem_ld_fence(r);
+        for (int c = 0; c < DP; c += 16) {  // few columns at a time: S holds the registers
+          uint32_t r[16];
+          tmem_ld_32x32b_x16(tmem_o + c, r);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * alpha);
-          tmem_st_32x32b_x32(tmem_o + c, r);
+          for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * alpha);
+          tmem_st_32x32b_x16(tmem_o + c, r);
         }
       }
     }
@@ -519,6 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   JobReader jobs{sh, p.status};
   Job job;
 
+  // The block was launched with 168 registers a thread: 200 * 256 + 96 * 128 fit.
   if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     const int stage = warp / 4;
@@ -528,7 +542,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t o_phase[2] = {0, 0}, stats_phase = 0;
     const int token_in_tile = row / p.pack;
     const int head_in_tile = row - token_in_tile * p.pack;
-    while (jobs.next(job)) {
+    for (; jobs.peek(); jobs.done()) {
+      const Job &job = jobs.here();
       const int token = token_in_tile + (PAIR ? stage * p.tokens : 0);  // of the job
       const bool valid = token_in_tile < p.tokens && token < job.count;
       int32_t limit = valid ? job.nk : 0;
@@ -590,40 +605,33 @@ __global__ void __launch_bounds__(kThreads, 1)
         part = p.part_o + at * p.dim;
         if (valid) p.part_lse[at] = none ? -INFINITY : m * p.scale_log2 + log2f(l);
       } else if (valid && p.lse != nullptr) {
-        p.lse[head * p.plan.total_q + out_row] = none ? -INFINITY : (m * p.scale_log2 + log2f(l)) * kLn2;
+        p.lse[static_cast<int64_t>(head) * p.plan.total_q + out_row] = none ? -INFINITY : (m * p.scale_log2 + log2f(l)) * kLn2;
       }
       const bool dirty = *reinterpret_cast<volatile int *>(&sh.dirty) != 0;
       if (live) {
+        const float g0 = f[0] * inv, g1 = f[1] * inv;
+        const uint32_t from = lanes + 256 + (PAIR ? 128 * stage : 0);
 #pragma unroll 1
         for (int c = 0; c < DP; c += 32) {
           if (c >= p.dim) break;
+          uint32_t r[32], r1[32];
+          if (have[0]) tmem_ld_32x32b_x32_issue(from + c, r);
+          if (!PAIR && have[1]) tmem_ld_32x32b_x32_issue(from + 128 + c, r1);
+          tmem_ld_wait();
+          if (have[0]) tmem_ld_fence(r);
+          if (!PAIR && have[1]) tmem_ld_fence(r1);
           float o[32];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) o[j] = 0.0f;
-          if (have[0]) {
-            uint32_t r[32];
-            tmem_ld_32x32b_x32_issue(lanes + 256 + (PAIR ? 128 * stage : 0) + c, r);
-            tmem_ld_wait();
-            tmem_ld_fence(r);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = f[0] == 0.0f ? 0.0f : __uint_as_float(r[j]) * f[0];
+          for (int j = 0; j < 32; ++j) {
+            o[j] = have[0] ? __uint_as_float(r[j]) * g0 : 0.0f;
+            if (!PAIR && have[1]) o[j] = fmaf(__uint_as_float(r1[j]), g1, o[j]);
           }
-          if (!PAIR && have[1]) {
-            uint32_t r[32];
-            tmem_ld_32x32b_x32_issue(lanes + 256 + 128 + c, r);
-            tmem_ld_wait();
-            tmem_ld_fence(r);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] += f[1] == 0.0f ? 0.0f : __uint_as_float(r[j]) * f[1];
-          }
-#pragma unroll
-          for (int j = 0; j < 32; ++j) o[j] = none ? 0.0f : o[j] * inv;
           if (valid && dirty && !none) {
             // the elements that were taken out, for the rows that see them
             const int kv_head = job.group * p.pack / p.group_heads;
-            const int64_t from = static_cast<int64_t>(max(job.first_masked, job.t0)) * kKeys;
+            const int64_t first = static_cast<int64_t>(max(job.first_masked, job.t0)) * kKeys;
             const T *v = static_cast<const T *>(p.v) + kv_head * p.v_head_stride + job.k0 * p.v_token_stride;
-            for (int64_t key = from; key < piece_end; ++key) {
+            for (int64_t key = first; key < piece_end; ++key) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) {
                 const float x = c + j < p.dim ? static_cast<float>(v[key * p.v_token_stride + c + j]) : 0.0f;
@@ -631,22 +639,25 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
           }
+          if (valid) {
 #pragma unroll
-          for (int j = 0; j < 32; j += 8) {
-            if (!valid || c + j >= p.dim) continue;
-            if (part != nullptr) {
-              float4 *dst = reinterpret_cast<float4 *>(part + c + j);
-              dst[0] = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-              dst[1] = make_float4(o[j + 4], o[j + 5], o[j + 6], o[j + 7]);
-            } else if (!job.behind || p.fill_tail) {
-              uint4 t;
-              t.x = pack2<T>(o[j], o[j + 1]);
-              t.y = pack2<T>(o[j + 2], o[j + 3]);
-              t.z = pack2<T>(o[j + 4], o[j + 5]);
-              t.w = pack2<T>(o[j + 6], o[j + 7]);
-              *reinterpret_cast<uint4 *>(out + c + j) = t;
+            for (int j = 0; j < 32; j += 8) {
+              if (c + j >= p.dim) break;
+              if (part != nullptr) {
+                float4 *dst = reinterpret_cast<float4 *>(part + c + j);
+                dst[0] = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                dst[1] = make_float4(o[j + 4], o[j + 5], o[j + 6], o[j + 7]);
+              } else if (!job.behind || p.fill_tail) {
+                uint4 t;
+                t.x = pack2<T>(o[j], o[j + 1]);
+                t.y = pack2<T>(o[j + 2], o[j + 3]);
+                t.z = pack2<T>(o[j + 4], o[j + 5]);
+                t.w = pack2<T>(o[j + 6], o[j + 7]);
+                *reinterpret_cast<uint4 *>(out + c + j) = t;
+              }
             }
           }
+          __syncwarp();
         }
       }
       tc_fence_before();
@@ -811,31 +822,35 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 11) {
       // ---------------- schedule ----------------
       attn::Order order;
+      bool alone = false;  // even shares: lane 0 goes on by itself
       if (p.split) {
         attn::Record record;
         order.init_share(p.plan, blockIdx.x, record);
         if (lane == 0) p.records[blockIdx.x] = record;
-        if (order.empty())  // a share cut to nothing may be counted among a job's pieces
+        if (__shfl_sync(0xffffffffu, order.empty(), 0))  // a share cut to nothing may be counted among a job's pieces
           for (int i = lane; i < kSlotRows; i += 32) p.part_lse[2ll * blockIdx.x * kSlotRows + i] = -INFINITY;
+        alone = true;
       } else {
-        order.init_whole(p.plan, blockIdx.x, gridDim.x);
+        order.init_whole(blockIdx.x, gridDim.x);
       }
       Segment seg;
       uint32_t phase = 1;
-      for (int slot = 0;;) {
-        const bool more = order.next(p.plan, seg);
-        if (more) describe<PAIR>(p, seg, job);
-        else job.count = -1;
-        if (!warp_wait_quick(&sh.job_empty[slot], phase, &sh.abort, p.status)) break;
-        if (lane == 0) {
-          sh.jobs[slot] = job;
-          mbar_arrive(&sh.job_full[slot]);
-        }
-        __syncwarp();
-        if (!more) break;
-        if (++slot == kJobs) {
-          slot = 0;
-          phase ^= 1;
+      if (!alone || lane == 0) {
+        for (int slot = 0;;) {
+          const bool more = order.next(p.plan, seg);
+          if (lane == 0) {
+            if (more) describe<PAIR>(p, seg, job);
+            else job.count = -1;
+            mbar_wait_through(&sh.job_empty[slot], phase, &sh.abort, p.status);
+            sh.jobs[slot] = job;
+            mbar_arrive(&sh.job_full[slot]);
+          }
+          if (!alone) __syncwarp();
+          if (!more || *const_cast<volatile int *>(&sh.abort)) break;
+          if (++slot == kJobs) {
+            slot = 0;
+            phase ^= 1;
+          }
         }
       }
     } else {
@@ -904,19 +919,18 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ---- joining the pieces of jobs that were cut ------------------------------------------
-constexpr int kJoinRows = 8;  // rows of one block, a warp each
+// Block (c - 1, y): the job whose first inner cut is cut c, a part of its rows; a
+// warp for a row at a time, four columns to a lane.
+constexpr int kJoinWarps = 8;
+constexpr int kJoinParts = 4;  // of a tile's rows
 
 template <typename T>
-__global__ void __launch_bounds__(32 * kJoinRows) attention_join_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(32 * kJoinWarps) attention_join_kernel(const __grid_constant__ Params p) {
   grid_dependency_wait();
   const int lane = threadIdx.x & 31;
   const int c = static_cast<int>(blockIdx.x) + 1;
   const attn::Record before = p.records[c - 1], job = p.records[c];
   if (!attn::join_starts(before, job)) return;
-  const int at = blockIdx.y * kJoinRows + (threadIdx.x >> 5);  // row of the slot
-  const int in_tile = at % kTile;
-  const int token = in_tile / p.pack + at / kTile * p.tokens;
-  if (in_tile / p.pack >= p.tokens || token >= job.count) return;
   int pieces = 1;  // and one for every record inside the job
   for (int i0 = c;; i0 += 32) {
     const int i = i0 + lane;
@@ -926,39 +940,49 @@ __global__ void __launch_bounds__(32 * kJoinRows) attention_join_kernel(const __
     if (others) break;
   }
   const int first = attn::join_first(before, job, c);
-  const auto slot_row = [&](int i) {
-    return static_cast<int64_t>(i == 0 ? first : 2 * (c + i - 1)) * kSlotRows + at;
-  };
-  float top = -INFINITY;
-  for (int i = lane; i < pieces; i += 32) top = max3_nan(top, p.part_lse[slot_row(i)], top);
-  for (int o = 16; o; o >>= 1) top = max3_nan(top, __shfl_xor_sync(0xffffffffu, top, o), top);
-  const float base = top == -INFINITY ? 0.0f : top;
-  float sum = 0.0f, acc[4] = {};
-  for (int i = 0; i < pieces; ++i) {
-    const float lse = p.part_lse[slot_row(i)];
-    if (lse == -INFINITY) continue;
-    const float weight = ex2(lse - base);
-    sum += weight;
-    if (lane * 4 < p.dim) {
-      const float4 o = *reinterpret_cast<const float4 *>(p.part_o + slot_row(i) * p.dim + 4 * lane);
-      acc[0] = fmaf(weight, o.x, acc[0]);
-      acc[1] = fmaf(weight, o.y, acc[1]);
-      acc[2] = fmaf(weight, o.z, acc[2]);
-      acc[3] = fmaf(weight, o.w, acc[3]);
+  for (int at = blockIdx.y * kJoinWarps + (threadIdx.x >> 5); at < kSlotRows; at += kJoinWarps * gridDim.y) {
+    const int in_tile = at % kTile;
+    const int token = in_tile / p.pack + at / kTile * p.tokens;
+    if (in_tile / p.pack >= p.tokens || token >= job.count) continue;
+    const auto slot_row = [&](int i) {
+      return static_cast<int64_t>(i == 0 ? first : 2 * (c + i - 1)) * kSlotRows + at;
+    };
+    float top = -INFINITY;
+    for (int i = lane; i < pieces; i += 32) top = max3_nan(top, p.part_lse[slot_row(i)], top);
+    for (int o = 16; o; o >>= 1) top = max3_nan(top, __shfl_xor_sync(0xffffffffu, top, o), top);
+    const float base = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f, acc[4] = {};
+    for (int i0 = 0; i0 < pieces; i0 += 32) {
+      const float weight = i0 + lane < pieces ? ex2(p.part_lse[slot_row(i0 + lane)] - base) : 0.0f;
+      sum += weight;
+      const int n = min(32, pieces - i0);
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const float w = __shfl_sync(0xffffffffu, weight, i);
+        // a piece without keys left its rows unwritten
+        if (lane * 4 < p.dim && w != 0.0f) {
+          const float4 o = *reinterpret_cast<const float4 *>(p.part_o + slot_row(i0 + i) * p.dim + 4 * lane);
+          acc[0] = fmaf(w, o.x, acc[0]);
+          acc[1] = fmaf(w, o.y, acc[1]);
+          acc[2] = fmaf(w, o.z, acc[2]);
+          acc[3] = fmaf(w, o.w, acc[3]);
+        }
+      }
     }
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    const float inv = top == -INFINITY ? 0.0f : 1.0f / sum;
+    const int head = job.group * p.pack + in_tile % p.pack;
+    const int64_t row = static_cast<int64_t>(job.row0) + token;
+    if (lane * 4 < p.dim) {
+      uint2 t;
+      t.x = pack2<T>(acc[0] * inv, acc[1] * inv);
+      t.y = pack2<T>(acc[2] * inv, acc[3] * inv);
+      *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + row * p.out_token_stride + head * p.out_head_stride +
+                                 4 * lane) = t;
+    }
+    if (lane == 0 && p.lse != nullptr)
+      p.lse[static_cast<int64_t>(head) * p.plan.total_q + row] = top == -INFINITY ? -INFINITY : (top + log2f(sum)) * kLn2;
   }
-  const float inv = top == -INFINITY ? 0.0f : 1.0f / sum;
-  const int head = job.group * p.pack + in_tile % p.pack;
-  const int64_t row = job.row0 + token;
-  if (lane * 4 < p.dim) {
-    uint2 t;
-    t.x = pack2<T>(acc[0] * inv, acc[1] * inv);
-    t.y = pack2<T>(acc[2] * inv, acc[3] * inv);
-    *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + row * p.out_token_stride + head * p.out_head_stride +
-                               4 * lane) = t;
-  }
-  if (lane == 0 && p.lse != nullptr)
-    p.lse[head * p.plan.total_q + row] = top == -INFINITY ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
 // ---- host side -------------------------------------------------------------------------
@@ -1055,8 +1079,8 @@ int launch(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, con
   cfg.numAttrs = 1;
   cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, q, k, v, p);
   if (err == cudaSuccess && p.split && p.plan.blocks > 1) {
-    cfg.gridDim = dim3(p.plan.blocks - 1, (PAIR ? 2 : 1) * kTile / kJoinRows, 1);
-    cfg.blockDim = dim3(32 * kJoinRows, 1, 1);
+    cfg.gridDim = dim3(p.plan.blocks - 1, kJoinParts * (PAIR ? 2 : 1), 1);
+    cfg.blockDim = dim3(32 * kJoinWarps, 1, 1);
     cfg.dynamicSmemBytes = 0;
     err = cudaLaunchKernelEx(&cfg, attention_join_kernel<T>, p);
   }
@@ -1098,14 +1122,15 @@ extern "C" int vfb_attention(const vfb_attention_args *args, void *stream) {
   p.plan.cu_q = a.cu_seqlens_q;
   p.plan.cu_k = a.cu_seqlens_k;
   p.plan.len_k = a.lengths_k;
-  p.plan.total_q = a.total_q;
-  p.plan.total_k = a.total_k;
+  p.plan.total_q = static_cast<int32_t>(a.total_q);
+  p.plan.total_k = static_cast<int32_t>(a.total_k);
   p.plan.batch = a.batch;
   p.plan.groups = c.groups;
-  p.plan.job_tokens = c.tokens * (c.pair ? 2 : 1);
+  attn::set_job_tokens(p.plan, c.tokens * (c.pair ? 2 : 1));
   p.plan.causal = a.causal != 0;
   p.plan.blocks = sms < kMaxBlocks ? sms : kMaxBlocks;
   p.plan.key_shift = c.pair ? 7 : 6;
+  p.plan.unit_shift = attn::unit_shift_for(c.jobs, a.total_q + a.total_k);
   p.v = a.v;
   p.out = a.out;
   p.lse = a.lse;
