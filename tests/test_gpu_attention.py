@@ -64,6 +64,10 @@ LENGTHS = [
     ([40, 300], [7, 130]),
     ([1], [5000]),
     ([64], [3000]),
+    ([300], [4000]),
+    ([700, 20], [5000, 3100]),
+    ([2500], [2500]),
+    ([5, 1, 0, 2], [9000, 3, 40, 6000]),
 ]
 
 

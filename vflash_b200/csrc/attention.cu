@@ -1010,8 +1010,23 @@ Choice choose(const vfb_attention_args &a) {
                             ? (a.total_q + tokens - 1) / tokens
                             : attn::min64(a.total_q, a.total_q / tokens + a.batch + 1);
   c.jobs = tiles * c.groups;
-  // Whole jobs balance by themselves when there are many; few keys are not worth cutting.
-  c.split = c.jobs < 4 * kMaxBlocks && a.total_k > 256;
+  // Even shares or whole jobs?  Shares cost the pieces' rows written and joined and
+  // the shares worked out: 20 us for PAIR, 10 us for ALT, the time of 1500 or 1100
+  // keys of a job.  They save what the blocks would idle: about a job's keys
+  // times the part of the blocks without one, half a job where there are more jobs
+  // than blocks, little when there are many.  Lengths are not known here, so a job
+  // is taken to have the average number of keys, twice that for keys of their own
+  // (caches differ more than prompts: there the longest job decides), and from
+  // 8192 cached keys on single tokens are always shared out.  Measured, whole against
+  // even (us): prompts of 2000 tokens of 32 / 8 heads 68 against 81, 4800 tokens of
+  // 16 / 2 heads 145 against 109; one token over 1000 keys 17 against 19, over 2000
+  // 27 against 20; 64 tokens over 1000 keys each 64 against 75, 32 over 1 to 8192
+  // 182 against 93.
+  int64_t keys = a.total_k / a.batch;
+  if (a.cu_seqlens_k != nullptr) keys = attn::min64(a.total_k, 2 * keys);
+  const int64_t idle = c.jobs < kMaxBlocks ? kMaxBlocks - c.jobs : kMaxBlocks / 2;
+  c.split = c.jobs < 4 * kMaxBlocks && (keys * idle > (c.pair ? 1500 : 1100) * kMaxBlocks ||
+                                        (!c.pair && a.total_k >= 8192));
   return c;
 }
 
