@@ -23,10 +23,13 @@
 //     quarters of a 128-row scale tile, whose scales for four groups are then
 //     64 consecutive bytes.
 //
-// A block has eight warps: WR row groups of RU units each, the steps of the
-// block's K range dealt out to the 8 / WR warps of a row group.  The warps'
-// sums are added in shared memory, those of the blocks of a cluster (one K
-// range each) through distributed shared memory, always in the same order.
+// A block's warps are WR row groups of RU units each, the steps of the block's K
+// range dealt out to the warps of a row group.  Every warp copies its steps into
+// a ring of its own in shared memory with cp.async, kDepth steps ahead, so that
+// the loads in flight hold no registers and wait for nothing but themselves; the
+// loop over the steps stays rolled and small.  The warps' sums are added in shared
+// memory, those of the blocks of a cluster (one K range each) through distributed
+// shared memory, always in the same order.
 #include <type_traits>
 
 #include "common.cuh"
@@ -34,8 +37,9 @@
 namespace vfb {
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kStep = 128;  // k of a step
+constexpr int kStep = 128;                   // k of a step
+constexpr int kUnitBytes = 16 * kStep / 2;  // codes of a unit's step
+constexpr int kUnitStage = kUnitBytes + 16 * 8;  // and their scales
 
 struct Args {
   const void *x;
@@ -50,24 +54,18 @@ struct Args {
   int32_t vector_x;   // rows of x are 16-byte aligned
 };
 
-// Loads that are skipped (the registers keep what they held) unless `in`.  The
-// results are only touched when they are multiplied, two steps later.
-__device__ __forceinline__ void load_stream(uint4 &v, const void *p, bool in) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.u32 p, %5, 0;\n\t"
-      "@p ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n\t}"
-      : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)
-      : "l"(p), "r"(static_cast<uint32_t>(in)));
+// Asynchronous copies to shared memory; nothing is read and zeros are written
+// unless `in`.
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
-
-__device__ __forceinline__ void load_word(uint32_t &v, const void *p, bool in) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.u32 p, %2, 0;\n\t"
-      "@p ld.global.nc.u32 %0, [%1];\n\t}"
-      : "+r"(v)
-      : "l"(p), "r"(static_cast<uint32_t>(in)));
+__device__ __forceinline__ void copy4(uint32_t dst, const void *src, bool in) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // Four bytes of e2m1 pairs -> four f16x2 (low nibble in the low half).
@@ -125,30 +123,27 @@ __device__ __forceinline__ int row_shift(uint32_t max_bits) {
   return min(14 - (min(e, 254) - 127), 126);
 }
 
-template <int NT, int RU, int WR>
+template <int NT, int RU, int WR, int WARPS>
 struct Shape {
   static constexpr int tokens = 8 * NT;
   static constexpr int rows = 16 * RU * WR;       // of the weight, in a block
-  static constexpr int k_warps = kWarps / WR;
+  static constexpr int k_warps = WARPS / WR;
+  static constexpr int depth = NT == 1 && WARPS == 16 ? 4 : 2;  // steps in flight, for a warp
+  static constexpr int stage = RU * kUnitStage;
+  static constexpr int ring_bytes = WARPS * depth * stage;
   static constexpr int row_bytes(int steps) { return steps * kStep * 2 + 64; }  // of x, padded against bank conflicts
-  static constexpr int sum_bytes = k_warps * rows * tokens * 4;
+  static constexpr int sum_row = rows + 4;        // likewise
+  static constexpr int sum_bytes = k_warps * sum_row * tokens * 4;
 };
 
-// Blocks that share an SM (by registers).
-template <int NT, int RU>
-constexpr int blocks_per_sm() { return NT == 1 && RU == 2 ? 3 : 2; }
-
-template <int RU>
-struct Batch {  // the weights of one step
-  uint4 w[RU][2];
-  uint32_t s[RU][2];  // four groups' scales, of which a lane uses two
-};
-
-template <typename T, int NT, int RU, int WR>
-__global__ void __launch_bounds__(32 * kWarps, blocks_per_sm<NT, RU>()) weight_only_kernel(const Args p) {
-  using S = Shape<NT, RU, WR>;
+template <typename T, int NT, int RU, int WR, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? (NT == 1 ? 3 : 2) : 1)
+    weight_only_kernel(const Args p) {
+  using S = Shape<NT, RU, WR, WARPS>;
   constexpr bool kScaled = std::is_same<T, __nv_bfloat16>::value;  // rows of x carry a power of two
+  constexpr int kThreads = 32 * WARPS;
   extern __shared__ __align__(128) uint8_t smem[];
+  uint8_t *xs = smem + S::ring_bytes;
   __shared__ uint32_t row_max[S::tokens];
   __shared__ float bias[S::rows];
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
@@ -156,44 +151,53 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm<NT, RU>()) weight_o
   const int part = blockIdx.x;
   const int m0 = blockIdx.z * S::tokens;
   const int tokens = min(S::tokens, p.M - m0);
-  const int unit0 = (blockIdx.y * WR + warp % WR) * RU;  // of 16 rows; eight units in 128 rows
-  const int64_t row_block = unit0 / 8;
+  const int first_unit = blockIdx.y * WR * RU;  // of 16 rows; eight units in 128 rows
   const int k_warp = warp / WR;
   const int k_begin = part * p.steps * kStep;
   const int steps = max(0, min(p.steps, (p.K - k_begin + kStep - 1) / kStep));
-
-  // weight row of row r of the block: a quarter's rows of all its units
+  const int own_steps = max(0, (steps - k_warp + S::k_warps - 1) / S::k_warps);
+  // weight row of row r of the block's output: a quarter's rows of all its units
   const auto feature = [&](int r) {
-    const int first = blockIdx.y * WR * RU, quarter_rows = 4 * RU * WR;
-    return static_cast<int64_t>(first / 8) * 128 + r / quarter_rows * 32 + 4 * (first % 8) + r % quarter_rows;
+    constexpr int quarter_rows = 4 * RU * WR;
+    const int unit = r % quarter_rows / 4;
+    return static_cast<int64_t>((first_unit + unit) / 8) * 128 + r / quarter_rows * 32 + 4 * ((first_unit + unit) % 8) +
+           r % 4;
   };
 
   grid_dependency_wait();
 
-  // rows g and g + 8 of unit u: see the header; 32-bit offsets inside the scale tile's 128 rows
+  // ---- copies: lane (g, t) brings 16 bytes of rows g and g + 8 and one word of scales ----
   const uint32_t half_k = p.K / 2;
-  const uint8_t *codes = p.codes + row_block * 128 * half_k;
-  const uint8_t *sf = p.sf + row_block * (p.K / 64) * 512;
-  const uint32_t in_quarter = 4 * (unit0 % 8) + g / 4;
-  const uint32_t code_at = ((g % 4) * 32 + in_quarter) * half_k + k_begin / 2 + 16 * t;
-  const uint32_t sf_at = (k_begin / 64 + t / 2) * 512 + in_quarter * 16 + (g % 4) * 4;
-  const int in_steps = max(0, (p.K - k_begin - 32 * t + kStep - 1) / kStep);
-  const auto load = [&](Batch<RU> &b, int step) {
-    const bool in = step < min(steps, in_steps);
+  const uint32_t ring = smem_u32(smem) + warp * S::depth * S::stage;
+  const int unit0 = first_unit + warp % WR * RU;
+  // rows g and g + 8 of unit u: see the header; 32-bit offsets inside the scale tile's 128 rows
+  const uint8_t *codes = p.codes + static_cast<int64_t>(unit0 / 8) * 128 * half_k;
+  const uint8_t *sf = p.sf + static_cast<int64_t>(unit0 / 8) * (p.K / 64) * 512;
+  const uint32_t code_at = ((g % 4) * 32 + 4 * (unit0 % 8) + g / 4) * half_k + k_begin / 2 + 16 * t;
+  // scales: 64 consecutive bytes for the 16 rows and four groups, in the order of (row / 4, row % 4)
+  const uint32_t sf_at = (k_begin / 64 + lane / 16) * 512 + 4 * (unit0 % 8) * 16 + lane % 16 * 4;
+  const int k_left = p.K - k_begin;
+  const auto copy = [&](int i) {  // the i-th of this warp's steps
+    if (i < own_steps) {
+      const int step = k_warp + i * S::k_warps;
+      const uint32_t stage = ring + i % S::depth * S::stage;
+      const bool in = step * kStep + 32 * t < k_left;  // K may end on half a step
+      const bool sf_in = step * kStep + lane / 16 * 64 < k_left;
 #pragma unroll
-    for (int u = 0; u < RU; ++u)
+      for (int u = 0; u < RU; ++u) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        load_stream(b.w[u][r], codes + (code_at + (4 * u + 2 * r) * half_k + step * (kStep / 2)), in);
-        load_word(b.s[u][r], sf + (sf_at + (4 * u + 2 * r) * 16 + step * 1024), in);
+        for (int r = 0; r < 2; ++r)
+          copy16(stage + u * kUnitStage + r * 512 + lane * 16,
+                 codes + (in ? code_at + (4 * u + 2 * r) * half_k + step * (kStep / 2) : 0u), in);
+        copy4(stage + u * kUnitStage + kUnitBytes + lane * 4, sf + (sf_in ? sf_at + u * 64 + step * 1024 : 0u), sf_in);
       }
+    }
+    copies_commit();
   };
-  Batch<RU> batch[2] = {};
-  load(batch[0], k_warp);
-  load(batch[1], k_warp + S::k_warps);
-
+#pragma unroll
+  for (int i = 0; i < S::depth; ++i) copy(i);
   const float alpha = __ldg(p.alpha);
-  if (tid < S::rows) bias[tid] = p.bias != nullptr ? __bfloat162float(p.bias[feature(tid)]) : 0.0f;
+  for (int r = tid; r < S::rows; r += kThreads) bias[r] = p.bias != nullptr ? __bfloat162float(p.bias[feature(r)]) : 0.0f;
 
   // ---- x to fp16 in shared memory ----
   const int row_bytes = S::row_bytes(p.steps);
@@ -203,22 +207,24 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm<NT, RU>()) weight_o
   const auto row_of = [&](int i) { return static_cast<int>(__umulhi(i, p.chunk_inverse)); };  // i / chunks
   // chunk 4 * t + i of a step is read by lane t in its i-th pair of products
   const auto place = [&](int m, int c) {
-    return reinterpret_cast<uint4 *>(smem + m * row_bytes + (c / 16) * 256 + (c % 4) * 64 + (c % 16) / 4 * 16);
+    return reinterpret_cast<uint4 *>(xs + m * row_bytes + (c / 16) * 256 + (c % 4) * 64 + (c % 16) / 4 * 16);
   };
   if (kScaled) {
     if (tid < S::tokens) row_max[tid] = 0;
     __syncthreads();
   }
-  for (int i0 = tid; i0 < items; i0 += 4 * 32 * kWarps) {
-    uint4 v[4];
+  constexpr int kFlight = NT == 1 ? 4 : 8;  // chunks of a thread in flight
+#pragma unroll 1
+  for (int i0 = tid; i0 < items; i0 += kFlight * kThreads) {
+    uint4 v[kFlight];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = i0 + j * 32 * kWarps, m = row_of(i), c = i - m * chunks;
+    for (int j = 0; j < kFlight; ++j) {
+      const int i = i0 + j * kThreads, m = row_of(i), c = i - m * chunks;
       if (i < items) v[j] = load_x8(x + m * p.ldx + k_begin + 8 * c, p.vector_x, p.K - k_begin - 8 * c);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = i0 + j * 32 * kWarps, m = row_of(i), c = i - m * chunks;
+    for (int j = 0; j < kFlight; ++j) {
+      const int i = i0 + j * kThreads, m = row_of(i), c = i - m * chunks;
       if (i >= items) break;  // for all 16 lanes of a row's piece at once
       *place(m, c) = v[j];
       if (!kScaled) continue;
@@ -236,7 +242,8 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm<NT, RU>()) weight_o
   }
   __syncthreads();
   if (kScaled) {
-    for (int i = tid; i < items; i += 32 * kWarps) {
+#pragma unroll 1
+    for (int i = tid; i < items; i += kThreads) {
       const int m = row_of(i), c = i - m * chunks;
       const float factor = power_of_two(row_shift(row_max[m]));
       uint4 v = *place(m, c);
@@ -254,34 +261,43 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm<NT, RU>()) weight_o
 
   // ---- products ----
   float acc[RU][NT][4] = {};
-  const auto multiply = [&](const Batch<RU> &b, int step) {
-    const bool in = step < in_steps;  // K may end on half a step: a zero scale makes any code 0
-    uint32_t scale[RU][2][2];         // unit, row, group: the scale in both halves
+  const uint8_t *own_ring = smem + warp * S::depth * S::stage;
+#pragma unroll 1
+  for (int i = 0; i < own_steps; ++i) {
+    copies_wait<S::depth - 1>();
+    __syncwarp();
+    const uint8_t *stage = own_ring + i % S::depth * S::stage;
+    const uint8_t *x_step = xs + g * row_bytes + (k_warp + i * S::k_warps) * 256 + t * 16;
+    uint4 w[RU][2];
+    uint32_t scale[RU][2][2];  // unit, row, group: the scale in both halves
 #pragma unroll
     for (int u = 0; u < RU; ++u)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const uint32_t h = decode_e4m3x2(in ? static_cast<uint16_t>(b.s[u][r] >> (16 * (t % 2))) : 0);
+        w[u][r] = *reinterpret_cast<const uint4 *>(stage + u * kUnitStage + r * 512 + lane * 16);
+        // lane's groups 2t and 2t + 1 of row g + 8r, which is row (g / 4 + 2r) of quarter g % 4
+        const uint16_t s = *reinterpret_cast<const uint16_t *>(stage + u * kUnitStage + kUnitBytes + t / 2 * 64 +
+                                                               (g / 4 + 2 * r) * 16 + g % 4 * 4 + t % 2 * 2);
+        const uint32_t h = decode_e4m3x2(s);
         scale[u][r][0] = __byte_perm(h, 0, 0x1010);
         scale[u][r][1] = __byte_perm(h, 0, 0x3232);
       }
-    const uint8_t *xs = smem + g * row_bytes + step * 256 + t * 16;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int q = 0; q < 4; ++q) {
       uint4 f[NT];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         f[n] = make_uint4(0, 0, 0, 0);
-        if (8 * n + g < tokens) f[n] = *reinterpret_cast<const uint4 *>(xs + 8 * n * row_bytes + i * 64);
+        if (8 * n + g < tokens) f[n] = *reinterpret_cast<const uint4 *>(x_step + 8 * n * row_bytes + q * 64);
       }
 #pragma unroll
       for (int u = 0; u < RU; ++u) {
         uint32_t a[2][4];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          decode_e2m1x8(reinterpret_cast<const uint32_t *>(&b.w[u][r])[i], a[r]);
+          decode_e2m1x8(reinterpret_cast<const uint32_t *>(&w[u][r])[q], a[r]);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) a[r][j] = mul_f16x2(a[r][j], scale[u][r][i / 2]);
+          for (int j = 0; j < 4; ++j) a[r][j] = mul_f16x2(a[r][j], scale[u][r][q / 2]);
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -290,106 +306,122 @@ __global__ void __launch_bounds__(32 * kWarps, blocks_per_sm<NT, RU>()) weight_o
         }
       }
     }
-  };
-  for (int step = k_warp; step < steps; step += 2 * S::k_warps) {
-    multiply(batch[0], step);
-    load(batch[0], step + 2 * S::k_warps);
-    if (step + S::k_warps < steps) multiply(batch[1], step + S::k_warps);
-    load(batch[1], step + 3 * S::k_warps);
+    __syncwarp();  // the stage is read by all lanes
+    copy(i + S::depth);
   }
+  copies_wait<0>();
 
   // ---- sums over the warps, then over the blocks of the cluster ----
-  __syncthreads();  // x is read
-  float *sums = reinterpret_cast<float *>(smem);  // [k warp][token][row]
+  __syncthreads();  // ring and x are read
+  float *sums = reinterpret_cast<float *>(smem);  // [k warp][token][row of the products]
 #pragma unroll
   for (int u = 0; u < RU; ++u)
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int row = (g % 4) * (4 * RU * WR) + 4 * ((warp % WR) * RU + u) + g / 4 + 2 * (j / 2);
-        const int token = 8 * n + 2 * t + j % 2;
-        sums[(k_warp * S::tokens + token) * S::rows + row] = acc[u][n][j];
-      }
+      for (int j = 0; j < 4; ++j)
+        sums[(k_warp * S::tokens + 8 * n + 2 * t + j % 2) * S::sum_row + ((warp % WR) * RU + u) * 16 + g + 8 * (j / 2)] =
+            acc[u][n][j];
   __syncthreads();
-  for (int i = tid; i < tokens * S::rows; i += 32 * kWarps) {
-    float v = sums[i];
+  // output row r of token m is row `row` of the products
+  const auto place_of = [&](int i, int &m, int &r) {
+    constexpr int quarter_rows = 4 * RU * WR;
+    m = i / S::rows;
+    r = i % S::rows;
+    return m * S::sum_row + r % quarter_rows / 4 * 16 + r % 4 * 4 + r / quarter_rows;
+  };
+  for (int i = tid; i < tokens * S::rows; i += kThreads) {
+    int m, r;
+    const int at = place_of(i, m, r);
+    float v = sums[at];
 #pragma unroll
-    for (int w = 1; w < S::k_warps; ++w) v += sums[w * S::tokens * S::rows + i];
+    for (int w = 1; w < S::k_warps; ++w) v += sums[w * S::tokens * S::sum_row + at];
     v *= alpha;
-    if (kScaled) v *= power_of_two(-row_shift(row_max[i / S::rows]));
-    sums[i] = v;
+    if (kScaled) v *= power_of_two(-row_shift(row_max[m]));
+    if (split == 1)
+      p.out[(m0 + m) * p.ldo + feature(r)] = __float2bfloat16_rn(v + bias[r]);
+    else
+      sums[at] = v;
   }
+  if (split == 1) return;
   cluster_sync();
-  for (int i = tid * split + part; i < tokens * S::rows; i += 32 * kWarps * split) {
+#pragma unroll 2
+  for (int i = part * kThreads + tid; i < tokens * S::rows; i += kThreads * split) {
+    int m, r;
+    const int at = place_of(i, m, r);
+    float other[8] = {};  // all in flight before the first is added
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (c < split)
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(other[c]) : "r"(map_to_rank(smem_u32(sums + at), c)));
     float v = 0.0f;
-    for (int c = 0; c < split; ++c) {
-      float other;
-      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(other) : "r"(map_to_rank(smem_u32(sums + i), c)));
-      v += other;
-    }
-    const int token = i / S::rows, row = i % S::rows;
-    p.out[(m0 + token) * p.ldo + feature(row)] = __float2bfloat16_rn(v + bias[row]);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) v += other[c];
+    p.out[(m0 + m) * p.ldo + feature(r)] = __float2bfloat16_rn(v + bias[r]);
   }
   cluster_sync();  // the others have read this block's sums
 }
 
-template <typename T, int NT, int RU, int WR>
+template <typename T, int NT, int RU, int WR, int WARPS>
 int launch(Args p, int split, cudaStream_t stream) {
-  using S = Shape<NT, RU, WR>;
-  auto kernel = weight_only_kernel<T, NT, RU, WR>;
+  using S = Shape<NT, RU, WR, WARPS>;
+  auto kernel = weight_only_kernel<T, NT, RU, WR, WARPS>;
   const int steps = (p.K + kStep - 1) / kStep;
   p.steps = (steps + split - 1) / split;
   p.chunk_inverse = static_cast<uint32_t>((1ull << 32) / (p.steps * 16)) + 1;
-  const int x_bytes = (p.M < S::tokens ? p.M : S::tokens) * S::row_bytes(p.steps);
-  const int smem = x_bytes > S::sum_bytes ? x_bytes : S::sum_bytes;
-  constexpr int kMost = 200 * 1024;
+  const int used = S::ring_bytes + (p.M < S::tokens ? p.M : S::tokens) * S::row_bytes(p.steps);
+  const int smem = used > S::sum_bytes ? used : S::sum_bytes;
+  constexpr int kMost = 220 * 1024;
   if (smem > kMost) return set_error(VFB_EINVAL, "vfb_nvfp4_weight_only: K is too large");
   static std::atomic<uint64_t> smem_set[kMaxAttrDevices];
   int rc = ensure_smem_optin(reinterpret_cast<const void *>(kernel), kMost, smem_set);
   if (rc != VFB_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(split, p.N / S::rows, (p.M + S::tokens - 1) / S::tokens);
-  cfg.blockDim = dim3(32 * kWarps, 1, 1);
+  cfg.blockDim = dim3(32 * WARPS, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = split;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = split;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
+  cfg.numAttrs = split > 1 ? 2 : 1;
   cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, p);
   if (err != cudaSuccess) return set_error(VFB_ECUDA, "vfb_nvfp4_weight_only launch: %s", cudaGetErrorString(err));
   return VFB_OK;
 }
 
-// Blocks along K: as many as still run at once, but every warp keeps two steps;
-// more where x of a K range would not let that many blocks share an SM.
-template <typename T, int NT, int RU, int WR>
-int launch_split(const Args &p, int sms, cudaStream_t stream) {
-  using S = Shape<NT, RU, WR>;
+// Blocks along K: as many as still run at once while every warp keeps two steps;
+// more where x of a K range would not leave room for `resident` blocks on an SM.
+template <typename T, int NT, int RU, int WR, int WARPS>
+int launch_split(const Args &p, int sms, int resident, cudaStream_t stream) {
+  using S = Shape<NT, RU, WR, WARPS>;
   const int steps = (p.K + kStep - 1) / kStep;
   const int tokens = p.M < S::tokens ? p.M : S::tokens;
   const int64_t blocks = static_cast<int64_t>(p.N / S::rows) * ((p.M + S::tokens - 1) / S::tokens);
-  const int resident = blocks_per_sm<NT, RU>();
-  const int x_most = 216 * 1024 / resident;
+  const int most = 224 * 1024 / resident - 2048 - S::ring_bytes;
   int split = 1;
   while (split < 8 && ((2 * blocks * split <= resident * sms && steps >= 4 * split * S::k_warps) ||
-                       tokens * S::row_bytes((steps + split - 1) / split) > x_most))
+                       tokens * S::row_bytes((steps + split - 1) / split) > most))
     split *= 2;
-  return launch<T, NT, RU, WR>(p, split, stream);
+  return launch<T, NT, RU, WR, WARPS>(p, split, stream);
 }
 
 template <typename T>
 int run(const Args &p, int sms, cudaStream_t s) {
-  if (p.M <= 2) return launch_split<T, 1, 2, 1>(p, sms, s);
-  if (p.M <= 8) return launch_split<T, 1, 4, 2>(p, sms, s);
-  if (p.M <= 16 || p.K > 16384) return launch_split<T, 2, 2, 4>(p, sms, s);
-  return launch_split<T, 4, 2, 4>(p, sms, s);
+  if (p.M <= 2) return launch_split<T, 1, 2, 2, 8>(p, sms, 3, s);
+  if (p.N % 256 == 0) {
+    if (p.M <= 8) return launch_split<T, 1, 2, 8, 16>(p, sms, 1, s);
+    if (p.M <= 16 || p.K > 16384) return launch_split<T, 2, 2, 8, 16>(p, sms, 1, s);
+    return launch_split<T, 4, 2, 8, 16>(p, sms, 1, s);
+  }
+  if (p.M <= 8) return launch_split<T, 1, 2, 4, 8>(p, sms, 2, s);
+  if (p.M <= 16 || p.K > 16384) return launch_split<T, 2, 2, 4, 8>(p, sms, 2, s);
+  return launch_split<T, 4, 2, 4, 8>(p, sms, 2, s);
 }
 
 constexpr int64_t kMaxK = 32768;
