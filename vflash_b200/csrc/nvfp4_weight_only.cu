@@ -137,7 +137,7 @@ struct Shape {
 };
 
 template <typename T, int NT, int RU, int WR, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? (NT == 1 ? 3 : 2) : 1)
+__global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 1)
     weight_only_kernel(const Args p) {
   using S = Shape<NT, RU, WR, WARPS>;
   constexpr bool kScaled = std::is_same<T, __nv_bfloat16>::value;  // rows of x carry a power of two
@@ -411,17 +411,22 @@ int launch_split(const Args &p, int sms, int resident, cudaStream_t stream) {
   return launch<T, NT, RU, WR, WARPS>(p, split, stream);
 }
 
+// Rows of a block: x is prepared once a block, so more weight rows share that work
+// the more rows x has, as long as the weight has enough of them for the SMs (and
+// for the two 128-row scale tiles of the widest block).  Measured, narrow against
+// wide block (us): 1 row, N = 12288, K = 4096 10.8 against 11.2; 5 rows 14.3
+// against 13.9; 8 rows, N = 28672, K = 5376 52.5 (128 rows) against 36.4 (256);
+// 16 rows, N = 4096, K = 16384 25.0 against 40.4, N = 16384, K = 4096 22.6 against
+// 20.3; 32 rows of the same 45.4 against 31.3.
 template <typename T>
 int run(const Args &p, int sms, cudaStream_t s) {
   if (p.M <= 2) return launch_split<T, 1, 2, 2, 8>(p, sms, 3, s);
-  if (p.N % 256 == 0) {
-    if (p.M <= 8) return launch_split<T, 1, 2, 8, 16>(p, sms, 1, s);
-    if (p.M <= 16 || p.K > 16384) return launch_split<T, 2, 2, 8, 16>(p, sms, 1, s);
-    return launch_split<T, 4, 2, 8, 16>(p, sms, 1, s);
-  }
-  if (p.M <= 8) return launch_split<T, 1, 2, 4, 8>(p, sms, 2, s);
-  if (p.M <= 16 || p.K > 16384) return launch_split<T, 2, 2, 4, 8>(p, sms, 2, s);
-  return launch_split<T, 4, 2, 4, 8>(p, sms, 2, s);
+  const bool wide = p.N % 256 == 0 && p.N >= (p.M <= 8 ? 24576 : 8192);
+  if (p.M <= 8)
+    return wide ? launch_split<T, 1, 2, 8, 16>(p, sms, 1, s) : launch_split<T, 1, 2, 4, 16>(p, sms, 1, s);
+  if (p.M <= 16 || p.K > 16384)
+    return wide ? launch_split<T, 2, 2, 8, 16>(p, sms, 1, s) : launch_split<T, 2, 2, 4, 16>(p, sms, 1, s);
+  return wide ? launch_split<T, 4, 2, 8, 16>(p, sms, 1, s) : launch_split<T, 4, 2, 4, 16>(p, sms, 1, s);
 }
 
 constexpr int64_t kMaxK = 32768;
