@@ -80,6 +80,16 @@ def test_model_sizes(n, k, rows):
     check(nvfp4_weight_only(x, weight.packed, weight.scales, weight.alpha), x, weight, None)
 
 
+@pytest.mark.parametrize("n,rows,k", [(128, 9, 8384), (128, 17, 4416), (128, 18, 8768), (128, 32, 16384),
+                                      (128, 32, 16448), (128, 8, 32768), (256, 33, 32768), (8192, 10, 7488),
+                                      (16384, 4, 18880), (16384, 3, 25280)])
+def test_rows_that_fill_shared_memory(n, rows, k):
+    """x takes most of a block's shared memory, or its K is dealt out so that it fits."""
+    weight = weight_of(n, k, 4)
+    x = activations(rows, k, 6, BF16)
+    check(nvfp4_weight_only(x, weight.packed, weight.scales, weight.alpha), x, weight, None)
+
+
 def test_every_code_and_scale_decodes_exactly():
     """One activation of 1 per row of x: the output is that weight times alpha, exact in bf16."""
     n, k = 128, 256

@@ -40,6 +40,7 @@ namespace {
 constexpr int kStep = 128;                   // k of a step
 constexpr int kUnitBytes = 16 * kStep / 2;  // codes of a unit's step
 constexpr int kUnitStage = kUnitBytes + 16 * 8;  // and their scales
+constexpr int kMostSmem = 222 * 1024;       // of a block alone on its SM; its static part takes less than 2 KB
 
 struct Args {
   const void *x;
@@ -100,16 +101,27 @@ __device__ __forceinline__ void mma_m16n8k16(float (&d)[4], uint32_t a0, uint32_
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Eight elements of a row of x, zeros behind `left`.
+// Eight elements of a row of x that lie anywhere.
 template <typename T>
-__device__ __forceinline__ uint4 load_x8(const T *p, bool vector, int left) {
-  if (vector && left >= 8) return __ldg(reinterpret_cast<const uint4 *>(p));
+__device__ __forceinline__ uint4 gather_x8(const T *p) {
   uint32_t w[4] = {};
   const uint16_t *u = reinterpret_cast<const uint16_t *>(p);
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (j < left) w[j / 2] |= static_cast<uint32_t>(__ldg(u + j)) << (16 * (j & 1));
+  for (int j = 0; j < 8; ++j) w[j / 2] |= static_cast<uint32_t>(__ldg(u + j)) << (16 * (j & 1));
   return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Largest magnitude of eight bf16 numbers, as the bits of an f32; NaN is left out.
+__device__ __forceinline__ uint32_t largest_x8(const uint4 &v) {
+  const auto magnitudes = [](uint32_t w) {
+    w &= 0x7FFF7FFFu;
+    return *reinterpret_cast<const __nv_bfloat162 *>(&w);
+  };
+  const __nv_bfloat162 two =
+      __hmax2(__hmax2(magnitudes(v.x), magnitudes(v.y)), __hmax2(magnitudes(v.z), magnitudes(v.w)));
+  const uint32_t w = *reinterpret_cast<const uint32_t *>(&two);
+  const uint32_t lo = w << 16, hi = w & 0xFFFF0000u;  // NaN where all four were
+  return max(lo > 0x7F800000u ? 0u : lo, hi > 0x7F800000u ? 0u : hi);
 }
 
 // 2^e for -126 <= e <= 127.
@@ -128,7 +140,7 @@ struct Shape {
   static constexpr int tokens = 8 * NT;
   static constexpr int rows = 16 * RU * WR;       // of the weight, in a block
   static constexpr int k_warps = WARPS / WR;
-  static constexpr int depth = NT == 1 && WARPS == 16 ? 4 : 2;  // steps in flight, for a warp
+  static constexpr int depth = 2;                 // steps in flight, for a warp
   static constexpr int stage = RU * kUnitStage;
   static constexpr int ring_bytes = WARPS * depth * stage;
   static constexpr int row_bytes(int steps) { return steps * kStep * 2 + 64; }  // of x, padded against bank conflicts
@@ -194,70 +206,96 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 1)
     }
     copies_commit();
   };
-#pragma unroll
-  for (int i = 0; i < S::depth; ++i) copy(i);
-  const float alpha = __ldg(p.alpha);
-  for (int r = tid; r < S::rows; r += kThreads) bias[r] = p.bias != nullptr ? __bfloat162float(p.bias[feature(r)]) : 0.0f;
 
-  // ---- x to fp16 in shared memory ----
+  // ---- x to fp16 in shared memory; its first loads go out before the copies, which would delay them ----
   const int row_bytes = S::row_bytes(p.steps);
   const T *x = static_cast<const T *>(p.x) + m0 * p.ldx;
   const int chunks = p.steps * (kStep / 8);  // of eight elements, in a row; a multiple of 16
   const int items = tokens * chunks;
   const auto row_of = [&](int i) { return static_cast<int>(__umulhi(i, p.chunk_inverse)); };  // i / chunks
   // chunk 4 * t + i of a step is read by lane t in its i-th pair of products
-  const auto place = [&](int m, int c) {
+  const auto place = [&](int i) {
+    const int m = row_of(i), c = i - m * chunks;
     return reinterpret_cast<uint4 *>(xs + m * row_bytes + (c / 16) * 256 + (c % 4) * 64 + (c % 16) / 4 * 16);
   };
+  const auto from = [&](int i) {
+    const int m = row_of(i), c = i - m * chunks;
+    return x + m * p.ldx + k_begin + 8 * c;
+  };
+  const auto inside = [&](int i) { return 8 * (i - row_of(i) * chunks) < k_left; };  // K is a multiple of eight
+  const auto note = [&](int i, const uint4 &v) {  // 16 lanes with one row's chunks
+    const uint32_t top = __reduce_max_sync(0xFFFFu << (lane & 16), largest_x8(v));
+    if (lane % 16 == 0 && top) atomicMax(&row_max[row_of(i)], top);
+  };
+  constexpr int kFlight = NT == 1 ? 8 : 12;  // chunks of a thread in flight
+  constexpr int kFlightItems = kFlight * kThreads;
+  uint4 v[kFlight];
+  const auto load = [&](int base) {
+#pragma unroll
+    for (int j = 0; j < kFlight; ++j) {
+      const int i = base + j * kThreads + tid;
+      if (i >= items) break;
+      v[j] = make_uint4(0, 0, 0, 0);
+      if (inside(i)) v[j] = __ldg(reinterpret_cast<const uint4 *>(from(i)));
+    }
+  };
+  if (p.vector_x) load(0);
+#pragma unroll
+  for (int i = 0; i < S::depth; ++i) copy(i);
+  const float alpha = __ldg(p.alpha);
+  for (int r = tid; r < S::rows; r += kThreads) bias[r] = p.bias != nullptr ? __bfloat162float(p.bias[feature(r)]) : 0.0f;
   if (kScaled) {
     if (tid < S::tokens) row_max[tid] = 0;
     __syncthreads();
   }
-  constexpr int kFlight = NT == 1 ? 4 : 8;  // chunks of a thread in flight
+  int base = 0;  // of the last flight, which stays in registers until the rows' maxima are known
+  if (p.vector_x) {
 #pragma unroll 1
-  for (int i0 = tid; i0 < items; i0 += kFlight * kThreads) {
-    uint4 v[kFlight];
+    for (;; base += kFlightItems, load(base)) {
+      if (kScaled) {
 #pragma unroll
-    for (int j = 0; j < kFlight; ++j) {
-      const int i = i0 + j * kThreads, m = row_of(i), c = i - m * chunks;
-      if (i < items) v[j] = load_x8(x + m * p.ldx + k_begin + 8 * c, p.vector_x, p.K - k_begin - 8 * c);
-    }
-#pragma unroll
-    for (int j = 0; j < kFlight; ++j) {
-      const int i = i0 + j * kThreads, m = row_of(i), c = i - m * chunks;
-      if (i >= items) break;  // for all 16 lanes of a row's piece at once
-      *place(m, c) = v[j];
-      if (!kScaled) continue;
-      const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-      uint32_t top = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {  // magnitudes compare as integers; NaN is left out
-        const uint32_t lo = (w[e] << 16) & 0x7FFFFFFFu, hi = w[e] & 0x7FFF0000u;
-        top = max(top, lo > 0x7F800000u ? 0u : lo);
-        top = max(top, hi > 0x7F800000u ? 0u : hi);
+        for (int j = 0; j < kFlight; ++j) {
+          const int i = base + j * kThreads + tid;
+          if (i >= items) break;
+          note(i, v[j]);
+        }
       }
-      top = __reduce_max_sync(0xFFFFu << (lane & 16), top);
-      if (lane % 16 == 0 && top) atomicMax(&row_max[m], top);
+      if (base + kFlightItems >= items) break;
+#pragma unroll
+      for (int j = 0; j < kFlight; ++j) *place(base + j * kThreads + tid) = v[j];
     }
-  }
-  __syncthreads();
-  if (kScaled) {
+  } else {
+    base = items;
 #pragma unroll 1
     for (int i = tid; i < items; i += kThreads) {
-      const int m = row_of(i), c = i - m * chunks;
-      const float factor = power_of_two(row_shift(row_max[m]));
-      uint4 v = *place(m, c);
-      uint32_t *w = reinterpret_cast<uint32_t *>(&v);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const __half2 h = __floats2half2_rn(__uint_as_float(w[e] << 16) * factor,
-                                            __uint_as_float(w[e] & 0xFFFF0000u) * factor);
-        w[e] = *reinterpret_cast<const uint32_t *>(&h);
-      }
-      *place(m, c) = v;
+      const uint4 c = inside(i) ? gather_x8(from(i)) : make_uint4(0, 0, 0, 0);
+      if (kScaled) note(i, c);
+      *place(i) = c;
     }
-    __syncthreads();
   }
+  const auto scaled = [&](uint4 c, float factor) {
+    uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const __half2 h =
+          __floats2half2_rn(__uint_as_float(w[e] << 16) * factor, __uint_as_float(w[e] & 0xFFFF0000u) * factor);
+      w[e] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  };
+  if (kScaled) {
+    __syncthreads();
+#pragma unroll 4
+    for (int i = tid; i < base; i += kThreads)
+      *place(i) = scaled(*place(i), power_of_two(row_shift(row_max[row_of(i)])));
+  }
+#pragma unroll
+  for (int j = 0; j < kFlight; ++j) {
+    const int i = base + j * kThreads + tid;
+    if (i >= items) break;
+    *place(i) = kScaled ? scaled(v[j], power_of_two(row_shift(row_max[row_of(i)]))) : v[j];
+  }
+  __syncthreads();
 
   // ---- products ----
   float acc[RU][NT][4] = {};
@@ -323,41 +361,49 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 1)
         sums[(k_warp * S::tokens + 8 * n + 2 * t + j % 2) * S::sum_row + ((warp % WR) * RU + u) * 16 + g + 8 * (j / 2)] =
             acc[u][n][j];
   __syncthreads();
-  // output row r of token m is row `row` of the products
-  const auto place_of = [&](int i, int &m, int &r) {
-    constexpr int quarter_rows = 4 * RU * WR;
-    m = i / S::rows;
-    r = i % S::rows;
-    return m * S::sum_row + r % quarter_rows / 4 * 16 + r % 4 * 4 + r / quarter_rows;
-  };
-  for (int i = tid; i < tokens * S::rows; i += kThreads) {
-    int m, r;
-    const int at = place_of(i, m, r);
-    float v = sums[at];
+  // four neighbours of the products' rows are the four quarters' rows of one place in them
+  const auto store = [&](int m, int l, const float4 &sum) {
+    const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+    const int64_t at = (m0 + m) * p.ldo + feature(l);
 #pragma unroll
-    for (int w = 1; w < S::k_warps; ++w) v += sums[w * S::tokens * S::sum_row + at];
-    v *= alpha;
-    if (kScaled) v *= power_of_two(-row_shift(row_max[m]));
+    for (int j = 0; j < 4; ++j) p.out[at + 32 * j] = __float2bfloat16_rn(v[j] + bias[j * (S::rows / 4) + l]);
+  };
+  const int fours = tokens * (S::rows / 4);
+#pragma unroll 2
+  for (int i = tid; i < fours; i += kThreads) {
+    const int m = i / (S::rows / 4), l = i % (S::rows / 4);
+    float4 *at = reinterpret_cast<float4 *>(sums + m * S::sum_row + 4 * l);
+    float4 sum = *at;
+#pragma unroll
+    for (int w = 1; w < S::k_warps; ++w) {
+      const float4 other = at[w * S::tokens * S::sum_row / 4];
+      sum.x += other.x, sum.y += other.y, sum.z += other.z, sum.w += other.w;
+    }
+    const float back = kScaled ? power_of_two(-row_shift(row_max[m])) : 1.0f;
+    sum = make_float4(sum.x * alpha * back, sum.y * alpha * back, sum.z * alpha * back, sum.w * alpha * back);
     if (split == 1)
-      p.out[(m0 + m) * p.ldo + feature(r)] = __float2bfloat16_rn(v + bias[r]);
+      store(m, l, sum);
     else
-      sums[at] = v;
+      *at = sum;
   }
   if (split == 1) return;
   cluster_sync();
-#pragma unroll 2
-  for (int i = part * kThreads + tid; i < tokens * S::rows; i += kThreads * split) {
-    int m, r;
-    const int at = place_of(i, m, r);
-    float other[8] = {};  // all in flight before the first is added
+#pragma unroll 1
+  for (int i = part * kThreads + tid; i < fours; i += kThreads * split) {
+    const int m = i / (S::rows / 4), l = i % (S::rows / 4);
+    const uint32_t at = smem_u32(sums + m * S::sum_row + 4 * l);
+    float4 other[8] = {};  // all in flight before the first is added
 #pragma unroll
     for (int c = 0; c < 8; ++c)
       if (c < split)
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(other[c]) : "r"(map_to_rank(smem_u32(sums + at), c)));
-    float v = 0.0f;
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(other[c].x), "=f"(other[c].y), "=f"(other[c].z), "=f"(other[c].w)
+                     : "r"(map_to_rank(at, c)));
+    float4 sum = other[0];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) v += other[c];
-    p.out[(m0 + m) * p.ldo + feature(r)] = __float2bfloat16_rn(v + bias[r]);
+    for (int c = 1; c < 8; ++c)
+      sum.x += other[c].x, sum.y += other[c].y, sum.z += other[c].z, sum.w += other[c].w;
+    store(m, l, sum);
   }
   cluster_sync();  // the others have read this block's sums
 }
@@ -371,10 +417,9 @@ int launch(Args p, int split, cudaStream_t stream) {
   p.chunk_inverse = static_cast<uint32_t>((1ull << 32) / (p.steps * 16)) + 1;
   const int used = S::ring_bytes + (p.M < S::tokens ? p.M : S::tokens) * S::row_bytes(p.steps);
   const int smem = used > S::sum_bytes ? used : S::sum_bytes;
-  constexpr int kMost = 220 * 1024;
-  if (smem > kMost) return set_error(VFB_EINVAL, "vfb_nvfp4_weight_only: K is too large");
+  if (smem > kMostSmem) return set_error(VFB_EINVAL, "vfb_nvfp4_weight_only: K is too large");
   static std::atomic<uint64_t> smem_set[kMaxAttrDevices];
-  int rc = ensure_smem_optin(reinterpret_cast<const void *>(kernel), kMost, smem_set);
+  int rc = ensure_smem_optin(reinterpret_cast<const void *>(kernel), kMostSmem, smem_set);
   if (rc != VFB_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(split, p.N / S::rows, (p.M + S::tokens - 1) / S::tokens);
@@ -397,13 +442,15 @@ int launch(Args p, int split, cudaStream_t stream) {
 
 // Blocks along K: as many as still run at once while every warp keeps two steps;
 // more where x of a K range would not leave room for `resident` blocks on an SM.
+// Powers of two only: three blocks of 16 warps in a cluster leave SMs unused (8
+// rows, N = 12288, K = 4096: 144 blocks in threes 22.8 us, 96 in pairs 15.1).
 template <typename T, int NT, int RU, int WR, int WARPS>
 int launch_split(const Args &p, int sms, int resident, cudaStream_t stream) {
   using S = Shape<NT, RU, WR, WARPS>;
   const int steps = (p.K + kStep - 1) / kStep;
   const int tokens = p.M < S::tokens ? p.M : S::tokens;
   const int64_t blocks = static_cast<int64_t>(p.N / S::rows) * ((p.M + S::tokens - 1) / S::tokens);
-  const int most = 224 * 1024 / resident - 2048 - S::ring_bytes;
+  const int most = (kMostSmem + 2048) / resident - 2048 - S::ring_bytes;
   int split = 1;
   while (split < 8 && ((2 * blocks * split <= resident * sms && steps >= 4 * split * S::k_warps) ||
                        tokens * S::row_bytes((steps + split - 1) / split) > most))
@@ -411,22 +458,26 @@ int launch_split(const Args &p, int sms, int resident, cudaStream_t stream) {
   return launch<T, NT, RU, WR, WARPS>(p, split, stream);
 }
 
-// Rows of a block: x is prepared once a block, so more weight rows share that work
-// the more rows x has, as long as the weight has enough of them for the SMs (and
-// for the two 128-row scale tiles of the widest block).  Measured, narrow against
-// wide block (us): 1 row, N = 12288, K = 4096 10.8 against 11.2; 5 rows 14.3
-// against 13.9; 8 rows, N = 28672, K = 5376 52.5 (128 rows) against 36.4 (256);
-// 16 rows, N = 4096, K = 16384 25.0 against 40.4, N = 16384, K = 4096 22.6 against
-// 20.3; 32 rows of the same 45.4 against 31.3.
+// Rows of the weight in a block.  Every block prepares x for itself, so tall
+// blocks share that work, the more the more rows x has; low blocks spread a low
+// weight over the SMs.  Measured (us, N x K):
+//   8 rows of x, 64 / 128 rows a block: 1152 x 1024 4.3 / 5.2, 128 x 16384 7.9 / 10.1,
+//   4096 x 4096 7.3 / 7.0, 12288 x 4096 14.6 / 12.8, 4096 x 16384 22.7 / 16.3;
+//   128 / 256 rows: 16384 x 4096 15.8 / 14.2, 28672 x 5376 33.8 / 26.6, and 12.2 / 12.0,
+//   23.9 / 22.7 for one row of x, but 12288 x 4096 12.8 / 13.5.
+//   32 rows of x, 128 / 256 rows a block (16 warps): 4096 x 4096 11.8 / 20.8,
+//   12288 x 4096 38.9 / 27.1, 28672 x 5376 99 / 76.
+// K > 16384 has no room for 32 rows of x.
 template <typename T>
 int run(const Args &p, int sms, cudaStream_t s) {
-  if (p.M <= 2) return launch_split<T, 1, 2, 2, 8>(p, sms, 3, s);
-  const bool wide = p.N % 256 == 0 && p.N >= (p.M <= 8 ? 24576 : 8192);
-  if (p.M <= 8)
-    return wide ? launch_split<T, 1, 2, 8, 16>(p, sms, 1, s) : launch_split<T, 1, 2, 4, 16>(p, sms, 1, s);
+  const bool tall = p.N % 256 == 0 && p.N >= (p.M <= 8 ? 16384 : 8192);
+  if (p.M <= 8) {
+    if (p.N <= 2048) return launch_split<T, 1, 2, 2, 8>(p, sms, 3, s);
+    return tall ? launch_split<T, 1, 2, 8, 16>(p, sms, 1, s) : launch_split<T, 1, 2, 4, 8>(p, sms, 3, s);
+  }
   if (p.M <= 16 || p.K > 16384)
-    return wide ? launch_split<T, 2, 2, 8, 16>(p, sms, 1, s) : launch_split<T, 2, 2, 4, 16>(p, sms, 1, s);
-  return wide ? launch_split<T, 4, 2, 8, 16>(p, sms, 1, s) : launch_split<T, 4, 2, 4, 16>(p, sms, 1, s);
+    return tall ? launch_split<T, 2, 2, 8, 16>(p, sms, 1, s) : launch_split<T, 2, 2, 4, 16>(p, sms, 1, s);
+  return tall ? launch_split<T, 4, 2, 8, 16>(p, sms, 1, s) : launch_split<T, 4, 2, 4, 16>(p, sms, 1, s);
 }
 
 constexpr int64_t kMaxK = 32768;
