@@ -11,12 +11,18 @@ device error or the output is not finite::
     python -m vflash_b200.profile_cases ffn --rows 8192 [--swiglu] [--one-kernel]
     python -m vflash_b200.profile_cases nvfp4_gemm --rows 8192 --n 4096
     python -m vflash_b200.profile_cases bf16_up --rows 32760
+    python -m vflash_b200.profile_cases attention --rows 8192 [--causal]
+    python -m vflash_b200.profile_cases attention_cached --rows 65536
+    python -m vflash_b200.profile_cases weight_only --rows 1 --n 65536
 
 Shapes other than the row count are those of the benchmark configurations:
 the merged QKV projection (N = 12288, K = 4096), the FFN (H = 4096,
 F = 16384; ``fp8_gemm_gelu`` is its up projection alone), the NVFP4
 linear (K = 4096) and a rank-32 low-rank up product (bf16, K = 32,
-N = 4096).
+N = 4096).  Attention runs 32 heads of 128: ``attention`` over one sequence of
+``rows`` tokens, ``attention_cached`` for one new token of each of 8 sequences
+that share ``rows`` cached keys evenly (8 key/value heads); ``weight_only`` is
+the weight-only NVFP4 product (K = 4096).
 """
 
 from __future__ import annotations
@@ -27,7 +33,8 @@ import sys
 import torch
 
 from . import _lib
-from .kernels import Epilogue, bf16_gemm, fp8_ffn, fp8_gemm, nvfp4_gemm, nvfp4_quantize, quantize_fp8_rows
+from .kernels import (Epilogue, attention, bf16_gemm, fp8_ffn, fp8_gemm, nvfp4_gemm, nvfp4_quantize, nvfp4_weight_only,
+                      quantize_fp8_rows)
 
 
 def _seeded(rows: int, cols: int, seed: int, std: float, device) -> torch.Tensor:
@@ -36,7 +43,7 @@ def _seeded(rows: int, cols: int, seed: int, std: float, device) -> torch.Tensor
 
 
 def run(case: str, rows: int, repeats: int, n: int = 4096, swiglu: bool = False,
-        one_kernel: bool = False) -> torch.Tensor:
+        one_kernel: bool = False, causal: bool = False) -> torch.Tensor:
     device = torch.device("cuda", 0)
     if case == "fp8_gemm":
         x = _seeded(rows, 4096, 1, 1.0, device)
@@ -77,6 +84,24 @@ def run(case: str, rows: int, repeats: int, n: int = 4096, swiglu: bool = False,
         up = _seeded(4096, 32, 2, 0.02, device)
         for _ in range(repeats):
             y = bf16_gemm(lo, up)
+    elif case == "attention":
+        q, k, v = (_seeded(rows, 32 * 128, i, 1.0, device).view(rows, 32, 128) for i in (1, 2, 3))
+        for _ in range(repeats):
+            y = attention(q, k, v, causal=causal)
+    elif case == "attention_cached":
+        q = _seeded(8, 32 * 128, 1, 1.0, device).view(8, 32, 128)
+        k, v = (_seeded(rows, 8 * 128, i, 1.0, device).view(rows, 8, 128) for i in (2, 3))
+        cu_q = torch.arange(9, dtype=torch.int32, device=device)
+        cu_k = cu_q * (rows // 8)
+        for _ in range(repeats):
+            y = attention(q, k, v, cu_q, cu_k, causal=True)
+    elif case == "weight_only":
+        x = _seeded(rows, 4096, 1, 1.0, device)
+        w = _seeded(n, 4096, 2, 0.02, device)
+        gsf_w = (448.0 * 6.0 / w.float().abs().max()).reshape(())
+        wp, wsc = nvfp4_quantize(w, gsf_w)
+        for _ in range(repeats):
+            y = nvfp4_weight_only(x, wp, wsc.view(n, 4096 // 16), (1.0 / gsf_w).to(torch.float32))
     else:
         raise ValueError(f"unknown case {case!r}")
     torch.cuda.synchronize(device)
@@ -85,14 +110,16 @@ def run(case: str, rows: int, repeats: int, n: int = 4096, swiglu: bool = False,
 
 def main(argv=None) -> int:
     parser = argparse.ArgumentParser(description=__doc__.split("\n\n")[0])
-    parser.add_argument("case", choices=["fp8_gemm", "fp8_gemm_gelu", "ffn", "nvfp4_gemm", "bf16_up"])
+    parser.add_argument("case", choices=["fp8_gemm", "fp8_gemm_gelu", "ffn", "nvfp4_gemm", "bf16_up", "attention",
+                                         "attention_cached", "weight_only"])
     parser.add_argument("--rows", type=int, default=4096)
     parser.add_argument("--n", type=int, default=4096, help="NVFP4 output features")
+    parser.add_argument("--causal", action="store_true", help="attention: mask later tokens")
     parser.add_argument("--repeats", type=int, default=3)
     parser.add_argument("--swiglu", action="store_true")
     parser.add_argument("--one-kernel", action="store_true")
     args = parser.parse_args(argv)
-    y = run(args.case, args.rows, args.repeats, args.n, args.swiglu, args.one_kernel)
+    y = run(args.case, args.rows, args.repeats, args.n, args.swiglu, args.one_kernel, args.causal)
     status = _lib.device_status(clear=True)
     finite = bool(torch.isfinite(y.float()).all())
     print(f"{args.case} rows={args.rows} status={status} finite={finite}")
