@@ -25,7 +25,7 @@
 //
 // A block's warps are WR row groups of RU units each, the steps of the block's K
 // range dealt out to the warps of a row group.  Every warp copies its steps into
-// a ring of its own in shared memory with cp.async, kDepth steps ahead, so that
+// a ring of its own in shared memory with cp.async, two steps ahead, so that
 // the loads in flight hold no registers and wait for nothing but themselves; the
 // loop over the steps stays rolled and small.  The warps' sums are added in shared
 // memory, those of the blocks of a cluster (one K range each) through distributed
@@ -460,21 +460,28 @@ int launch_split(const Args &p, int sms, int resident, cudaStream_t stream) {
 
 // Rows of the weight in a block.  Every block prepares x for itself, so tall
 // blocks share that work, the more the more rows x has; low blocks spread a low
-// weight over the SMs.  Measured (us, N x K):
+// weight over the SMs, and three of them share an SM, so that a last round of
+// few blocks costs less.  Measured (us, N x K):
 //   8 rows of x, 64 / 128 rows a block: 1152 x 1024 4.3 / 5.2, 128 x 16384 7.9 / 10.1,
 //   4096 x 4096 7.3 / 7.0, 12288 x 4096 14.6 / 12.8, 4096 x 16384 22.7 / 16.3;
-//   128 / 256 rows: 16384 x 4096 15.8 / 14.2, 28672 x 5376 33.8 / 26.6, and 12.2 / 12.0,
-//   23.9 / 22.7 for one row of x, but 12288 x 4096 12.8 / 13.5.
+//   128 / 256 rows, with tall blocks that fill the rounds on 148 SMs: 14336 x 5376
+//   21.3 / 16.8, 16384 x 4096 15.8 / 14.2, 28672 x 5376 33.8 / 26.6, 36864 x 4096
+//   29.1 / 22.8, and for one row of x 14.7 / 14.0, 12.2 / 12.0, 23.9 / 22.7, 19.8 / 19.5;
+//   where they do not: 12288 x 4096 12.8 / 13.5, 40960 x 4096 31.7 / 39.0 (one row
+//   of x 25.3 / 32.6).
 //   32 rows of x, 128 / 256 rows a block (16 warps): 4096 x 4096 11.8 / 20.8,
-//   12288 x 4096 38.9 / 27.1, 28672 x 5376 99 / 76.
+//   12288 x 4096 38.9 / 27.1, 28672 x 5376 99 / 76, 40960 x 4096 94.8 / 77.8.
 // K > 16384 has no room for 32 rows of x.
 template <typename T>
 int run(const Args &p, int sms, cudaStream_t s) {
-  const bool tall = p.N % 256 == 0 && p.N >= (p.M <= 8 ? 16384 : 8192);
+  const int64_t blocks = p.N % 256 ? 0 : (2 * p.N / 256 <= sms ? 2 : 1) * (p.N / 256);  // tall ones, with two along K
+  const int64_t rounds = (blocks + sms - 1) / sms;
   if (p.M <= 8) {
     if (p.N <= 2048) return launch_split<T, 1, 2, 2, 8>(p, sms, 3, s);
+    const bool tall = blocks > 0 && p.N >= 14336 && 10 * blocks >= 7 * rounds * sms;
     return tall ? launch_split<T, 1, 2, 8, 16>(p, sms, 1, s) : launch_split<T, 1, 2, 4, 8>(p, sms, 3, s);
   }
+  const bool tall = blocks > 0 && p.N >= 8192;
   if (p.M <= 16 || p.K > 16384)
     return tall ? launch_split<T, 2, 2, 8, 16>(p, sms, 1, s) : launch_split<T, 2, 2, 4, 16>(p, sms, 1, s);
   return tall ? launch_split<T, 4, 2, 8, 16>(p, sms, 1, s) : launch_split<T, 4, 2, 4, 16>(p, sms, 1, s);
