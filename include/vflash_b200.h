@@ -435,7 +435,7 @@ typedef struct vfb_attention_args {
   const int32_t *cu_seqlens_q, *cu_seqlens_k, *lengths_k;
   int32_t batch;               /* sequences (1 when cu_seqlens_q == NULL) */
   int32_t causal;
-  float scale;                 /* positive, finite */
+  float scale;                 /* positive, at most 1e30 */
   int32_t fill_tail;
   void *workspace;             /* vfb_attention_workspace_bytes() bytes, 256-byte aligned; NULL when that is 0. */
   int64_t workspace_bytes;     /* No other call in flight may use it. */

@@ -57,6 +57,7 @@ def test_operand_refusals(change, match):
     (dict(scale=0.0), "scale"),
     (dict(scale=-1.0), "scale"),
     (dict(scale=float("inf")), "scale"),
+    (dict(scale=3e38), "scale"),
     (dict(scale=float("nan")), "scale"),
     (dict(out=torch.zeros(6, 4, 32, dtype=BF16)), "out"),
     (dict(out=torch.zeros(6, 4, 64, dtype=torch.float16)), "out"),
@@ -95,7 +96,7 @@ def valid_args() -> _lib.AttentionArgs:
 @pytest.mark.parametrize("field,value", [
     ("total_q", -1), ("total_k", 2**31), ("heads", 3), ("heads", 0), ("kv_heads", 0), ("dim", 4), ("dim", 60),
     ("dim", 136), ("dtype", 2), ("batch", 0), ("batch", 2), ("cu_seqlens_k", 256), ("scale", 0.0),
-    ("scale", float("nan")), ("scale", float("inf")), ("q_token_stride", 60), ("k_head_stride", 0),
+    ("scale", float("nan")), ("scale", 3e38), ("scale", float("inf")), ("q_token_stride", 60), ("k_head_stride", 0),
     ("v_token_stride", 250), ("out_head_stride", -64)])
 def test_c_entry_refuses(field, value):
     lib = _lib.load()

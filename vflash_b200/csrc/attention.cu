@@ -1043,8 +1043,8 @@ int check_args(const vfb_attention_args *a) {
     return set_error(VFB_EINVAL, "vfb_attention: batch must be >= 1, and 1 without cu_seqlens_q");
   if (a->cu_seqlens_q != nullptr && a->cu_seqlens_k == nullptr && a->total_k != a->total_q)
     return set_error(VFB_EINVAL, "vfb_attention: keys of another length need cu_seqlens_k");
-  if (!(a->scale > 0.0f) || a->scale > 3.0e38f)
-    return set_error(VFB_EINVAL, "vfb_attention: scale must be positive and finite");
+  if (!(a->scale > 0.0f) || a->scale > 1.0e30f)  // times log2(e) it stays finite
+    return set_error(VFB_EINVAL, "vfb_attention: scale must be positive, at most 1e30");
   const int64_t strides[] = {a->q_token_stride, a->q_head_stride, a->k_token_stride,   a->k_head_stride,
                              a->v_token_stride, a->v_head_stride, a->out_token_stride, a->out_head_stride};
   for (int64_t s : strides)

@@ -620,7 +620,7 @@ def nvfp4_weight_only(matrix: torch.Tensor, w_packed: torch.Tensor, w_scales: to
     if rows > 1 and matrix.stride(0) < k:
         matrix = matrix.contiguous()  # expanded or overlapping rows
     if out is None:
-        out = torch.empty((rows, n), device=device, dtype=BF16)
+        out = torch.empty(rows, n, device=device, dtype=BF16)
     elif out.dtype != BF16 or out.shape != (rows, n) or out.stride(1) != 1 or rows > 1 and out.stride(0) < n:
         raise KernelInputError("the weight-only NVFP4 output must be bf16 [M, N] with unit column stride")
     elif out.device != device:
@@ -644,6 +644,8 @@ def nvfp4_weight_only(matrix: torch.Tensor, w_packed: torch.Tensor, w_scales: to
 def _strides(t: torch.Tensor, name: str) -> tuple[int, int]:
     """Token and head strides of a ``[rows, heads, dim]`` tensor; a dimension of one element takes a packed stride."""
     rows, heads, dim = t.shape
+    if t.is_contiguous():
+        return heads * dim, dim
     token, head, unit = t.stride()
     if unit != 1:
         raise KernelInputError(f"attention {name} needs a unit stride over the head dimension")
@@ -689,7 +691,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: t
     total_q, heads, dim = q.shape
     total_k, kv_heads = k.shape[:2]
     device = q.device
-    if q.dtype not in (BF16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+    dtype = q.dtype
+    if dtype not in (BF16, torch.float16) or k.dtype != dtype or v.dtype != dtype:
         raise KernelInputError("attention needs q, k and v all bf16 or all fp16")
     if k.shape != v.shape or k.shape[2] != dim or kv_heads < 1 or heads < 1 or heads % kv_heads:
         raise KernelInputError("attention needs k and v of one shape, q's dim, and heads divisible by kv_heads")
@@ -700,11 +703,11 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: t
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         raise KernelInputError("attention is inference-only")
     scale = dim ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < float("inf"):
-        raise KernelInputError("attention scale must be positive and finite")
+    if not 0.0 < scale <= 1e30:  # times log2(e) it stays finite
+        raise KernelInputError("attention scale must be positive, at most 1e30")
     if k.device != device or v.device != device:
         raise KernelInputError("attention operands must share one device")
-    at_q = at_k = at_n = None
+    at_q = at_k = at_n = 0
     batch = 1
     if cu_seqlens_q is not None:
         _check_offsets(cu_seqlens_q, None, device, "cu_seqlens_q")
@@ -724,14 +727,15 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: t
         at_n = lengths_k.data_ptr()
     fresh = out is None
     if fresh:
-        out = torch.empty((total_q, heads, dim), device=device, dtype=q.dtype)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != device:
+        out = torch.empty(total_q, heads, dim, device=device, dtype=dtype)
+    elif out.shape != q.shape or out.dtype != dtype or out.device != device:
         raise KernelInputError("attention out differs from q's shape, type or device")
-    lse = torch.empty((heads, total_q), device=device, dtype=torch.float32) if return_lse else None
-    args = _lib.AttentionArgs(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
-        *_strides(q, "q"), *_strides(k, "k"), *_strides(v, "v"), *_strides(out, "out"), total_q, total_k, heads,
-        kv_heads, dim, 0 if q.dtype == BF16 else 1, at_q, at_k, at_n, batch, causal, scale, fresh)
+    lse = torch.empty(heads, total_q, device=device, dtype=torch.float32) if return_lse else None
+    args = _lib.attention_args(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0,
+        *_strides(q, "q"), *_strides(k, "k"), *_strides(v, "v"),
+        *((heads * dim, dim) if fresh else _strides(out, "out")), total_q, total_k, heads, kv_heads, dim,
+        0 if dtype == BF16 else 1, at_q, at_k, at_n, batch, bool(causal), scale, fresh, 0, 0)
     lib = _lib.load()
     address = ctypes.byref(args)
     need = lib.vfb_attention_workspace_bytes(address)  # checks strides and alignment too
