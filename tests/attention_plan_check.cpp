@@ -3,7 +3,7 @@
 // exactly the pieces of each job that was cut.
 //
 // Reads cases from standard input, one a line:
-//   split blocks key_shift unit_shift grid groups job_tokens causal has_offsets batch total_q total_k  cu_q...  cu_k...  lengths_or_-1...
+//   split blocks key_shift band_keys unit_shift grid groups job_tokens causal has_offsets batch total_q total_k  cu_q...  cu_k...  lengths_or_-1...
 // and prints "ok <cases> <cut jobs>" or the first contradiction.
 #include <cstdio>
 #include <cstdlib>
@@ -28,6 +28,7 @@ int main() {
     Plan p = {};
     p.blocks = static_cast<int32_t>(read_int());
     p.key_shift = static_cast<int32_t>(read_int());
+    p.band_keys = static_cast<int32_t>(read_int());
     p.unit_shift = static_cast<int32_t>(read_int());
     const long long grid = read_int();
     p.groups = static_cast<int32_t>(read_int());
@@ -55,17 +56,23 @@ int main() {
     const int n = static_cast<int>(split ? p.blocks : grid);
     std::map<Job, bool> whole;
     for (int block = 0; block < n; ++block) {
-      Order order;
+      Share share;
+      uint32_t next = block;  // of the whole jobs
       if (split) {
         Record record;
-        order.init_share(p, block, record);
+        share.init(p, block, record);
         records.push_back(record);
-        if (order.empty()) empty_slots.insert(2 * block);
-      } else {
-        order.init_whole(block, static_cast<int32_t>(grid));
+        if (share.empty()) empty_slots.insert(2 * block);
       }
       Segment s;
-      while (order.next(p, s)) {
+      std::map<std::pair<int, int>, int> last;  // tile of a head group in a sequence
+      while (split ? share.next(p, s) : whole_job(p, next, s)) {
+        next += static_cast<uint32_t>(grid);
+        if (!split && p.causal && grid == 1) {  // in a head group's sequence the longest come first
+          const auto at = last.emplace(std::make_pair(s.b, s.group), s.seq.tiles).first;
+          if (s.tile != at->second - 1) return std::printf("order\n"), 1;
+          at->second = s.tile;
+        }
         const Job job{s.b, s.group, s.tile};
         if (s.seq.tiles <= s.tile || s.tile < 0 || s.group < 0 || s.group >= p.groups) return std::printf("bad job\n"), 1;
         const int tiles = tiles_of(p, s.seq, s.tile);

@@ -40,8 +40,9 @@ def case(rng: random.Random) -> str:
         total_k = max(0, total_k - 50)
     used = [rng.choice([0, x, x // 2, x + 5]) for x in nk] if rng.random() < 0.4 else [-1] * batch
     per_tile = total_q // tokens + batch + 1 if offsets else -(-total_q // tokens)
-    grid = max(1, min(total_q, per_tile) * groups if rng.random() < 0.5 else 148)
-    return " ".join(map(str, [int(split), blocks, rng.choice([6, 7]), rng.choice([0, 0, 0, 2, 9]), grid, groups, tokens, causal, int(offsets), batch, total_q, total_k,
+    grid = max(1, min(total_q, per_tile) * groups if rng.random() < 0.3 else rng.choice([1, 1, 148]))
+    band_keys = rng.choice([1, 700, 4000, 98304])
+    return " ".join(map(str, [int(split), blocks, rng.choice([6, 7]), band_keys, rng.choice([0, 0, 0, 2, 9]), grid, groups, tokens, causal, int(offsets), batch, total_q, total_k,
                               *cu_q, *cu_k, *used]))
 
 

@@ -16,7 +16,10 @@
 //   warp 8          TMA loads: Q tiles, then K and V tiles through one ring
 //   warp 9          MMA issue, one thread
 //   warp 10         cleans the V tiles that hold keys some row must not see
-//   warp 11         works out the block's jobs and hands them to the others
+//   warp 11         works out the block's jobs and hands them to the others; whole
+//                   jobs it takes, when it needs one, from the blocks of the grid that
+//                   have not begun (clusterlaunchcontrol: the list needs no counter in
+//                   memory, and blocks with short jobs take more of them)
 // The two stages keep the tensor cores busy with one tile's products while the
 // other's exponentials run.  They are
 //   PAIR: two tiles of query rows against the same keys (many query rows), or
@@ -88,7 +91,7 @@ struct Params {
   void *out;
   float *lse;
   int64_t v_token_stride, v_head_stride, out_token_stride, out_head_stride;
-  int32_t heads, pack, tokens;    // heads in a tile, tokens in a tile (pack * tokens <= 128)
+  int32_t pack, tokens;           // heads in a tile, tokens in a tile (pack * tokens <= 128)
   int32_t group_heads;            // query heads of one key/value head
   int32_t dim, fill_tail, split;
   float scale_log2;
@@ -222,6 +225,11 @@ __device__ __forceinline__ constexpr uint32_t exponent_mask() {  // both halves 
   return std::is_same<T, __nv_bfloat16>::value ? 0x7F807F80u : 0x7C007C00u;
 }
 
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t exponent_one() {  // its last bit
+  return std::is_same<T, __nv_bfloat16>::value ? 0x00800080u : 0x04000400u;
+}
+
 // ---- a job (or a piece of one) as the roles see it -----------------------------------
 struct Job {
   int64_t row0, k0;     // first query row of the job in q, first key row of its sequence
@@ -276,6 +284,8 @@ struct Shared {
   uint64_t v_todo[kRingSlots], v_clean[kRingSlots];
   uint64_t stats_full, stats_empty, drain;
   uint64_t job_full[kJobs], job_empty[kJobs];
+  alignas(16) uint64_t taken[2];  // the answer to take_block()
+  uint64_t taken_full;
   Job jobs[kJobs];
   uint32_t tmem;
   int abort;
@@ -284,6 +294,34 @@ struct Shared {
 };
 static_assert(sizeof(Shared) + Layout<128, true>::smem <= 232448 && sizeof(Shared) + Layout<128, false>::smem <= 232448,
               "shared memory of a block");
+
+// Takes a block of the grid that has not begun off it: its index, or -1 if all
+// have begun (then this must not be called again).  By a whole warp.
+__device__ __forceinline__ int64_t take_block(Shared &sh, uint32_t phase, int *status) {
+  if ((threadIdx.x & 31) == 0) {
+    mbar_arrive_expect_tx(&sh.taken_full, 16);
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                     smem_u32(sh.taken)),
+                 "r"(smem_u32(&sh.taken_full))
+                 : "memory");
+  }
+  __syncwarp();
+  if (!warp_wait_quick(&sh.taken_full, phase, &sh.abort, status)) return -1;
+  const volatile uint64_t *answer = sh.taken;
+  uint32_t taken, block;
+  asm volatile(
+      "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
+      "mov.b128 h, {%2, %3};\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+      : "=r"(taken), "=r"(block)
+      : "l"(answer[0]), "l"(answer[1]));
+  fence_proxy_async_smem();  // read before the next answer is written
+  __syncwarp();
+  return taken ? static_cast<int64_t>(block) : -1;
+}
 
 // A role's way through the schedule.
 struct JobReader {
@@ -509,6 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&sh.stats_full, 4);
     mbar_init(&sh.stats_empty, 4);
     mbar_init(&sh.drain, 1);
+    mbar_init(&sh.taken_full, 1);
     sh.abort = 0;
     sh.dirty = 0;
     fence_mbar_init();
@@ -821,37 +860,50 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     } else if (warp == 11) {
       // ---------------- schedule ----------------
-      attn::Order order;
-      bool alone = false;  // even shares: lane 0 goes on by itself
-      if (p.split) {
-        attn::Record record;
-        order.init_share(p.plan, blockIdx.x, record);
-        if (lane == 0) p.records[blockIdx.x] = record;
-        if (__shfl_sync(0xffffffffu, order.empty(), 0))  // a share cut to nothing may be counted among a job's pieces
-          for (int i = lane; i < kSlotRows; i += 32) p.part_lse[2ll * blockIdx.x * kSlotRows + i] = -INFINITY;
-        alone = true;
-      } else {
-        order.init_whole(blockIdx.x, gridDim.x);
-      }
       Segment seg;
+      int slot = 0;
       uint32_t phase = 1;
-      if (!alone || lane == 0) {
-        for (int slot = 0;;) {
-          const bool more = order.next(p.plan, seg);
-          if (lane == 0) {
-            if (more) describe<PAIR>(p, seg, job);
-            else job.count = -1;
-            mbar_wait_through(&sh.job_empty[slot], phase, &sh.abort, p.status);
-            sh.jobs[slot] = job;
-            mbar_arrive(&sh.job_full[slot]);
-          }
-          if (!alone) __syncwarp();
-          if (!more || *const_cast<volatile int *>(&sh.abort)) break;
-          if (++slot == kJobs) {
-            slot = 0;
-            phase ^= 1;
-          }
+      const auto hand_out = [&](bool more) {  // by lane 0
+        if (more) describe<PAIR>(p, seg, job);
+        else job.count = -1;
+        mbar_wait_through(&sh.job_empty[slot], phase, &sh.abort, p.status);
+        sh.jobs[slot] = job;
+        mbar_arrive(&sh.job_full[slot]);
+      };
+      const auto step = [&]() {
+        if (++slot == kJobs) {
+          slot = 0;
+          phase ^= 1;
         }
+      };
+      if (p.split) {
+        attn::Share share;
+        attn::Record record;
+        share.init(p.plan, blockIdx.x, record);
+        if (lane == 0) p.records[blockIdx.x] = record;
+        if (__shfl_sync(0xffffffffu, share.empty(), 0))  // a share cut to nothing may be counted among a job's pieces
+          for (int i = lane; i < kSlotRows; i += 32) p.part_lse[2ll * blockIdx.x * kSlotRows + i] = -INFINITY;
+        if (lane == 0)
+          for (bool more = true; more; step()) {
+            more = share.next(p.plan, seg);
+            hand_out(more);
+            if (*const_cast<volatile int *>(&sh.abort)) break;
+          }
+      } else {
+        uint32_t taken_phase = 0;
+        int64_t next = blockIdx.x;
+        while (next >= 0) {
+          if (attn::whole_job(p.plan, static_cast<uint32_t>(next), seg)) {
+            if (lane == 0) hand_out(true);
+            __syncwarp();
+            step();
+            // no job is taken before there is room for it
+            if (!warp_wait_quick(&sh.job_empty[slot], phase, &sh.abort, p.status)) break;
+          }
+          next = take_block(sh, taken_phase, p.status);
+          taken_phase ^= 1;
+        }
+        if (lane == 0) hand_out(false);
       }
     } else {
       // ---------------- cleaning of V tiles ----------------
@@ -869,21 +921,27 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int panel = 0; panel < L::panels; ++panel) {
           uint8_t *column = tile + panel * L::kv_panel + lane % 8 * 16;
-#pragma unroll 4
-          for (int r = all + row; r < end; r += 4) {
-            uint4 *at = reinterpret_cast<uint4 *>(column + r * 128);
-            uint4 x = *at;
-            uint32_t *word = reinterpret_cast<uint32_t *>(&x);
-            uint32_t bad = 0;
+          // Eight rows of a lane in flight; an element is not finite if adding one to its
+          // exponent carries into the sign.  None is, as a rule.
+#pragma unroll 1
+          for (int r0 = all + row; r0 < end; r0 += 32) {
+            uint32_t carry = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const uint32_t hit = __vcmpeq2(word[j] & exponent_mask<T>(), exponent_mask<T>());
-              word[j] &= ~hit;
-              bad |= hit;
+            for (int i = 0; i < 8; ++i) {
+              const int r = r0 + 4 * i;
+              uint4 x = make_uint4(0, 0, 0, 0);
+              if (r < end) x = *reinterpret_cast<const uint4 *>(column + r * 128);
+              const uint32_t word[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j) carry |= (word[j] & exponent_mask<T>()) + exponent_one<T>();
             }
-            if (bad) {
-              *at = x;
-              *reinterpret_cast<volatile int *>(&sh.dirty) = 1;
+            if (!(carry & 0x80008000u)) continue;
+            *reinterpret_cast<volatile int *>(&sh.dirty) = 1;
+#pragma unroll 1
+            for (int r = r0; r < min(r0 + 32, end); r += 4) {
+              uint32_t *word = reinterpret_cast<uint32_t *>(column + r * 128);
+#pragma unroll 1
+              for (int j = 0; j < 4; ++j) word[j] &= ~__vcmpeq2(word[j] & exponent_mask<T>(), exponent_mask<T>());
             }
           }
 #pragma unroll 4
@@ -988,6 +1046,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attention_join_kernel(const _
 // ---- host side -------------------------------------------------------------------------
 constexpr int kMaxBlocks = 148;  // SMs of a B200: blocks that even shares are cut for
 
+constexpr int kBandBytes = 48 << 20;  // of K and V that stay in L2 (126 MB) beside the rows read and written
+
 struct Choice {
   int pack, tokens, groups;
   bool pair, split;
@@ -1075,7 +1135,7 @@ int make_map(CUtensorMap *map, const void *base, int dtype, int64_t dim, int64_t
 }
 
 template <typename T, int DP, bool PAIR>
-int launch(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, const Params &p, int64_t jobs, int sms,
+int launch(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, const Params &p, int64_t jobs,
            cudaStream_t stream) {
   using L = Layout<DP, PAIR>;
   auto kernel = attention_kernel<T, DP, PAIR>;
@@ -1083,7 +1143,7 @@ int launch(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, con
   int rc = ensure_smem_optin(reinterpret_cast<const void *>(kernel), L::smem, smem_set);
   if (rc != VFB_OK) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.split ? p.plan.blocks : attn::min64(jobs, sms)), 1, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(p.split ? p.plan.blocks : jobs), 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
   cfg.dynamicSmemBytes = L::smem;
   cfg.stream = stream;
@@ -1145,6 +1205,7 @@ extern "C" int vfb_attention(const vfb_attention_args *args, void *stream) {
   p.plan.causal = a.causal != 0;
   p.plan.blocks = sms < kMaxBlocks ? sms : kMaxBlocks;
   p.plan.key_shift = c.pair ? 7 : 6;
+  p.plan.band_keys = kBandBytes / (4 * a.dim);
   p.plan.unit_shift = attn::unit_shift_for(c.jobs, a.total_q + a.total_k);
   p.v = a.v;
   p.out = a.out;
@@ -1153,7 +1214,6 @@ extern "C" int vfb_attention(const vfb_attention_args *args, void *stream) {
   p.v_head_stride = a.v_head_stride;
   p.out_token_stride = a.out_token_stride;
   p.out_head_stride = a.out_head_stride;
-  p.heads = a.heads;
   p.pack = c.pack;
   p.tokens = c.tokens;
   p.group_heads = a.heads / a.kv_heads;
@@ -1184,10 +1244,10 @@ extern "C" int vfb_attention(const vfb_attention_args *args, void *stream) {
   const auto go = [&](auto type) {
     using T = decltype(type);
     if (a.dim > 64)
-      return c.pair ? launch<T, 128, true>(mq, mk, mv, p, c.jobs, sms, s)
-                    : launch<T, 128, false>(mq, mk, mv, p, c.jobs, sms, s);
-    return c.pair ? launch<T, 64, true>(mq, mk, mv, p, c.jobs, sms, s)
-                  : launch<T, 64, false>(mq, mk, mv, p, c.jobs, sms, s);
+      return c.pair ? launch<T, 128, true>(mq, mk, mv, p, c.jobs, s)
+                    : launch<T, 128, false>(mq, mk, mv, p, c.jobs, s);
+    return c.pair ? launch<T, 64, true>(mq, mk, mv, p, c.jobs, s)
+                  : launch<T, 64, false>(mq, mk, mv, p, c.jobs, s);
   };
   return a.dtype == 0 ? go(__nv_bfloat16()) : go(__half());
 }
