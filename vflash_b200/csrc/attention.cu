@@ -80,7 +80,7 @@ struct Layout {
   static constexpr int q_tile = panels * kQPanel;
   static constexpr int kv_tile = panels * kv_panel;
   static constexpr int q_bytes = (PAIR ? 2 : 1) * q_tile;
-  static constexpr int ring = DP == 128 ? (PAIR ? 5 : 12) : (PAIR ? 8 : 16);
+  static constexpr int ring = DP == 128 ? (PAIR ? 5 : 11) : (PAIR ? 8 : 16);
   static constexpr int ahead = PAIR ? 1 : 4;  // key tiles whose S is issued before the first P V
   static constexpr int smem = 1024 + q_bytes + ring * kv_tile;  // tiles start on 1024 bytes
 };
@@ -230,6 +230,25 @@ __device__ __forceinline__ constexpr uint32_t exponent_one() {  // its last bit
   return std::is_same<T, __nv_bfloat16>::value ? 0x00800080u : 0x04000400u;
 }
 
+// Lane i of four gets the i-th of u from each of them, in the order of the lanes.
+__device__ __forceinline__ void transpose_in_four(uint4 (&u)[4], int lane) {
+  const auto exchange = [&](uint4 &keep_low, uint4 &keep_high, int with) {
+    const bool high = lane & with;
+    const uint4 give = high ? keep_low : keep_high;
+    uint4 got;
+    got.x = __shfl_xor_sync(0xffffffffu, give.x, with);
+    got.y = __shfl_xor_sync(0xffffffffu, give.y, with);
+    got.z = __shfl_xor_sync(0xffffffffu, give.z, with);
+    got.w = __shfl_xor_sync(0xffffffffu, give.w, with);
+    if (high) keep_low = got;
+    else keep_high = got;
+  };
+  exchange(u[0], u[1], 1);
+  exchange(u[2], u[3], 1);
+  exchange(u[0], u[2], 2);
+  exchange(u[1], u[3], 2);
+}
+
 // ---- a job (or a piece of one) as the roles see it -----------------------------------
 struct Job {
   int64_t row0, k0;     // first query row of the job in q, first key row of its sequence
@@ -290,9 +309,9 @@ struct Shared {
   uint32_t tmem;
   int abort;
   int dirty;  // a non-finite element of V was taken out of a tile
-  float2 stats[kTile];  // ALT: (m, l) of stage 1's rows
 };
-static_assert(sizeof(Shared) + Layout<128, true>::smem <= 232448 && sizeof(Shared) + Layout<128, false>::smem <= 232448,
+static_assert(sizeof(Shared) + Layout<128, true>::smem <= 232448 &&
+                  sizeof(Shared) + 2 * kTile * sizeof(float2) + Layout<128, false>::smem <= 232448,
               "shared memory of a block");
 
 // Takes a block of the grid that has not begun off it: its index, or -1 if all
@@ -517,6 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t *s_q = smem;
   uint8_t *s_kv = smem + L::q_bytes;
   __shared__ Shared sh;
+  __shared__ float2 stats[PAIR ? 1 : 2][PAIR ? 1 : kTile];  // (m, l) of each stage's rows
 
   const int warp = threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
@@ -542,10 +562,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&sh.p_tail[i][1], 4);
       mbar_init(&sh.pv_done[i], 1);
       mbar_init(&sh.o_full[i], 1);
-      mbar_init(&sh.o_empty[i], 4);
+      mbar_init(&sh.o_empty[i], PAIR ? 4 : 8);  // warps that read it
     }
-    mbar_init(&sh.stats_full, 4);
-    mbar_init(&sh.stats_empty, 4);
+    mbar_init(&sh.stats_full, 8);
+    mbar_init(&sh.stats_empty, 8);
     mbar_init(&sh.drain, 1);
     mbar_init(&sh.taken_full, 1);
     sh.abort = 0;
@@ -592,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool live = __any_sync(0xffffffffu, valid);
       if (!sm.run(PAIR ? job.t0 : job.t0 + stage, job.n[stage], PAIR ? 1 : 2, limit, live, valid)) break;
       float m = sm.m, l = sm.l;
-      bool have[2] = {job.n[stage] > 0, false};  // accumulators that hold something for this row
+      bool have[2] = {job.n[stage] > 0, false};  // (PAIR) accumulators that hold something for this row
       float f[2] = {1.0f, 0.0f};
       if (PAIR) {
         if (have[0]) {
@@ -600,34 +620,30 @@ __global__ void __launch_bounds__(kThreads, 1)
           o_phase[stage] ^= 1;
         }
       } else {
-        // stage 1 hands its statistics over; stage 0 joins the two accumulators
-        if (stage == 1) {
-          if (!warp_wait_quick(&sh.stats_empty, stats_phase ^ 1, &sh.abort, p.status)) break;
-          sh.stats[row] = make_float2(m, l);
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.stats_full);
-          stats_phase ^= 1;
-          continue;
-        }
+        // The stages exchange their statistics; each joins half the columns of the accumulators.
+        if (!warp_wait_quick(&sh.stats_empty, stats_phase ^ 1, &sh.abort, p.status)) break;
+        stats[stage][row] = make_float2(m, l);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.stats_full);
         if (!warp_wait_quick(&sh.stats_full, stats_phase, &sh.abort, p.status)) break;
         stats_phase ^= 1;
-        const float2 other = sh.stats[row];
+        const float2 s0 = stats[0][row], s1 = stats[PAIR ? 0 : 1][row];
         __syncwarp();
         if (lane == 0) mbar_arrive(&sh.stats_empty);
         bool ok = true;
+#pragma unroll
         for (int i = 0; i < 2; ++i) {
-          if (job.n[i] == 0) continue;
+          have[i] = job.n[i] > 0;
+          if (!have[i]) continue;
           ok = ok && warp_wait_quick(&sh.o_full[i], o_phase[i], &sh.abort, p.status);
           o_phase[i] ^= 1;
         }
         if (!ok) break;
-        have[1] = job.n[1] > 0;
-        const float joint = max3_nan(m, other.x, m);
-        const float shift = joint == -INFINITY ? 0.0f : joint;
-        f[0] = m == -INFINITY ? 0.0f : ex2((m - shift) * p.scale_log2);
-        f[1] = other.x == -INFINITY ? 0.0f : ex2((other.x - shift) * p.scale_log2);
-        m = joint;
-        l = l * f[0] + other.y * f[1];
+        m = max3_nan(s0.x, s1.x, s0.x);
+        const float shift = m == -INFINITY ? 0.0f : m;
+        f[0] = s0.x == -INFINITY ? 0.0f : ex2((s0.x - shift) * p.scale_log2);
+        f[1] = s1.x == -INFINITY ? 0.0f : ex2((s1.x - shift) * p.scale_log2);
+        l = s0.y * f[0] + s1.y * f[1];
       }
       tc_fence_after();
       // A row of infinite scores is NaN however its exponentials were rounded.
@@ -642,28 +658,39 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (job.slot >= 0) {
         const int64_t at = static_cast<int64_t>(job.slot) * kSlotRows + (PAIR ? stage * kTile : 0) + row;
         part = p.part_o + at * p.dim;
-        if (valid) p.part_lse[at] = none ? -INFINITY : m * p.scale_log2 + log2f(l);
-      } else if (valid && p.lse != nullptr) {
+        if (valid && (PAIR || stage == 0)) p.part_lse[at] = none ? -INFINITY : m * p.scale_log2 + log2f(l);
+      } else if (valid && (PAIR || stage == 0) && p.lse != nullptr) {
         p.lse[static_cast<int64_t>(head) * p.plan.total_q + out_row] = none ? -INFINITY : (m * p.scale_log2 + log2f(l)) * kLn2;
       }
       const bool dirty = *reinterpret_cast<volatile int *>(&sh.dirty) != 0;
       if (live) {
+        // Stores: four lanes exchange their rows' pieces and write 64 bytes of each row
+        // together.  (Every lane its own row: 32 lines for an instruction, 1.7 us a job.)
+        const unsigned valid_rows = __ballot_sync(0xffffffffu, valid) >> (lane & ~3);
         const float g0 = f[0] * inv, g1 = f[1] * inv;
         const uint32_t from = lanes + 256 + (PAIR ? 128 * stage : 0);
 #pragma unroll 1
-        for (int c = 0; c < DP; c += 32) {
+        for (int c = PAIR ? 0 : stage * (DP / 2); c < (PAIR || stage == 1 ? DP : DP / 2); c += 32) {
           if (c >= p.dim) break;
-          uint32_t r[32], r1[32];
-          if (have[0]) tmem_ld_32x32b_x32_issue(from + c, r);
-          if (!PAIR && have[1]) tmem_ld_32x32b_x32_issue(from + 128 + c, r1);
-          tmem_ld_wait();
-          if (have[0]) tmem_ld_fence(r);
-          if (!PAIR && have[1]) tmem_ld_fence(r1);
           float o[32];
+          {
+            uint32_t(&r)[32] = reinterpret_cast<uint32_t(&)[32]>(o);
+            if (have[0]) {
+              tmem_ld_32x32b_x32_issue(from + c, r);
+              tmem_ld_wait();
+              tmem_ld_fence(r);
+            }
+          }
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            o[j] = have[0] ? __uint_as_float(r[j]) * g0 : 0.0f;
-            if (!PAIR && have[1]) o[j] = fmaf(__uint_as_float(r1[j]), g1, o[j]);
+          for (int j = 0; j < 32; ++j) o[j] = have[0] ? o[j] * g0 : 0.0f;
+          if (!PAIR && have[1]) {
+#pragma unroll
+            for (int h = 0; h < 32; h += 16) {
+              uint32_t r[16];
+              tmem_ld_32x32b_x16(from + 128 + c + h, r);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) o[h + j] = fmaf(__uint_as_float(r[j]), g1, o[h + j]);
+            }
           }
           if (valid && dirty && !none) {
             // the elements that were taken out, for the rows that see them
@@ -678,22 +705,35 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
           }
-          if (valid) {
+          const int part_of_row = lane % 4;
+          uint4 u[4];
+          if (job.slot >= 0) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 8) {
-              if (c + j >= p.dim) break;
-              if (part != nullptr) {
-                float4 *dst = reinterpret_cast<float4 *>(part + c + j);
-                dst[0] = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-                dst[1] = make_float4(o[j + 4], o[j + 5], o[j + 6], o[j + 7]);
-              } else if (!job.behind || p.fill_tail) {
-                uint4 t;
-                t.x = pack2<T>(o[j], o[j + 1]);
-                t.y = pack2<T>(o[j + 2], o[j + 3]);
-                t.z = pack2<T>(o[j + 4], o[j + 5]);
-                t.w = pack2<T>(o[j + 6], o[j + 7]);
-                *reinterpret_cast<uint4 *>(out + c + j) = t;
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float *x = o + 16 * h + 4 * j;
+                u[j] = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
               }
+              transpose_in_four(u, lane);
+              const int column = c + 16 * h + 4 * part_of_row;
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if ((valid_rows >> j & 1) && column < p.dim)
+                  *reinterpret_cast<uint4 *>(part + (j - part_of_row) * p.dim + column) = u[j];
+            }
+          } else if (!job.behind || p.fill_tail) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float *x = o + 8 * j;
+              u[j] = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
+            }
+            transpose_in_four(u, lane);
+            const int column = c + 8 * part_of_row;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              T *row_j = reinterpret_cast<T *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(out), j, 4));
+              if ((valid_rows >> j & 1) && column < p.dim) *reinterpret_cast<uint4 *>(row_j + column) = u[j];
             }
           }
           __syncwarp();
@@ -770,14 +810,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t q_desc = sw128_kmajor_desc(smem_u32(s_q)), k_desc = sw128_kmajor_desc(smem_u32(s_kv));
         const uint64_t v_desc = sw128_mnmajor_desc(smem_u32(s_kv), L::kv_panel);
         RingPos<L::ring> pos;      // the item that is waited for next
-        uint32_t q_phase = 0, o_phase[2] = {1, 1};
-        uint32_t issued[2] = {0, 0}, joined[2] = {0, 0};  // S and P V of each stage so far, over all jobs
+        // Of the stages, in a field of 16 bits each (an array would live in local memory):
+        // S and P V so far, over all jobs, modulo 4, and the phase of o_empty.
+        uint32_t q_phase = 0, issued = 0, joined = 0, o_phase = 0x10001;
         uint32_t v_phase = 0;  // a bit for every slot
         const auto wait = [&](uint64_t *bar, uint32_t phase) { mbar_wait_through(bar, phase, &sh.abort, p.status); };
         const auto product_s = [&](int stage, int slot) {  // S = Q K^T
           const uint64_t a = q_desc + (PAIR ? stage * (L::q_tile >> 4) : 0);
           const uint64_t b = k_desc + slot * (L::kv_tile >> 4);
-          const uint32_t buffer = issued[stage]++ % kBuffers;
+          const uint32_t buffer = issued >> 16 * stage & (kBuffers - 1);
+          issued = (issued + (1u << 16 * stage)) & 0x30003u;
 #pragma unroll
           for (int k = 0; k < DP / 16; ++k)
             mma_f16(tmem + 128 * stage + kKeys * buffer, a + ((k / 4 * kQPanel + k % 4 * 32) >> 4),
@@ -785,12 +827,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_commit(&sh.s_full[stage][buffer]);
         };
         const auto product_o = [&](int stage, int slot, bool first, bool last) {  // O (+)= P V
-          const uint32_t buffer = joined[stage] % kBuffers, phase = joined[stage] / kBuffers & 1;
-          ++joined[stage];
+          const uint32_t count = joined >> 16 * stage, buffer = count & (kBuffers - 1), phase = count / kBuffers & 1;
+          joined = (joined + (1u << 16 * stage)) & 0x30003u;
           wait(&sh.p_full[stage][buffer], phase);
           if (first) {
-            wait(&sh.o_empty[stage], o_phase[stage]);
-            o_phase[stage] ^= 1;
+            wait(&sh.o_empty[stage], o_phase >> 16 * stage & 1);
+            o_phase ^= 1u << 16 * stage;
           }
           tc_fence_after();
           const uint64_t b = v_desc + slot * (L::kv_tile >> 4);
