@@ -49,6 +49,8 @@
 // zeroes, in the key tiles that any row of the block sees only in part, the V
 // rows behind the sequence's end and (causal) every element that is not
 // finite; the latter are added back at the end to the rows that do see them.
+#include <cmath>
+
 #include "common.cuh"
 #include "attention_plan.h"
 
@@ -1112,23 +1114,31 @@ Choice choose(const vfb_attention_args &a) {
                             ? (a.total_q + tokens - 1) / tokens
                             : attn::min64(a.total_q, a.total_q / tokens + a.batch + 1);
   c.jobs = tiles * c.groups;
-  // Even shares or whole jobs?  Shares cost the pieces' rows written and joined and
-  // the shares worked out: 20 us for PAIR, 10 us for ALT, the time of 1500 or 1100
-  // keys of a job.  They save what the blocks would idle: about a job's keys
-  // times the part of the blocks without one, half a job where there are more jobs
-  // than blocks, little when there are many.  Lengths are not known here, so a job
-  // is taken to have the average number of keys, twice that for keys of their own
-  // (caches differ more than prompts: there the longest job decides), and from
-  // 8192 cached keys on single tokens are always shared out.  Measured, whole against
-  // even (us): prompts of 2000 tokens of 32 / 8 heads 68 against 81, 4800 tokens of
-  // 16 / 2 heads 145 against 109; one token over 1000 keys 17 against 19, over 2000
-  // 27 against 20; 64 tokens over 1000 keys each 64 against 75, 32 over 1 to 8192
-  // 182 against 93.
-  int64_t keys = a.total_k / a.batch;
-  if (a.cu_seqlens_k != nullptr) keys = attn::min64(a.total_k, 2 * keys);
-  const int64_t idle = c.jobs < kMaxBlocks ? kMaxBlocks - c.jobs : kMaxBlocks / 2;
-  c.split = c.jobs < 4 * kMaxBlocks && (keys * idle > (c.pair ? 1500 : 1100) * kMaxBlocks ||
-                                        (!c.pair && a.total_k >= 8192));
+  // Even shares or whole jobs?  Both estimated, in the time of a key of a job (15 ns
+  // with two tiles of rows, 10 ns with one): a whole job costs a fixed time besides its
+  // keys, shares cost writing and joining the pieces and going through more short
+  // ones, and whole jobs leave blocks idle, all of them for the longest job where
+  // there are no more jobs than blocks.  Lengths are not known here.  Prompts count
+  // as equally long (the longest jobs go first).  Keys of their own are caches: half
+  // equal, half with one of twice the average, which may come last; with lengths inside
+  // of slots, half filled on average.  Measured, whole against even (us, 32 / 8
+  // heads of 128): prompts of 1000 tokens 24 / 40, 5000 188 / 215, all tokens seen 4000
+  // 245 / 247; 512 tokens after 1024, 4096, 16384 cached ones 30 / 40, 74 / 59, 247 / 135;
+  // single tokens of 1 sequence on 1000 and 2000 keys 16 / 19, 26 / 20, of 64 on 500 and 1000 36 / 54,
+  // 56 / 70, of 16 on 4000 50 / 61, of 32 on 1 to 8192 in slots 162 / 82.
+  const double fixed = c.pair ? 350 : 600, join = c.pair ? 2000 : 1900, slope = c.pair ? 1.05 : 1.2;
+  const double nk = static_cast<double>(a.total_k) / a.batch, nq = static_cast<double>(a.total_q) / a.batch;
+  const double mean = a.lengths_k != nullptr ? nk / 2 : a.causal ? nk - (nq < nk ? nq : nk) / 2 : nk;
+  const double rounds = static_cast<double>(c.jobs) / kMaxBlocks;
+  const bool few = c.jobs <= kMaxBlocks;
+  const double sorted = few ? fixed + nk : (a.causal ? rounds : std::ceil(rounds)) * (fixed + mean);
+  double whole = sorted;
+  if (a.lengths_k != nullptr || (a.cu_seqlens_k != nullptr && a.batch > 1)) {
+    const double longest = a.lengths_k != nullptr ? nk : 2 * nk;
+    const double uneven = few ? fixed + longest : rounds * (fixed + mean) + (fixed + longest) / 2;
+    whole = a.lengths_k != nullptr ? uneven : (sorted + uneven) / 2;
+  }
+  c.split = c.jobs < 4 * kMaxBlocks && whole > join + rounds * (mean + attn::OVERHEAD) * slope;
   return c;
 }
 
