@@ -147,6 +147,35 @@ def test_cache_slots(lengths, nq, heads, kv_heads):
     assert torch.equal(got.view(torch.int16), want.view(torch.int16))
 
 
+@pytest.mark.parametrize("nq,heads,kv_heads,lengths,slot", [
+    (1, 8, 2, [1, 5000, 0, 9000, 64, 3000], 9000), (20, 8, 2, [20, 5000, 0, 9000], 9000), (200, 8, 8, [200, 6000, 131], 6000),
+    (1, 16, 2, [30000], 32768)])
+def test_long_cache_slots(nq, heads, kv_heads, lengths, slot):
+    """Slots whose keys are shared out over the blocks, much of them unused."""
+    lengths_q = [nq] * len(lengths)
+    q, k, v = operands(lengths_q, lengths, heads, kv_heads, 128, BF16, slot=slot)
+    used = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    got, lse = attention(q, k, v, offsets(lengths_q), offsets(lengths, slot), lengths_k=used, causal=True,
+                         return_lse=True)
+    check(got, lse, q, k, v, lengths_q, lengths, True, slot=slot)
+
+
+def test_head_groups_whose_keys_do_not_fit_together():
+    """A causal sequence so long that its jobs go a few head groups at a time, more of them than blocks."""
+    q, k, v = operands([1500], [20000], 24, 12, 128, BF16)
+    got, lse = attention(q, k, v, offsets([1500]), offsets([20000]), causal=True, return_lse=True)
+    check(got, lse, q, k, v, [1500], [20000], True)
+
+
+def test_few_sequences_with_rows_among_many_without():
+    """Far more blocks are launched than there are jobs."""
+    lengths = [0] * 3000
+    lengths[17], lengths[2990] = 400, 2700
+    q, k, v = operands(lengths, lengths, 4, 2, 64, BF16)
+    got, lse = attention(q, k, v, offsets(lengths), causal=True, return_lse=True)
+    check(got, lse, q, k, v, lengths, lengths, True)
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_hidden_keys_never_reach_a_row(bad, dim):

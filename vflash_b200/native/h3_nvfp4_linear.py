@@ -201,8 +201,8 @@ class NVFP4Execution:
         ``W[n, k] = e2m1(code) * e4m3(scale)`` exactly; ``weight.input_scale``
         (the W4A4 path's activation calibration) plays no part.  For single
         tokens and small batches, where ``linear`` would pad to a 128-row tile
-        and quantise the activations for nothing: the call is bound by reading
-        the weight once.  fp32 values are first rounded to bf16, as in
+        and quantise the activations for nothing (from about a dozen rows on
+        ``linear`` is faster, where 4-bit activations will do).  fp32 values are first rounded to bf16, as in
         ``linear``; sums are fp32, with one rounding after the bias.
         """
         packed = weight.packed
