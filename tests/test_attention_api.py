@@ -67,6 +67,13 @@ def test_option_refusals(kwargs, match):
         attention(*operands(), **kwargs)
 
 
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_out_may_not_be_an_operand(which):
+    planes = [torch.zeros(6, 4, 64, dtype=BF16) for _ in range(3)]
+    with pytest.raises(KernelInputError, match="overlap"):
+        attention(*planes, out=planes[which])
+
+
 def test_other_key_count_needs_offsets():
     q, _, _ = operands()
     _, k, v = operands(rows=9)
@@ -95,7 +102,7 @@ def valid_args() -> _lib.AttentionArgs:
 
 @pytest.mark.parametrize("field,value", [
     ("total_q", -1), ("total_k", 2**31), ("heads", 3), ("heads", 0), ("kv_heads", 0), ("dim", 4), ("dim", 60),
-    ("dim", 136), ("dtype", 2), ("batch", 0), ("batch", 2), ("cu_seqlens_k", 256), ("scale", 0.0),
+    ("dim", 136), ("dtype", 2), ("batch", 0), ("batch", 2), ("batch", 2**31 - 1), ("cu_seqlens_k", 256), ("scale", 0.0),
     ("scale", float("nan")), ("scale", 3e38), ("scale", float("inf")), ("q_token_stride", 60), ("k_head_stride", 0),
     ("v_token_stride", 250), ("out_head_stride", -64)])
 def test_c_entry_refuses(field, value):

@@ -1151,8 +1151,8 @@ int check_args(const vfb_attention_args *a) {
   if (a->dim < 8 || a->dim > 128 || a->dim % 8)
     return set_error(VFB_EINVAL, "vfb_attention: dim must be a multiple of 8 from 8 to 128");
   if (a->dtype != 0 && a->dtype != 1) return set_error(VFB_EINVAL, "vfb_attention: dtype must be 0 (bf16) or 1 (fp16)");
-  if (a->batch < 1 || (a->cu_seqlens_q == nullptr && (a->batch != 1 || a->cu_seqlens_k != nullptr)))
-    return set_error(VFB_EINVAL, "vfb_attention: batch must be >= 1, and 1 without cu_seqlens_q");
+  if (a->batch < 1 || a->batch >= (1 << 30) || (a->cu_seqlens_q == nullptr && (a->batch != 1 || a->cu_seqlens_k != nullptr)))
+    return set_error(VFB_EINVAL, "vfb_attention: batch must be >= 1, below 2^30, and 1 without cu_seqlens_q");
   if (a->cu_seqlens_q != nullptr && a->cu_seqlens_k == nullptr && a->total_k != a->total_q)
     return set_error(VFB_EINVAL, "vfb_attention: keys of another length need cu_seqlens_k");
   if (!(a->scale > 0.0f) || a->scale > 1.0e30f)  // times log2(e) it stays finite

@@ -683,8 +683,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: t
     Returns ``[total_q, heads, dim]`` in the inputs' type, with ``return_lse``
     also the fp32 ``[heads, total_q]`` log-sum-exp of the scaled scores.  A row
     without keys is 0 (lse -inf), and so is a row behind the last sequence,
-    except in a given ``out``, where those rows stay as they were.  Inference
-    only; the scores never leave the SM.
+    except in a given ``out``, where those rows stay as they were.  ``out`` may be
+    strided as the inputs and may not overlap them.  Inference only; the scores
+    never leave the SM.
     """
     if q.ndim != 3 or k.ndim != 3 or v.ndim != 3:
         raise KernelInputError("attention operands must be [rows, heads, dim]")
@@ -730,6 +731,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: t
         out = torch.empty(total_q, heads, dim, device=device, dtype=dtype)
     elif out.shape != q.shape or out.dtype != dtype or out.device != device:
         raise KernelInputError("attention out differs from q's shape, type or device")
+    elif total_q and out.data_ptr() in (q.data_ptr(), k.data_ptr(), v.data_ptr()):
+        raise KernelInputError("attention out may not overlap q, k or v")
     lse = torch.empty(heads, total_q, device=device, dtype=torch.float32) if return_lse else None
     args = _lib.attention_args(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0,
