@@ -542,15 +542,17 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int warp = threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
-  if (threadIdx.x == 0) {
+  if (threadIdx.x < L::ring) {  // side by side: one thread takes half a microsecond for all of them
+    const int i = threadIdx.x;
+    mbar_init(&sh.kv_full[i], 1);
+    mbar_init(&sh.kv_empty[i], 1);
+    mbar_init(&sh.v_todo[i], 1);
+    mbar_init(&sh.v_clean[i], 1);
+    fence_mbar_init();
+  }
+  if (threadIdx.x == 32) {
     mbar_init(&sh.q_full, 1);
     mbar_init(&sh.q_empty, 1);
-    for (int i = 0; i < L::ring; ++i) {
-      mbar_init(&sh.kv_full[i], 1);
-      mbar_init(&sh.kv_empty[i], 1);
-      mbar_init(&sh.v_todo[i], 1);
-      mbar_init(&sh.v_clean[i], 1);
-    }
     for (int i = 0; i < kJobs; ++i) {
       mbar_init(&sh.job_full[i], 1);
       mbar_init(&sh.job_empty[i], kJobReaders);
