@@ -44,6 +44,15 @@
 // power limit here and the extra instructions cost clock (2 of 8: 15.1 against
 // 14.6 ms at the limit, 13.2 against 12.8 ms before it is reached).
 //
+// Measured (replayed graphs): 32760 tokens of 32 heads, all pairs, 14.1 to 15.0 ms
+// (1170 to 1250 TFLOP/s, at the power limit); causal prompts of 8192 to 1 tokens, 32 on 8
+// heads, 658 us (1140); 48 prompts of 1 to 300 tokens, heads of 64, 24 us; 17
+// tokens 7.7 us, all latency; one token of 32 requests on 1 to 8192 cached keys
+// 82 us (4.8 TB/s), of one on 131072 102 us (5.3 TB/s).
+//
+// P is rounded to the operands' type because the second product takes 16 bits;
+// the sum l is of the exponentials before that rounding, in fp32.
+//
 // Keys behind a row's limit: their scores become -inf, so P = 0; but 0 * inf
 // and 0 * NaN would still spoil the second product.  Warp 10 therefore
 // zeroes, in the key tiles that any row of the block sees only in part, the V

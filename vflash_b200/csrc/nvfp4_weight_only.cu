@@ -30,6 +30,11 @@
 // loop over the steps stays rolled and small.  The warps' sums are added in shared
 // memory, those of the blocks of a cluster (one K range each) through distributed
 // shared memory, always in the same order.
+//
+// Measured (replayed graphs): 1 row, N = 12288, K = 4096 9.9 us (2.9 TB/s with 4 us of
+// it start and end), N = 28672, K = 5376 21.6 us (4.0 TB/s); 7 rows of that 22.8 us;
+// 32 rows, N = 12288, K = 4096 26.8 us: bringing x to fp16 a third of a block's
+// time, products and decoding, with 96 of 148 SMs, most of the rest.
 #include <type_traits>
 
 #include "common.cuh"
