@@ -81,7 +81,7 @@ def test_model_sizes(n, k, rows):
 
 
 @pytest.mark.parametrize("n,rows,k", [(128, 9, 8384), (128, 17, 4416), (128, 18, 8768), (128, 32, 16384),
-                                      (128, 32, 16448), (128, 8, 32768), (256, 33, 32768), (8192, 10, 7488),
+                                      (128, 32, 16448), (128, 8, 32768), (256, 33, 32768), (4096, 20, 16384), (8192, 10, 7488),
                                       (16384, 4, 18880), (16384, 3, 25280)])
 def test_rows_that_fill_shared_memory(n, rows, k):
     """x takes most of a block's shared memory, or its K is dealt out so that it fits."""

@@ -32,8 +32,8 @@
 // shared memory, always in the same order.
 //
 // Measured (replayed graphs): 1 row, N = 12288, K = 4096 9.9 us (2.9 TB/s with 4 us of
-// it start and end), N = 28672, K = 5376 21.6 us (4.0 TB/s); 7 rows of that 22.8 us;
-// 32 rows, N = 12288, K = 4096 26.8 us: bringing x to fp16 a third of a block's
+// it start and end), N = 28672, K = 5376 21.6 us (4.0 TB/s); 7 rows of that 23 us;
+// 32 rows, N = 12288, K = 4096 24.7 us: bringing x to fp16 a quarter of a block's
 // time, products and decoding, with 96 of 148 SMs, most of the rest.
 #include <type_traits>
 
@@ -157,6 +157,7 @@ template <typename T, int NT, int RU, int WR, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 1)
     weight_only_kernel(const Args p) {
   using S = Shape<NT, RU, WR, WARPS>;
+  static_assert(NT == 1 || S::tokens <= 2 * WARPS, "a warp prepares at most two rows");
   constexpr bool kScaled = std::is_same<T, __nv_bfloat16>::value;  // rows of x carry a power of two
   constexpr int kThreads = 32 * WARPS;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -216,29 +217,40 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 1)
   const int row_bytes = S::row_bytes(p.steps);
   const T *x = static_cast<const T *>(p.x) + m0 * p.ldx;
   const int chunks = p.steps * (kStep / 8);  // of eight elements, in a row; a multiple of 16
-  const int items = tokens * chunks;
-  const auto row_of = [&](int i) { return static_cast<int>(__umulhi(i, p.chunk_inverse)); };  // i / chunks
+  // Up to eight rows: all threads share them.  More: a warp has one or two rows to
+  // itself and needs no other's maximum (32 rows, N = 12288, K = 4096: 24.7 us, before that 27.0).
+  constexpr bool kOwnRows = NT > 1;
+  constexpr int kStride = kOwnRows ? 32 : kThreads;
+  const int first = kOwnRows ? lane : tid;
+  const int items = (kOwnRows ? (tokens - warp + WARPS - 1) / WARPS : tokens) * chunks;
+  const auto nth_row = [&](int i) { return static_cast<int>(__umulhi(i, p.chunk_inverse)); };  // i / chunks
+  const auto row_of = [&](int i) { return kOwnRows ? warp + WARPS * nth_row(i) : nth_row(i); };
+  const auto chunk_of = [&](int i) { return i - nth_row(i) * chunks; };
   // chunk 4 * t + i of a step is read by lane t in its i-th pair of products
   const auto place = [&](int i) {
-    const int m = row_of(i), c = i - m * chunks;
-    return reinterpret_cast<uint4 *>(xs + m * row_bytes + (c / 16) * 256 + (c % 4) * 64 + (c % 16) / 4 * 16);
+    const int c = chunk_of(i);
+    return reinterpret_cast<uint4 *>(xs + row_of(i) * row_bytes + (c / 16) * 256 + (c % 4) * 64 + (c % 16) / 4 * 16);
   };
-  const auto from = [&](int i) {
-    const int m = row_of(i), c = i - m * chunks;
-    return x + m * p.ldx + k_begin + 8 * c;
-  };
-  const auto inside = [&](int i) { return 8 * (i - row_of(i) * chunks) < k_left; };  // K is a multiple of eight
-  const auto note = [&](int i, const uint4 &v) {  // 16 lanes with one row's chunks
-    const uint32_t top = __reduce_max_sync(0xFFFFu << (lane & 16), largest_x8(v));
-    if (lane % 16 == 0 && top) atomicMax(&row_max[row_of(i)], top);
+  const auto from = [&](int i) { return x + row_of(i) * p.ldx + k_begin + 8 * chunk_of(i); };
+  const auto inside = [&](int i) { return 8 * chunk_of(i) < k_left; };  // K is a multiple of eight
+  uint32_t best[2] = {0, 0};  // of a warp's own rows
+  const auto note = [&](int i, const uint4 &v) {
+    const uint32_t largest = largest_x8(v);
+    if (kOwnRows) {
+      if (nth_row(i) == 0) best[0] = max(best[0], largest);
+      else best[1] = max(best[1], largest);
+    } else {  // 16 lanes with one row's chunks
+      const uint32_t top = __reduce_max_sync(0xFFFFu << (lane & 16), largest);
+      if (lane % 16 == 0 && top) atomicMax(&row_max[row_of(i)], top);
+    }
   };
   constexpr int kFlight = NT == 1 ? 8 : 12;  // chunks of a thread in flight
-  constexpr int kFlightItems = kFlight * kThreads;
+  constexpr int kFlightItems = kFlight * kStride;
   uint4 v[kFlight];
   const auto load = [&](int base) {
 #pragma unroll
     for (int j = 0; j < kFlight; ++j) {
-      const int i = base + j * kThreads + tid;
+      const int i = base + j * kStride + first;
       if (i >= items) break;
       v[j] = make_uint4(0, 0, 0, 0);
       if (inside(i)) v[j] = __ldg(reinterpret_cast<const uint4 *>(from(i)));
@@ -249,7 +261,7 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 1)
   for (int i = 0; i < S::depth; ++i) copy(i);
   const float alpha = __ldg(p.alpha);
   for (int r = tid; r < S::rows; r += kThreads) bias[r] = p.bias != nullptr ? __bfloat162float(p.bias[feature(r)]) : 0.0f;
-  if (kScaled) {
+  if (kScaled && !kOwnRows) {
     if (tid < S::tokens) row_max[tid] = 0;
     __syncthreads();
   }
@@ -260,19 +272,19 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 1)
       if (kScaled) {
 #pragma unroll
         for (int j = 0; j < kFlight; ++j) {
-          const int i = base + j * kThreads + tid;
+          const int i = base + j * kStride + first;
           if (i >= items) break;
           note(i, v[j]);
         }
       }
       if (base + kFlightItems >= items) break;
 #pragma unroll
-      for (int j = 0; j < kFlight; ++j) *place(base + j * kThreads + tid) = v[j];
+      for (int j = 0; j < kFlight; ++j) *place(base + j * kStride + first) = v[j];
     }
   } else {
     base = items;
 #pragma unroll 1
-    for (int i = tid; i < items; i += kThreads) {
+    for (int i = first; i < items; i += kStride) {
       const uint4 c = inside(i) ? gather_x8(from(i)) : make_uint4(0, 0, 0, 0);
       if (kScaled) note(i, c);
       *place(i) = c;
@@ -289,14 +301,23 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 1)
     return make_uint4(w[0], w[1], w[2], w[3]);
   };
   if (kScaled) {
-    __syncthreads();
+    if (kOwnRows) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, best[r]);
+        if (lane == 0 && warp + r * WARPS < S::tokens) row_max[warp + r * WARPS] = top;
+      }
+      __syncwarp();
+    } else {
+      __syncthreads();
+    }
 #pragma unroll 4
-    for (int i = tid; i < base; i += kThreads)
+    for (int i = first; i < base; i += kStride)
       *place(i) = scaled(*place(i), power_of_two(row_shift(row_max[row_of(i)])));
   }
 #pragma unroll
   for (int j = 0; j < kFlight; ++j) {
-    const int i = base + j * kThreads + tid;
+    const int i = base + j * kStride + first;
     if (i >= items) break;
     *place(i) = kScaled ? scaled(v[j], power_of_two(row_shift(row_max[row_of(i)]))) : v[j];
   }
@@ -475,8 +496,13 @@ int launch_split(const Args &p, int sms, int resident, cudaStream_t stream) {
 //   where they do not: 12288 x 4096 12.8 / 13.5, 40960 x 4096 31.7 / 39.0 (one row
 //   of x 25.3 / 32.6).
 //   32 rows of x, 128 / 256 rows a block (16 warps): 4096 x 4096 11.8 / 20.8,
-//   12288 x 4096 38.9 / 27.1, 28672 x 5376 99 / 76, 40960 x 4096 94.8 / 77.8.
-// K > 16384 has no room for 32 rows of x.
+//   12288 x 4096 38.9 / 27.1, 28672 x 5376 99 / 76, 40960 x 4096 94.8 / 77.8 (before
+//   warps had rows of x to themselves, which took 10 % off all of these).
+// 32 rows of x (sixteen at a time otherwise) do not fit for K > 16384, and where they
+// only fit with K dealt out to eight blocks, these take more than one round unless
+// the weight is low: 4096 x 16384, 20 rows 45.7 / 35.3, 17 rows (four blocks along K) 27.3 /
+// 34.9; 4096 x 12288, 24 rows 22.0 / 27.7, 32 rows 41.4 / 29.4; 1024 x 16384, 32 rows
+// 17.4 / 22.2.
 template <typename T>
 int run(const Args &p, int sms, cudaStream_t s) {
   const int64_t blocks = p.N % 256 ? 0 : (2 * p.N / 256 <= sms ? 2 : 1) * (p.N / 256);  // tall ones, with two along K
@@ -487,7 +513,9 @@ int run(const Args &p, int sms, cudaStream_t s) {
     return tall ? launch_split<T, 1, 2, 8, 16>(p, sms, 1, s) : launch_split<T, 1, 2, 4, 8>(p, sms, 3, s);
   }
   const bool tall = blocks > 0 && p.N >= 8192;
-  if (p.M <= 16 || p.K > 16384)
+  const int64_t x_block = static_cast<int64_t>(p.M < 32 ? p.M : 32) * p.K;
+  const bool deep = p.K > 16384 || (x_block > 300000 && 8 * (p.N / 128) > sms);
+  if (p.M <= 16 || deep)
     return tall ? launch_split<T, 2, 2, 8, 16>(p, sms, 1, s) : launch_split<T, 2, 2, 4, 16>(p, sms, 1, s);
   return tall ? launch_split<T, 4, 2, 8, 16>(p, sms, 1, s) : launch_split<T, 4, 2, 4, 16>(p, sms, 1, s);
 }
