@@ -354,3 +354,18 @@ def test_block_stack_with_attention():
     replay = resident.capture(x, gate, attention=attend, cu_seqlens=cu)
     assert torch.equal(replay(), want)
     assert not torch.equal(streamed.forward(x, gate), want)
+
+
+@pytest.mark.parametrize("at_peak", [1.0, 0.0])
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+@pytest.mark.parametrize("nq,nk", [(1, 131072), (3, 1000), (300, 700)])
+def test_many_keys_far_below_the_peak_count(nq, nk, dtype, at_peak):
+    """One key carries the maximum, all others 18 nats less: below what fp16 holds of the largest, but many."""
+    q = torch.zeros(nq, 2, 64, dtype=dtype, device=DEV)
+    q[..., 0] = 1
+    k = torch.zeros(nk, 1, 64, dtype=dtype, device=DEV)
+    k[1:, :, 0] = -18
+    v = torch.ones(nk, 1, 64, dtype=dtype, device=DEV)
+    v[0] = at_peak
+    got, lse = attention(q, k, v, offsets([nq]), offsets([nk]), scale=1.0, return_lse=True)
+    check(got, lse, q, k, v, [nq], [nk], False, scale=1.0)

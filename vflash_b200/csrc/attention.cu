@@ -8,8 +8,9 @@
 //   O = O * 2^(m - m') + P V      tcgen05, P (16 bit) read from TMEM
 //   out = O / l,  lse = m * scale + ln l
 // S and O never leave the SM.  m only moves (and O is only multiplied) when the
-// maximum grows by more than kHold binary orders, so P may reach 2^kHold; the
-// result is the same to rounding and the pass over O in TMEM is rare.
+// maximum grows by more than kHold binary orders, so P may reach 2^kHold (in fp16
+// all of P lies 2^kLift higher); the result is the same to rounding and the pass over
+// O in TMEM is rare.
 //
 // Roles of a block of twelve warps, one block on an SM:
 //   warps 0-3, 4-7  softmax of stage 0 and stage 1, one thread per row
@@ -77,6 +78,12 @@ constexpr int kRingSlots = 16;       // at most
 constexpr int kJobs = 2;             // jobs that the scheduler may be ahead
 constexpr int kJobReaders = 11;      // warps that follow the schedule
 constexpr float kHold = 8.0f;
+// P carries a factor of 2^kLift, which cancels in O / l and comes off the
+// log-sum-exp.  fp16 ends at 2^-24, and many keys that each round to 0 there may hold
+// a good part of l; P is at most 2^kHold, so 2^7 more still fit below 65504, and what
+// is lost of a probability is at most 2^-32 of the largest.  bf16 has fp32's range.
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? 7.0f : 0.0f;
 constexpr float kLn2 = 0.693147180559945309f;
 
 // Rows of a workspace slot (one piece of a job): both tiles of PAIR.
@@ -503,7 +510,7 @@ struct Softmax {
       }
     }
     const float base = m == -INFINITY ? 0.0f : m * p.scale_log2;
-    const f32x2 scale2 = pair(p.scale_log2, p.scale_log2), base2 = pair(-base, -base);
+    const f32x2 scale2 = pair(p.scale_log2, p.scale_log2), base2 = pair(kLift<T> - base, kLift<T> - base);
     f32x2 sum[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
 #pragma unroll
     for (int h = 0; h < N / 32; ++h) {
@@ -671,9 +678,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (job.slot >= 0) {
         const int64_t at = static_cast<int64_t>(job.slot) * kSlotRows + (PAIR ? stage * kTile : 0) + row;
         part = p.part_o + at * p.dim;
-        if (valid && (PAIR || stage == 0)) p.part_lse[at] = none ? -INFINITY : m * p.scale_log2 + log2f(l);
+        if (valid && (PAIR || stage == 0)) p.part_lse[at] = none ? -INFINITY : m * p.scale_log2 + (log2f(l) - kLift<T>);
       } else if (valid && (PAIR || stage == 0) && p.lse != nullptr) {
-        p.lse[static_cast<int64_t>(head) * p.plan.total_q + out_row] = none ? -INFINITY : (m * p.scale_log2 + log2f(l)) * kLn2;
+        p.lse[static_cast<int64_t>(head) * p.plan.total_q + out_row] =
+            none ? -INFINITY : (m * p.scale_log2 + (log2f(l) - kLift<T>)) * kLn2;
       }
       const bool dirty = *reinterpret_cast<volatile int *>(&sh.dirty) != 0;
       if (live) {
