@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
@@ -369,3 +371,78 @@ def test_many_keys_far_below_the_peak_count(nq, nk, dtype, at_peak):
     v[0] = at_peak
     got, lse = attention(q, k, v, offsets([nq]), offsets([nk]), scale=1.0, return_lse=True)
     check(got, lse, q, k, v, [nq], [nk], False, scale=1.0)
+
+
+def workspace_bytes(q, k, batch, causal, slots=False):
+    """What the call reserves for pieces of jobs: 0 where it runs whole jobs."""
+    rows, heads, dim = q.shape
+    kv = k.shape[1]
+    at = q.data_ptr()
+    args = _lib.attention_args(
+        at, k.data_ptr(), k.data_ptr(), at + q.numel() * 2, 0, heads * dim, dim, kv * dim, dim, kv * dim, dim, heads * dim, dim, rows,
+        k.shape[0], heads, kv, dim, 0 if q.dtype == BF16 else 1, at, at, at if slots else 0, batch, causal, 1.0, 0, 0, 0)
+    need = _lib.load().vfb_attention_workspace_bytes(ctypes.byref(args))
+    assert need >= 0
+    return need
+
+
+CUT = [(1, 9000, 2, 1, 64, True), (3, 9001, 8, 2, 128, True), (40, 9000, 4, 4, 128, True), (300, 4001, 2, 1, 128, True),
+       (300, 4001, 4, 4, 64, True), (3, 500, 8, 2, 128, False), (300, 700, 4, 4, 64, False)]  # the last ones are whole
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("nq,nk,heads,kv_heads,dim,cut", CUT)
+def test_values_that_are_not_finite_where_the_keys_have_no_weight(nq, nk, heads, kv_heads, dim, cut, bad):
+    """Seen keys whose exponentials vanish beside the others' still bring their NaN and infinities (0 * inf)."""
+    q, k, v = operands([nq], [nk], heads, kv_heads, dim, BF16)
+    assert (workspace_bytes(q, k, 1, False) > 0) == cut
+    q[..., 0], k[..., 0] = 1, 0
+    low = nk // 3
+    k[:low, :, 0] = -1000  # at scale 1: far more than 126 binary orders below, in pieces of their own when cut
+    run = lambda values: attention(q, k, values, offsets([nq]), offsets([nk]), scale=1.0, return_lse=True)  # noqa: E731
+    want, want_lse = run(v)
+    check(want, want_lse, q, k, v, [nq], [nk], False, scale=1.0)
+    v[7, 0, 5] = bad
+    v[low - 1, 0, 6] = bad
+    got, lse = run(v)
+    assert not torch.isfinite(got[:, :heads // kv_heads, 5:7].float()).any()
+    got[:, :heads // kv_heads, 5:7] = want[:, :heads // kv_heads, 5:7]
+    assert torch.equal(got, want) and torch.equal(lse, want_lse)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("nq,nk,heads,kv_heads,dim,cut", CUT)
+def test_values_that_are_not_finite_at_the_end_of_a_job(nq, nk, heads, kv_heads, dim, cut, bad):
+    """Keys that only later rows see: taken out of the tile for the others, added back for those that see them."""
+    q, k, v = operands([nq], [nk], heads, kv_heads, dim, BF16)
+    assert (workspace_bytes(q, k, 1, True) > 0) == cut
+    run = lambda values: attention(q, k, values, offsets([nq]), offsets([nk]), causal=True, return_lse=True)  # noqa: E731
+    want, want_lse = run(v)
+    check(want, want_lse, q, k, v, [nq], [nk], True)
+    first = nq // 2  # the row from which on this key is seen
+    v[nk - nq + first, 0, 5] = bad
+    got, lse = run(v)
+    column = got[first:, :heads // kv_heads, 5].float()
+    assert (column != column).all() if bad != bad else (column == bad).all()
+    got[first:, :heads // kv_heads, 5] = want[first:, :heads // kv_heads, 5]
+    assert torch.equal(got, want) and torch.equal(lse, want_lse)
+    # a key that is not finite: every row that sees it is NaN, the others are as they were
+    k[nk - nq + first, 0, 3] = float("nan")
+    got, _ = run(torch.where(torch.isfinite(v), v, 0))
+    assert torch.isnan(got[first:, :heads // kv_heads].float()).all()
+    assert torch.equal(got[:first, :, 6:], want[:first, :, 6:])
+
+
+@pytest.mark.parametrize("nq,nk,heads,kv_heads,dim,cut", CUT)
+def test_scores_of_minus_infinity(nq, nk, heads, kv_heads, dim, cut):
+    """Keys with scores of -inf have no weight; a row that sees nothing else is 0 / 0, whether its job is cut or not."""
+    q, k, v = operands([nq], [nk], heads, kv_heads, dim, BF16)
+    assert (workspace_bytes(q, k, 1, False) > 0) == cut
+    q[..., 0] = 1
+    low = nk // 3 + 1
+    k[:low, :, 0] = float("-inf")
+    got, lse = attention(q, k, v, offsets([nq]), offsets([nk]), return_lse=True)
+    check(got, lse, q, k[low:], v[low:], [nq], [nk - low], False)
+    k[..., 0] = float("-inf")
+    got, lse = attention(q, k, v, offsets([nq]), offsets([nk]), return_lse=True)
+    assert torch.isnan(got.float()).all() and (lse == -torch.inf).all()

@@ -85,6 +85,9 @@ constexpr float kHold = 8.0f;
 template <typename T>
 constexpr float kLift = std::is_same<T, __half>::value ? 7.0f : 0.0f;
 constexpr float kLn2 = 0.693147180559945309f;
+// Log-sum-exp of a piece whose keys' scores are all -inf: it has no weight beside
+// others, yet is no piece without keys (-inf), whose rows may be unwritten.
+constexpr float kNoWeight = -3.402823466e38f;
 
 // Rows of a workspace slot (one piece of a job): both tiles of PAIR.
 constexpr int kSlotRows = 2 * kTile;
@@ -670,7 +673,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (m == INFINITY) l = NAN;
       const int64_t piece_end = attn::min64(limit, static_cast<int64_t>(job.t1) * kKeys);
       const bool none = piece_end <= static_cast<int64_t>(job.t0) * kKeys;
-      const float inv = none ? 0.0f : 1.0f / l;
+      // (l == 0: all scores are -inf.  Alone that is 0 / 0; a piece leaves its sums as they are.)
+      const float inv = none ? 0.0f : job.slot >= 0 && l == 0.0f ? 1.0f : 1.0f / l;
       const int64_t out_row = job.row0 + token;
       const int head = job.group * p.pack + head_in_tile;
       T *out = static_cast<T *>(p.out) + out_row * p.out_token_stride + head * p.out_head_stride;
@@ -678,7 +682,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (job.slot >= 0) {
         const int64_t at = static_cast<int64_t>(job.slot) * kSlotRows + (PAIR ? stage * kTile : 0) + row;
         part = p.part_o + at * p.dim;
-        if (valid && (PAIR || stage == 0)) p.part_lse[at] = none ? -INFINITY : m * p.scale_log2 + (log2f(l) - kLift<T>);
+        if (valid && (PAIR || stage == 0))
+          p.part_lse[at] = none ? -INFINITY : l == 0.0f ? kNoWeight : m * p.scale_log2 + (log2f(l) - kLift<T>);
       } else if (valid && (PAIR || stage == 0) && p.lse != nullptr) {
         p.lse[static_cast<int64_t>(head) * p.plan.total_q + out_row] =
             none ? -INFINITY : (m * p.scale_log2 + (log2f(l) - kLift<T>)) * kLn2;
@@ -1074,14 +1079,17 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attention_join_kernel(const _
     const float base = top == -INFINITY ? 0.0f : top;
     float sum = 0.0f, acc[4] = {};
     for (int i0 = 0; i0 < pieces; i0 += 32) {
-      const float weight = i0 + lane < pieces ? ex2(p.part_lse[slot_row(i0 + lane)] - base) : 0.0f;
+      const float part = i0 + lane < pieces ? p.part_lse[slot_row(i0 + lane)] : -INFINITY;
+      const float weight = ex2(part - base);
+      const unsigned written = __ballot_sync(0xffffffffu, part != -INFINITY);
       sum += weight;
       const int n = min(32, pieces - i0);
 #pragma unroll 4
       for (int i = 0; i < n; ++i) {
         const float w = __shfl_sync(0xffffffffu, weight, i);
-        // a piece without keys left its rows unwritten
-        if (lane * 4 < p.dim && w != 0.0f) {
+        // A piece without keys may have left its rows unwritten.  One with a weight of 0 is
+        // read: what it saw of infinities and NaN stays, as it does inside a job.
+        if (lane * 4 < p.dim && (written >> i & 1)) {
           const float4 o = *reinterpret_cast<const float4 *>(p.part_o + slot_row(i0 + i) * p.dim + 4 * lane);
           acc[0] = fmaf(w, o.x, acc[0]);
           acc[1] = fmaf(w, o.y, acc[1]);
@@ -1091,7 +1099,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attention_join_kernel(const _
       }
     }
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const float inv = top == -INFINITY ? 0.0f : 1.0f / sum;
+    const float inv = top == -INFINITY ? 0.0f : top == kNoWeight ? NAN : 1.0f / sum;
     const int head = job.group * p.pack + in_tile % p.pack;
     const int64_t row = static_cast<int64_t>(job.row0) + token;
     if (lane * 4 < p.dim) {
@@ -1102,7 +1110,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attention_join_kernel(const _
                                  4 * lane) = t;
     }
     if (lane == 0 && p.lse != nullptr)
-      p.lse[static_cast<int64_t>(head) * p.plan.total_q + row] = top == -INFINITY ? -INFINITY : (top + log2f(sum)) * kLn2;
+      p.lse[static_cast<int64_t>(head) * p.plan.total_q + row] =
+          top == -INFINITY || top == kNoWeight ? -INFINITY : (top + log2f(sum)) * kLn2;
   }
 }
 
