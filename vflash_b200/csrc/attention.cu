@@ -462,7 +462,13 @@ struct Softmax {
   __device__ __forceinline__ void hand_over(uint64_t (&bar)[2]) {
     tc_fence_before();
     __syncwarp();
-    if ((threadIdx.x & 31) == 0) mbar_arrive(&bar[count % kBuffers]);
+    // by predicate: the lanes stay together for the next store to TMEM
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.eq.u32 p, %1, 0;\n\t"
+        "@p mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];\n\t}" ::"r"(smem_u32(&bar[count % kBuffers])),
+        "r"(threadIdx.x & 31)
+        : "memory");
   }
 
   __device__ __forceinline__ bool tile(int32_t key0, int32_t limit, bool scale_o, bool valid) {

@@ -464,17 +464,19 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volati
   return __all_sync(0xffffffffu, ok);
 }
 
-// warp_wait for roles that wait several times for every product they issue: no
-// vote while the phase is there or comes soon (38 cycles when it is there, warp_wait
-// 112).  The warp is converged and all lanes ask with one instruction, so
-// they get one answer; only giving up is voted on.
+// warp_wait for roles that wait several times for every product they issue: the
+// lanes vote on every try instead of once behind a loop of their own (a late lane may
+// see a phase that others have not seen yet), and no clock is read while the phase is
+// there or comes soon.  All control flow hangs on votes, so no lane can leave for
+// another warp-wide instruction while the others still wait; the vote also brings the lanes
+// together when only one of them has just issued a copy or an arrival.
 __device__ __forceinline__ bool warp_wait_quick(uint64_t *bar, uint32_t parity, volatile int *abort_flag,
                                                 int *status) {
-  if (mbar_try_wait(bar, parity)) return true;
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
   const uint64_t start = global_timer_ns();
   for (;;) {
     for (int spin = 0; spin < 256; ++spin)
-      if (mbar_try_wait(bar, parity)) return true;
+      if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
     const bool expired = global_timer_ns() - start > VFB_WAIT_TIMEOUT_NS;
     if (__any_sync(0xffffffffu, expired || *abort_flag)) {
       if (expired) {
