@@ -386,7 +386,8 @@ VFB_API int vfb_nvfp4_gemm_quant(const void *A, const void *sfa, const void *W, 
  * bf16 (dtype 0) or fp16 (dtype 1) [M,K], row stride ldx >= K, any alignment
  * of its element type.  w_codes / w_sf: the packed weight [N,K/2] and its 128x4 scales as in
  * vfb_nvfp4_gemm.  alpha: fp32 device scalar.  bias: bf16 [N] or NULL.  out:
- * bf16 [M,N], row stride ldo >= N, no overlap with x.  Requires K % 64 == 0, K <= 32768,
+ * bf16 [M,N], row stride ldo >= N, no overlap with x, the weight, alpha or bias
+ * (refused unless apart or interleaved with one period).  Requires K % 64 == 0, K <= 32768,
  * N % 128 == 0, N <= 1048576, M <= 524288, 16-byte aligned w_codes, 4-byte
  * aligned w_sf.
  * bf16 rows are brought to fp16 by a power of two of their own (exact for
@@ -422,8 +423,9 @@ VFB_API int vfb_nvfp4_weight_only(const void *x, int32_t dtype, int64_t M, int64
  * as they are; rows of `lse` behind it become -inf. */
 typedef struct vfb_attention_args {
   const void *q, *k, *v;       /* bf16 (dtype 0) or fp16 (dtype 1), [rows, heads, dim], unit dim stride */
-  void *out;                   /* the same type, [total_q, heads, dim]; may not alias q, k or v */
-  float *lse;                  /* [heads, total_q] contiguous, or NULL */
+  void *out;                   /* the same type, [total_q, heads, dim] */
+  float *lse;                  /* [heads, total_q] contiguous, or NULL; out and lse may not overlap q, k, v or each
+                                * other (refused unless apart or interleaved with one period) */
   int64_t q_token_stride, q_head_stride;  /* strides in elements, multiples of 8; bases 16-byte aligned */
   int64_t k_token_stride, k_head_stride;
   int64_t v_token_stride, v_head_stride;

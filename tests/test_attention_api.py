@@ -142,3 +142,48 @@ def test_packed_attention_checks():
         PackedAttention(heads=1)(*[torch.zeros(2, 64, dtype=BF16)] * 3, out=torch.zeros(64, 2, dtype=BF16).T)
     with pytest.raises(ValueError, match="cu_seqlens"):
         block_linears(None, {}, None, None, cu_seqlens=cu(0, 1))
+
+
+def launch_refusal(**fields) -> str:
+    """What vfb_attention answers for planes that lie apart but for ``fields``, and a workspace that is missing."""
+    a = valid_args()
+    for i, name in enumerate(("q", "k", "v", "out")):
+        setattr(a, name, (i + 1) << 26)
+    a.total_k, a.cu_seqlens_q, a.cu_seqlens_k = 20000, 256, 256
+    for name, value in fields.items():
+        setattr(a, name, value)
+    lib = _lib.load()
+    assert lib.vfb_attention_workspace_bytes(ctypes.byref(a)) > 0  # so the call is refused here or there, on any machine
+    assert lib.vfb_attention(ctypes.byref(a), None) == _lib.VFB_EINVAL
+    return _lib.last_error()
+
+
+Q, K, V, OUT = ((i + 1) << 26 for i in range(4))
+ROW = 2 * 256  # bytes of a packed row of 4 heads of 64
+
+
+@pytest.mark.parametrize("fields", [
+    dict(out=Q), dict(out=Q + ROW), dict(out=Q - ROW), dict(out=Q + 5 * ROW), dict(out=K + 16), dict(out=V - 5 * ROW), dict(out=V + 19999 * ROW),
+    dict(out=Q + ROW // 2, q_token_stride=512, out_token_stride=512),  # half a row on, the other half in the next gap
+    dict(q=1 << 16, out=(1 << 16) + 128, q_head_stride=128, out_head_stride=64, q_token_stride=512),
+    dict(out=1 << 16, q=(1 << 16) + 6 * 128 - 16, q_token_stride=64, q_head_stride=6 * 64, out_token_stride=64,
+         out_head_stride=6 * 64),
+    dict(lse=Q), dict(lse=K + 19999 * ROW + ROW // 2 - 4), dict(lse=OUT + 100)])
+def test_launch_refuses_overlap(fields):
+    assert "overlap" in launch_refusal(**fields)
+
+
+@pytest.mark.parametrize("fields", [
+    {}, dict(out=Q + 6 * ROW), dict(out=Q - 6 * ROW), dict(out=V + 20000 * ROW), dict(lse=OUT + 6 * ROW),
+    # columns of one buffer beside q's, k's and v's
+    dict(q=Q, k=Q + ROW, v=Q + ROW + ROW // 2, out=Q + 2 * ROW,
+         **{f"{n}_token_stride": 3 * 256 for n in ("q", "k", "v", "out")}),
+    dict(q=Q + 2 * ROW, k=Q + ROW, v=Q + ROW + ROW // 2, out=Q,
+         **{f"{n}_token_stride": 3 * 256 for n in ("q", "k", "v", "out")}),
+    # behind q inside every head, and planes of heads in turn
+    dict(out=Q + 128, q_head_stride=128, out_head_stride=128, q_token_stride=512, out_token_stride=512),
+    dict(out=Q + 6 * 128, q_token_stride=64, out_token_stride=64, q_head_stride=2 * 6 * 64, out_head_stride=2 * 6 * 64),
+    # one row: its stride says nothing
+    dict(out=Q + ROW, total_q=1)])
+def test_launch_accepts_tensors_that_lie_apart(fields):
+    assert "workspace" in launch_refusal(**fields)

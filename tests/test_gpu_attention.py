@@ -9,7 +9,7 @@ import torch
 
 from oracle.attention import reference
 from vflash_b200 import _lib
-from vflash_b200.kernels import attention
+from vflash_b200.kernels import KernelInputError, attention
 from vflash_b200.native.h3_attention import PackedAttention
 
 pytestmark = pytest.mark.gpu
@@ -446,3 +446,16 @@ def test_scores_of_minus_infinity(nq, nk, heads, kv_heads, dim, cut):
     k[..., 0] = float("-inf")
     got, lse = attention(q, k, v, offsets([nq]), offsets([nk]), return_lse=True)
     assert torch.isnan(got.float()).all() and (lse == -torch.inf).all()
+
+
+def test_an_out_over_its_operands_is_refused_and_columns_of_one_buffer_are_not():
+    rows, heads, dim = 300, 4, 64
+    merged = normal((rows + 1, 4, heads, dim), 3, BF16)
+    q, k, v, free = (merged[:rows, i] for i in range(4))
+    want = attention(q, k, v, causal=True)
+    with pytest.raises(KernelInputError, match="overlap"):
+        attention(q, k, v, causal=True, out=merged[1:, 0])
+    with pytest.raises(KernelInputError, match="overlap"):
+        attention(q, k, v, causal=True, out=merged[:rows, 2, :, :])
+    assert attention(q, k, v, causal=True, out=free) is free
+    assert torch.equal(free, want)

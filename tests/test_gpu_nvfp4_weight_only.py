@@ -15,7 +15,7 @@ import torch
 
 from oracle import nvfp4
 from vflash_b200 import _lib
-from vflash_b200.kernels import attention, nvfp4_quantize, nvfp4_weight_only
+from vflash_b200.kernels import KernelInputError, attention, nvfp4_quantize, nvfp4_weight_only
 from vflash_b200.native.h3_attention import PackedAttention
 from vflash_b200.native.h3_nvfp4_linear import NVFP4Execution, NVFP4Weight
 
@@ -233,3 +233,14 @@ def test_single_token_step():
             # one rounding of the output and one of every probability, and 2^-12 for all that is kept in fp32
             bound = 2.0**-8 * ref.abs() + (2.0**-8 + 2.0**-12) * size
             assert ((y[b, h * dim:(h + 1) * dim].double() - ref).abs() <= bound).all()
+
+
+def test_an_out_over_the_activations_is_refused():
+    weight = weight_of(128, 128, 2)
+    both = activations(9, 256, 3, BF16)
+    x, beside = both[:, :128], both[:, 128:]
+    want = nvfp4_weight_only(x, weight.packed, weight.scales, weight.alpha)
+    for out in (x, both[:, 64:192]):
+        with pytest.raises(KernelInputError, match="overlap"):
+            nvfp4_weight_only(x, weight.packed, weight.scales, weight.alpha, out=out)
+    assert torch.equal(nvfp4_weight_only(x, weight.packed, weight.scales, weight.alpha, out=beside), want)

@@ -85,3 +85,20 @@ def test_execution_checks(monkeypatch):
     monkeypatch.setattr(nv, "nvfp4_weight_only", product)
     assert engine.weight_only_linear(torch.zeros(2, 3, 64), weight).shape == (2, 3, 128)
     assert engine.calls == 1 and engine.rows == 6
+
+
+X, CODES, SF, ALPHA, BIAS, OUT = (i << 20 for i in range(1, 7))
+
+
+@pytest.mark.parametrize("changed,refused", [
+    ({}, False), ({10: X}, True), ({10: X + 2 * 64}, True), ({10: X - 2 * 128 * 3 + 2}, True), ({10: X - 2 * 128 * 3}, False),
+    ({10: X + 2 * 64 * 3}, False), ({10: CODES + 100}, True), ({10: SF + 511}, True), ({10: ALPHA - 4}, True),
+    ({10: BIAS + 254}, True), ({10: BIAS + 256}, False), ({7: None, 10: BIAS}, False),
+    ({3: 192, 11: 192, 10: X + 2 * 64}, False), ({3: 192, 11: 192, 10: X + 2 * 62}, True),  # columns of one buffer
+    ({3: 192, 11: 192, 10: X - 2 * 128}, False), ({3: 192, 11: 256, 10: X + 2 * 64}, True), ({2: 1, 10: X + 2 * 64}, False)])
+def test_c_entry_refuses_an_out_over_its_operands(changed, refused):
+    args = [X, 0, 3, 64, CODES, SF + 2, ALPHA, BIAS, 128, 64, OUT, 128, None]  # the scales' alignment is refused later
+    for index, value in changed.items():
+        args[index] = value
+    assert _lib.load().vfb_nvfp4_weight_only(*args) == _lib.VFB_EINVAL
+    assert ("overlap" if refused else "aligned") in _lib.last_error()

@@ -1202,6 +1202,23 @@ int check_args(const vfb_attention_args *a) {
   return VFB_OK;
 }
 
+// Blocks write rows while others still read theirs.
+int check_overlap(const vfb_attention_args &a) {
+  const auto extent = [&](const void *base, int64_t rows, int64_t heads, int64_t token_stride, int64_t head_stride) {
+    return Extent{base, 2ll * a.dim, {rows, heads}, {2 * token_stride, 2 * head_stride}};
+  };
+  const Extent out = extent(a.out, a.total_q, a.heads, a.out_token_stride, a.out_head_stride);
+  const Extent lse{a.lse, 4 * a.total_q * a.heads, {a.lse != nullptr, 1}, {}};
+  const Extent operands[] = {extent(a.q, a.total_q, a.heads, a.q_token_stride, a.q_head_stride),
+                             extent(a.k, a.total_k, a.kv_heads, a.k_token_stride, a.k_head_stride),
+                             extent(a.v, a.total_k, a.kv_heads, a.v_token_stride, a.v_head_stride)};
+  for (const Extent &t : operands)
+    if (may_overlap(out, t) || may_overlap(lse, t))
+      return set_error(VFB_EINVAL, "vfb_attention: out and lse may not overlap q, k or v");
+  if (may_overlap(out, lse)) return set_error(VFB_EINVAL, "vfb_attention: out and lse may not overlap");
+  return VFB_OK;
+}
+
 // [rows, heads, dim] as (dim, heads, rows), boxes of 64 x box_heads x box_rows.
 int make_map(CUtensorMap *map, const void *base, int dtype, int64_t dim, int64_t heads, int64_t rows,
              int64_t head_stride, int64_t token_stride, int box_heads, int box_rows) {
@@ -1271,6 +1288,8 @@ extern "C" int vfb_attention(const vfb_attention_args *args, void *stream) {
   if (a.total_q == 0) return VFB_OK;
   if (!a.q || !a.out || (a.total_k > 0 && (!a.k || !a.v)))
     return set_error(VFB_EINVAL, "vfb_attention: NULL pointer");
+  rc = check_overlap(a);
+  if (rc != VFB_OK) return rc;
   const Choice c = choose(a);
   const int64_t need = vfb_attention_workspace_bytes(args);
   if (a.workspace_bytes < need || (need > 0 && (!a.workspace || reinterpret_cast<uintptr_t>(a.workspace) % 256)))

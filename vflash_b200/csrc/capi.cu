@@ -123,6 +123,37 @@ int ensure_smem_optin(const void *kernel, int bytes, std::atomic<uint64_t> *done
   return VFB_OK;
 }
 
+bool may_overlap(const Extent &a, const Extent &b) {
+  const auto end = [](const Extent &t) {
+    uintptr_t at = reinterpret_cast<uintptr_t>(t.base) + t.width;
+    for (int i = 0; i < 2; ++i)
+      if (t.counts[i] > 1) at += (t.counts[i] - 1) * t.strides[i];
+    return at;
+  };
+  const uintptr_t from_a = reinterpret_cast<uintptr_t>(a.base), from_b = reinterpret_cast<uintptr_t>(b.base);
+  for (const Extent *t : {&a, &b})
+    for (int64_t n : t->counts)
+      if (n < 1) return false;
+  if (end(a) <= from_b || end(b) <= from_a) return false;
+  // Modulo a period, what is left of each is its run and the dimensions whose strides
+  // are no multiples of it.
+  const auto inside = [](const Extent &t, int64_t period) {
+    int64_t bytes = t.width;
+    for (int i = 0; i < 2; ++i)
+      if (t.counts[i] > 1 && t.strides[i] % period) bytes += (t.counts[i] - 1) * t.strides[i];
+    return bytes;
+  };
+  for (const Extent *t : {&a, &b})
+    for (int i = 0; i < 2; ++i) {
+      const int64_t period = t->strides[i];
+      if (t->counts[i] < 2) continue;
+      const int64_t apart =
+          static_cast<int64_t>(from_b >= from_a ? (from_b - from_a) % period : (period - (from_a - from_b) % period) % period);
+      if (apart >= inside(a, period) && apart + inside(b, period) <= period) return false;
+    }
+  return true;
+}
+
 // cuTensorMapEncodeTiled from the driver, looked up once through the runtime
 // (no link-time dependency on libcuda).
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {

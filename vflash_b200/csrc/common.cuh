@@ -680,4 +680,14 @@ int make_map_u8(CUtensorMap *map, const void *base, int64_t rows, int64_t cols, 
 int make_map_out(CUtensorMap *map, void *base, int64_t width, int64_t rows, int64_t planes, int64_t ld,
                  int64_t plane_stride);
 bool aligned16(const void *ptr);
+
+// A tensor's bytes: runs of `width`, `counts` of them at `strides` (0: no such dimension).
+struct Extent {
+  const void *base;
+  int64_t width;
+  int64_t counts[2], strides[2];
+};
+// False when the two are known to have no byte in common: apart, or interleaved
+// with a period that both keep (columns of one merged buffer, planes of heads).
+bool may_overlap(const Extent &a, const Extent &b);
 }  // namespace vfb

@@ -538,6 +538,16 @@ extern "C" int vfb_nvfp4_weight_only(const void *x, int32_t dtype, int64_t M, in
   if (M == 0) return VFB_OK;
   if (!x || !w_codes || !w_sf || !alpha || !out)
     return set_error(VFB_EINVAL, "vfb_nvfp4_weight_only: NULL pointer");
+  // Blocks write their part of out while others still read.
+  const Extent written{out, 2 * N, {M, 1}, {2 * ldo, 0}};
+  const Extent read[] = {{x, 2 * K, {M, 1}, {2 * ldx, 0}},
+                         {w_codes, N * K / 2, {1, 1}, {}},
+                         {w_sf, N * K / 16, {1, 1}, {}},
+                         {alpha, 4, {1, 1}, {}},
+                         {bias, 2 * N, {bias != nullptr, 1}, {}}};
+  for (const Extent &t : read)
+    if (may_overlap(written, t))
+      return set_error(VFB_EINVAL, "vfb_nvfp4_weight_only: out may not overlap x, the weight, alpha or bias");
   if (!aligned16(w_codes) || reinterpret_cast<uintptr_t>(w_sf) % 4)
     return set_error(VFB_EINVAL, "vfb_nvfp4_weight_only: codes must be 16-byte aligned, scales 4-byte aligned");
   int sms = 0;

@@ -572,6 +572,13 @@ def _on(device: torch.device):
     return _SAME_DEVICE if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
+def _refuse(rc: int, what: str) -> None:
+    """Raises for a library call that did not run: KernelInputError where it refused its arguments."""
+    if rc == _lib.VFB_EINVAL:
+        raise KernelInputError(_lib.last_error())
+    _lib.check(rc, what)
+
+
 def _check_weight_only(matrix, w_packed, w_scales, alpha, bias) -> None:
     k = matrix.shape[1]
     if (w_packed.dtype != torch.uint8 or w_packed.ndim != 2 or 2 * w_packed.shape[1] != k
@@ -603,7 +610,8 @@ def nvfp4_weight_only(matrix: torch.Tensor, w_packed: torch.Tensor, w_scales: to
     ``nvfp4_gemm`` takes them, ``alpha`` an fp32 scalar tensor, ``bias`` bf16
     ``[N]``.  K % 64 == 0, K <= 32768, N % 128 == 0.  Made for few rows (one token,
     a small batch); more rows work too, re-reading the weight for every 32.
-    ``out`` may be a strided view and may not overlap ``matrix``.  ``checked``
+    ``out`` may be a strided view and may not overlap an operand (columns of one
+    buffer beside ``matrix`` are apart).  ``checked``
     skips the checks of the weight and the bias, for a caller that made them
     (an ``NVFP4Weight`` is checked when it is made); the library still checks
     sizes and alignment.
@@ -634,7 +642,7 @@ def nvfp4_weight_only(matrix: torch.Tensor, w_packed: torch.Tensor, w_scales: to
             w_packed.data_ptr(), w_scales.data_ptr(), alpha.data_ptr(), None if bias is None else bias.data_ptr(),
             n, k, out.data_ptr(), max(out.stride(0), n), _lib.stream_handle(device))
     if rc:
-        _lib.check(rc, "vfb_nvfp4_weight_only")
+        _refuse(rc, "vfb_nvfp4_weight_only")
     return out
 
 
@@ -684,7 +692,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: t
     also the fp32 ``[heads, total_q]`` log-sum-exp of the scaled scores.  A row
     without keys is 0 (lse -inf), and so is a row behind the last sequence,
     except in a given ``out``, where those rows stay as they were.  ``out`` may be
-    strided as the inputs and may not overlap them.  Inference only; the scores
+    strided as the inputs and may not overlap them (columns or planes of one buffer
+    beside theirs are apart).  Inference only; the scores
     never leave the SM.
     """
     if q.ndim != 3 or k.ndim != 3 or v.ndim != 3:
@@ -754,5 +763,5 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: t
                 args.workspace_bytes = need
             rc = lib.vfb_attention(address, _lib.stream_handle(device))
         if rc:
-            _lib.check(rc, "vfb_attention")
+            _refuse(rc, "vfb_attention")
     return (out, lse) if return_lse else out
