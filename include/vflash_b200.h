@@ -435,7 +435,7 @@ typedef struct vfb_attention_args {
   int32_t dim;                 /* 8 <= dim <= 128, dim % 8 == 0 */
   int32_t dtype;
   const int32_t *cu_seqlens_q, *cu_seqlens_k, *lengths_k;
-  int32_t batch;               /* sequences, 1 to 2^30 - 1 (1 when cu_seqlens_q == NULL) */
+  int32_t batch;               /* sequences, 1 to 2^24 - 1 (1 when cu_seqlens_q == NULL) */
   int32_t causal;
   float scale;                 /* positive, at most 1e30 */
   int32_t fill_tail;

@@ -187,3 +187,15 @@ def test_launch_refuses_overlap(fields):
     dict(out=Q + ROW, total_q=1)])
 def test_launch_accepts_tensors_that_lie_apart(fields):
     assert "workspace" in launch_refusal(**fields)
+
+
+def test_batches_that_take_too_long_to_pass_over_are_refused():
+    lib = _lib.load()
+    a = valid_args()
+    a.cu_seqlens_q, a.batch = 256, 2**24 - 1
+    assert lib.vfb_attention_workspace_bytes(ctypes.byref(a)) >= 0
+    a.batch = 2**24
+    assert lib.vfb_attention_workspace_bytes(ctypes.byref(a)) == -1
+    assert "2^24" in _lib.last_error()
+    with pytest.raises(KernelInputError, match="2\\^24"):
+        attention(*operands(), torch.zeros(2**24 + 1, dtype=torch.int32))

@@ -58,3 +58,27 @@ def test_every_key_tile_is_visited_once(tmp_path):
     assert result.returncode == 0, result.stdout
     word, cases, cuts = result.stdout.split()
     assert word == "ok" and int(cases) == 400 and int(cuts) > 300
+
+
+def build(tmp_path, source: str) -> Path:
+    if shutil.which("g++") is None:
+        pytest.skip("g++ is not installed")
+    exe = tmp_path / source
+    subprocess.run(["g++", "-std=c++17", "-O2", "-Wall", "-Werror", f"-I{ROOT / 'vflash_b200' / 'csrc'}",
+                    str(ROOT / "tests" / f"{source}.cpp"), "-o", str(exe)], check=True)
+    return exe
+
+
+@pytest.mark.parametrize("n,blocks,groups,tokens,top", [(1, 3, 2, 64, 900), (300, 5, 3, 64, 300), (2000, 9, 2, 16, 40),
+                                                        (300000, 4, 8, 32, 2)])
+def test_blocks_go_on_where_they_last_were(tmp_path, n, blocks, groups, tokens, top):
+    """The same jobs as by a search from the first sequence, and each block passes over the sequences once."""
+    rng = random.Random(n)
+    lengths = [rng.randint(0, top) for _ in range(n)]
+    result = subprocess.run([str(build(tmp_path, "attention_cursor_check"))], capture_output=True, text=True, timeout=60,
+                            input=" ".join(map(str, [n, blocks, groups, tokens, *lengths])))
+    assert result.returncode == 0, result.stdout
+    word, jobs, passed = result.stdout.split()
+    assert word == "ok" and int(jobs) >= sum(x > 0 for x in lengths) * groups
+    if n > 3000:
+        assert int(passed) <= blocks * (n + 1)

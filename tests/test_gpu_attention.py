@@ -459,3 +459,31 @@ def test_an_out_over_its_operands_is_refused_and_columns_of_one_buffer_are_not()
         attention(q, k, v, causal=True, out=merged[:rows, 2, :, :])
     assert attention(q, k, v, causal=True, out=free) is free
     assert torch.equal(free, want)
+
+
+def test_a_hundred_thousand_prompts_of_one_token():
+    """One key each: every row is its own value, exactly."""
+    n = 100_000
+    q, k, v = operands([n], [n], 4, 2, 64, BF16)
+    cu = torch.arange(n + 1, dtype=torch.int32, device=DEV)
+    got, lse = attention(q, k, v, cu, causal=True, return_lse=True)
+    assert torch.equal(got, v.repeat_interleave(2, dim=1))
+    products = q.double() * k.double().repeat_interleave(2, dim=1) * 64**-0.5
+    want, size = products.sum(dim=2).T, products.abs().sum(dim=2).T
+    # 64 products summed and scaled in fp32, and four roundings (twice ln 2, its inverse, the logarithm of 1) of the result
+    assert ((lse.double() - want).abs() <= (68 * size + 4 * want.abs()) * 2.0**-24 + 1e-7).all()
+    assert _lib.device_status(clear=True) == _lib.VFB_OK
+
+
+@pytest.mark.parametrize("keys", [0, 20000])
+def test_rows_at_both_ends_of_the_largest_batch(keys):
+    """2^24 - 1 sequences, all but the first and the last empty: passed over 32 at a time, and one by one by a share."""
+    batch = 2**24 - 1
+    nq, nk = [3, 2], [3 + keys, 2 + keys]
+    q, k, v = operands(nq, nk, 4, 2, 64, BF16)
+    cu_q = torch.full((batch + 1,), nq[0], dtype=torch.int32, device=DEV)
+    cu_k = torch.full((batch + 1,), nk[0], dtype=torch.int32, device=DEV)
+    cu_q[0] = cu_k[0] = 0
+    cu_q[-1], cu_k[-1] = sum(nq), sum(nk)
+    got, lse = attention(q, k, v, cu_q, cu_k, causal=True, return_lse=True)
+    check(got, lse, q, k, v, nq, nk, True)

@@ -965,9 +965,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
       } else {
         uint32_t taken_phase = 0;
+        attn::Cursor at{0, 0};
         int64_t next = blockIdx.x;
         while (next >= 0) {
-          if (attn::whole_job(p.plan, static_cast<uint32_t>(next), seg)) {
+          if (attn::whole_job(p.plan, static_cast<uint32_t>(next), seg, at)) {
             if (lane == 0) hand_out(true);
             __syncwarp();
             step();
@@ -1124,6 +1125,10 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attention_join_kernel(const _
 // ---- host side -------------------------------------------------------------------------
 constexpr int kMaxBlocks = 148;  // SMs of a B200: blocks that even shares are cut for
 
+// Sequences of a call, below: a block passes over all of them (32 at a time, one
+// by one where a share goes on behind empty ones) while its other warps wait.
+constexpr int kMaxBatch = 1 << 24;
+
 constexpr int kBandBytes = 48 << 20;  // of K and V that stay in L2 (126 MB) beside the rows read and written
 
 struct Choice {
@@ -1185,8 +1190,8 @@ int check_args(const vfb_attention_args *a) {
   if (a->dim < 8 || a->dim > 128 || a->dim % 8)
     return set_error(VFB_EINVAL, "vfb_attention: dim must be a multiple of 8 from 8 to 128");
   if (a->dtype != 0 && a->dtype != 1) return set_error(VFB_EINVAL, "vfb_attention: dtype must be 0 (bf16) or 1 (fp16)");
-  if (a->batch < 1 || a->batch >= (1 << 30) || (a->cu_seqlens_q == nullptr && (a->batch != 1 || a->cu_seqlens_k != nullptr)))
-    return set_error(VFB_EINVAL, "vfb_attention: batch must be >= 1, below 2^30, and 1 without cu_seqlens_q");
+  if (a->batch < 1 || a->batch >= kMaxBatch || (a->cu_seqlens_q == nullptr && (a->batch != 1 || a->cu_seqlens_k != nullptr)))
+    return set_error(VFB_EINVAL, "vfb_attention: batch must be >= 1, below 2^24, and 1 without cu_seqlens_q");
   if (a->cu_seqlens_q != nullptr && a->cu_seqlens_k == nullptr && a->total_k != a->total_q)
     return set_error(VFB_EINVAL, "vfb_attention: keys of another length need cu_seqlens_k");
   if (!(a->scale > 0.0f) || a->scale > 1.0e30f)  // times log2(e) it stays finite

@@ -170,27 +170,43 @@ __device__ __forceinline__ uint32_t warp_upto(uint32_t own) {  // inclusive sum 
 }
 #endif
 
+// Where a block's way through the list of whole jobs stands: the sequences from
+// `b` on hold the jobs from `before` on.  The jobs that a block takes come later and later
+// in the list, as a rule, so it passes over the sequences once.  (From the first
+// sequence for every job: 4096 prompts of 64 tokens, 4 heads of 64, 3.0 ms instead of
+// 0.26, 131072 of one token 1.4 s instead of 6.9 ms.)
+struct Cursor {
+  int32_t b;
+  uint32_t before;
+};
+
 // Whole jobs: the sequence in which job `x` of the list lies, -1 behind the end;
 // `x` becomes its place inside the sequence.
-VFB_HD int32_t locate_job(const Plan &p, uint32_t &x) {
+VFB_HD int32_t locate_job(const Plan &p, uint32_t &x, Cursor &at) {
+  if (x < at.before) at = Cursor{0, 0};
+  x -= at.before;
 #ifdef __CUDA_ARCH__
   const int lane = threadIdx.x & 31;
-  for (int32_t b0 = 0; b0 < num_seqs(p); b0 += 32) {
-    const uint32_t own = b0 + lane < num_seqs(p) ? static_cast<uint32_t>(sequence(p, b0 + lane).tiles) * p.groups : 0u;
+  for (; at.b < num_seqs(p); at.b += 32) {
+    const int32_t b = at.b + lane;
+    const uint32_t own = b < num_seqs(p) ? static_cast<uint32_t>(sequence(p, b).tiles) * p.groups : 0u;
     const uint32_t upto = warp_upto(own);
     const unsigned hit = __ballot_sync(0xffffffffu, x < upto);
     if (hit) {
-      const int at = __ffs(hit) - 1;
-      x -= __shfl_sync(0xffffffffu, upto - own, at);
-      return b0 + at;
+      const int first = __ffs(hit) - 1;
+      x -= __shfl_sync(0xffffffffu, upto - own, first);
+      return at.b + first;
     }
-    x -= __shfl_sync(0xffffffffu, upto, 31);
+    const uint32_t all = __shfl_sync(0xffffffffu, upto, 31);
+    x -= all;
+    at.before += all;
   }
 #else
-  for (int32_t b = 0; b < num_seqs(p); ++b) {
-    const uint32_t own = static_cast<uint32_t>(sequence(p, b).tiles) * p.groups;
-    if (x < own) return b;
+  for (; at.b < num_seqs(p); ++at.b) {
+    const uint32_t own = static_cast<uint32_t>(sequence(p, at.b).tiles) * p.groups;
+    if (x < own) return at.b;
     x -= own;
+    at.before += own;
   }
 #endif
   return -1;
@@ -205,8 +221,8 @@ struct Segment {
 };
 
 // Whole jobs: job `x` of the list; false behind its end.
-VFB_HD bool whole_job(const Plan &p, uint32_t x, Segment &s) {
-  s.b = locate_job(p, x);
+VFB_HD bool whole_job(const Plan &p, uint32_t x, Segment &s, Cursor &at) {
+  s.b = locate_job(p, x, at);
   if (s.b < 0) return false;
   s.seq = sequence(p, s.b);
   const uint32_t tiles = s.seq.tiles;
@@ -225,6 +241,11 @@ VFB_HD bool whole_job(const Plan &p, uint32_t x, Segment &s) {
   s.t1 = tiles_of(p, s.seq, s.tile);
   s.slot = -1;
   return true;
+}
+
+VFB_HD bool whole_job(const Plan &p, uint32_t x, Segment &s) {
+  Cursor at{0, 0};
+  return whole_job(p, x, s, at);
 }
 
 // Even shares: a job, and the key tile of it where a share begins or ends.

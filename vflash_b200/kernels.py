@@ -722,8 +722,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: t
     if cu_seqlens_q is not None:
         _check_offsets(cu_seqlens_q, None, device, "cu_seqlens_q")
         batch = cu_seqlens_q.shape[0] - 1
-        if batch < 1:
-            raise KernelInputError("attention cu_seqlens_q needs at least two entries")
+        if not 1 <= batch < 2**24:
+            raise KernelInputError("attention cu_seqlens_q needs at least two entries, and fewer than 2^24 sequences")
         at_q = cu_seqlens_q.data_ptr()
         if cu_seqlens_k is not None:
             _check_offsets(cu_seqlens_k, batch + 1, device, "cu_seqlens_k")
