@@ -487,3 +487,18 @@ def test_rows_at_both_ends_of_the_largest_batch(keys):
     cu_q[-1], cu_k[-1] = sum(nq), sum(nk)
     got, lse = attention(q, k, v, cu_q, cu_k, causal=True, return_lse=True)
     check(got, lse, q, k, v, nq, nk, True)
+
+
+def test_a_job_longer_than_the_limit_of_a_wait():
+    """600 million keys in every job: the warps that wait for a job's end wait longer than for a tile."""
+    nq, nk = 146 * 256, 600_000_000
+    k = torch.zeros(nk, 1, 8, dtype=BF16, device=DEV)
+    k[nk // 2, 0, 0] = 40  # all the weight: the others have e^-40 each
+    q = torch.zeros(nq, 1, 8, dtype=BF16, device=DEV)
+    q[..., 0] = 1
+    cu_q = offsets([nq])
+    assert workspace_bytes(q, k, 1, False) == 0
+    out = torch.zeros_like(q)
+    attention(q, k, k, cu_q, offsets([nk]), scale=1.0, out=out)
+    assert _lib.device_status(clear=True) == _lib.VFB_OK
+    assert torch.equal(out, 40 * q)

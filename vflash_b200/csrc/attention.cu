@@ -77,6 +77,10 @@ constexpr int kThreads = 384;
 constexpr int kRingSlots = 16;       // at most
 constexpr int kJobs = 2;             // jobs that the scheduler may be ahead
 constexpr int kJobReaders = 11;      // warps that follow the schedule
+// Waits for a whole job of other warps (for the next one, for room in the schedule,
+// for a job's last tiles): a job of 2^31 keys takes about 30 s.  The waits inside a job
+// have the usual limit, and whichever runs out first ends all of them.
+constexpr uint64_t kJobTimeoutNs = 120000000000ull;
 constexpr float kHold = 8.0f;
 // P carries a factor of 2^kLift, which cancels in O / l and comes off the
 // log-sum-exp.  fp16 ends at 2^-24, and many keys that each round to 0 there may hold
@@ -372,7 +376,7 @@ struct JobReader {
 
   // `next` for a role of one thread.
   __device__ __forceinline__ bool next_alone(Job &j) {
-    mbar_wait_through(&sh.job_full[slot], phase, &sh.abort, status);
+    mbar_wait_through(&sh.job_full[slot], phase, &sh.abort, status, kJobTimeoutNs);
     if (*const_cast<volatile int *>(&sh.abort)) return false;
     j = sh.jobs[slot];
     mbar_arrive(&sh.job_empty[slot]);
@@ -386,7 +390,7 @@ struct JobReader {
   // The next job in place, for a warp that reads its fields when it needs them (the
   // softmax warps have no register to spare) and gives it back with done().
   __device__ __forceinline__ bool peek() {
-    return warp_wait_quick(&sh.job_full[slot], phase, &sh.abort, status) && here().count >= 0;
+    return warp_wait_quick(&sh.job_full[slot], phase, &sh.abort, status, kJobTimeoutNs) && here().count >= 0;
   }
   __device__ __forceinline__ const Job &here() const { return sh.jobs[slot]; }
   __device__ __forceinline__ void done() {
@@ -400,7 +404,7 @@ struct JobReader {
 
   // The next job; false when there is none (or a wait ran out).
   __device__ __forceinline__ bool next(Job &j) {
-    if (!warp_wait_quick(&sh.job_full[slot], phase, &sh.abort, status)) return false;
+    if (!warp_wait_quick(&sh.job_full[slot], phase, &sh.abort, status, kJobTimeoutNs)) return false;
     j = sh.jobs[slot];
     __syncwarp();
     if ((threadIdx.x & 31) == 0) mbar_arrive(&sh.job_empty[slot]);
@@ -940,7 +944,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const auto hand_out = [&](bool more) {  // by lane 0
         if (more) describe<PAIR>(p, seg, job);
         else job.count = -1;
-        mbar_wait_through(&sh.job_empty[slot], phase, &sh.abort, p.status);
+        mbar_wait_through(&sh.job_empty[slot], phase, &sh.abort, p.status, kJobTimeoutNs);
         sh.jobs[slot] = job;
         mbar_arrive(&sh.job_full[slot]);
       };
@@ -973,7 +977,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             step();
             // no job is taken before there is room for it
-            if (!warp_wait_quick(&sh.job_empty[slot], phase, &sh.abort, p.status)) break;
+            if (!warp_wait_quick(&sh.job_empty[slot], phase, &sh.abort, p.status, kJobTimeoutNs)) break;
           }
           next = take_block(sh, taken_phase, p.status);
           taken_phase ^= 1;
@@ -986,7 +990,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t todo_phase = 0;  // a bit for every slot
       const auto clean = [&](int32_t t) {
         const int slot = pos.slot;
-        if (!warp_wait_quick(&sh.v_todo[slot], todo_phase >> slot & 1, &sh.abort, p.status)) return false;
+        if (!warp_wait_quick(&sh.v_todo[slot], todo_phase >> slot & 1, &sh.abort, p.status, kJobTimeoutNs)) return false;
         todo_phase ^= 1u << slot;
         if (!warp_wait_quick(&sh.kv_full[slot], pos.phase, &sh.abort, p.status)) return false;
         uint8_t *tile = s_kv + slot * L::kv_tile;

@@ -1,7 +1,7 @@
 // Device-side building blocks shared by the sm_100a kernels: mbarriers with
 // bounded waits, TMA tile loads, tcgen05 (TMEM allocation, MMA issue, commit,
 // TMEM loads) and strict BF16 rounding helpers.  Every wait in this file gives
-// up after VFB_WAIT_TIMEOUT_NS of wall time, records VFB_ETIMEOUT in the
+// up after VFB_WAIT_TIMEOUT_NS of wall time (or a limit it is given), records VFB_ETIMEOUT in the
 // device status word and returns false, so a broken pipeline ends the kernel
 // instead of hanging the GPU.
 #pragma once
@@ -471,13 +471,13 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volati
 // another warp-wide instruction while the others still wait; the vote also brings the lanes
 // together when only one of them has just issued a copy or an arrival.
 __device__ __forceinline__ bool warp_wait_quick(uint64_t *bar, uint32_t parity, volatile int *abort_flag,
-                                                int *status) {
+                                                int *status, uint64_t timeout_ns = VFB_WAIT_TIMEOUT_NS) {
   if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
   const uint64_t start = global_timer_ns();
   for (;;) {
     for (int spin = 0; spin < 256; ++spin)
       if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-    const bool expired = global_timer_ns() - start > VFB_WAIT_TIMEOUT_NS;
+    const bool expired = global_timer_ns() - start > timeout_ns;
     if (__any_sync(0xffffffffu, expired || *abort_flag)) {
       if (expired) {
         *abort_flag = 1;
@@ -494,12 +494,12 @@ __device__ __forceinline__ bool warp_wait_quick(uint64_t *bar, uint32_t parity, 
 // that does not depend on the wait stays warp-uniform for the compiler, which
 // then keeps the products' operands in uniform registers.
 __device__ __forceinline__ void mbar_wait_through(uint64_t *bar, uint32_t parity, volatile int *abort_flag,
-                                                  int *status) {
+                                                  int *status, uint64_t timeout_ns = VFB_WAIT_TIMEOUT_NS) {
   if (mbar_try_wait(bar, parity)) return;
   const uint64_t start = global_timer_ns();
   while (!mbar_try_wait(bar, parity)) {
     if (*abort_flag) return;
-    if (global_timer_ns() - start > VFB_WAIT_TIMEOUT_NS) {
+    if (global_timer_ns() - start > timeout_ns) {
       *abort_flag = 1;
       record_status(status, VFB_ETIMEOUT);
       return;
