@@ -502,3 +502,35 @@ def test_a_job_longer_than_the_limit_of_a_wait():
     attention(q, k, k, cu_q, offsets([nk]), scale=1.0, out=out)
     assert _lib.device_status(clear=True) == _lib.VFB_OK
     assert torch.equal(out, 40 * q)
+
+
+@pytest.mark.parametrize("rows,keys,heads,cut", [(200, 200, 2, False), (700, 700, 24, False), (3, 9000, 4, True), (300, 4001, 4, True)])
+@pytest.mark.parametrize("fill_tail", [0, 1])
+def test_bad_offsets_write_nothing_beside_the_outputs(rows, keys, heads, cut, fill_tail):
+    """Offsets and lengths that decrease, repeat or leave the buffers: what lies around out, lse and the workspace stays."""
+    dim, guard = 64, 300
+    q, k, v = operands([rows], [keys], heads, heads, dim, BF16)
+    lists = [[0, 500_000], [0, -7, rows], [0, rows - 1, 1, rows], [5, 5, 5], [2**31 - 1, -(2**31), 2**31 - 1, 0], [rows, 0],
+             [-1, rows + 1, rows, 0, rows]]
+    for at in lists:
+        for keys_at in (at, [x * keys // rows if abs(x) < 2**20 else x for x in at], [0] * len(at), [keys] * len(at)):
+            for lengths in (None, [2**31 - 1] * (len(at) - 1), [-5] * (len(at) - 1), [1] * (len(at) - 1)):
+                out = torch.full((rows + 2 * guard, heads, dim), 7.0, dtype=BF16, device=DEV)
+                lse = torch.full((heads * rows + 2 * guard,), 7.0, device=DEV)
+                cu_q, cu_k = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in (at, keys_at))
+                used = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=DEV)
+                args = _lib.attention_args(
+                    q.data_ptr(), k.data_ptr(), v.data_ptr(), out[guard:].data_ptr(), lse[guard:].data_ptr(),
+                    *(heads * dim, dim) * 4, rows, keys, heads, heads, dim, 0, cu_q.data_ptr(), cu_k.data_ptr(),
+                    0 if used is None else used.data_ptr(), len(at) - 1, 1, 0.125, fill_tail, 0, 0)
+                need = _lib.load().vfb_attention_workspace_bytes(ctypes.byref(args))
+                if len(at) == 2 and lengths is None:
+                    assert (need > 0) == cut
+                workspace = torch.full((need + 512,), 99, dtype=torch.uint8, device=DEV)
+                if need:
+                    args.workspace, args.workspace_bytes = workspace[256:].data_ptr(), need
+                _lib.check(_lib.load().vfb_attention(ctypes.byref(args), _lib.stream_handle(q.device)), "vfb_attention")
+                assert (out[:guard] == 7).all() and (out[guard + rows:] == 7).all()
+                assert (lse[:guard] == 7).all() and (lse[guard + heads * rows:] == 7).all()
+                assert (workspace[:256] == 99).all() and (workspace[256 + need:] == 99).all()
+                assert _lib.device_status(clear=True) == _lib.VFB_OK
