@@ -390,9 +390,10 @@ VFB_API int vfb_nvfp4_gemm_quant(const void *A, const void *sfa, const void *W, 
  * (refused unless apart or interleaved with one period).  Requires K % 64 == 0, K <= 32768,
  * N % 128 == 0, N <= 1048576, M <= 524288, 16-byte aligned w_codes, 4-byte
  * aligned w_sf.
- * bf16 rows are brought to fp16 by a power of two of their own (exact for
- * elements within 2^-30 of the row's largest magnitude).  No reference
- * counterpart: the reference always quantises the activations. */
+ * bf16 rows are brought to fp16 by a power of two of their own, or kept in bf16
+ * where that would lose bits: products are exact down to 2^-160 of the row's
+ * largest magnitude.  No reference counterpart: the reference always quantises the
+ * activations. */
 VFB_API int vfb_nvfp4_weight_only(const void *x, int32_t dtype, int64_t M, int64_t ldx,
                                   const void *w_codes, const void *w_sf, const float *alpha,
                                   const void *bias, int64_t N, int64_t K, void *out, int64_t ldo,

@@ -244,3 +244,61 @@ def test_an_out_over_the_activations_is_refused():
         with pytest.raises(KernelInputError, match="overlap"):
             nvfp4_weight_only(x, weight.packed, weight.scales, weight.alpha, out=out)
     assert torch.equal(nvfp4_weight_only(x, weight.packed, weight.scales, weight.alpha, out=beside), want)
+
+
+def without_column(weight, column):
+    """The weight with zeros in one input column."""
+    weight.packed[:, column // 2] &= 0xF0 if column % 2 == 0 else 0x0F
+    return weight
+
+
+def check_without_loss(got, x, weight):
+    """``check`` without its term for what fp16 loses of small activations."""
+    w, xd, alpha = decoded(weight), x.double(), weight.alpha.double()
+    want, size = alpha * (xd @ w.T), alpha * (xd.abs() @ w.abs().T)
+    bound = 2.0**-8 * want.abs() + (x.shape[1] / 16 + 68) * 2.0**-24 * size + 1e-38
+    error = (got.double() - want).abs()
+    assert (error <= bound).all(), f"{(error / bound).max().item():.2f} times the bound"
+    assert _lib.device_status(clear=True) == _lib.VFB_OK
+
+
+@pytest.mark.parametrize("rows", [1, 3, 8, 9, 20, 33])
+@pytest.mark.parametrize("n,k,column,shift", [(128, 64, 5, 0), (256, 192, 190, 0), (384, 1024, 700, 0), (384, 1024, 1, 3),
+                                              (4096, 4096, 4095, 0), (128, 16384, 9000, 0), (256, 32768, 0, 0),
+                                              (16384, 512, 77, 0)])
+def test_an_outlier_on_a_weight_of_zero_takes_nothing_from_the_others(rows, n, k, column, shift):
+    """Only some blocks of a K that is dealt out hold the outlier; the bits are those without it."""
+    weight = without_column(weight_of(n, k, 5), column)
+    x = torch.zeros(rows, k + 8, dtype=BF16, device=DEV)[:, shift:shift + k]  # rows off 16 bytes where shifted
+    x.copy_(activations(rows, k, 6, BF16))
+    x[:, column] = 0
+    want = nvfp4_weight_only(x, weight.packed, weight.scales, weight.alpha)
+    check_without_loss(want, x, weight)
+    for big in (1e30, -3e38, 1e9):
+        x[rows // 2, column] = big
+        got = nvfp4_weight_only(x, weight.packed, weight.scales, weight.alpha)
+        check_without_loss(got, x, weight)
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("rows", [2, 12, 32])
+@pytest.mark.parametrize("below", [16, 28, 29, 30, 31, 32, 33, 40, 80, 120, 150])
+def test_activations_far_below_their_row_s_largest(rows, below):
+    weight = without_column(weight_of(256, 384, 5), 100)
+    x = activations(rows, 384, 6, BF16)
+    x = torch.where(x == 0, 1, x) * 2.0**(40 - below)
+    x[:, 100] = 2.0**45
+    x[0, 7] = 0
+    check_without_loss(nvfp4_weight_only(x, weight.packed, weight.scales, weight.alpha), x, weight)
+
+
+def test_subnormal_and_largest_activations():
+    weight = without_column(weight_of(128, 256, 5), 3)
+    x = activations(4, 256, 6, BF16)
+    x[0] = (x[0].float() * 2.0**-128).to(BF16)  # subnormal ones alone
+    x[1] = (x[1].float() * 2.0**-100).to(BF16)  # far below the largest, normal
+    x[1:3, 3] = 1e6
+    x[2, 9] = 2.0**-60
+    x[3] = (x[3].float().clamp(-4, 4) * 2.0**100).to(BF16)
+    got = nvfp4_weight_only(x, weight.packed, weight.scales, weight.alpha)
+    check_without_loss(got, x, weight)

@@ -12,9 +12,11 @@
 //   * a decoded weight e2m1 * e4m3 has at most six significant bits and lies in
 //     2^-10 .. 2688, so it is exact in fp16: cvt.f16x2.e2m1x2 and one HMUL2.
 //     x is brought to fp16 too, each row multiplied by a power of two that puts
-//     its largest magnitude (of the block's K range) into [2^14, 2^15): exact
-//     for elements down to 2^-30 of it, 2^-39 of it absolute below.  Products
-//     are exact, sums fp32.
+//     its largest magnitude (of the block's K range) into [2^14, 2^15), which is
+//     exact for elements down to 2^-31 of it.  Where a row of the block has others
+//     than 0 below, the block takes bf16 for both operands: a decoded weight is exact there
+//     too, but takes three more instructions for a pair (1.5 times as many in the
+//     loop).  Products are exact either way, sums fp32, and both give the same bits.
 //   * the order of k inside a product is free as long as both operands agree.
 //     A lane takes 32 consecutive weights of a row (one 16-byte load), a quad 128
 //     of them (a "step": 64 bytes of every row), and x is laid out in shared
@@ -98,12 +100,41 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
   return r;
 }
 
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// ---- decoded weights in bf16, times 2^-kWideShift: 2^-22 .. 0.66 ------------------
+// An e2m1 number as fp16 has its sign, five bits of exponent and one of mantissa; the
+// same bits three places further down are its bf16 form times 2^-112 (15 and 127 are the
+// exponents' biases).
+constexpr int kWideShift = 12;
+__device__ __forceinline__ uint32_t low_bf16x2(uint32_t h) { return (h >> 3 & 0x0FFF0FFFu) | (h & 0x80008000u); }
+
+// The two scales of an e4m3 pair as f16x2, each twice as bf16 and times 2^(112 - kWideShift).
+__device__ __forceinline__ void wide_scales(uint32_t h, uint32_t (&s)[2]) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
+  const float up = __int_as_float((112 - kWideShift + 127) << 23);
+  const __nv_bfloat162 a = __float2bfloat162_rn(f.x * up), b = __float2bfloat162_rn(f.y * up);
+  s[0] = *reinterpret_cast<const uint32_t *>(&a);
+  s[1] = *reinterpret_cast<const uint32_t *>(&b);
+}
+
+template <bool BF16>
 __device__ __forceinline__ void mma_m16n8k16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                              uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  if (BF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 // Eight elements of a row of x that lie anywhere.
@@ -129,6 +160,16 @@ __device__ __forceinline__ uint32_t largest_x8(const uint4 &v) {
   return max(lo > 0x7F800000u ? 0u : lo, hi > 0x7F800000u ? 0u : hi);
 }
 
+// Smallest magnitude other than 0 of eight bf16 numbers and of those behind `low`,
+// whose halves are magnitudes' bits less 1: 0 becomes 2^16 - 1 there, the largest.
+constexpr uint32_t kNoneLow = 0xFFFFFFFFu;
+__device__ __forceinline__ uint32_t smallest_x8(const uint4 &v, uint32_t low) {
+  const auto with = [&](uint32_t w) { low = __viaddmin_u16x2(w & 0x7FFF7FFFu, 0xFFFFFFFFu, low); };
+  with(v.x), with(v.y), with(v.z), with(v.w);
+  return low;
+}
+__device__ __forceinline__ uint32_t lower_half(uint32_t low) { return min(low & 0xFFFFu, low >> 16); }
+
 // 2^e for -126 <= e <= 127.
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
 
@@ -138,6 +179,22 @@ __device__ __forceinline__ int row_shift(uint32_t max_bits) {
   const int e = static_cast<int>(max_bits >> 23);  // biased; 0 for subnormals and zero
   if (max_bits == 0) return 0;
   return min(14 - (min(e, 254) - 127), 126);
+}
+
+// True when a row so multiplied has numbers of which fp16 loses bits: below 2^-17, its
+// last place being 2^-24 and bf16's significand eight bits long.
+__device__ __forceinline__ bool loses_bits(uint32_t max_bits, uint32_t low) {
+  const int smallest = max(static_cast<int>(low + 1) >> 7, 1);  // its exponent, biased; subnormals share that of the smallest normal one
+  return low != 0xFFFFu && smallest - 127 + row_shift(max_bits) < -17;
+}
+
+// The power of two of a row whose block takes bf16: it puts the largest magnitude at
+// 2^60, so that sums of 2^15 products stay far from overflow and products with the
+// smallest weight keep all their bits down to 2^-160 of the largest.
+__device__ __forceinline__ int wide_row_shift(uint32_t max_bits) {
+  const int e = static_cast<int>(max_bits >> 23);
+  if (max_bits == 0) return 0;
+  return min(60 - (min(e, 254) - 127), 126);
 }
 
 template <int NT, int RU, int WR, int WARPS>
@@ -163,6 +220,7 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 1)
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t *xs = smem + S::ring_bytes;
   __shared__ uint32_t row_max[S::tokens];
+  __shared__ uint32_t row_low[S::tokens];  // of each row's smallest magnitude other than 0, see smallest_x8
   __shared__ float bias[S::rows];
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
   const int split = gridDim.x;  // cluster: blocks along K
@@ -233,15 +291,19 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 1)
   };
   const auto from = [&](int i) { return x + row_of(i) * p.ldx + k_begin + 8 * chunk_of(i); };
   const auto inside = [&](int i) { return 8 * chunk_of(i) < k_left; };  // K is a multiple of eight
-  uint32_t best[2] = {0, 0};  // of a warp's own rows
+  uint32_t best[2] = {0, 0}, low[2] = {kNoneLow, kNoneLow};  // of a warp's own rows
   const auto note = [&](int i, const uint4 &v) {
     const uint32_t largest = largest_x8(v);
     if (kOwnRows) {
-      if (nth_row(i) == 0) best[0] = max(best[0], largest);
-      else best[1] = max(best[1], largest);
+      if (nth_row(i) == 0) best[0] = max(best[0], largest), low[0] = smallest_x8(v, low[0]);
+      else best[1] = max(best[1], largest), low[1] = smallest_x8(v, low[1]);
     } else {  // 16 lanes with one row's chunks
       const uint32_t top = __reduce_max_sync(0xFFFFu << (lane & 16), largest);
-      if (lane % 16 == 0 && top) atomicMax(&row_max[row_of(i)], top);
+      const uint32_t least = __reduce_min_sync(0xFFFFu << (lane & 16), lower_half(smallest_x8(v, kNoneLow)));
+      if (lane % 16 == 0 && top) {
+        atomicMax(&row_max[row_of(i)], top);
+        atomicMin(&row_low[row_of(i)], least);
+      }
     }
   };
   constexpr int kFlight = NT == 1 ? 8 : 12;  // chunks of a thread in flight
@@ -262,7 +324,7 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 1)
   const float alpha = __ldg(p.alpha);
   for (int r = tid; r < S::rows; r += kThreads) bias[r] = p.bias != nullptr ? __bfloat162float(p.bias[feature(r)]) : 0.0f;
   if (kScaled && !kOwnRows) {
-    if (tid < S::tokens) row_max[tid] = 0;
+    if (tid < S::tokens) row_max[tid] = 0, row_low[tid] = 0xFFFF;
     __syncthreads();
   }
   int base = 0;  // of the last flight, which stays in registers until the rows' maxima are known
@@ -305,7 +367,8 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 1)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, best[r]);
-        if (lane == 0 && warp + r * WARPS < S::tokens) row_max[warp + r * WARPS] = top;
+        const uint32_t least = __reduce_min_sync(0xFFFFFFFFu, lower_half(low[r]));
+        if (lane == 0 && warp + r * WARPS < S::tokens) row_max[warp + r * WARPS] = top, row_low[warp + r * WARPS] = least;
       }
       __syncwarp();
     } else {
@@ -323,56 +386,84 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 1)
   }
   __syncthreads();
 
+  // ---- rows whose numbers lie too far apart for fp16: all of x again, in bf16 ----
+  const bool wide =
+      kScaled && __any_sync(0xFFFFFFFFu, lane < tokens && loses_bits(row_max[min(lane, tokens - 1)], row_low[min(lane, tokens - 1)]));
+  if (wide) {
+#pragma unroll 1
+    for (int i = first; i < items; i += kStride) {
+      uint4 c = make_uint4(0, 0, 0, 0);
+      if (inside(i)) c = p.vector_x ? __ldg(reinterpret_cast<const uint4 *>(from(i))) : gather_x8(from(i));
+      const float factor = power_of_two(wide_row_shift(row_max[row_of(i)]));
+      uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        w[e] = pack_bf16x2(__uint_as_float(w[e] << 16) * factor, __uint_as_float(w[e] & 0xFFFF0000u) * factor);
+      *place(i) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __syncthreads();
+  }
+
   // ---- products ----
   float acc[RU][NT][4] = {};
   const uint8_t *own_ring = smem + warp * S::depth * S::stage;
+  const auto products = [&](auto as_bf16) {
+    constexpr bool kWide = decltype(as_bf16)::value;
 #pragma unroll 1
-  for (int i = 0; i < own_steps; ++i) {
-    copies_wait<S::depth - 1>();
-    __syncwarp();
-    const uint8_t *stage = own_ring + i % S::depth * S::stage;
-    const uint8_t *x_step = xs + g * row_bytes + (k_warp + i * S::k_warps) * 256 + t * 16;
-    uint4 w[RU][2];
-    uint32_t scale[RU][2][2];  // unit, row, group: the scale in both halves
+    for (int i = 0; i < own_steps; ++i) {
+      copies_wait<S::depth - 1>();
+      __syncwarp();
+      const uint8_t *stage = own_ring + i % S::depth * S::stage;
+      const uint8_t *x_step = xs + g * row_bytes + (k_warp + i * S::k_warps) * 256 + t * 16;
+      uint4 w[RU][2];
+      uint32_t scale[RU][2][2];  // unit, row, group: the scale in both halves
 #pragma unroll
-    for (int u = 0; u < RU; ++u)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        w[u][r] = *reinterpret_cast<const uint4 *>(stage + u * kUnitStage + r * 512 + lane * 16);
-        // lane's groups 2t and 2t + 1 of row g + 8r, which is row (g / 4 + 2r) of quarter g % 4
-        const uint16_t s = *reinterpret_cast<const uint16_t *>(stage + u * kUnitStage + kUnitBytes + t / 2 * 64 +
-                                                               (g / 4 + 2 * r) * 16 + g % 4 * 4 + t % 2 * 2);
-        const uint32_t h = decode_e4m3x2(s);
-        scale[u][r][0] = __byte_perm(h, 0, 0x1010);
-        scale[u][r][1] = __byte_perm(h, 0, 0x3232);
-      }
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      uint4 f[NT];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        f[n] = make_uint4(0, 0, 0, 0);
-        if (8 * n + g < tokens) f[n] = *reinterpret_cast<const uint4 *>(x_step + 8 * n * row_bytes + q * 64);
-      }
-#pragma unroll
-      for (int u = 0; u < RU; ++u) {
-        uint32_t a[2][4];
+      for (int u = 0; u < RU; ++u)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          decode_e2m1x8(reinterpret_cast<const uint32_t *>(&w[u][r])[q], a[r]);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) a[r][j] = mul_f16x2(a[r][j], scale[u][r][q / 2]);
+          w[u][r] = *reinterpret_cast<const uint4 *>(stage + u * kUnitStage + r * 512 + lane * 16);
+          // lane's groups 2t and 2t + 1 of row g + 8r, which is row (g / 4 + 2r) of quarter g % 4
+          const uint16_t s = *reinterpret_cast<const uint16_t *>(stage + u * kUnitStage + kUnitBytes + t / 2 * 64 +
+                                                                 (g / 4 + 2 * r) * 16 + g % 4 * 4 + t % 2 * 2);
+          const uint32_t h = decode_e4m3x2(s);
+          if (kWide) {
+            wide_scales(h, scale[u][r]);
+          } else {
+            scale[u][r][0] = __byte_perm(h, 0, 0x1010);
+            scale[u][r][1] = __byte_perm(h, 0, 0x3232);
+          }
         }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        uint4 f[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-          mma_m16n8k16(acc[u][n], a[0][0], a[1][0], a[0][1], a[1][1], f[n].x, f[n].y);
-          mma_m16n8k16(acc[u][n], a[0][2], a[1][2], a[0][3], a[1][3], f[n].z, f[n].w);
+          f[n] = make_uint4(0, 0, 0, 0);
+          if (8 * n + g < tokens) f[n] = *reinterpret_cast<const uint4 *>(x_step + 8 * n * row_bytes + q * 64);
+        }
+#pragma unroll
+        for (int u = 0; u < RU; ++u) {
+          uint32_t a[2][4];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            decode_e2m1x8(reinterpret_cast<const uint32_t *>(&w[u][r])[q], a[r]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              a[r][j] = kWide ? mul_bf16x2(low_bf16x2(a[r][j]), scale[u][r][q / 2]) : mul_f16x2(a[r][j], scale[u][r][q / 2]);
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma_m16n8k16<kWide>(acc[u][n], a[0][0], a[1][0], a[0][1], a[1][1], f[n].x, f[n].y);
+            mma_m16n8k16<kWide>(acc[u][n], a[0][2], a[1][2], a[0][3], a[1][3], f[n].z, f[n].w);
+          }
         }
       }
+      __syncwarp();  // the stage is read by all lanes
+      copy(i + S::depth);
     }
-    __syncwarp();  // the stage is read by all lanes
-    copy(i + S::depth);
-  }
+  };
+  if (wide) products(std::true_type());
+  else products(std::false_type());
   copies_wait<0>();
 
   // ---- sums over the warps, then over the blocks of the cluster ----
@@ -405,7 +496,8 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 1)
       const float4 other = at[w * S::tokens * S::sum_row / 4];
       sum.x += other.x, sum.y += other.y, sum.z += other.z, sum.w += other.w;
     }
-    const float back = kScaled ? power_of_two(-row_shift(row_max[m])) : 1.0f;
+    const float back =
+        !kScaled ? 1.0f : power_of_two(wide ? kWideShift - wide_row_shift(row_max[m]) : -row_shift(row_max[m]));
     sum = make_float4(sum.x * alpha * back, sum.y * alpha * back, sum.z * alpha * back, sum.w * alpha * back);
     if (split == 1)
       store(m, l, sum);
