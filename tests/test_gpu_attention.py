@@ -534,3 +534,31 @@ def test_bad_offsets_write_nothing_beside_the_outputs(rows, keys, heads, cut, fi
                 assert (lse[:guard] == 7).all() and (lse[guard + heads * rows:] == 7).all()
                 assert (workspace[:256] == 99).all() and (workspace[256 + need:] == 99).all()
                 assert _lib.device_status(clear=True) == _lib.VFB_OK
+
+
+def test_a_captured_stack_keeps_what_it_reads():
+    """Inputs that only the graph still needs (the offsets of a packed batch, the gate, the weights) stay as they were."""
+    import gc
+    import weakref
+
+    from tests.helpers import fp8_weight
+    from vflash_b200.native.h3_block_stack import FP8BlockStack, block_shapes
+    from vflash_b200.native.h3_parallel import FP8Weight
+
+    hidden = 256
+    parts = {name: fp8_weight(n, k, j) for j, (name, n, k) in enumerate(block_shapes(hidden, 1024))}
+    blocks = [{name: FP8Weight(c.to(DEV), s.to(DEV)) for name, (c, s) in parts.items()}]
+    x = normal((300, 1, hidden), 5, BF16)
+    gate = torch.full((1, hidden), 1 / 32, dtype=BF16, device=DEV)
+    cu = offsets([170, 130])
+    attend = PackedAttention(heads=4)
+    stack = FP8BlockStack(blocks, hidden, 1024, DEV, resident=True, chunk_bytes=1 << 20)
+    want = stack.forward(x, gate, attention=attend, cu_seqlens=cu)
+    replay = stack.capture(x, gate, attention=attend, cu_seqlens=cu)
+    kept = [weakref.ref(t) for t in (x, gate, cu, stack)]
+    del x, gate, cu, stack
+    gc.collect()
+    assert all(ref() is not None for ref in kept)
+    others = [torch.full((n,), -1, dtype=torch.int32, device=DEV) for n in (3, 128, 300 * 128) for _ in range(50)]
+    assert torch.equal(replay(), want)
+    del others

@@ -128,9 +128,9 @@ class FP8BlockStack:
 
         The stack runs once eagerly first (loading every block and setting up
         the kernels), then the block loop is captured; a replay reads the
-        current contents of ``hidden`` and ``gate`` (and ``cu_seqlens``) and
-        rewrites the returned output tensor.  One graph launch replaces the per-block host work of
-        issuing 8 kernels per block.
+        current contents of ``hidden`` and ``gate`` (and ``cu_seqlens``), which it
+        keeps alive with the stack, and rewrites the returned output tensor.  One graph
+        launch replaces the per-block host work of issuing 8 kernels per block.
         """
         if not self.ring.resident:
             raise ValueError("graph capture needs a resident stack")
@@ -145,6 +145,7 @@ class FP8BlockStack:
             return out
 
         replay.graph = graph
+        replay.reads = (self, hidden, gate, cu_seqlens)  # by address: they live as long as the graph
         return replay
 
     def _block(self, gate, attention, cu_seqlens):
