@@ -15,8 +15,9 @@
 //     its largest magnitude (of the block's K range) into [2^14, 2^15), which is
 //     exact for elements down to 2^-31 of it.  Where a row of the block has others
 //     than 0 below, the block takes bf16 for both operands: a decoded weight is exact there
-//     too, but takes three more instructions for a pair (1.5 times as many in the
-//     loop).  Products are exact either way, sums fp32, and both give the same bits.
+//     too, but takes three more instructions for a pair (1 row, 12288 x 4096 14.6 us
+//     instead of 10.0, 32 rows, 16384 x 4096 33.8 instead of 24.8).  Products are exact
+//     either way, sums fp32, and both give the same bits.
 //   * the order of k inside a product is free as long as both operands agree.
 //     A lane takes 32 consecutive weights of a row (one 16-byte load), a quad 128
 //     of them (a "step": 64 bytes of every row), and x is laid out in shared
@@ -582,6 +583,9 @@ int launch_split(const Args &p, int sms, int resident, cudaStream_t stream) {
 // few blocks costs less.  Measured (us, N x K):
 //   8 rows of x, 64 / 128 rows a block: 1152 x 1024 4.3 / 5.2, 128 x 16384 7.9 / 10.1,
 //   4096 x 4096 7.3 / 7.0, 12288 x 4096 14.6 / 12.8, 4096 x 16384 22.7 / 16.3;
+//   one row 1152 x 1024 3.2 / 4.3, 128 x 16384 5.5 / 7.8, 1152 x 16384 8.0 / 8.7,
+//   2048 x 16384 8.6 / 11.2, 4096 x 4096 6.3 / 6.1, 4096 x 16384 12.9 / 12.4 (two rows
+//   12% more on either side);
 //   128 / 256 rows, with tall blocks that fill the rounds on 148 SMs: 14336 x 5376
 //   21.3 / 16.8, 16384 x 4096 15.8 / 14.2, 28672 x 5376 33.8 / 26.6, 36864 x 4096
 //   29.1 / 22.8, and for one row of x 14.7 / 14.0, 12.2 / 12.0, 23.9 / 22.7, 19.8 / 19.5;
