@@ -562,3 +562,17 @@ def test_a_captured_stack_keeps_what_it_reads():
     others = [torch.full((n,), -1, dtype=torch.int32, device=DEV) for n in (3, 128, 300 * 128) for _ in range(50)]
     assert torch.equal(replay(), want)
     del others
+
+
+def test_the_largest_number_of_keys():
+    """2^31 - 1 keys and rows of both tiles of a job: key counts rounded up to tiles pass 31 bits."""
+    nq, nk = 256, 2**31 - 1
+    k = torch.zeros(nk, 1, 8, dtype=BF16, device=DEV)
+    k[-1, 0, 0] = 40  # all the weight: the others have e^-40 each
+    q = torch.zeros(nq, 1, 8, dtype=BF16, device=DEV)
+    q[..., 0] = 1
+    assert workspace_bytes(q, k, 1, False) > 0
+    got, lse = attention(q, k, k, scale=1.0, return_lse=True)
+    assert _lib.device_status(clear=True) == _lib.VFB_OK
+    assert torch.equal(got, 40 * q)
+    assert ((lse - 40).abs() <= 1e-4).all()  # 2^31 e^-40 is 9e-9

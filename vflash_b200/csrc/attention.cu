@@ -309,8 +309,8 @@ __device__ __forceinline__ void describe(const Params &p, const Segment &s, Job 
   const int32_t tiles = max(s.t1 - s.t0, 0);
   if (PAIR) {
     // stage 0's rows may see fewer keys than the job's last row
-    const int32_t seen0 = attn::keys_seen(p.plan, s.seq, j.rows0 + min(p.tokens, j.count));
-    j.n[0] = max(min(s.t1, (seen0 + 127) / 128) - s.t0, 0);
+    const uint32_t seen0 = attn::keys_seen(p.plan, s.seq, j.rows0 + min(p.tokens, j.count));
+    j.n[0] = max(min(s.t1, static_cast<int32_t>((seen0 + 127) / 128)) - s.t0, 0);  // unsigned: up to 2^31 - 1 keys
     j.n[1] = j.count > p.tokens ? tiles : 0;
   } else {
     j.n[0] = (tiles + 1) / 2;
@@ -1320,7 +1320,7 @@ extern "C" int vfb_attention(const vfb_attention_args *args, void *stream) {
   p.plan.blocks = sms < kMaxBlocks ? sms : kMaxBlocks;
   p.plan.key_shift = c.pair ? 7 : 6;
   p.plan.band_keys = kBandBytes / (4 * a.dim);
-  p.plan.unit_shift = attn::unit_shift_for(c.jobs, a.total_q + a.total_k);
+  p.plan.unit_shift = c.split ? attn::unit_shift_for(c.jobs, a.total_q + a.total_k) : 0;
   p.v = a.v;
   p.out = a.out;
   p.lse = a.lse;
