@@ -81,6 +81,7 @@ constexpr int kJobReaders = 11;      // warps that follow the schedule
 // for a job's last tiles): a job of 2^31 keys takes about 30 s.  The waits inside a job
 // have the usual limit, and whichever runs out first ends all of them.
 constexpr uint64_t kJobTimeoutNs = 120000000000ull;
+constexpr uint64_t kDrainNs = 100000000;  // for the products in flight when a block ends
 constexpr float kHold = 8.0f;
 // P carries a factor of 2^kLift, which cancels in O / l and comes off the
 // log-sum-exp.  fp16 ends at 2^-24, and many keys that each round to 0 there may hold
@@ -828,7 +829,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             load(&map_k, kv_head, k0 + static_cast<int64_t>(i + L::ahead) * kKeys, false);
         }
       }
-      // every load has landed before the block ends (a finished run waits for nothing here)
+      // every load has landed before the block ends (a finished run waits for nothing here;
+      // after an abort 256 tries each, far longer than a load takes)
       if (q_loaded) warp_wait_quick(&sh.q_full, q_phase ^ 1, &sh.abort, p.status);
       for (int i = 0; i < L::ring; ++i) {
         const uint32_t last = i < pos.slot ? pos.phase : pos.phase ^ 1;
@@ -934,7 +936,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // the products issued last are over before the block ends
         tc_commit(&sh.drain);
-        wait(&sh.drain, 0);
+        mbar_drain(&sh.drain, 0, kDrainNs);
       }
     } else if (warp == 11) {
       // ---------------- schedule ----------------

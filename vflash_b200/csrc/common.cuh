@@ -488,6 +488,15 @@ __device__ __forceinline__ bool warp_wait_quick(uint64_t *bar, uint32_t parity, 
   }
 }
 
+// For a role's own copies and products in flight, before its block ends: they are waited
+// for after an abort too, if not for ever.  No clock is read where they are there already.
+__device__ __forceinline__ void mbar_drain(uint64_t *bar, uint32_t parity, uint64_t timeout_ns) {
+  if (mbar_try_wait(bar, parity)) return;
+  const uint64_t start = global_timer_ns();
+  while (!mbar_try_wait(bar, parity) && global_timer_ns() - start < timeout_ns) {
+  }
+}
+
 // A bounded wait without an answer, for the MMA issuer: after one that ran out
 // (or another role's abort) the caller goes on, its later waits return at
 // once, and what it issues is discarded with the rest of the run.  Control flow
