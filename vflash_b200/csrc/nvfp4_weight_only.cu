@@ -221,7 +221,6 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 1)
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t *xs = smem + S::ring_bytes;
   __shared__ uint32_t row_max[S::tokens];
-  __shared__ uint32_t row_low[S::tokens];  // of each row's smallest magnitude other than 0, see smallest_x8
   __shared__ float bias[S::rows];
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane / 4, t = lane % 4;
   const int split = gridDim.x;  // cluster: blocks along K
@@ -300,11 +299,7 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 1)
       else best[1] = max(best[1], largest), low[1] = smallest_x8(v, low[1]);
     } else {  // 16 lanes with one row's chunks
       const uint32_t top = __reduce_max_sync(0xFFFFu << (lane & 16), largest);
-      const uint32_t least = __reduce_min_sync(0xFFFFu << (lane & 16), lower_half(smallest_x8(v, kNoneLow)));
-      if (lane % 16 == 0 && top) {
-        atomicMax(&row_max[row_of(i)], top);
-        atomicMin(&row_low[row_of(i)], least);
-      }
+      if (lane % 16 == 0 && top) atomicMax(&row_max[row_of(i)], top);
     }
   };
   constexpr int kFlight = NT == 1 ? 8 : 12;  // chunks of a thread in flight
@@ -325,7 +320,7 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 1)
   const float alpha = __ldg(p.alpha);
   for (int r = tid; r < S::rows; r += kThreads) bias[r] = p.bias != nullptr ? __bfloat162float(p.bias[feature(r)]) : 0.0f;
   if (kScaled && !kOwnRows) {
-    if (tid < S::tokens) row_max[tid] = 0, row_low[tid] = 0xFFFF;
+    if (tid < S::tokens) row_max[tid] = 0;
     __syncthreads();
   }
   int base = 0;  // of the last flight, which stays in registers until the rows' maxima are known
@@ -353,7 +348,10 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 1)
       *place(i) = c;
     }
   }
-  const auto scaled = [&](uint4 c, float factor) {
+  bool lossy = false;  // this thread has numbers that lose bits in fp16
+  const auto scaled = [&](uint4 c, uint32_t max_bits) {
+    const float factor = power_of_two(row_shift(max_bits));
+    if (!kOwnRows) lossy |= loses_bits(max_bits, lower_half(smallest_x8(c, kNoneLow)));
     uint32_t w[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -368,8 +366,8 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 1)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, best[r]);
-        const uint32_t least = __reduce_min_sync(0xFFFFFFFFu, lower_half(low[r]));
-        if (lane == 0 && warp + r * WARPS < S::tokens) row_max[warp + r * WARPS] = top, row_low[warp + r * WARPS] = least;
+        lossy |= loses_bits(top, lower_half(low[r]));
+        if (lane == 0 && warp + r * WARPS < S::tokens) row_max[warp + r * WARPS] = top;
       }
       __syncwarp();
     } else {
@@ -377,19 +375,17 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 1)
     }
 #pragma unroll 4
     for (int i = first; i < base; i += kStride)
-      *place(i) = scaled(*place(i), power_of_two(row_shift(row_max[row_of(i)])));
+      *place(i) = scaled(*place(i), row_max[row_of(i)]);
   }
 #pragma unroll
   for (int j = 0; j < kFlight; ++j) {
     const int i = base + j * kStride + first;
     if (i >= items) break;
-    *place(i) = kScaled ? scaled(v[j], power_of_two(row_shift(row_max[row_of(i)]))) : v[j];
+    *place(i) = kScaled ? scaled(v[j], row_max[row_of(i)]) : v[j];
   }
-  __syncthreads();
 
   // ---- rows whose numbers lie too far apart for fp16: all of x again, in bf16 ----
-  const bool wide =
-      kScaled && __any_sync(0xFFFFFFFFu, lane < tokens && loses_bits(row_max[min(lane, tokens - 1)], row_low[min(lane, tokens - 1)]));
+  const bool wide = __syncthreads_or(lossy) && kScaled;
   if (wide) {
 #pragma unroll 1
     for (int i = first; i < items; i += kStride) {
