@@ -148,17 +148,19 @@ __device__ __forceinline__ uint4 gather_x8(const T *p) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Largest magnitude of eight bf16 numbers, as the bits of an f32; NaN is left out.
-__device__ __forceinline__ uint32_t largest_x8(const uint4 &v) {
+// Largest magnitudes of the even and the odd ones of eight bf16 numbers and of those
+// behind `two`; NaN is left out.
+__device__ __forceinline__ __nv_bfloat162 largest_x8(const uint4 &v, __nv_bfloat162 two) {
   const auto magnitudes = [](uint32_t w) {
     w &= 0x7FFF7FFFu;
     return *reinterpret_cast<const __nv_bfloat162 *>(&w);
   };
-  const __nv_bfloat162 two =
-      __hmax2(__hmax2(magnitudes(v.x), magnitudes(v.y)), __hmax2(magnitudes(v.z), magnitudes(v.w)));
+  return __hmax2(__hmax2(__hmax2(magnitudes(v.x), magnitudes(v.y)), __hmax2(magnitudes(v.z), magnitudes(v.w))), two);
+}
+// The larger one, as the bits of an f32.
+__device__ __forceinline__ uint32_t upper_half(__nv_bfloat162 two) {
   const uint32_t w = *reinterpret_cast<const uint32_t *>(&two);
-  const uint32_t lo = w << 16, hi = w & 0xFFFF0000u;  // NaN where all four were
-  return max(lo > 0x7F800000u ? 0u : lo, hi > 0x7F800000u ? 0u : hi);
+  return max(w << 16, w & 0xFFFF0000u);
 }
 
 // Smallest magnitude other than 0 of eight bf16 numbers and of those behind `low`,
@@ -291,14 +293,18 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 1)
   };
   const auto from = [&](int i) { return x + row_of(i) * p.ldx + k_begin + 8 * chunk_of(i); };
   const auto inside = [&](int i) { return 8 * chunk_of(i) < k_left; };  // K is a multiple of eight
-  uint32_t best[2] = {0, 0}, low[2] = {kNoneLow, kNoneLow};  // of a warp's own rows
+  // of a warp's own rows; the smallest without own rows of all of them
+  __nv_bfloat162 best[2] = {__nv_bfloat162(0.0f, 0.0f), __nv_bfloat162(0.0f, 0.0f)};
+  uint32_t low[2] = {kNoneLow, kNoneLow};
   const auto note = [&](int i, const uint4 &v) {
-    const uint32_t largest = largest_x8(v);
+    const int r = kOwnRows ? nth_row(i) : 0;
+    if (r == 0) low[0] = smallest_x8(v, low[0]);
+    else low[1] = smallest_x8(v, low[1]);
     if (kOwnRows) {
-      if (nth_row(i) == 0) best[0] = max(best[0], largest), low[0] = smallest_x8(v, low[0]);
-      else best[1] = max(best[1], largest), low[1] = smallest_x8(v, low[1]);
+      if (r == 0) best[0] = largest_x8(v, best[0]);
+      else best[1] = largest_x8(v, best[1]);
     } else {  // 16 lanes with one row's chunks
-      const uint32_t top = __reduce_max_sync(0xFFFFu << (lane & 16), largest);
+      const uint32_t top = __reduce_max_sync(0xFFFFu << (lane & 16), upper_half(largest_x8(v, best[0])));
       if (lane % 16 == 0 && top) atomicMax(&row_max[row_of(i)], top);
     }
   };
@@ -349,9 +355,7 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 1)
     }
   }
   bool lossy = false;  // this thread has numbers that lose bits in fp16
-  const auto scaled = [&](uint4 c, uint32_t max_bits) {
-    const float factor = power_of_two(row_shift(max_bits));
-    if (!kOwnRows) lossy |= loses_bits(max_bits, lower_half(smallest_x8(c, kNoneLow)));
+  const auto scaled = [&](uint4 c, float factor) {
     uint32_t w[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -365,23 +369,24 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 1)
     if (kOwnRows) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, best[r]);
+        const uint32_t top = __reduce_max_sync(0xFFFFFFFFu, upper_half(best[r]));
         lossy |= loses_bits(top, lower_half(low[r]));
         if (lane == 0 && warp + r * WARPS < S::tokens) row_max[warp + r * WARPS] = top;
       }
       __syncwarp();
-    } else {
+    } else {  // its smallest number beside the largest of all rows: never too few are found
       __syncthreads();
+      lossy = loses_bits(__reduce_max_sync(0xFFFFFFFFu, lane < tokens ? row_max[lane] : 0u), lower_half(low[0]));
     }
 #pragma unroll 4
     for (int i = first; i < base; i += kStride)
-      *place(i) = scaled(*place(i), row_max[row_of(i)]);
+      *place(i) = scaled(*place(i), power_of_two(row_shift(row_max[row_of(i)])));
   }
 #pragma unroll
   for (int j = 0; j < kFlight; ++j) {
     const int i = base + j * kStride + first;
     if (i >= items) break;
-    *place(i) = kScaled ? scaled(v[j], row_max[row_of(i)]) : v[j];
+    *place(i) = kScaled ? scaled(v[j], power_of_two(row_shift(row_max[row_of(i)]))) : v[j];
   }
 
   // ---- rows whose numbers lie too far apart for fp16: all of x again, in bf16 ----
