@@ -427,7 +427,7 @@ typedef struct vfb_attention_args {
   void *out;                   /* the same type, [total_q, heads, dim] */
   float *lse;                  /* [heads, total_q] contiguous, or NULL; out and lse may not overlap q, k, v or each
                                 * other (refused unless apart or interleaved with one period) */
-  int64_t q_token_stride, q_head_stride;  /* strides in elements, multiples of 8; bases 16-byte aligned */
+  int64_t q_token_stride, q_head_stride;  /* strides in elements, multiples of 8, >= dim; bases 16-byte aligned */
   int64_t k_token_stride, k_head_stride;
   int64_t v_token_stride, v_head_stride;
   int64_t out_token_stride, out_head_stride;

@@ -6,9 +6,9 @@
 // is built around many wide loads in flight and few instructions for a weight:
 //   * mma.m16n8k16 with the weights as the 16-row operand and up to 8 rows of x
 //     as the 8 columns: one instruction multiplies 256 weights, whatever M <= 8.
-//     (tcgen05 wants its operands in shared memory, 128 rows at a time: the
-//     decoded weights would make a round trip that the product is too small to
-//     pay for.)
+//     (tcgen05 reads its operands from shared memory, the first also from TMEM, 128
+//     rows at a time: the decoded weights would make a round trip through either, which a
+//     few columns do not pay for.)
 //   * a decoded weight e2m1 * e4m3 has at most six significant bits and lies in
 //     2^-10 .. 2688, so it is exact in fp16: cvt.f16x2.e2m1x2 and one HMUL2.
 //     x is brought to fp16 too, each row multiplied by a power of two that puts
@@ -34,10 +34,11 @@
 // memory, those of the blocks of a cluster (one K range each) through distributed
 // shared memory, always in the same order.
 //
-// Measured (replayed graphs): 1 row, N = 12288, K = 4096 9.9 us (2.9 TB/s with 4 us of
-// it start and end), N = 28672, K = 5376 21.6 us (4.0 TB/s); 7 rows of that 23 us;
-// 32 rows, N = 12288, K = 4096 24.7 us: bringing x to fp16 a quarter of a block's
-// time, products and decoding, with 96 of 148 SMs, most of the rest.
+// Measured (replayed graphs, weights that left L2): 1 row, N = 12288, K = 4096 10.2 us
+// (2.8 TB/s with 4 us of it start and end), N = 28672, K = 5376 22.3 us (3.9 TB/s); 7
+// rows of that 26.5 us, in fp16, which needs no power of two, 22.9; 32 rows, N = 12288,
+// K = 4096 24.1 us: bringing x to fp16 a quarter of a block's time, products and
+// decoding, with 96 of 148 SMs, most of the rest.
 #include <type_traits>
 
 #include "common.cuh"

@@ -609,7 +609,8 @@ def nvfp4_weight_only(matrix: torch.Tensor, w_packed: torch.Tensor, w_scales: to
     ``w_packed`` uint8 ``[N, K/2]`` and ``w_scales`` uint8 (128x4 layout) as
     ``nvfp4_gemm`` takes them, ``alpha`` an fp32 scalar tensor, ``bias`` bf16
     ``[N]``.  K % 64 == 0, K <= 32768, N % 128 == 0.  Made for few rows (one token,
-    a small batch); more rows work too, re-reading the weight for every 32.
+    a small batch); more rows work too, re-reading the weight for every 32 (every 16
+    for a deep weight).  Activations of a row may lie as far apart as bf16 allows.
     ``out`` may be a strided view and may not overlap an operand (columns of one
     buffer beside ``matrix`` are apart).  ``checked``
     skips the checks of the weight and the bias, for a caller that made them
@@ -679,7 +680,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: t
 
     ``q`` ``[total_q, heads, dim]``, ``k`` and ``v`` ``[total_k, kv_heads, dim]``,
     all bf16 or all fp16, ``dim`` a multiple of 8 up to 128 with unit stride,
-    other strides free (multiples of 8 elements); head ``h`` reads key head
+    other strides free (multiples of 8 elements, at least ``dim``); head ``h`` reads key head
     ``h // (heads // kv_heads)``.  Sequence ``b`` has the query rows
     ``cu_seqlens_q[b]:cu_seqlens_q[b+1]`` and the keys of the same entries of
     ``cu_seqlens_k`` (default: the queries' offsets), of which only the first
