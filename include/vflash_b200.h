@@ -390,9 +390,11 @@ VFB_API int vfb_nvfp4_gemm_quant(const void *A, const void *sfa, const void *W, 
  * (refused unless apart or interleaved with one period).  Requires K % 64 == 0, K <= 32768,
  * N % 128 == 0, N <= 1048576, M <= 524288, 16-byte aligned w_codes, 4-byte
  * aligned w_sf.
- * bf16 rows are brought to fp16 by a power of two of their own, or kept in bf16
- * where that would lose bits: products are exact down to 2^-160 of the row's
- * largest magnitude.  No reference counterpart: the reference always quantises the
+ * bf16 rows are brought to fp16 by a power of two of their own: products are exact
+ * for elements down to 2^-31 of the row's largest magnitude, and of smaller ones 2^-39
+ * of it may be lost where one element in sixteen (of the K range of a block) lies within
+ * 2^-12 of the largest.  Other rows are kept in bf16, where products are exact down to
+ * 2^-160 of the largest.  No reference counterpart: the reference always quantises the
  * activations. */
 VFB_API int vfb_nvfp4_weight_only(const void *x, int32_t dtype, int64_t M, int64_t ldx,
                                   const void *w_codes, const void *w_sf, const float *alpha,

@@ -302,3 +302,26 @@ def test_subnormal_and_largest_activations():
     x[3] = (x[3].float().clamp(-4, 4) * 2.0**100).to(BF16)
     got = nvfp4_weight_only(x, weight.packed, weight.scales, weight.alpha)
     check_without_loss(got, x, weight)
+
+
+@pytest.mark.parametrize("rows,n,k", [(1, 4096, 4096), (3, 256, 512), (8, 128, 16384), (9, 384, 1024), (32, 256, 4096)])
+@pytest.mark.parametrize("outlier", [0.0, 2e4])
+def test_activations_behind_a_gelu(rows, n, k, outlier):
+    """A row's long tail towards zero, with and without an outlier on a weight of zero."""
+    weight = without_column(weight_of(n, k, 5), 40)
+    x = torch.nn.functional.gelu(3 * activations(rows, k, 6, torch.float32), approximate="tanh").to(BF16)
+    x[:, 40] = outlier
+    check_without_loss(nvfp4_weight_only(x, weight.packed, weight.scales, weight.alpha), x, weight)
+
+
+@pytest.mark.parametrize("rows,n,k", [(1, 4096, 4096), (8, 128, 16384), (32, 256, 4096)])
+@pytest.mark.parametrize("outlier", [0.0, 2e4])
+def test_activations_over_many_orders(rows, n, k, outlier):
+    """Evenly spread from 2^-43 to 1 on a logarithmic scale: enough large ones that what fp16 leaves of the small
+    ones is nothing beside their sums, unless there is an outlier on a weight of zero."""
+    weight = without_column(weight_of(n, k, 5), 40)
+    gen = torch.Generator(device=DEV).manual_seed(7)
+    x = torch.exp(-30 * torch.rand(rows, k, generator=gen, device=DEV))
+    x = (x * torch.where(torch.rand(rows, k, generator=gen, device=DEV) < 0.5, -1, 1)).to(BF16)
+    x[:, 40] = outlier
+    check_without_loss(nvfp4_weight_only(x, weight.packed, weight.scales, weight.alpha), x, weight)

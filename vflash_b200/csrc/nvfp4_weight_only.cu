@@ -13,11 +13,15 @@
 //     2^-10 .. 2688, so it is exact in fp16: cvt.f16x2.e2m1x2 and one HMUL2.
 //     x is brought to fp16 too, each row multiplied by a power of two that puts
 //     its largest magnitude (of the block's K range) into [2^14, 2^15), which is
-//     exact for elements down to 2^-31 of it.  Where a row of the block has others
-//     than 0 below, the block takes bf16 for both operands: a decoded weight is exact there
-//     too, but takes three more instructions for a pair (1 row, 12288 x 4096 14.6 us
-//     instead of 10.0, 32 rows, 16384 x 4096 33.8 instead of 24.8).  Products are exact
-//     either way, sums fp32, and both give the same bits.
+//     exact for elements down to 2^-31 of it and leaves 2^-39 of it of those below.
+//     That is nothing beside the rest where at least one element in sixteen lies
+//     within 2^-12 of the largest: for weights of like size 2^-23 of their products,
+//     fp32's own roundings.  A row that is a few large elements and many small ones
+//     would lose the small ones, and all of the result where the large ones meet
+//     weights of 0.  A block with such a row takes bf16 for both operands: a decoded
+//     weight is exact there too, but takes three more instructions for a pair (1 row,
+//     12288 x 4096 14.9 us instead of 10.3, 32 rows, 16384 x 4096 35.2 instead of 24.7).
+//     Sums are fp32 either way.
 //   * the order of k inside a product is free as long as both operands agree.
 //     A lane takes 32 consecutive weights of a row (one 16-byte load), a quad 128
 //     of them (a "step": 64 bytes of every row), and x is laid out in shared
@@ -190,6 +194,12 @@ __device__ __forceinline__ int row_shift(uint32_t max_bits) {
 __device__ __forceinline__ bool loses_bits(uint32_t max_bits, uint32_t low) {
   const int smallest = max(static_cast<int>(low + 1) >> 7, 1);  // its exponent, biased; subnormals share that of the smallest normal one
   return low != 0xFFFFu && smallest - 127 + row_shift(max_bits) < -17;
+}
+
+// How many of eight fp16 numbers are at least 4, 2^-12 of the largest that a row may hold.
+__device__ __forceinline__ int large_x8(const uint4 &h) {
+  const auto signs = [](uint32_t w) { return ((w & 0x7FFF7FFFu) + 0x3C003C00u) & 0x80008000u; };  // 4 is 0x4400
+  return __popc(signs(h.x) | signs(h.y) >> 1 | signs(h.z) >> 2 | signs(h.w) >> 3);
 }
 
 // The power of two of a row whose block takes bf16: it puts the largest magnitude at
@@ -391,7 +401,19 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 1)
   }
 
   // ---- rows whose numbers lie too far apart for fp16: all of x again, in bf16 ----
-  const bool wide = __syncthreads_or(lossy) && kScaled;
+  bool wide = __syncthreads_or(lossy) && kScaled;
+  if (wide) {  // unless enough of every row are large: a few lanes count them, one warp a row
+    bool few = false;
+    for (int r = warp; r < tokens; r += WARPS) {
+      int large = 0;
+      for (int at = 16 * lane; at < 256 * p.steps; at += 512) {
+        const uint4 h = *reinterpret_cast<const uint4 *>(xs + r * row_bytes + at);
+        large += large_x8(h);
+      }
+      few |= row_max[r] != 0 && 16 * __reduce_add_sync(0xFFFFFFFFu, large) < min(p.steps * kStep, k_left);
+    }
+    wide = __syncthreads_or(few);
+  }
   if (wide) {
 #pragma unroll 1
     for (int i = first; i < items; i += kStride) {

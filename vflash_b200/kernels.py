@@ -610,7 +610,7 @@ def nvfp4_weight_only(matrix: torch.Tensor, w_packed: torch.Tensor, w_scales: to
     ``nvfp4_gemm`` takes them, ``alpha`` an fp32 scalar tensor, ``bias`` bf16
     ``[N]``.  K % 64 == 0, K <= 32768, N % 128 == 0.  Made for few rows (one token,
     a small batch); more rows work too, re-reading the weight for every 32 (every 16
-    for a deep weight).  Activations of a row may lie as far apart as bf16 allows.
+    for a deep weight).  A few large activations take nothing from the others of their row.
     ``out`` may be a strided view and may not overlap an operand (columns of one
     buffer beside ``matrix`` are apart).  ``checked``
     skips the checks of the weight and the bias, for a caller that made them
