@@ -576,3 +576,29 @@ def test_the_largest_number_of_keys():
     assert _lib.device_status(clear=True) == _lib.VFB_OK
     assert torch.equal(got, 40 * q)
     assert ((lse - 40).abs() <= 1e-4).all()  # 2^31 e^-40 is 9e-9
+
+
+@pytest.mark.parametrize("dtype,size", [(FP16, 300.0), (FP16, 5000.0), (FP16, 60000.0), (BF16, 1e4), (BF16, 1e9), (BF16, 1e17)])
+@pytest.mark.parametrize("nq,nk,heads,kv_heads,dim,cut", CUT)
+def test_huge_scores_pick_the_largest(nq, nk, heads, kv_heads, dim, cut, dtype, size):
+    """Scores far beyond 2^24 and far apart: every row is the value of its best key, and stays finite."""
+    q, k, v = operands([nq], [nk], heads, kv_heads, dim, dtype)
+    assert (workspace_bytes(q, k, 1, False) > 0) == cut
+    q.zero_()
+    k.zero_()
+    gen = torch.Generator().manual_seed(4)
+    sign = torch.where(torch.rand(nq, heads, generator=gen) < 0.5, -1.0, 1.0).to(DEV)
+    q[..., 3] = (size * sign).to(dtype)
+    # keys by their place: steps of a 64th of the size, so that neighbours are far apart in the scores too
+    place = torch.randint(-64, 65, (nk, kv_heads), generator=gen).to(DEV)
+    best, worst = nk // 3, nk - 2
+    place[best], place[worst] = 65, -65
+    k[..., 3] = (size * place / 66).to(dtype)
+    got, lse = attention(q, k, v, offsets([nq]), offsets([nk]), scale=1.0, return_lse=True)
+    wide = lambda row: v[row].repeat_interleave(heads // kv_heads, dim=0).expand(nq, heads, dim)  # noqa: E731
+    want = torch.where(sign[..., None] > 0, wide(best), wide(worst))
+    assert torch.equal(got, want)
+    peak = torch.where(sign > 0, k[best, :, 3].repeat_interleave(heads // kv_heads).double(),
+                       -k[worst, :, 3].repeat_interleave(heads // kv_heads).double()) * q[..., 3].abs().double()
+    assert ((lse.double().T - peak).abs() <= 2.0**-22 * peak).all()  # the score and its way through log2 and back
+    assert _lib.device_status(clear=True) == _lib.VFB_OK

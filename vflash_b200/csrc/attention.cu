@@ -49,7 +49,7 @@
 // 32760 tokens of 32 heads, all pairs, 15.3 to 15.6 ms (13.5 while cool, then 14.9; 1130 to
 // 1300 TFLOP/s, at the power limit); causal prompts of 8192 to 1 tokens, 32 on 8 heads, 754 to
 // 770 us (657: 1140 TFLOP/s at a higher clock); 48 prompts of 1 to 300 tokens, heads of 64,
-// 24 us (25); 17 tokens 12.5 us, bound by the host (8.5, all latency); one token of 32
+// 25 us (25); 17 tokens 12.5 us, bound by the host (8.5, all latency); one token of 32
 // requests on 1 to 8192 cached keys 86 to 91 us (86: 4.5 TB/s), of one on 131072 keys
 // 104 to 112 us (106: 5.1 TB/s).
 //
@@ -89,6 +89,12 @@ constexpr float kHold = 8.0f;
 // log-sum-exp.  fp16 ends at 2^-24, and many keys that each round to 0 there may hold
 // a good part of l; P is at most 2^kHold, so 2^7 more still fit below 65504, and what
 // is lost of a probability is at most 2^-32 of the largest.  bf16 has fp32's range.
+// The maximum times the scale is rounded before it is taken off the scores' products,
+// by up to 2^-4 here and 2^-24 of it beyond, which P has no room for.  From the tile
+// on in which some row's maximum goes beyond, a warp takes the maximum off those rows'
+// scores first, in a loop of its own (one packed addition more for every pair: 15.97
+// instead of 15.35 ms for 32760 tokens).
+constexpr float kFar = 1048576.0f;
 template <typename T>
 constexpr float kLift = std::is_same<T, __half>::value ? 7.0f : 0.0f;
 constexpr float kLn2 = 0.693147180559945309f;
@@ -453,15 +459,23 @@ struct Softmax {
   __device__ __forceinline__ bool run(int32_t t0, int32_t n, int32_t stride, int32_t limit, bool live, bool valid) {
     m = -INFINITY;
     l = 0.0f;
-    for (int32_t i = 0; i < n; ++i, ++count) {
+    int32_t i = 0;
+    for (; i < n; ++i, ++count) {
       if (!wait(&sh.s_full[stage][count % kBuffers], count / kBuffers & 1)) return false;
       tc_fence_after();
       if (live) {
-        if (!tile((t0 + i * stride) * N, limit, i > 0, valid)) return false;
+        const int done = tile<false>((t0 + i * stride) * N, limit, i > 0, valid);
+        if (done < 0) break;
+        if (done == 0) return false;
       } else {
         hand_over(sh.p_full[stage]);
         hand_over(sh.p_tail[stage]);
       }
+    }
+    for (bool first = true; i < n; ++i, ++count, first = false) {
+      if (!first && !wait(&sh.s_full[stage][count % kBuffers], count / kBuffers & 1)) return false;
+      tc_fence_after();
+      if (tile<true>((t0 + i * stride) * N, limit, i > 0, valid) == 0) return false;
     }
     return true;
   }
@@ -478,7 +492,9 @@ struct Softmax {
         : "memory");
   }
 
-  __device__ __forceinline__ bool tile(int32_t key0, int32_t limit, bool scale_o, bool valid) {
+  // 1 when done, 0 after a wait that ran out, -1 (nothing done) where only tile<true> will do.
+  template <bool FAR>
+  __device__ __forceinline__ int tile(int32_t key0, int32_t limit, bool scale_o, bool valid) {
     const uint32_t at = tmem_s + N * (count % kBuffers);
     float s[N];
     {
@@ -506,6 +522,7 @@ struct Softmax {
     // true also for a NaN score; not while no key has been seen
     const bool move = valid && !((peak - m) * p.scale_log2 <= kHold) && peak != -INFINITY;
     if (__any_sync(0xffffffffu, move)) {
+      if (!FAR && __any_sync(0xffffffffu, move && fabsf(peak * p.scale_log2) > kFar)) return -1;
       const float alpha = !move ? 1.0f : m == -INFINITY ? 0.0f : ex2((m - peak) * p.scale_log2);
       if (move) {
         m = peak;
@@ -513,7 +530,7 @@ struct Softmax {
       }
       if (scale_o) {
         // S(count) came behind the P V that freed its buffer, so at most one phase of pv_done is open here.
-        if (!wait(&sh.pv_done[stage], (count - 1) & 1)) return false;
+        if (!wait(&sh.pv_done[stage], (count - 1) & 1)) return 0;
         tc_fence_after();
 #pragma unroll 1
         for (int c = 0; c < DP; c += 16) {  // few columns at a time: S holds the registers
@@ -525,7 +542,13 @@ struct Softmax {
         }
       }
     }
-    const float base = m == -INFINITY ? 0.0f : m * p.scale_log2;
+    float base = m == -INFINITY ? 0.0f : m * p.scale_log2;
+    if (FAR) {
+      const float off = fabsf(base) > kFar ? m : 0.0f;  // the other rows' bits stay as they are
+#pragma unroll
+      for (int j = 0; j < N; ++j) s[j] -= off;
+      if (off != 0.0f) base = 0.0f;
+    }
     const f32x2 scale2 = pair(p.scale_log2, p.scale_log2), base2 = pair(kLift<T> - base, kLift<T> - base);
     f32x2 sum[2] = {pair(0.0f, 0.0f), pair(0.0f, 0.0f)};
 #pragma unroll
@@ -553,7 +576,7 @@ struct Softmax {
     split(sum[0], a, b);
     split(sum[1], c, d);
     l += (a + b) + (c + d);
-    return true;
+    return 1;
   }
 };
 
