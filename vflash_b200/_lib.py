@@ -233,6 +233,8 @@ def ptr(tensor) -> int | None:
 def stream_handle(device) -> int:
     import torch
 
+    if not isinstance(device, torch.device):  # None, an index or a name
+        return torch.cuda.current_stream(device).cuda_stream
     # the raw handle: building a torch.cuda.Stream object costs 2 us a call
     index = torch.cuda.current_device() if device.index is None else device.index
     return torch._C._cuda_getCurrentRawStream(index)
