@@ -5,7 +5,8 @@ may see (nothing behind a mask is touched).  ``bound`` is per element, from the
 roundings that any kernel of this contract makes, u being half a step of the
 operand type (``torch.finfo(t).eps / 2``) and e = 2^-24 that of fp32:
 
-* the output's rounding: u |o|;
+* the output's rounding: u |o|, and half the smallest subnormal (2^-25 in fp16,
+  nothing measurable in bf16) where it is subnormal;
 * every exp value rounded to the type before the second product:
   u sum_j p_j |v_j| / l, plus half the smallest subnormal for each key
   (2^-25 in fp16, nothing measurable in bf16) times |v_j|, with l >= 1; a kernel
@@ -38,7 +39,7 @@ def reference(q, k, v, lengths_q, lengths_k, *, causal: bool, scale: float, slot
     heads, dim = q.shape[1:]
     group = heads // k.shape[1]
     u, e = torch.finfo(q.dtype).eps / 2, 2.0**-24
-    tiny = 2.0**-32 if q.dtype == torch.float16 else 0.0
+    tiny, subnormal = (2.0**-32, 2.0**-25) if q.dtype == torch.float16 else (0.0, 0.0)
     out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
     lse = torch.full((heads, q.shape[0]), -torch.inf, dtype=torch.float64, device=q.device)
     out_bound, lse_bound = torch.zeros_like(out), torch.zeros_like(lse)
@@ -67,6 +68,6 @@ def reference(q, k, v, lengths_q, lengths_k, *, causal: bool, scale: float, slot
             peak = s.masked_fill(~seen, 0).abs().amax(dim=1, keepdim=True)
             relative = 2 * (score + 4 * e * peak) + 2.0**-17 + (nk + 64) * e
             out_bound[rows, h] = (u * out[rows, h].abs() + (u + 2 * relative) * (p @ vs.abs())
-                                  + tiny * (seen.double() @ vs.abs()) + 2.0**-40)
+                                  + tiny * (seen.double() @ vs.abs()) + subnormal + 2.0**-40)
             lse_bound[h, rows] = (relative + 4 * e * (z.abs() + peak) + 1e-7)[:, 0]
     return out, lse, out_bound, lse_bound
