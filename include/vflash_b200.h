@@ -392,7 +392,7 @@ VFB_API int vfb_nvfp4_gemm_quant(const void *A, const void *sfa, const void *W, 
  * aligned w_sf.
  * bf16 rows are brought to fp16 by a power of two of their own: products are exact
  * for elements down to 2^-31 of the row's largest magnitude, and of smaller ones 2^-39
- * of it may be lost where one element in sixteen (of the K range of a block) lies within
+ * of it may be lost where one element in four (of the K range of a block) lies within
  * 2^-12 of the largest.  Other rows are kept in bf16, where products are exact down to
  * 2^-160 of the largest.  No reference counterpart: the reference always quantises the
  * activations. */

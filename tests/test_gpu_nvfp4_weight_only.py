@@ -325,3 +325,16 @@ def test_activations_over_many_orders(rows, n, k, outlier):
     x = (x * torch.where(torch.rand(rows, k, generator=gen, device=DEV) < 0.5, -1, 1)).to(BF16)
     x[:, 40] = outlier
     check_without_loss(nvfp4_weight_only(x, weight.packed, weight.scales, weight.alpha), x, weight)
+
+
+@pytest.mark.parametrize("rows", [1, 8, 20])
+@pytest.mark.parametrize("k,outliers", [(64, 5), (64, 15), (512, 60), (4096, 300)])
+def test_many_outliers_of_several_sizes(rows, k, outliers):
+    """Up to a quarter of a row may be large numbers on weights of zero."""
+    weight = weight_of(2048, k, 5)
+    x = activations(rows, k, 6, BF16)
+    gen = torch.Generator().manual_seed(8)
+    for i, column in enumerate(torch.randperm(k, generator=gen)[:outliers].tolist()):
+        without_column(weight, column)
+        x[:, column] = (1e30, -2e30, 1e20, 4e29)[i % 4]
+    check_without_loss(nvfp4_weight_only(x, weight.packed, weight.scales, weight.alpha), x, weight)

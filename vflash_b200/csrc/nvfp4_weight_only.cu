@@ -14,9 +14,9 @@
 //     x is brought to fp16 too, each row multiplied by a power of two that puts
 //     its largest magnitude (of the block's K range) into [2^14, 2^15), which is
 //     exact for elements down to 2^-31 of it and leaves 2^-39 of it of those below.
-//     That is nothing beside the rest where at least one element in sixteen lies
-//     within 2^-12 of the largest: for weights of like size 2^-23 of their products,
-//     fp32's own roundings.  A row that is a few large elements and many small ones
+//     That is nothing beside the rest where at least one element in four lies
+//     within 2^-12 of the largest: for weights of like size 2^-25 of their products,
+//     below fp32's own roundings.  A row that is a few large elements and many small ones
 //     would lose the small ones, and all of the result where the large ones meet
 //     weights of 0.  A block with such a row takes bf16 for both operands: a decoded
 //     weight is exact there too, but takes three more instructions for a pair (1 row,
@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 3 : 1)
         const uint4 h = *reinterpret_cast<const uint4 *>(xs + r * row_bytes + at);
         large += large_x8(h);
       }
-      few |= row_max[r] != 0 && 16 * __reduce_add_sync(0xFFFFFFFFu, large) < min(p.steps * kStep, k_left);
+      few |= row_max[r] != 0 && 4 * __reduce_add_sync(0xFFFFFFFFu, large) < min(p.steps * kStep, k_left);
     }
     wide = __syncthreads_or(few);
   }
