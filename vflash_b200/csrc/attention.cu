@@ -48,7 +48,7 @@
 // Measured, repeated calls (replayed graphs in brackets, inputs that left L2):
 // 32760 tokens of 32 heads, all pairs, 15.3 to 15.6 ms (13.5 while cool, then 14.9; 1130 to
 // 1300 TFLOP/s, at the power limit); causal prompts of 8192 to 1 tokens, 32 on 8 heads, 754 to
-// 770 us (657: 1140 TFLOP/s at a higher clock); 48 prompts of 1 to 300 tokens, heads of 64,
+// 775 us (657: 1140 TFLOP/s at a higher clock); 48 prompts of 1 to 300 tokens, heads of 64,
 // 25 us (25); 17 tokens 12.5 us, bound by the host (8.5, all latency); one token of 32
 // requests on 1 to 8192 cached keys 86 to 91 us (86: 4.5 TB/s), of one on 131072 keys
 // 104 to 112 us (106: 5.1 TB/s).
